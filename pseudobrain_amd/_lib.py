@@ -1,4 +1,5 @@
-"""ctypes binding of libpbgdn.so (the C ABI declared in include/pbgdn.h).
+"""ctypes binding of libpbgdn.so (the C ABI declared in include/pbgdn.h) and
+libpbattn.so (include/pbattn.h).
 
 torch is imported first so that its HIP runtime is the one in the process:
 the library links libamdhip64 by soname and binds to whatever is loaded.
@@ -17,6 +18,10 @@ LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libpbgdn.so
 # The debug build of the same sources (build.py): LDS and outputs poisoned with NaN.
 DEBUG_LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libpbgdn_debug.so")
 ABI_VERSION = 15
+# The attention operators (include/pbattn.h), a library of their own.
+ATTN_LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libpbattn.so")
+ATTN_DEBUG_LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libpbattn_debug.so")
+ATTN_ABI_VERSION = 1
 
 F32, BF16, F16 = 0, 1, 2
 OK, ERR_INVALID_ARGUMENT, ERR_UNSUPPORTED, ERR_LAUNCH, ERR_SCRATCH = 0, 1, 2, 3, 4
@@ -63,8 +68,23 @@ SIGNATURES = {
     "pbgdn_stream_probe": ([_vp, _vp, ctypes.c_int64, _vp], _i),
 }
 
+_sz = ctypes.c_size_t
+ATTN_SIGNATURES = {
+    "pbattn_abi_version": ([], _i),
+    "pbattn_window_fwd": ([_vp, _vp, _vp, _i, _vp, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _f, _i, _i, _vp],
+                          _i),
+    "pbattn_window_bwd": ([_vp, _vp, _vp, _i, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+                           _i, _i, _i, _i, _i, _i, _f, _i, _i, _vp, _sz, _vp], _i),
+    "pbattn_window_bwd_workspace_size": ([_i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i], _sz),
+    "pbattn_paged_decode": ([_vp, _vp, _vp, _i, _vp, _i, _i, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _f, _i, _i,
+                             _vp, _sz, _vp], _i),
+    "pbattn_paged_decode_workspace_size": ([_i, _i, _i, _i, _i], _sz),
+    "pbattn_paged_write": ([_vp, _vp, _i, _vp, _vp, _vp, _vp, _i, _i, _vp, _i, _i, _i, _vp], _i),
+}
+
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
+_attn: ctypes.CDLL | None = None
 
 
 class PbgdnError(RuntimeError):
@@ -75,27 +95,32 @@ class PbgdnError(RuntimeError):
         super().__init__(f"{where}: pbgdn status {status}: {status_string(status)}")
 
 
-def _declare(handle: ctypes.CDLL, name: str) -> None:
+def _declare(handle: ctypes.CDLL, name: str, signatures) -> None:
     fn = getattr(handle, name)
-    fn.argtypes, fn.restype = SIGNATURES[name]
+    fn.argtypes, fn.restype = signatures[name]
 
 
-def _load(path: str) -> ctypes.CDLL:
+def _load(path: str, signatures=SIGNATURES, version_fn: str = "pbgdn_abi_version",
+          expected: int = ABI_VERSION) -> ctypes.CDLL:
     if not os.path.exists(path):
         raise RuntimeError(
             f"pbgdn HIP library not found at {path}; build it with "
             "`python -m pseudobrain_amd.build` (there is no CPU fallback)")
     handle = ctypes.CDLL(path)
     try:  # the version before the other symbols: an older library lacks some of them
-        _declare(handle, "pbgdn_abi_version")
-        version = handle.pbgdn_abi_version()
-        if version != ABI_VERSION:
-            raise RuntimeError(f"{os.path.basename(path)} ABI version {version}, expected {ABI_VERSION}; rebuild it")
-        for name in SIGNATURES:
-            _declare(handle, name)
+        _declare(handle, version_fn, signatures)
+        version = getattr(handle, version_fn)()
+        if version != expected:
+            raise RuntimeError(f"{os.path.basename(path)} ABI version {version}, expected {expected}; rebuild it")
+        for name in signatures:
+            _declare(handle, name, signatures)
     except AttributeError as e:
-        raise RuntimeError(f"{os.path.basename(path)} lacks a function of ABI {ABI_VERSION} ({e}); rebuild it") from e
+        raise RuntimeError(f"{os.path.basename(path)} lacks a function of ABI {expected} ({e}); rebuild it") from e
     return handle
+
+
+def _load_attn(path: str) -> ctypes.CDLL:
+    return _load(path, ATTN_SIGNATURES, "pbattn_abi_version", ATTN_ABI_VERSION)
 
 
 def lib() -> ctypes.CDLL:
@@ -109,25 +134,39 @@ def lib() -> ctypes.CDLL:
     return _lib
 
 
+def attn_lib() -> ctypes.CDLL:
+    """The loaded attention library; raises RuntimeError when it is not built."""
+    global _attn
+    if _attn is not None:
+        return _attn
+    with _lock:
+        if _attn is None:
+            _attn = _load_attn(ATTN_LIB_PATH)
+    return _attn
+
+
 _debug: ctypes.CDLL | None = None
+_attn_debug: ctypes.CDLL | None = None
 
 
 @contextlib.contextmanager
 def debug_library():
-    """Within the block every call of this package goes to libpbgdn_debug.so,
-    whose kernels fill their LDS with NaN before use and whose entry points
+    """Within the block every call of this package goes to libpbgdn_debug.so and
+    libpbattn_debug.so, whose kernels fill their LDS with NaN before use and whose entry points
     fill their outputs and workspaces with NaN before launching (a test aid:
     an unwritten output element or a read of unwritten LDS then shows as NaN).
     Not thread-safe: the other library is restored on exit."""
-    global _lib, _debug
-    prev = lib()
+    global _lib, _debug, _attn, _attn_debug
+    prev, prev_attn = lib(), attn_lib()
     if _debug is None:
         _debug = _load(DEBUG_LIB_PATH)
-    _lib = _debug
+    if _attn_debug is None:
+        _attn_debug = _load_attn(ATTN_DEBUG_LIB_PATH)
+    _lib, _attn = _debug, _attn_debug
     try:
         yield _debug
     finally:
-        _lib = prev
+        _lib, _attn = prev, prev_attn
 
 
 def status_string(status: int) -> str:

@@ -1,9 +1,10 @@
-"""Build the HIP library of the operator for gfx950: pseudobrain_amd/libpbgdn.so.
+"""Build the HIP libraries for gfx950: pseudobrain_amd/libpbgdn.so, the operator
+(the C ABI of include/pbgdn.h), and pseudobrain_amd/libpbattn.so, the attention
+operators (include/pbattn.h).
 
-One shared library holds both kernels and the C ABI declared in include/pbgdn.h.
-It is compiled in-tree with hipcc (objects in parallel, then one link) and loaded
-with ctypes by pseudobrain_amd._lib; it links the HIP runtime by soname, so in a
-process that imported torch it binds to the runtime torch already loaded.
+They are compiled in-tree with hipcc (objects in parallel, then the links) and
+loaded with ctypes by pseudobrain_amd._lib; they link the HIP runtime by soname, so
+in a process that imported torch they bind to the runtime torch already loaded.
 
     python -m pseudobrain_amd.build
 """
@@ -27,6 +28,9 @@ DEBUG_LIB = os.path.join(PKG, "libpbgdn_debug.so")
 SOURCES = ("abi.hip", "recurrent.hip", "chunk.hip", "chunk_prep.hip", "chunk_scan.hip", "chunk_wide.hip",
            "chunk_k256.hip", "chunk_bwd.hip", "chunk_residuals.hip",
            "layer.hip", "decode_layer.hip", "device.hip")
+ATTN_LIB = os.path.join(PKG, "libpbattn.so")
+ATTN_DEBUG_LIB = os.path.join(PKG, "libpbattn_debug.so")
+ATTN_SOURCES = ("attn_fwd.hip", "attn_bwd.hip", "attn_decode.hip", "device.hip")
 ARCH = "gfx950"
 
 # Packed fp32 VALU instructions are disabled (-packed-fp32-ops): the kernels
@@ -53,20 +57,21 @@ def _run(cmd):
 
 
 def build(verbose: bool = False) -> str:
-    """Compile every source and link libpbgdn.so and libpbgdn_debug.so; returns
-    the path of the first."""
+    """Compile every source and link libpbgdn.so, libpbattn.so and their debug
+    builds; returns the path of the first."""
     cc = hipcc()
     libs = []  # (library, objects)
     jobs = []
-    for lib, objdir, extra in ((LIB, "_build", []), (DEBUG_LIB, "_build_debug", ["-DPBGDN_DEBUG"])):
+    for both, objdir, extra in (((LIB, ATTN_LIB), "_build", []),
+                                ((DEBUG_LIB, ATTN_DEBUG_LIB), "_build_debug", ["-DPBGDN_DEBUG"])):
         objdir = os.path.join(PKG, objdir)
         os.makedirs(objdir, exist_ok=True)
-        objs = []
-        for src in SOURCES:
-            obj = os.path.join(objdir, src.replace(".hip", ".o"))
-            objs.append(obj)
-            jobs.append([cc, *HIPCC_FLAGS, *extra, f"-I{INCLUDE}", "-c", os.path.join(CSRC, src), "-o", obj])
-        libs.append((lib, objs))
+        for lib, sources in zip(both, (SOURCES, ATTN_SOURCES)):
+            libs.append((lib, [os.path.join(objdir, src.replace(".hip", ".o")) for src in sources]))
+        # the longest compilations first
+        for src in dict.fromkeys(ATTN_SOURCES + SOURCES):
+            jobs.append([cc, *HIPCC_FLAGS, *extra, f"-I{INCLUDE}", "-c", os.path.join(CSRC, src), "-o",
+                         os.path.join(objdir, src.replace(".hip", ".o"))])
     with ThreadPoolExecutor(max_workers=min(len(jobs), os.cpu_count() or 8)) as pool:
         for proc in pool.map(_run, jobs):
             if verbose and proc.stderr:

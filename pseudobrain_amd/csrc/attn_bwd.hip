@@ -1,0 +1,756 @@
+// Windowed attention, backward (pbattn_window_bwd).
+//
+// Four kernels, none with an atomic sum:
+//   stat_kernel   per (token, head): lse in powers of two and
+//                 delta = do . o - dlse, stored by (batch, key head) in the
+//                 row order of the tiles below; float16 also takes the maxima
+//                 that bound ds
+//   dkdv_kernel   a wave owns 32 keys, with K and V rows and the sums of dK^T
+//                 and dV^T in registers, and walks the queries that see them
+//                 (all heads of the group): S = Q K^T, P, dV^T += dO^T P,
+//                 dP = dO V^T, dS, dK^T += Q^T dS. Long or few walks are split
+//                 into parts; the sinks, which every later query sees, are
+//                 always walked in parts beyond their window
+//   dq_kernel     the forward's walk over keys: S^T, dP^T, dS^T, dQ^T += K^T dS^T
+//   join_kernel   sums of parts, in a fixed order
+// Recomputing S and dP on both sides costs two products of seven, and saves
+// float32 sums of dQ in memory and their atomics.
+#include <atomic>
+
+#include "attn.hpp"
+#include "attn_tile.hpp"
+#include "device.hpp"
+
+namespace pbgdn {
+
+constexpr int QR = 32;            // rows of a query tile of dkdv_kernel
+constexpr int TAIL_TOKENS = 512;  // query tokens of one part of the sinks' walk
+constexpr int MAX_PARTS = 16;     // parts of an ordinary key tile's walk
+
+struct BwdParams {
+  WindowParams f;
+  const void *grad_o, *o;
+  const float *lse, *grad_lse;
+  void *dq, *dk, *dv;
+  float2 *stat;       // [B][Hk][Tq G]: (lse log2(e), delta); +inf for a row that sees nothing
+  uint32_t *range;    // float16: bits of max |do|, |v|, |delta|
+  float *part;        // [2][parts][B][Hk][Tk][D] when parts > 1
+  float *tail;        // [2][tail slots][Hk][sink tiles 32][D]
+  float scale, c;     // signed
+  int B, D;
+  int parts;          // parts of a key tile's walk
+  int key_slots;      // key tiles of a (batch, key head)
+  int sink_tiles;     // 32-key tiles that hold sinks, 0 when no query is beyond their window
+  int tail_slots;     // parts of the sinks' walk over all sequences, and slot 0 of each: the window's own part
+  // query tiles: `heads` heads of `tokens` tokens each, `splits` tiles for the heads of a token
+  int heads, tokens, splits;
+};
+
+// Sequence n's slots in the parts of the sinks: the window's part, then one per TAIL_TOKENS tokens.
+__device__ __forceinline__ int tail_start(const BwdParams &p, int seq) {
+  if (!p.f.cu_q) return seq * ((p.f.Tq + TAIL_TOKENS - 1) / TAIL_TOKENS + 1);
+  return boundary(p.f.cu_q, seq, p.f.Tq) / TAIL_TOKENS + 2 * seq;
+}
+inline long tail_slot_count(int Tq, int nseq, bool packed) {
+  return packed ? Tq / TAIL_TOKENS + 2L * nseq : nseq * ((Tq + TAIL_TOKENS - 1L) / TAIL_TOKENS + 1);
+}
+
+// ---------------------------------------------------------------------------
+// float16's range: ds is bounded by max |do| max |v| D + max |delta|; a power
+// of two brings that bound to 2^14.
+// ---------------------------------------------------------------------------
+template <int DT, int D>
+__device__ __forceinline__ float range_scale(const uint32_t *range) {
+  if constexpr (DT != PBGDN_F16) return 1.0f;
+  const float bound = __uint_as_float(range[0]) * __uint_as_float(range[1]) * D + __uint_as_float(range[2]);
+  if (!(bound > 0.0f && bound < 1e30f)) return 1.0f;
+  int e;
+  frexpf(bound, &e);
+  e = 14 - e;
+  e = e > 100 ? 100 : e < -100 ? -100 : e;
+  return ldexpf(1.0f, e);
+}
+
+__global__ void range_zero_kernel(uint32_t *range) {
+  if (threadIdx.x < 4) range[threadIdx.x] = 0;
+}
+
+// max |v| over rows of D elements (float16).
+template <int D>
+__global__ __launch_bounds__(256) void range_v_kernel(View v, int B, int Tk, int Hk, uint32_t *range) {
+  constexpr int LPR = D / 8;  // lanes of a row
+  const long rows = static_cast<long>(B) * Tk * Hk;
+  float top = 0.0f;
+  for (long r = blockIdx.x * (256L / LPR) + threadIdx.x / LPR; r < rows; r += gridDim.x * (256L / LPR)) {
+    const long b = r / (static_cast<long>(Tk) * Hk), t = r / Hk % Tk, h = r % Hk;
+    const half8_t x = *reinterpret_cast<const half8_t *>(v.base + b * v.batch + t * v.token + h * v.head +
+                                                         (threadIdx.x % LPR) * 16);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(static_cast<float>(x[i])));
+  }
+  top = wave_max(top);
+  if ((threadIdx.x & 63) == 0) atomicMax(range + 1, __float_as_uint(top));
+}
+
+template <int DT, int D>
+__global__ __launch_bounds__(256) void stat_kernel(const BwdParams p) {
+  using E = Elem<DT>;
+  constexpr int PER = 16 / E::BYTES, LPR = D / PER < 64 ? D / PER : 64, RPB = 256 / LPR;  // lanes a row, rows a block
+  constexpr int UNITS = D / PER / LPR;
+  const long rows = static_cast<long>(p.B) * p.f.Tq * p.f.Hq;
+  float top_do = 0.0f, top_delta = 0.0f;
+  for (long r = blockIdx.x * static_cast<long>(RPB) + threadIdx.x / LPR; r < rows; r += gridDim.x * static_cast<long>(RPB)) {
+    float sum = 0.0f;
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) {
+      const long at = r * D * E::BYTES + (u * LPR + threadIdx.x % LPR) * 16;
+      const v4u32_t x = *reinterpret_cast<const v4u32_t *>(static_cast<const unsigned char *>(p.o) + at);
+      const v4u32_t y = *reinterpret_cast<const v4u32_t *>(static_cast<const unsigned char *>(p.grad_o) + at);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (E::BYTES == 2) {
+          sum += E::low(x[i]) * E::low(y[i]) + E::high(x[i]) * E::high(y[i]);
+          if constexpr (DT == PBGDN_F16) top_do = fmaxf(top_do, fmaxf(fabsf(E::low(y[i])), fabsf(E::high(y[i]))));
+        } else {
+          sum += __uint_as_float(x[i]) * __uint_as_float(y[i]);
+        }
+      }
+    }
+#pragma unroll
+    for (int w = LPR / 2; w > 0; w >>= 1) sum += __shfl_xor(sum, w, 64);
+    if (threadIdx.x % LPR == 0) {
+      const float lse = p.lse[r];
+      const bool empty = lse == -INFINITY;
+      const float delta = empty ? 0.0f : p.grad_lse ? sum - p.grad_lse[r] : sum;
+      const int h = static_cast<int>(r % p.f.Hq), G = p.f.group;
+      const long bt = r / p.f.Hq, b = bt / p.f.Tq, t = bt % p.f.Tq;
+      p.stat[((b * p.f.Hk + h / G) * p.f.Tq + t) * G + h % G] = make_float2(empty ? INFINITY : lse * LOG2E, delta);
+      top_delta = fmaxf(top_delta, fabsf(delta));
+    }
+  }
+  if constexpr (DT == PBGDN_F16) {
+    top_do = wave_max(top_do);
+    top_delta = wave_max(top_delta);
+    if ((threadIdx.x & 63) == 0) {
+      atomicMax(p.range, __float_as_uint(top_do));
+      atomicMax(p.range + 2, __float_as_uint(top_delta));
+    }
+  }
+}
+
+// A row of transposed accumulators: column d of z[d / 32], times f, as DT.
+template <int DT, int D>
+__device__ __forceinline__ void store_row(void *dst, const float16_t *z, int h, float f) {
+  using E = Elem<DT>;
+#pragma unroll
+  for (int m = 0; m < D / 32; ++m)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float4_t x = {z[m][4 * e] * f, z[m][4 * e + 1] * f, z[m][4 * e + 2] * f, z[m][4 * e + 3] * f};
+      const int d = 32 * m + 8 * e + 4 * h;
+      if constexpr (E::BYTES == 2) {
+        *reinterpret_cast<v2u32_t *>(static_cast<unsigned char *>(dst) + 2 * d) =
+            v2u32_t{E::pack(x[0], x[1]), E::pack(x[2], x[3])};
+      } else {
+        *reinterpret_cast<float4_t *>(static_cast<unsigned char *>(dst) + 4 * d) = x;
+      }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// dK and dV. TAIL: the sinks' keys against the queries beyond their window.
+// ---------------------------------------------------------------------------
+template <int DT, int D, int NW>
+struct Dkdv {
+  using L = Tile<DT, D>;
+  static constexpr int BN = 32 * NW, TILE = QR * L::ROW, STAT = QR * 8, BUF = 2 * TILE + STAT, LDS = 2 * BUF;
+  static constexpr int LOADS = QR / L::PER_DMA;  // of one tensor, all waves
+  // float32 rows of 256: K and V rows are read from LDS instead of registers
+  static constexpr bool HELD = L::STEPS <= 32;
+  static constexpr int KV = HELD ? 0 : 2 * BN * L::ROW, BUFS = HELD ? 2 : 1;
+  static constexpr int BYTES = KV + BUFS * BUF;
+};
+
+template <int DT, int D, int NW, bool TAIL, int WAVES>
+__global__ __launch_bounds__(NW * 64, WAVES) void dkdv_kernel(const BwdParams p) {
+  using K = Dkdv<DT, D, NW>;
+  using L = typename K::L;
+  using E = typename L::E;
+  constexpr int S = L::STEPS, MB = L::MB;
+  extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
+  PBGDN_POISON_LDS(lds, K::BYTES);
+  PBGDN_POISON_SYNC();
+
+  const WindowParams &f = p.f;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const int n = lane & 31, h = lane >> 5, G = f.group;
+
+  // which keys, which part of their queries
+  int b, hk, seq, tile, part, slot = 0;
+  if constexpr (TAIL) {
+    int id = blockIdx.x;
+    tile = id % p.sink_tiles;
+    id /= p.sink_tiles;
+    hk = id % f.Hk;
+    slot = id / f.Hk;
+    // bisection over the sequences' first slots
+    int lo = 0, hi = f.nseq - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (tail_start(p, mid) <= slot)
+        lo = mid;
+      else
+        hi = mid - 1;
+    }
+    seq = lo;
+    b = f.cu_q ? 0 : seq;
+    part = slot - tail_start(p, seq) - 1;
+  } else {
+    const int groups = gridDim.x / (p.key_slots * p.parts);
+    int grp, s;
+    place(blockIdx.x, groups, p.key_slots * p.parts, grp, s);
+    s = p.key_slots * p.parts - 1 - s;  // the first keys, which most queries see, first
+    b = grp / f.Hk;
+    hk = grp % f.Hk;
+    part = s % p.parts;
+    tile = s / p.parts;
+    seq = b;
+    const int32_t *cu = f.cu_k ? f.cu_k : f.cu_q;
+    if (f.cu_q) {
+      seq = slot_sequence(cu, f.nseq, f.Tk, 1, K::BN, tile);
+      tile -= slot_start(cu, seq, f.Tk, 1, K::BN);
+    }
+  }
+  const Seq sq = sequence<true>(f.cu_q, f.cu_k, seq, f.nseq, f.Tq, f.Tk);
+  const int j0 = tile * K::BN;
+  if (part < 0 || tile < 0 || j0 >= sq.nk) return;
+  const int off = sq.nk - sq.nq;  // position of query token 0
+
+  // the query tokens [t0, t1) of this part
+  int t0, t1;
+  if constexpr (TAIL) {
+    t0 = j0 + f.window - off;  // the first beyond the window of the tile's first key
+    t0 = t0 > 0 ? t0 : 0;
+    t0 = t0 > part * TAIL_TOKENS ? t0 : part * TAIL_TOKENS;
+    t1 = (part + 1) * TAIL_TOKENS < sq.nq ? (part + 1) * TAIL_TOKENS : sq.nq;
+    if (part * TAIL_TOKENS >= sq.nq) return;
+  } else {
+    const int jl = (j0 + K::BN < sq.nk ? j0 + K::BN : sq.nk) - 1;
+    t0 = j0 - off > 0 ? j0 - off : 0;
+    t1 = jl < sq.nk - f.window ? jl + f.window - off : sq.nq;
+    t1 = t1 < 0 ? 0 : t1;
+    if (p.parts > 1) {
+      int step = (t1 - t0 + p.parts - 1) / p.parts;
+      step = (step + p.tokens - 1) / p.tokens * p.tokens;
+      t0 = t0 + part * step;
+      t1 = t1 < t0 + step ? t1 : t0 + step;
+    }
+  }
+  const int tiles = t1 > t0 ? (t1 - t0 + p.tokens - 1) / p.tokens * p.splits : 0;
+
+  // this wave's keys
+  const int key = j0 + wave * 32 + n;
+  const int kc = key < sq.nk ? key : sq.nk - 1;
+  const unsigned char *krow = f.k.base + b * f.k.batch + hk * f.k.head + (sq.k0 + kc) * f.k.token;
+  const unsigned char *vrow = f.v.base + b * f.v.batch + hk * f.v.head + (sq.k0 + kc) * f.v.token;
+  v4u32_t kf[K::HELD ? S : 1], vf[K::HELD ? S : 1];
+  unsigned char *const kl = lds + wave * 32 * L::ROW, *const vl = kl + K::BN * L::ROW;
+  const uint32_t rbase = L::rows_base(n, h), cbase = L::cols_base(lane);
+#pragma unroll
+  for (int s = 0; s < S; ++s) {
+    const v4u32_t x = *reinterpret_cast<const v4u32_t *>(krow + (2 * s + h) * 16);
+    const v4u32_t y = *reinterpret_cast<const v4u32_t *>(vrow + (2 * s + h) * 16);
+    if constexpr (K::HELD) {
+      kf[s] = x;
+      vf[s] = y;
+    } else {
+      const uint32_t at = (rbase ^ ((2 * s) % 16 * 16)) + (2 * s) / 16 * 256;
+      *reinterpret_cast<v4u32_t *>(kl + at) = x;
+      *reinterpret_cast<v4u32_t *>(vl + at) = y;
+    }
+  }
+  const auto k_unit = [&](int s) { return K::HELD ? kf[K::HELD ? s : 0] : L::rows(kl, rbase, 0, s); };
+  const auto v_unit = [&](int s) { return K::HELD ? vf[K::HELD ? s : 0] : L::rows(vl, rbase, 0, s); };
+
+  float16_t dk[MB], dv[MB];
+#pragma unroll
+  for (int m = 0; m < MB; ++m) dk[m] = dv[m] = zero16();
+  const float range = range_scale<DT, D>(p.range);
+
+  // staging of query tile i: `tokens` tokens from its first, `heads` heads
+  const unsigned char *qb = f.q.base + b * f.q.batch + sq.q0 * f.q.token + hk * G * f.q.head;
+  const unsigned char *gb = static_cast<const unsigned char *>(p.grad_o) +
+                            ((static_cast<long>(b) * f.Tq + sq.q0) * f.Hq + hk * G) * static_cast<long>(L::ROW);
+  const long g_token = static_cast<long>(f.Hq) * L::ROW;
+  const float2 *sb = p.stat + ((static_cast<long>(b) * f.Hk + hk) * f.Tq + sq.q0) * G;
+  unsigned char *const bufs = lds + K::KV;
+  const auto stage = [&](int i) {
+    const int group = p.splits == 1 ? i : i / p.splits, split = p.splits == 1 ? 0 : i % p.splits;
+    const int t = t0 + group * p.tokens, g0 = split * QR;
+    const int tn = t1 - t < p.tokens ? t1 - t : p.tokens, hn = G - g0 < p.heads ? G - g0 : p.heads;
+    const uint32_t to = uniform(lds_address(bufs + (K::BUFS == 2 ? (i & 1) * K::BUF : 0)));
+    const v4u32_t dq_ = dma_desc(qb + t * f.q.token + g0 * f.q.head,
+                                 (tn - 1) * f.q.token + (hn - 1) * f.q.head + L::ROW);
+    const v4u32_t dg_ = dma_desc(gb + t * g_token + g0 * L::ROW, (tn - 1) * g_token + (hn - 1) * L::ROW + L::ROW);
+#pragma unroll
+    for (int w = 0; w < (K::LOADS + NW - 1) / NW; ++w) {
+      const int inst = wave + NW * w;
+      const int row = inst * L::PER_DMA + lane / L::UNITS;
+      const int tt = row / p.heads, gg = row - tt * p.heads;
+      const uint32_t unit = ((lane % L::UNITS) ^ L::swz(row)) * 16;
+      const bool in = tt < tn && gg < hn;
+      dma(dq_, in ? tt * static_cast<uint32_t>(f.q.token) + gg * static_cast<uint32_t>(f.q.head) + unit : OUT_OF_RANGE,
+          to + inst * 1024);
+      dma(dg_, in ? tt * static_cast<uint32_t>(g_token) + gg * L::ROW + unit : OUT_OF_RANGE, to + K::TILE + inst * 1024);
+    }
+    if (wave == 0) {
+      const int rows = p.splits == 1 ? tn * G : hn;
+      dma4(dma_desc(sb + static_cast<long>(t) * G + g0, rows * 8L), lane * 4, to + 2 * K::TILE);
+    }
+  };
+
+  const int w_lo = j0 + wave * 32, w_hi = w_lo + 31;
+  if (tiles > 0 && K::BUFS == 2) stage(0);
+  for (int i = 0; i < tiles; ++i) {
+    if constexpr (K::BUFS == 2) {
+      wait_dma();
+      block_sync();
+      if (i + 1 < tiles) stage(i + 1);
+    } else {
+      block_sync();
+      stage(i);
+      wait_dma();
+      block_sync();
+    }
+    const unsigned char *qt = bufs + (K::BUFS == 2 ? (i & 1) * K::BUF : 0), *gt = qt + K::TILE;
+    const float4_t *st = reinterpret_cast<const float4_t *>(qt + 2 * K::TILE);
+    const int tok = t0 + (p.splits == 1 ? i : i / p.splits) * p.tokens;
+    const int p_lo = tok + off, p_hi = (tok + p.tokens < t1 ? tok + p.tokens : t1) - 1 + off;
+    bool whole, none;
+    if constexpr (TAIL) {
+      whole = w_hi < f.sinks && w_hi <= p_lo - f.window;
+      none = w_lo >= f.sinks || w_lo > p_hi - f.window;
+    } else {
+      whole = w_hi <= p_lo && w_lo > p_hi - f.window;
+      none = w_lo > p_hi || w_hi <= p_lo - f.window;
+    }
+    if (none) continue;
+
+    float16_t x = zero16(), y = zero16();
+#pragma unroll
+    for (int s = 0; s < S; ++s) x = E::mma(L::rows(qt, rbase, 0, s), k_unit(s), x);
+#pragma unroll
+    for (int s = 0; s < S; ++s) y = E::mma(L::rows(gt, rbase, 0, s), v_unit(s), y);
+    if (!whole) {
+      const uint32_t inv = 65536 / p.heads + 1;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int pos = p_lo + static_cast<int>((acc_row(e, h) * inv) >> 16);
+        const bool seen = TAIL ? (key < f.sinks) & (key <= pos - f.window) : (key <= pos) & (key > pos - f.window);
+        x[e] = seen ? x[e] : -INFINITY;
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 16; e += 4) {
+      // rows 2 e + 4 h .. + 3: (lse, delta) pairs
+      const float4_t a = st[e + 2 * h], c = st[e + 2 * h + 1];
+      const float lse[4] = {a[0], a[2], c[0], c[2]}, delta[4] = {a[1], a[3], c[1], c[3]};
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float w = __builtin_amdgcn_exp2f(x[e + r] == -INFINITY ? x[e + r] : __builtin_fmaf(x[e + r], p.c, -lse[r]));
+        x[e + r] = w;
+        float d = y[e + r] - delta[r];
+        if constexpr (DT == PBGDN_F16) d *= range;
+        y[e + r] = w == 0.0f ? 0.0f : w * d;
+      }
+    }
+    L::cols_product(gt, cbase, 0, L::operand(x), dv);
+    L::cols_product(qt, cbase, 0, L::operand(y), dk);
+  }
+
+  if (key >= sq.nk) return;
+  const float fk = p.scale / range;
+  const long row = (static_cast<long>(b) * f.Tk + sq.k0 + key) * f.Hk + hk;
+  if constexpr (TAIL) {
+    const long at = ((static_cast<long>(slot) * f.Hk + hk) * p.sink_tiles * 32 + key) * D;
+    const long half = static_cast<long>(p.tail_slots) * f.Hk * p.sink_tiles * 32 * D;
+    store_row<PBGDN_F32, D>(p.tail + at, dk, h, fk);
+    store_row<PBGDN_F32, D>(p.tail + half + at, dv, h, 1.0f);
+  } else if (p.parts > 1) {
+    const long half = static_cast<long>(p.B) * f.Tk * f.Hk * D;
+    store_row<PBGDN_F32, D>(p.part + part * half + row * D, dk, h, fk);
+    store_row<PBGDN_F32, D>(p.part + (p.parts + part) * half + row * D, dv, h, 1.0f);
+  } else if (key < p.sink_tiles * 32 && seq < f.nseq) {
+    const long at = ((static_cast<long>(tail_start(p, seq)) * f.Hk + hk) * p.sink_tiles * 32 + key) * D;
+    const long half = static_cast<long>(p.tail_slots) * f.Hk * p.sink_tiles * 32 * D;
+    store_row<PBGDN_F32, D>(p.tail + at, dk, h, fk);
+    store_row<PBGDN_F32, D>(p.tail + half + at, dv, h, 1.0f);
+  } else {
+    store_row<DT, D>(static_cast<unsigned char *>(p.dk) + row * L::ROW, dk, h, fk);
+    store_row<DT, D>(static_cast<unsigned char *>(p.dv) + row * L::ROW, dv, h, 1.0f);
+  }
+}
+
+// Sums the parts of dk and dv, in order: the window's parts of every key when
+// p.parts > 1, and the sinks' parts. Each thread four elements of a key's row.
+template <int DT, int D>
+__global__ __launch_bounds__(256) void join_kernel(const BwdParams p, long rows, bool sinks_only) {
+  using E = Elem<DT>;
+  const WindowParams &f = p.f;
+  constexpr int TPR = D / 4;
+  const long half = static_cast<long>(p.B) * f.Tk * f.Hk * D;
+  const int sinkpad = p.sink_tiles * 32;
+  const long tail_half = static_cast<long>(p.tail_slots) * f.Hk * sinkpad * D;
+  for (long i = blockIdx.x * 256L + threadIdx.x; i < rows * TPR; i += gridDim.x * 256L) {
+    const long r = i / TPR;
+    const int d = static_cast<int>(i % TPR) * 4;
+    int seq, hk, key;
+    long row;  // of dk and dv
+    if (sinks_only) {
+      key = static_cast<int>(r % sinkpad);
+      hk = static_cast<int>(r / sinkpad % f.Hk);
+      seq = static_cast<int>(r / sinkpad / f.Hk);
+    } else {
+      hk = static_cast<int>(r % f.Hk);
+      const long token = r / f.Hk;
+      seq = static_cast<int>(token / f.Tk);
+      key = static_cast<int>(token % f.Tk);
+      if (f.cu_q) {
+        const int32_t *cu = f.cu_k ? f.cu_k : f.cu_q;
+        int lo = 0, hi = f.nseq - 1;
+        while (lo < hi) {
+          const int mid = (lo + hi + 1) >> 1;
+          if (boundary(cu, mid, f.Tk) <= key)
+            lo = mid;
+          else
+            hi = mid - 1;
+        }
+        seq = lo;
+      }
+    }
+    const Seq sq = sequence<true>(f.cu_q, f.cu_k, seq, f.nseq, f.Tq, f.Tk);
+    if (sinks_only) {
+      if (key >= sq.nk) continue;
+      row = ((f.cu_q ? 0 : static_cast<long>(seq) * f.Tk) + sq.k0 + key) * f.Hk + hk;
+    } else {
+      row = r;
+      if (f.cu_q) key -= sq.k0;
+    }
+    const bool inside = key >= 0 && key < sq.nk;
+    const int tails = (sq.nq + TAIL_TOKENS - 1) / TAIL_TOKENS;
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      float4_t sum = {0.0f, 0.0f, 0.0f, 0.0f};
+      if (!sinks_only && inside)
+        for (int a = 0; a < p.parts; ++a)
+          sum += *reinterpret_cast<const float4_t *>(p.part + (which * p.parts + a) * half + row * D + d);
+      if (inside && key < sinkpad) {
+        const long slot = tail_start(p, seq);
+        for (int a = sinks_only ? 0 : 1; a <= tails; ++a)
+          sum += *reinterpret_cast<const float4_t *>(p.tail + which * tail_half +
+                                                     (((slot + a) * f.Hk + hk) * sinkpad + key) * D + d);
+      }
+      void *dst = which ? p.dv : p.dk;
+      if constexpr (E::BYTES == 2) {
+        reinterpret_cast<v2u32_t *>(dst)[(row * D + d) / 4] = v2u32_t{E::pack(sum[0], sum[1]), E::pack(sum[2], sum[3])};
+      } else {
+        reinterpret_cast<float4_t *>(dst)[(row * D + d) / 4] = sum;
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// dQ: the forward's rows and walk.
+// ---------------------------------------------------------------------------
+template <int DT, int D, int NW, int BN>
+struct Dq {
+  using L = Tile<DT, D>;
+  static constexpr int BM = 32 * NW, TILE = BN * L::ROW, LDS = 4 * TILE;
+};
+
+template <int DT, int D, int NW, int BN, int WAVES>
+__global__ __launch_bounds__(NW * 64, WAVES) void dq_kernel(const BwdParams p) {
+  using F = Dq<DT, D, NW, BN>;
+  using L = typename F::L;
+  using E = typename L::E;
+  constexpr int S = L::STEPS, MB = L::MB;
+  extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
+  PBGDN_POISON_LDS(lds, F::LDS);
+  PBGDN_POISON_SYNC();
+
+  const WindowParams &f = p.f;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const int n = lane & 31, h = lane >> 5, G = f.group;
+  const int groups = gridDim.x / f.slots;
+  int grp, slot;
+  place(blockIdx.x, groups, f.slots, grp, slot);
+  const int b = grp / f.Hk, hk = grp % f.Hk;
+  int seq = b;
+  if (f.cu_q) {
+    seq = slot_sequence(f.cu_q, f.nseq, f.Tq, G, F::BM, slot);
+    slot -= slot_start(f.cu_q, seq, f.Tq, G, F::BM);
+  }
+  const Seq sq = sequence<false>(f.cu_q, f.cu_k, seq, f.nseq, f.Tq, f.Tk);
+  const long total = static_cast<long>(sq.nq) * G, row0 = static_cast<long>(slot) * F::BM;
+  if (slot < 0 || row0 >= total) return;
+  const int off = sq.nk - sq.nq;
+  const auto position = [&](long row) { return static_cast<int>((row < total ? row : total - 1) / G) + off; };
+  const KeyRange range = key_range(position(row0), position(row0 + F::BM - 1), f.window, f.sinks);
+  const long wrow = row0 + wave * 32;
+  const int w_first = position(wrow), w_last = position(wrow + 31);
+
+  const unsigned char *kb_ = f.k.base + b * f.k.batch + hk * f.k.head + sq.k0 * f.k.token;
+  const unsigned char *vb_ = f.v.base + b * f.v.batch + hk * f.v.head + sq.k0 * f.v.token;
+  using Stage = KeyStage<DT, D, BN, NW>;
+  const int tiles = (range.count + BN - 1) / BN;
+  if (tiles > 0) {
+    Stage::tile(kb_, f.k.token, range, 0, lds, wave, lane);
+    Stage::tile(vb_, f.v.token, range, 0, lds + 2 * F::TILE, wave, lane);
+  }
+
+  const long row = wrow + n, r = row < total ? row : total - 1;
+  const int t = static_cast<int>(r / G), head = hk * G + static_cast<int>(r % G), pos = t + off;
+  const long out = (static_cast<long>(b) * f.Tq + sq.q0 + t) * f.Hq + head;
+  const unsigned char *qrow = f.q.base + b * f.q.batch + (sq.q0 + t) * f.q.token + head * f.q.head;
+  const unsigned char *grow = static_cast<const unsigned char *>(p.grad_o) + out * L::ROW;
+  v4u32_t qf[S], gf[S];
+#pragma unroll
+  for (int s = 0; s < S; ++s) {
+    qf[s] = *reinterpret_cast<const v4u32_t *>(qrow + (2 * s + h) * 16);
+    gf[s] = *reinterpret_cast<const v4u32_t *>(grow + (2 * s + h) * 16);
+  }
+  const float2 st = p.stat[((static_cast<long>(b) * f.Hk + hk) * f.Tq + sq.q0) * G + r];
+  const float scale16 = range_scale<DT, D>(p.range);
+  float16_t dq[MB];
+#pragma unroll
+  for (int m = 0; m < MB; ++m) dq[m] = zero16();
+
+  const uint32_t rbase = L::rows_base(n, h), cbase = L::cols_base(lane);
+  for (int it = 0; it < tiles; ++it) {
+    wait_dma();
+    block_sync();
+    const unsigned char *kt = lds + (it & 1) * F::TILE, *vt = kt + 2 * F::TILE;
+    if (it + 1 < tiles) {
+      unsigned char *next = lds + ((it + 1) & 1) * F::TILE;
+      Stage::tile(kb_, f.k.token, range, (it + 1) * BN, next, wave, lane);
+      Stage::tile(vb_, f.v.token, range, (it + 1) * BN, next + 2 * F::TILE, wave, lane);
+    }
+    const int u0 = it * BN;
+    const int first = u0 < range.sinks ? u0 : u0 + range.delta, last = u0 + BN - 1 + range.delta;
+    const bool whole = u0 >= range.sinks && last <= w_first && first > w_last - f.window;
+    if (first > w_last) continue;
+#pragma unroll
+    for (int kb = 0; kb < BN / 32; ++kb) {
+      float16_t x = L::rows_product(kt, rbase, 32 * kb, qf), y = L::rows_product(vt, rbase, 32 * kb, gf);
+      if (!whole) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int u = u0 + 32 * kb + acc_row(i, h);
+          x[i] = sees(pos, u < range.sinks ? u : u + range.delta, f.window, f.sinks) ? x[i] : -INFINITY;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float w = __builtin_amdgcn_exp2f(x[i] == -INFINITY ? x[i] : __builtin_fmaf(x[i], p.c, -st.x));
+        float d = y[i] - st.y;
+        if constexpr (DT == PBGDN_F16) d *= scale16;
+        x[i] = w == 0.0f ? 0.0f : w * d;
+      }
+      L::cols_product(kt, cbase, 32 * kb, L::operand(x), dq);
+    }
+  }
+  if (row < total) store_row<DT, D>(static_cast<unsigned char *>(p.dq) + out * L::ROW, dq, h, p.scale / scale16);
+}
+
+// ---------------------------------------------------------------------------
+// Launches.
+// ---------------------------------------------------------------------------
+// Waves (of 32 keys) of a workgroup of dkdv_kernel.
+template <int DT, int D>
+constexpr int dkdv_waves() { return DT == PBGDN_F32 && D == 256 ? 1 : DT == PBGDN_F32 || D == 256 ? 2 : 4; }
+
+static bool sinks_beyond(const WindowParams &f) { return f.sinks > 0 && f.window < f.Tk; }
+static int sink_tiles(const WindowParams &f) {
+  if (!sinks_beyond(f)) return 0;
+  const int s = f.sinks < f.Tk ? f.sinks : f.Tk;
+  return (s + 31) / 32;
+}
+
+// Parts of a key tile's walk: enough workgroups for every CU several times
+// over, none shorter than about 16 query tiles.
+static int walk_parts(const WindowParams &f, int B, int bn, int cus) {
+  const long tiles = (static_cast<long>(f.Tk) * (f.cu_q ? 1 : B) + bn - 1) / bn * f.Hk;
+  const long walk = (f.window < f.Tq ? static_cast<long>(f.window) + bn : f.Tq) * f.group / QR;
+  long parts = tiles > 0 ? (4L * cus + tiles - 1) / tiles : 1;
+  if (parts > walk / 16) parts = walk / 16;
+  return parts < 2 ? 1 : parts > MAX_PARTS ? MAX_PARTS : static_cast<int>(parts);
+}
+
+template <int DT, int D>
+static int launch_bwd(BwdParams &p, hipStream_t stream) {
+  WindowParams &f = p.f;
+  const int nb = f.cu_q ? 1 : p.B;
+  DeviceShape shape;
+  if (!device_shape(shape)) return PBGDN_ERR_LAUNCH;
+  if constexpr (DT == PBGDN_F16) {
+    hipLaunchKernelGGL(range_zero_kernel, dim3(1), dim3(64), 0, stream, p.range);
+    if (f.Tk > 0)
+      hipLaunchKernelGGL(range_v_kernel<D>, dim3(shape.cus * 4), dim3(256), 0, stream, f.v, p.B, f.Tk, f.Hk, p.range);
+  }
+  hipLaunchKernelGGL((stat_kernel<DT, D>), dim3(shape.cus * 8), dim3(256), 0, stream, p);
+
+  constexpr int NW = dkdv_waves<DT, D>(), BN = 32 * NW;
+  if (f.Tk > 0) {
+    {
+      using K = Dkdv<DT, D, NW>;
+      constexpr int W = 1;
+      static std::atomic<bool> flags[MAX_DEVICES];
+      const auto kernel = dkdv_kernel<DT, D, NW, false, W>;
+      if (!smem_configured(reinterpret_cast<const void *>(kernel), K::BYTES, flags)) return PBGDN_ERR_LAUNCH;
+      const long slots = f.cu_q ? f.Tk / BN + f.nseq + 1 : (f.Tk + BN - 1) / BN;
+      const long blocks = slots * p.parts * nb * f.Hk;
+      if (blocks > 0x7fffffffL) return PBGDN_ERR_UNSUPPORTED;
+      p.key_slots = static_cast<int>(slots);
+      hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(NW * 64), K::BYTES, stream, p);
+    }
+    if (p.sink_tiles) {
+      using K = Dkdv<DT, D, 1>;
+      static std::atomic<bool> flags[MAX_DEVICES];
+      const auto kernel = dkdv_kernel<DT, D, 1, true, 1>;
+      if (!smem_configured(reinterpret_cast<const void *>(kernel), K::BYTES, flags)) return PBGDN_ERR_LAUNCH;
+      const long blocks = static_cast<long>(p.tail_slots) * f.Hk * p.sink_tiles;
+      if (blocks > 0x7fffffffL) return PBGDN_ERR_UNSUPPORTED;
+      hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(64), K::BYTES, stream, p);
+    }
+    if (p.parts > 1 || p.sink_tiles) {
+      const bool sinks_only = p.parts == 1;
+      const long rows = sinks_only ? static_cast<long>(f.nseq) * f.Hk * p.sink_tiles * 32
+                                   : static_cast<long>(p.B) * f.Tk * f.Hk;
+      const long want = (rows * (D / 4) + 255) / 256;
+      hipLaunchKernelGGL((join_kernel<DT, D>), dim3(static_cast<unsigned>(want < 65536 ? want : 65536)), dim3(256), 0,
+                         stream, p, rows, sinks_only);
+    }
+  }
+  {
+    constexpr int DQ_NW = 4, DQ_BN = DT == PBGDN_F32 ? (D == 64 ? 64 : 32) : D == 256 ? 32 : 64;
+    constexpr int W = DT != PBGDN_F32 && D <= 128 ? 2 : 1;
+    using F = Dq<DT, D, DQ_NW, DQ_BN>;
+    static std::atomic<bool> flags[MAX_DEVICES];
+    const auto kernel = dq_kernel<DT, D, DQ_NW, DQ_BN, W>;
+    if (!smem_configured(reinterpret_cast<const void *>(kernel), F::LDS, flags)) return PBGDN_ERR_LAUNCH;
+    const long slots = window_slots(f, F::BM), blocks = slots * nb * f.Hk;
+    if (blocks > 0x7fffffffL) return PBGDN_ERR_UNSUPPORTED;
+    f.slots = static_cast<int>(slots);
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(DQ_NW * 64), F::LDS, stream, p);
+  }
+  return hipGetLastError() == hipSuccess ? PBGDN_OK : PBGDN_ERR_LAUNCH;
+}
+
+// The workspace: statistics, the float16 range, the parts.
+struct Plan {
+  size_t stat, range, part, tail, bytes;
+  int parts, sink_tiles, tail_slots;
+};
+static int key_tile(int dtype, int D) {
+  return 32 * (dtype == PBGDN_F32 ? (D == 256 ? 1 : 2) : D == 256 ? 2 : 4);
+}
+static bool plan(Plan &w, const WindowParams &f, int dtype, int B, int D) {
+  DeviceShape shape;
+  if (!device_shape(shape)) shape.cus = 256;  // sizes are asked for without a device too
+  w.parts = walk_parts(f, B, key_tile(dtype, D), shape.cus);
+  w.sink_tiles = sink_tiles(f);
+  const long slots = w.sink_tiles ? tail_slot_count(f.Tq, f.nseq, f.cu_q != nullptr) : 0;
+  if (slots > 0x7fffffffL) return false;
+  w.tail_slots = static_cast<int>(slots);
+  const auto round = [](size_t x) { return (x + 255) & ~static_cast<size_t>(255); };
+  w.stat = 0;
+  w.range = round(static_cast<size_t>(B) * f.Tq * f.Hq * sizeof(float2));
+  w.part = w.range + 256;
+  w.tail = w.part + round(w.parts > 1 ? 2 * sizeof(float) * w.parts * B * f.Tk * f.Hk * static_cast<size_t>(D) : 0);
+  w.bytes = w.tail + round(2 * sizeof(float) * slots * f.Hk * w.sink_tiles * 32 * static_cast<size_t>(D));
+  return true;
+}
+
+}  // namespace pbgdn
+
+extern "C" size_t pbattn_window_bwd_workspace_size(int B, int Tq, int Tk, int Hq, int Hk, int D, int num_seqs,
+                                                   int dtype, int packed, int window, int sinks) {
+  using namespace pbgdn;
+  if (B < 0 || Tq < 0 || Tk < 0 || Hq <= 0 || Hk <= 0 || Hq % Hk != 0 || num_seqs < 0 || sinks < 0 ||
+      !attn_dtype(dtype) || (D != 64 && D != 128 && D != 256)) {
+    return 0;
+  }
+  WindowParams f{};
+  const int32_t some = 0;
+  f.cu_q = packed ? &some : nullptr;
+  f.nseq = num_seqs;
+  f.Tq = Tq;
+  f.Tk = Tk;
+  f.Hq = Hq;
+  f.Hk = Hk;
+  f.group = Hq / Hk;
+  f.window = window <= 0 || window > NO_WINDOW ? NO_WINDOW : window;
+  f.sinks = sinks < NO_WINDOW ? sinks : NO_WINDOW;
+  Plan w;
+  return plan(w, f, dtype, B, D) ? w.bytes : 0;
+}
+
+extern "C" int pbattn_window_bwd(const void *q, const void *k, const void *v, int dtype, const int64_t *strides,
+                                 const int32_t *cu_q, const int32_t *cu_k, int num_seqs, const void *o,
+                                 const float *lse, const void *grad_o, const float *grad_lse, void *dq, void *dk,
+                                 void *dv, int B, int Tq, int Tk, int Hq, int Hk, int D, float scale, int window,
+                                 int sinks, void *workspace, size_t workspace_bytes, void *stream) {
+  using namespace pbgdn;
+  BwdParams p{};
+  const int status = window_params(p.f, q, k, v, dtype, strides, cu_q, cu_k, num_seqs, B, Tq, Tk, Hq, Hk, D, scale,
+                                   window, sinks);
+  if (status != PBGDN_OK || p.f.nseq == 0) return status;
+  if (!o || !lse || !grad_o || !dq || (Tk > 0 && (!dk || !dv)) || !workspace) return PBGDN_ERR_INVALID_ARGUMENT;
+  if (!aligned16(o) || !aligned16(grad_o) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv) ||
+      !aligned16(workspace)) {
+    return PBGDN_ERR_INVALID_ARGUMENT;
+  }
+  Plan w;
+  if (!plan(w, p.f, dtype, B, D)) return PBGDN_ERR_UNSUPPORTED;
+  if (workspace_bytes < w.bytes) return PBGDN_ERR_INVALID_ARGUMENT;
+  unsigned char *ws = static_cast<unsigned char *>(workspace);
+  p.o = o;
+  p.lse = lse;
+  p.grad_o = grad_o;
+  p.grad_lse = grad_lse;
+  p.dq = dq;
+  p.dk = dk;
+  p.dv = dv;
+  p.stat = reinterpret_cast<float2 *>(ws + w.stat);
+  p.range = reinterpret_cast<uint32_t *>(ws + w.range);
+  p.part = reinterpret_cast<float *>(ws + w.part);
+  p.tail = reinterpret_cast<float *>(ws + w.tail);
+  p.scale = scale;
+  p.c = scale * LOG2E;
+  p.B = B;
+  p.D = D;
+  p.parts = w.parts;
+  p.sink_tiles = w.sink_tiles;
+  p.tail_slots = w.tail_slots;
+  p.heads = p.f.group < QR ? p.f.group : QR;
+  p.tokens = QR / p.heads;
+  p.splits = (p.f.group + QR - 1) / QR;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  debug_poison(dq, static_cast<size_t>(B) * Tq * Hq * D * attn_bytes(dtype), st);
+  debug_poison(dk, static_cast<size_t>(B) * Tk * Hk * D * attn_bytes(dtype), st);
+  debug_poison(dv, static_cast<size_t>(B) * Tk * Hk * D * attn_bytes(dtype), st);
+  debug_poison(workspace, w.bytes, st);
+#define PBATTN_BWD(T)                                    \
+  switch (D) {                                           \
+    case 64: return launch_bwd<T, 64>(p, st);            \
+    case 128: return launch_bwd<T, 128>(p, st);          \
+    default: return launch_bwd<T, 256>(p, st);           \
+  }
+  switch (dtype) {
+    case PBGDN_F32: PBATTN_BWD(PBGDN_F32)
+    case PBGDN_BF16: PBATTN_BWD(PBGDN_BF16)
+    default: PBATTN_BWD(PBGDN_F16)
+  }
+#undef PBATTN_BWD
+}

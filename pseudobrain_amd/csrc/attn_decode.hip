@@ -1,0 +1,645 @@
+// Attention of the newest tokens over a paged cache (pbattn_paged_decode) and
+// the cache's writes (pbattn_paged_write).
+//
+// Decoding reads every visible key and value once and computes little with
+// them, so the kernel is built around loads: each wave takes blocks of 32 keys
+// by itself, straight from the cache into the registers the matrix
+// instructions read, with no LDS in between. Scores come from 16x16 products
+// S^T = K Q^T whose 16 columns are the (token, head) rows that share the key
+// head. For O^T = V^T P the wave loads 8 (16-bit) whole value rows such that
+// each lane holds an 8 x 8 block of V, and transposes it in place.
+//
+// The visible blocks of all sequences are shared out evenly from the lengths:
+// every workgroup derives the same shares, so a batch of uneven contexts needs
+// neither a host's knowledge of the lengths nor a list made by another kernel.
+#include "attn.hpp"
+#include "attn_tile.hpp"
+#include "device.hpp"
+
+namespace pbgdn {
+
+constexpr int DEC_WAVES = 4;         // waves of a workgroup
+constexpr int DEC_KEYS = 32;         // keys of a block
+constexpr int DEC_MIN = DEC_WAVES;   // fewest blocks of a part: one a wave
+constexpr int DEC_ROWS = 16;         // rows of a matrix tile
+
+struct DecodeParams {
+  const unsigned char *q, *k, *v;
+  long token, head;  // strides of the caches, bytes
+  int page_rows;     // a page's stride in token strides
+  int page, num_pages, max_pages;
+  const int32_t *table, *lengths;
+  void *o;
+  float *lse;
+  float *part;     // [slots][Hk][rows][D] unnormalised outputs
+  float2 *stat;    // [slots][Hk][rows] (maximum in powers of two, sum)
+  int B, T, Hq, Hk, group, rows, row_tiles, window, sinks, target;
+  float c;
+  int negate;
+};
+
+// The keys sequence b's queries see, and its blocks.
+__device__ __forceinline__ int seq_length(const DecodeParams &p, int b) {
+  const int n = p.num_pages > 0 ? p.lengths[b] : 0;
+  return n > 0 ? n : 0;
+}
+__device__ __forceinline__ KeyRange seq_keys(const DecodeParams &p, int len) {
+  return key_range(len - p.T, len - 1, p.window, p.sinks);
+}
+__device__ __forceinline__ int seq_blocks(const DecodeParams &p, int b) {
+  const int len = seq_length(p, b);
+  return (seq_keys(p, len).count + DEC_KEYS - 1) / DEC_KEYS;
+}
+
+// The shares: every part takes `per` blocks (the last of a sequence what is
+// left), a sequence at least one part.
+struct Share {
+  int seq, part, parts, per, first;  // first: the sequence's first slot
+};
+__device__ __forceinline__ long wave_sum_long(long x) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off, 64);
+  return x;
+}
+// Blocks per part, the same in every workgroup.
+__device__ __forceinline__ int share_size(const DecodeParams &p, int lane) {
+  long total = 0;
+  for (int b = lane; b < p.B; b += 64) total += seq_blocks(p, b);
+  total = wave_sum_long(total);
+  const int per = static_cast<int>((total + p.target - 1) / p.target);
+  const int whole = (per + DEC_MIN - 1) / DEC_MIN * DEC_MIN;
+  return whole > DEC_MIN ? whole : DEC_MIN;
+}
+__device__ __forceinline__ int seq_parts(const DecodeParams &p, int b, int per) {
+  const int n = (seq_blocks(p, b) + per - 1) / per;
+  return n > 0 ? n : 1;
+}
+// Whose slot it is: a scan over the sequences, 64 at a time. seq = -1 past the last.
+__device__ __forceinline__ Share share_of_slot(const DecodeParams &p, int slot, int lane) {
+  Share s;
+  s.per = share_size(p, lane);
+  s.seq = -1;
+  int base = 0;
+  for (int b0 = 0; b0 < p.B; b0 += 64) {
+    const int mine = b0 + lane < p.B ? seq_parts(p, b0 + lane, s.per) : 0;
+    int scan = mine;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int x = __shfl_up(scan, off, 64);
+      if (lane >= off) scan += x;
+    }
+    const uint64_t past = __ballot(base + scan > slot);
+    if (past) {
+      const int l = __builtin_ctzll(past);
+      s.seq = b0 + l;
+      s.parts = __shfl(mine, l, 64);
+      s.first = base + __shfl(scan, l, 64) - s.parts;
+      s.part = slot - s.first;
+      return s;
+    }
+    base += __shfl(scan, 63, 64);
+  }
+  return s;
+}
+// The first slot of sequence b.
+__device__ __forceinline__ int first_slot(const DecodeParams &p, int b, int per, int lane) {
+  long before = 0;
+  for (int i = lane; i < b; i += 64) before += seq_parts(p, i, per);
+  return static_cast<int>(wave_sum_long(before));
+}
+
+template <int DT, int D>
+struct Dec {
+  using E = Elem<DT>;
+  static constexpr bool SHORT = E::BYTES == 2;
+  static constexpr int ROW = D * E::BYTES;
+  static constexpr int KSTEPS = ROW / 64;           // 16-byte units a lane reads of a key
+  static constexpr int VB = SHORT && D == 64 ? 8 : 16;  // bytes a lane reads of a value row at once
+  static constexpr int VLOADS = ROW / 16 / VB;      // times it does
+  static constexpr int VE = VB / E::BYTES;          // elements of one such read
+  static constexpr int OT = D / 16;                 // 16-wide output tiles: VLOADS * VE
+};
+
+// Scores of 16 keys: x += K rows (a lane's units) times Q rows.
+template <int DT>
+__device__ __forceinline__ float4_t key_mma(v4u32_t k, v4u32_t q, float4_t x) {
+  if constexpr (DT == PBGDN_F32) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      x = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[e]), __uint_as_float(q[e]), x, 0, 0, 0);
+    return x;
+  } else {
+    return Elem<DT>::mma16(k, q, x);
+  }
+}
+
+// max / sum over the four lanes (one of each 16) that hold a row.
+__device__ __forceinline__ float max_rows(float x) {
+  float a = x, b = x;
+  swap16(a, b);
+  a = fmaxf(a, b);
+  b = a;
+  swap32(a, b);
+  return fmaxf(a, b);
+}
+
+template <int DT, int D, int RB, int OCC>
+__global__ __launch_bounds__(DEC_WAVES * 64, OCC) void decode_kernel(const DecodeParams p) {
+  using K = Dec<DT, D>;
+  using E = typename K::E;
+  constexpr int KS = K::KSTEPS, OT = K::OT;
+  // waves joined at a time: pairs, or one after the other where two would not fit
+  constexpr int JOINS = RB * D <= 256 ? 2 : 1;
+  __shared__ __attribute__((aligned(16))) float merge[JOINS][RB * DEC_ROWS * (D + 2)];
+  PBGDN_POISON_LDS(merge, sizeof(merge));
+  PBGDN_POISON_SYNC();
+
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const int c = lane & 15, g = lane >> 4;
+  int id = blockIdx.x;
+  const int hk = id % p.Hk;
+  id /= p.Hk;
+  const int row0 = id % p.row_tiles * (RB * DEC_ROWS);
+  const int slot = id / p.row_tiles;
+  const Share share = share_of_slot(p, slot, lane);
+  if (share.seq < 0) return;
+  const int b = uniform(share.seq), len = uniform(seq_length(p, b));
+  const KeyRange range = seq_keys(p, len);
+  const int blocks = (range.count + DEC_KEYS - 1) / DEC_KEYS;
+  const int begin = uniform(share.part * share.per);
+  const int end = uniform(begin + share.per < blocks ? begin + share.per : blocks);
+
+  // this lane's rows of Q (column c of every row block)
+  v4u32_t qf[RB][KS];
+  int pos[RB];
+#pragma unroll
+  for (int r = 0; r < RB; ++r) {
+    const int row = row0 + r * DEC_ROWS + c;
+    const int rr = row < p.rows ? row : p.rows - 1;
+    const int t = rr / p.group;
+    pos[r] = len - p.T + t;
+    const unsigned char *src = p.q + ((static_cast<long>(b) * p.T + t) * p.Hq + hk * p.group + rr % p.group) * K::ROW;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      qf[r][s] = *reinterpret_cast<const v4u32_t *>(src + (4 * s + g) * 16);
+      if (p.negate) qf[r][s] ^= K::SHORT ? 0x80008000u : 0x80000000u;
+    }
+  }
+  float m[RB], l[RB];
+  float4_t o[RB][OT];
+#pragma unroll
+  for (int r = 0; r < RB; ++r) {
+    m[r] = -INFINITY;
+    l[r] = 0.0f;
+#pragma unroll
+    for (int j = 0; j < OT; ++j) o[r][j] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+
+  const unsigned char *kbase = p.k + hk * p.head, *vbase = p.v + hk * p.head;
+  const int32_t *table = p.table + static_cast<long>(b) * p.max_pages;
+  // the cache row of key `lane & 31` of a block, -1 where there is none
+  const auto lookup = [&](int blk) {
+    const int u = blk * DEC_KEYS + (lane & 31);
+    if (u >= range.count) return -1;
+    const int j = u < range.sinks ? u : u + range.delta;
+    const int pg = j / p.page;
+    const int at = pg < p.max_pages ? table[pg] : -1;
+    return at >= 0 && at < p.num_pages ? at * p.page_rows + (j - pg * p.page) : -1;
+  };
+  int rows = begin + wave < end ? lookup(begin + wave) : -1;
+  for (int blk = begin + wave; blk < end; blk += DEC_WAVES) {
+    const bool all = __ballot(rows >= 0) == ~0ull;
+    const int safe = rows >= 0 ? rows : 0;
+    v4u32_t kf[2][KS];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+      const unsigned char *src = kbase + static_cast<long>(__shfl(safe, 16 * kb + c, 64)) * p.token;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) kf[kb][s] = *reinterpret_cast<const v4u32_t *>(src + (4 * s + g) * 16);
+    }
+    uint32_t vf[8][K::VLOADS][K::VB / 4];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int key = (i < 4 ? 0 : 16) + 4 * g + i % 4;
+      const unsigned char *src = vbase + static_cast<long>(__shfl(safe, key, 64)) * p.token;
+#pragma unroll
+      for (int x = 0; x < K::VLOADS; ++x) {
+        if constexpr (K::VB == 16) {
+          const v4u32_t w = *reinterpret_cast<const v4u32_t *>(src + x * 16 * K::VB + c * K::VB);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) vf[i][x][e] = w[e];
+        } else {
+          const v2u32_t w = *reinterpret_cast<const v2u32_t *>(src + x * 16 * K::VB + c * K::VB);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) vf[i][x][e] = w[e];
+        }
+      }
+    }
+    const int valid = rows;
+    if (blk + DEC_WAVES < end) rows = lookup(blk + DEC_WAVES);
+
+    if (!all) {  // values of absent keys: zeros, whatever the row they were read from holds
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const bool in = __shfl(valid, (i < 4 ? 0 : 16) + 4 * g + i % 4, 64) >= 0;
+#pragma unroll
+        for (int x = 0; x < K::VLOADS; ++x)
+#pragma unroll
+          for (int e = 0; e < K::VB / 4; ++e) vf[i][x][e] = in ? vf[i][x][e] : 0u;
+      }
+    }
+    const int u0 = blk * DEC_KEYS;
+    const int j0 = u0 < range.sinks ? u0 : u0 + range.delta, j1 = u0 + DEC_KEYS - 1 + range.delta;
+    const bool whole = all && u0 >= range.sinks && j1 <= len - p.T && j0 > len - 1 - p.window;
+#pragma unroll
+    for (int r = 0; r < RB; ++r) {
+      float4_t s[2];
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+        s[kb] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int k = 0; k < KS; ++k) s[kb] = key_mma<DT>(kf[kb][k], qf[r][k], s[kb]);
+      }
+      if (!whole) {
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int key = 16 * kb + 4 * g + i, u = u0 + key;
+            const int j = u < range.sinks ? u : u + range.delta;
+            const bool seen = (__shfl(valid, key, 64) >= 0) & sees(pos[r], j, p.window, p.sinks);
+            s[kb][i] = seen ? s[kb][i] : -INFINITY;
+          }
+      }
+      float mx = s[0][0];
+#pragma unroll
+      for (int i = 1; i < 8; ++i) mx = fmaxf(mx, s[i / 4][i % 4]);
+      const float top = fmaxf(m[r], max_rows(mx)), base = top == -INFINITY ? 0.0f : top, at = base * p.c;
+      const float alpha = __builtin_amdgcn_exp2f((m[r] - base) * p.c);
+      m[r] = top;
+      float sum = 0.0f;
+      const bool far = __any(fabsf(at) > EXACT_SCORES);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float x = s[i / 4][i % 4];
+        s[i / 4][i % 4] = __builtin_amdgcn_exp2f(far ? (x - base) * p.c : __builtin_fmaf(x, p.c, -at));
+        sum += s[i / 4][i % 4];
+      }
+      l[r] = l[r] * alpha + sum;
+#pragma unroll
+      for (int j = 0; j < OT; ++j) o[r][j] *= alpha;
+      if constexpr (K::SHORT) {
+        const v4u32_t w = {E::pack(s[0][0], s[0][1]), E::pack(s[0][2], s[0][3]), E::pack(s[1][0], s[1][1]),
+                           E::pack(s[1][2], s[1][3])};
+#pragma unroll
+        for (int x = 0; x < K::VLOADS; ++x)
+#pragma unroll
+          for (int e = 0; e < K::VE; ++e) {
+            v4u32_t a;  // element e of the lane's eight value rows
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              a[i] = __builtin_amdgcn_perm(vf[2 * i + 1][x][e / 2], vf[2 * i][x][e / 2],
+                                           e % 2 ? 0x07060302u : 0x05040100u);
+            o[r][x * K::VE + e] = E::mma16(a, w, o[r][x * K::VE + e]);
+          }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+          for (int x = 0; x < K::VLOADS; ++x)
+#pragma unroll
+            for (int e = 0; e < K::VE; ++e)
+              o[r][x * K::VE + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                  __uint_as_float(vf[i][x][e]), s[i / 4][i % 4], o[r][x * K::VE + e], 0, 0, 0);
+      }
+    }
+  }
+
+#pragma unroll
+  for (int r = 0; r < RB; ++r) l[r] = add_xor32(add_xor16(l[r]));
+  // from here on maxima in powers of two
+#pragma unroll
+  for (int r = 0; r < RB; ++r) m[r] *= p.c;
+  // join the waves into wave 0: the upper half into the lower, or one by one
+  constexpr int ROUNDS = JOINS == 2 ? 2 : DEC_WAVES - 1;
+#pragma unroll
+  for (int round = 0; round < ROUNDS; ++round) {
+    const int from = JOINS == 2 ? DEC_WAVES / 2 >> round : round + 1, count = JOINS == 2 ? from : 1;
+    if (wave >= from && wave < from + count) {
+      float *dst = merge[wave - from];
+#pragma unroll
+      for (int r = 0; r < RB; ++r) {
+#pragma unroll
+        for (int j = 0; j < OT; ++j)
+          *reinterpret_cast<float4_t *>(dst + ((r * OT + j) * 64 + lane) * 4) = o[r][j];
+        if (g == 0) {
+          dst[RB * DEC_ROWS * D + (r * 16 + c) * 2] = m[r];
+          dst[RB * DEC_ROWS * D + (r * 16 + c) * 2 + 1] = l[r];
+        }
+      }
+    }
+    __syncthreads();
+    if (wave < count) {
+      const float *src = merge[wave];
+#pragma unroll
+      for (int r = 0; r < RB; ++r) {
+        const float m2 = src[RB * DEC_ROWS * D + (r * 16 + c) * 2], l2 = src[RB * DEC_ROWS * D + (r * 16 + c) * 2 + 1];
+        const float top = fmaxf(m[r], m2), at = top == -INFINITY ? 0.0f : top;
+        const float f1 = __builtin_amdgcn_exp2f(m[r] - at), f2 = __builtin_amdgcn_exp2f(m2 - at);
+        m[r] = top;
+        l[r] = l[r] * f1 + l2 * f2;
+#pragma unroll
+        for (int j = 0; j < OT; ++j)
+          o[r][j] = o[r][j] * f1 + *reinterpret_cast<const float4_t *>(src + ((r * OT + j) * 64 + lane) * 4) * f2;
+      }
+    }
+    __syncthreads();
+  }
+  if (wave != 0) return;
+
+#pragma unroll
+  for (int r = 0; r < RB; ++r) {
+    const int row = row0 + r * DEC_ROWS + c;
+    if (row >= p.rows) continue;
+    const bool last = share.parts == 1;
+    const float f = last && l[r] > 0.0f ? 1.0f / l[r] : 1.0f;
+    const long at = last ? (static_cast<long>(b) * p.T + row / p.group) * p.Hq + hk * p.group + row % p.group
+                         : (static_cast<long>(slot) * p.Hk + hk) * p.rows + row;
+    if (g == 0) {
+      if (!last) {
+        p.stat[at] = make_float2(m[r], l[r]);
+      } else if (p.lse) {
+        p.lse[at] = l[r] > 0.0f ? (m[r] + __builtin_amdgcn_logf(l[r])) * LN2 : l[r] == 0.0f ? -INFINITY : l[r];
+      }
+    }
+    // element j of the lane's i-th matrix row: column VE (4 g + i) + j of a run of 16 VE
+#pragma unroll
+    for (int x = 0; x < K::VLOADS; ++x)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < K::VE; e += 4) {
+          const long d = at * D + x * 16 * K::VE + (4 * g + i) * K::VE + e;
+          const float4_t y = {o[r][x * K::VE + e][i] * f, o[r][x * K::VE + e + 1][i] * f,
+                              o[r][x * K::VE + e + 2][i] * f, o[r][x * K::VE + e + 3][i] * f};
+          if (!last || !K::SHORT) {
+            *reinterpret_cast<float4_t *>((last ? static_cast<float *>(p.o) : p.part) + d) = y;
+          } else if constexpr (K::SHORT) {
+            *reinterpret_cast<v2u32_t *>(static_cast<unsigned char *>(p.o) + 2 * d) =
+                v2u32_t{E::pack(y[0], y[1]), E::pack(y[2], y[3])};
+          }
+        }
+  }
+}
+
+// Joins a sequence's parts: a workgroup per (sequence, query row and head),
+// a quarter of the parts to a wave.
+template <int DT, int D>
+__global__ __launch_bounds__(256) void decode_join_kernel(const DecodeParams p) {
+  using E = Elem<DT>;
+  constexpr int VEC = D / 64;
+  __shared__ float acc[4][D], stat[4][2];
+  PBGDN_POISON_LDS(acc, sizeof(acc));
+  PBGDN_POISON_SYNC();
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  int id = blockIdx.x;
+  const int row = id % p.rows;
+  id /= p.rows;
+  const int hk = id % p.Hk, b = id / p.Hk;
+  const int per = uniform(share_size(p, lane));
+  const int parts = uniform(seq_parts(p, b, per));
+  if (parts == 1) return;  // written by the first kernel
+  const int first = uniform(first_slot(p, b, per, lane));
+  float m = -INFINITY, l = 0.0f, o[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) o[e] = 0.0f;
+  for (int i = wave; i < parts; i += 4) {
+    const long at = (static_cast<long>(first + i) * p.Hk + hk) * p.rows + row;
+    const float2 s = p.stat[at];
+    const float top = fmaxf(m, s.x), base = top == -INFINITY ? 0.0f : top;
+    const float f1 = __builtin_amdgcn_exp2f(m - base), f2 = __builtin_amdgcn_exp2f(s.x - base);
+    m = top;
+    l = l * f1 + s.y * f2;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) o[e] = o[e] * f1 + p.part[at * D + lane * VEC + e] * f2;
+  }
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) acc[wave][lane * VEC + e] = o[e];
+  if (lane == 0) {
+    stat[wave][0] = m;
+    stat[wave][1] = l;
+  }
+  __syncthreads();
+  const float top = fmaxf(fmaxf(stat[0][0], stat[1][0]), fmaxf(stat[2][0], stat[3][0]));
+  const float base = top == -INFINITY ? 0.0f : top;
+  float f[4], sum = 0.0f;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    f[w] = __builtin_amdgcn_exp2f(stat[w][0] - base);
+    sum += stat[w][1] * f[w];
+  }
+  const float inv = sum > 0.0f ? 1.0f / sum : sum;
+  const long at = (static_cast<long>(b) * p.T + row / p.group) * p.Hq + hk * p.group + row % p.group;
+  if (threadIdx.x < D) {
+    float x = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) x += acc[w][threadIdx.x] * f[w];
+    store_elem(p.o, at * D + threadIdx.x, DT, x * inv);
+  }
+  if (p.lse && threadIdx.x == 0)
+    p.lse[at] = sum > 0.0f ? (top + __builtin_amdgcn_logf(sum)) * LN2 : sum == 0.0f ? -INFINITY : sum;
+}
+
+// ---------------------------------------------------------------------------
+// Writes into the pages: 16 bytes a thread, the threads of a token together.
+// ---------------------------------------------------------------------------
+struct WriteParams {
+  const unsigned char *k, *v;
+  long k_token, k_head, v_token, v_head;
+  unsigned char *kc, *vc;
+  long page_stride, token, head;
+  const int64_t *slots;
+  long total;
+  int page, units, N, Hk;  // 16-byte units of a head
+};
+__global__ __launch_bounds__(256) void paged_write_kernel(const WriteParams p) {
+  const int per = p.Hk * p.units;  // units of a token, of one cache
+  const long n = static_cast<long>(p.N) * per;
+  for (long i = blockIdx.x * 256L + threadIdx.x; i < n; i += gridDim.x * 256L) {
+    const int tok = static_cast<int>(i / per), x = static_cast<int>(i - static_cast<long>(tok) * per);
+    const int64_t slot = p.slots[tok];
+    if (slot < 0 || slot >= p.total) continue;
+    const int hd = x / p.units, u = x - hd * p.units;
+    const int64_t pg = slot / p.page;
+    const long to = pg * p.page_stride + (slot - pg * p.page) * p.token + hd * p.head + u * 16;
+    const v4u32_t a = *reinterpret_cast<const v4u32_t *>(p.k + tok * p.k_token + hd * p.k_head + u * 16);
+    const v4u32_t b = *reinterpret_cast<const v4u32_t *>(p.v + tok * p.v_token + hd * p.v_head + u * 16);
+    *reinterpret_cast<v4u32_t *>(p.kc + to) = a;
+    *reinterpret_cast<v4u32_t *>(p.vc + to) = b;
+  }
+}
+
+template <int DT, int D>
+static int launch_decode(DecodeParams &p, hipStream_t stream) {
+  const long slots = static_cast<long>(p.target) + p.B;
+  const auto run = [&](auto kernel, int rb) {
+    p.row_tiles = (p.rows + rb * DEC_ROWS - 1) / (rb * DEC_ROWS);
+    const long blocks = slots * p.Hk * p.row_tiles;
+    if (blocks > 0x7fffffffL || static_cast<long>(p.B) * p.Hk * p.rows > 0x7fffffffL) return false;
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(DEC_WAVES * 64), 0, stream, p);
+    return true;
+  };
+  constexpr int WIDE = D * Elem<DT>::BYTES;
+  const bool ok = p.rows <= DEC_ROWS ? run(decode_kernel<DT, D, 1, WIDE <= 256 ? 2 : 1>, 1)
+                                     : run(decode_kernel<DT, D, 2, WIDE <= 256 ? 2 : 1>, 2);
+  if (!ok) return PBGDN_ERR_UNSUPPORTED;
+  hipLaunchKernelGGL((decode_join_kernel<DT, D>), dim3(static_cast<unsigned>(p.B * p.Hk * p.rows)), dim3(256), 0,
+                     stream, p);
+  return hipGetLastError() == hipSuccess ? PBGDN_OK : PBGDN_ERR_LAUNCH;
+}
+
+template <int DT>
+static int dispatch_decode(DecodeParams &p, int D, hipStream_t stream) {
+  switch (D) {
+    case 64: return launch_decode<DT, 64>(p, stream);
+    case 128: return launch_decode<DT, 128>(p, stream);
+    case 256: return launch_decode<DT, 256>(p, stream);
+    default: return PBGDN_ERR_UNSUPPORTED;
+  }
+}
+
+// Parts wanted over all sequences: workgroups for every CU a few times over.
+static int decode_target(int Hk, int rows) {
+  DeviceShape shape;
+  if (!device_shape(shape)) shape.cus = 256;
+  const int tiles = (rows + 2 * DEC_ROWS - 1) / (2 * DEC_ROWS);
+  const int t = 4 * shape.cus / (Hk * tiles);
+  return t > 1 ? t : 1;
+}
+static bool decode_sizes_ok(int B, int T, int Hq, int Hk, int D) {
+  return B >= 0 && T >= 1 && T <= PBATTN_MAX_DRAFT && Hq > 0 && Hk > 0 && Hq % Hk == 0 && D > 0;
+}
+
+// The cache's strides in bytes; false when they cannot be.
+static bool cache_strides(const int64_t *s, int bytes, int page_size, int num_pages, long out[3]) {
+  for (int a = 0; a < 3; ++a) {
+    if (s[a] < 0 || s[a] * bytes % 16 != 0) return false;
+    out[a] = s[a] * bytes;
+  }
+  return true;
+}
+
+}  // namespace pbgdn
+
+extern "C" size_t pbattn_paged_decode_workspace_size(int B, int T, int Hq, int Hk, int D) {
+  using namespace pbgdn;
+  if (!decode_sizes_ok(B, T, Hq, Hk, D)) return 0;
+  const int rows = Hq / Hk * T;
+  const size_t slots = static_cast<size_t>(decode_target(Hk, rows)) + B;
+  return slots * Hk * rows * (D * sizeof(float) + sizeof(float2));
+}
+
+extern "C" int pbattn_paged_decode(const void *q, const void *k_cache, const void *v_cache, int dtype,
+                                   const int64_t *strides, int page_size, int num_pages, const int32_t *page_table,
+                                   int max_pages, const int32_t *lengths, void *o, float *lse, int B, int T, int Hq,
+                                   int Hk, int D, float scale, int window, int sinks, void *workspace,
+                                   size_t workspace_bytes, void *stream) {
+  using namespace pbgdn;
+  if (!decode_sizes_ok(B, T, Hq, Hk, D) || !attn_dtype(dtype) || !strides || page_size <= 0 || num_pages < 0 ||
+      max_pages < 0 || sinks < 0 || !(scale - scale == 0.0f)) {
+    return PBGDN_ERR_INVALID_ARGUMENT;
+  }
+  if (B == 0) return PBGDN_OK;
+  if (!q || !o || !lengths || (max_pages > 0 && !page_table) || (num_pages > 0 && (!k_cache || !v_cache)) || !workspace ||
+      !aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(o) || !aligned16(workspace)) {
+    return PBGDN_ERR_INVALID_ARGUMENT;
+  }
+  long st[3];
+  if (!cache_strides(strides, attn_bytes(dtype), page_size, num_pages, st)) return PBGDN_ERR_INVALID_ARGUMENT;
+  if (num_pages > 1 || page_size > 1) {
+    if (st[1] <= 0 || st[0] % st[1] != 0) return PBGDN_ERR_INVALID_ARGUMENT;
+  }
+  const long page_rows = st[1] > 0 ? st[0] / st[1] : 0;
+  if (page_rows * (num_pages > 0 ? num_pages - 1 : 0) + page_size > 0x7fffffffL) return PBGDN_ERR_UNSUPPORTED;
+  if (workspace_bytes < pbattn_paged_decode_workspace_size(B, T, Hq, Hk, D)) return PBGDN_ERR_INVALID_ARGUMENT;
+  DecodeParams p{};
+  p.q = static_cast<const unsigned char *>(q);
+  p.k = static_cast<const unsigned char *>(k_cache);
+  p.v = static_cast<const unsigned char *>(v_cache);
+  p.token = st[1];
+  p.head = st[2];
+  p.page_rows = static_cast<int>(page_rows);
+  p.page = page_size;
+  p.num_pages = num_pages;
+  p.max_pages = max_pages;
+  p.table = page_table;
+  p.lengths = lengths;
+  p.o = o;
+  p.lse = lse;
+  p.B = B;
+  p.T = T;
+  p.Hq = Hq;
+  p.Hk = Hk;
+  p.group = Hq / Hk;
+  p.rows = p.group * T;
+  p.window = window <= 0 || window > NO_WINDOW ? NO_WINDOW : window;
+  p.sinks = sinks < NO_WINDOW ? sinks : NO_WINDOW;
+  p.target = decode_target(Hk, p.rows);
+  const float c = __builtin_fabsf(scale) * LOG2E;
+  p.c = c > 1.17549435e-38f ? c : 1.17549435e-38f;
+  p.negate = scale < 0.0f;
+  const size_t rows = (static_cast<size_t>(p.target) + B) * Hk * p.rows;
+  p.part = static_cast<float *>(workspace);
+  p.stat = reinterpret_cast<float2 *>(p.part + rows * D);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  debug_poison(o, static_cast<size_t>(B) * T * Hq * D * attn_bytes(dtype), s);
+  if (lse) debug_poison(lse, static_cast<size_t>(B) * T * Hq * sizeof(float), s);
+  debug_poison(workspace, rows * (D * sizeof(float) + sizeof(float2)), s);
+  switch (dtype) {
+    case PBGDN_F32: return dispatch_decode<PBGDN_F32>(p, D, s);
+    case PBGDN_BF16: return dispatch_decode<PBGDN_BF16>(p, D, s);
+    default: return dispatch_decode<PBGDN_F16>(p, D, s);
+  }
+}
+
+extern "C" int pbattn_paged_write(const void *k, const void *v, int dtype, const int64_t *kv_strides, void *k_cache,
+                                  void *v_cache, const int64_t *strides, int page_size, int num_pages,
+                                  const int64_t *slots, int N, int Hk, int D, void *stream) {
+  using namespace pbgdn;
+  if (N < 0 || Hk <= 0 || D <= 0 || !attn_dtype(dtype) || !kv_strides || !strides || page_size <= 0 || num_pages < 0) {
+    return PBGDN_ERR_INVALID_ARGUMENT;
+  }
+  if (N == 0 || num_pages == 0) return PBGDN_OK;
+  const int bytes = attn_bytes(dtype);
+  if (D * bytes % 16 != 0) return PBGDN_ERR_UNSUPPORTED;
+  if (!k || !v || !k_cache || !v_cache || !slots || !aligned16(k) || !aligned16(v) || !aligned16(k_cache) ||
+      !aligned16(v_cache)) {
+    return PBGDN_ERR_INVALID_ARGUMENT;
+  }
+  long st[3];
+  if (!cache_strides(strides, bytes, page_size, num_pages, st)) return PBGDN_ERR_INVALID_ARGUMENT;
+  for (int a = 0; a < 4; ++a)
+    if (kv_strides[a] < 0 || kv_strides[a] * bytes % 16 != 0) return PBGDN_ERR_INVALID_ARGUMENT;
+  WriteParams p{};
+  p.k = static_cast<const unsigned char *>(k);
+  p.v = static_cast<const unsigned char *>(v);
+  p.k_token = kv_strides[0] * bytes;
+  p.k_head = kv_strides[1] * bytes;
+  p.v_token = kv_strides[2] * bytes;
+  p.v_head = kv_strides[3] * bytes;
+  p.kc = static_cast<unsigned char *>(k_cache);
+  p.vc = static_cast<unsigned char *>(v_cache);
+  p.page_stride = st[0];
+  p.token = st[1];
+  p.head = st[2];
+  p.slots = slots;
+  p.total = static_cast<long>(num_pages) * page_size;
+  p.page = page_size;
+  p.units = D * bytes / 16;
+  p.N = N;
+  p.Hk = Hk;
+  const long want = (static_cast<long>(N) * Hk * p.units + 255) / 256;
+  hipLaunchKernelGGL(paged_write_kernel, dim3(static_cast<unsigned>(want < 65536 ? want : 65536)), dim3(256), 0,
+                     static_cast<hipStream_t>(stream), p);
+  return hipGetLastError() == hipSuccess ? PBGDN_OK : PBGDN_ERR_LAUNCH;
+}

@@ -1,0 +1,372 @@
+// Tiles of the attention kernels (gfx950): rows of D elements in LDS, staged by
+// direct-to-LDS loads, and the two matrix products every kernel is made of.
+//
+// All kernels keep scores transposed or not so that one side of every product
+// lives in registers, on the 32x32 matrix instructions (lane l: n = l & 31,
+// h = l >> 5; an accumulator holds rows 8 (i / 4) + 4 h + i % 4 of column n in
+// its element i):
+//
+//   rows product   X[r][n] = sum_d M[r][d] Y[n][d]
+//                  M a tile in LDS, read 16 bytes of a row at a time; Y held by
+//                  the wave, lane (n, h) with units 2 s + h of row n.
+//   cols product   Z[d][n] += sum_r M[r][d] X[r][n]
+//                  X as the rows product left it: its accumulator is the B
+//                  operand as it stands, because the order of the contraction
+//                  index is free as long as both operands agree; M's columns
+//                  come from LDS by transposing reads (16-bit) or single
+//                  elements (float32).
+//
+// So S = K Q^T then O^T = V^T P needs no exchange between lanes: a query is one
+// lane pair's column from the score to the output.
+#pragma once
+
+#include "common.hpp"
+#include "pbattn.h"
+
+namespace pbgdn {
+
+typedef float float16_t __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+typedef short i16x4_t __attribute__((ext_vector_type(4)));
+
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+
+// Weights are exp2(s c - m c), one fused operation a score: the rounding of m c
+// is the same for every score of a row and cancels in its sum. Past this |m c|
+// it would no longer stay near 1 (2^-24 of it), and the kernels subtract first.
+constexpr float EXACT_SCORES = 65536.0f;
+
+// Element types: bytes, one matrix step of the rows product (a 16-byte unit per
+// lane and side) and the packing of two float32 values.
+template <int DT>
+struct Elem;
+
+template <>
+struct Elem<PBGDN_BF16> {
+  static constexpr int BYTES = 2;
+  using T = u16;
+  __device__ static float16_t mma(v4u32_t a, v4u32_t b, float16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c,
+                                                   0, 0, 0);
+  }
+  __device__ static float4_t mma16(v4u32_t a, v4u32_t b, float4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c,
+                                                   0, 0, 0);
+  }
+  __device__ static uint32_t pack(float x, float y) {
+    return __builtin_bit_cast(uint32_t, bf16x2_t{static_cast<__bf16>(x), static_cast<__bf16>(y)});
+  }
+  __device__ static float low(uint32_t w) { return __uint_as_float(w << 16); }
+  __device__ static float high(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+};
+
+template <>
+struct Elem<PBGDN_F16> {
+  static constexpr int BYTES = 2;
+  using T = half_t;
+  __device__ static float16_t mma(v4u32_t a, v4u32_t b, float16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0,
+                                                  0, 0);
+  }
+  __device__ static float4_t mma16(v4u32_t a, v4u32_t b, float4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0,
+                                                  0, 0);
+  }
+  __device__ static uint32_t pack(float x, float y) {
+    return __builtin_bit_cast(uint32_t, half2_t{static_cast<half_t>(x), static_cast<half_t>(y)});
+  }
+  __device__ static float low(uint32_t w) { return static_cast<float>(__builtin_bit_cast(half2_t, w)[0]); }
+  __device__ static float high(uint32_t w) { return static_cast<float>(__builtin_bit_cast(half2_t, w)[1]); }
+};
+
+template <>
+struct Elem<PBGDN_F32> {
+  static constexpr int BYTES = 4;
+  using T = float;
+  __device__ static float16_t mma(v4u32_t a, v4u32_t b, float16_t c) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[i]), __uint_as_float(b[i]), c, 0, 0, 0);
+    return c;
+  }
+};
+
+__device__ __forceinline__ float16_t zero16() {
+  float16_t z;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) z[i] = 0.0f;
+  return z;
+}
+
+// Row, within 32, of element i of an accumulator in lane half h.
+__device__ __forceinline__ constexpr int acc_row(int i, int h) { return 8 * (i / 4) + 4 * h + i % 4; }
+
+// ---------------------------------------------------------------------------
+// A tile's place in LDS: row r at r * ROW bytes, its 16-byte unit u at unit
+// u ^ swz(r). The permutation spreads both read patterns over all 64 banks: the
+// 16 rows of a quarter wave's rows-product read fall on 16 different units of
+// 256 bytes, and the 4 rows x 64 bytes of a transposing read on one line.
+// ---------------------------------------------------------------------------
+template <int DT, int D>
+struct Tile {
+  using E = Elem<DT>;
+  static constexpr int ROW = D * E::BYTES;  // bytes of a row
+  static constexpr int UNITS = ROW / 16;
+  static constexpr int STEPS = UNITS / 2;   // matrix steps of a rows product
+  static constexpr int MB = D / 32;         // 32-row blocks of a cols product's result
+  static constexpr int PER_DMA = 64 / UNITS > 0 ? 64 / UNITS : 1;  // rows a wave-wide load fills (UNITS <= 64)
+  static_assert(UNITS == 8 || UNITS == 16 || UNITS == 32 || UNITS == 64, "rows of 128 to 1024 bytes");
+
+  __device__ static __forceinline__ int swz(int r) {
+    return UNITS == 8 ? (((r >> 1) & 1) << 2) | ((r >> 2) & 3) : ((r & 3) << 2) | ((r >> 2) & 3);
+  }
+
+  // Rows product's read: lane base, then unit 2 s of rows r0 .. r0 + 31.
+  __device__ static __forceinline__ uint32_t rows_base(int n, int h) { return n * ROW + ((h ^ swz(n)) * 16); }
+  __device__ static __forceinline__ v4u32_t rows(const unsigned char *tile, uint32_t base, int r0, int s) {
+    const uint32_t lo = (2 * s) % 16, hi = (2 * s) / 16;
+    return *reinterpret_cast<const v4u32_t *>(tile + ((base ^ (lo * 16)) + hi * 256 + r0 * ROW));
+  }
+
+  // Cols product's read, 16-bit: the A operand of matrix step t (16 rows from
+  // r0 + 16 t) for columns 32 m .. 32 m + 31.
+  __device__ static __forceinline__ uint32_t cols_base(int lane) {
+    if constexpr (E::BYTES == 2) {
+      const int c = lane & 15, dh = (lane >> 4) & 1, h = lane >> 5;
+      const int r = 4 * h + (c >> 2);
+      return r * ROW + (((2 * dh + ((c & 3) >> 1)) ^ swz(r)) * 16) + 8 * (c & 1);
+    } else {
+      const int n = lane & 31, h = lane >> 5;
+      return 4 * h * ROW + (((n >> 2) ^ h) * 16) + 4 * (n & 3);
+    }
+  }
+  __device__ static __forceinline__ v2u32_t tr(const unsigned char *tile, uint32_t base, int row, int m, int b) {
+    const uint32_t lo = ((4 * m) % UNITS % 16) ^ (2 * b), hi = (4 * m) / 16;
+    const uint32_t at = (base ^ (lo * 16)) + hi * 256 + row * ROW;
+    return __builtin_bit_cast(v2u32_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                           (__attribute__((address_space(3))) i16x4_t *)(tile + at)));
+  }
+  __device__ static __forceinline__ v4u32_t cols(const unsigned char *tile, uint32_t base, int r0, int t, int m) {
+    const v2u32_t x = tr(tile, base, r0 + 16 * t, m, 0), y = tr(tile, base, r0 + 16 * t + 8, m, 1);
+    return v4u32_t{x[0], x[1], y[0], y[1]};
+  }
+  // The same, float32: element i of the contraction.
+  __device__ static __forceinline__ float col1(const unsigned char *tile, uint32_t base, int r0, int i, int m) {
+    const uint32_t k = ((8 * m) % 16) ^ ((i % 4) << 2) ^ ((2 * (i / 4)) & 3), hi = (8 * m) / 16;
+    return *reinterpret_cast<const float *>(tile + ((base ^ (k * 16)) + hi * 256 + (r0 + 8 * (i / 4) + i % 4) * ROW));
+  }
+
+  // X = M[r0 .. r0 + 31] Y^T; y: STEPS units a lane.
+  __device__ static __forceinline__ float16_t rows_product(const unsigned char *tile, uint32_t base, int r0,
+                                                           const v4u32_t *y) {
+    float16_t x = zero16();
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) x = E::mma(rows(tile, base, r0, s), y[s], x);
+    return x;
+  }
+
+  // X as the B operand of a cols product.
+  struct Operand {
+    v4u32_t w[E::BYTES == 2 ? 2 : 4];
+  };
+  __device__ static __forceinline__ Operand operand(const float16_t &x) {
+    Operand o;
+    if constexpr (E::BYTES == 2) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o.w[t][j] = E::pack(x[8 * t + 2 * j], x[8 * t + 2 * j + 1]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o.w[i / 4][i % 4] = __float_as_uint(x[i]);
+    }
+    return o;
+  }
+  // z[m] += columns 32 m .. of M[r0 .. r0 + 31] times X, every m.
+  __device__ static __forceinline__ void cols_product(const unsigned char *tile, uint32_t base, int r0,
+                                                      const Operand &x, float16_t *z) {
+    if constexpr (E::BYTES == 2) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int m = 0; m < MB; ++m) z[m] = E::mma(cols(tile, base, r0, t, m), x.w[t], z[m]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+#pragma unroll
+        for (int m = 0; m < MB; ++m)
+          z[m] = __builtin_amdgcn_mfma_f32_32x32x2f32(col1(tile, base, r0, i, m), __uint_as_float(x.w[i / 4][i % 4]),
+                                                      z[m], 0, 0, 0);
+    }
+  }
+};
+
+// ---------------------------------------------------------------------------
+// Direct-to-LDS loads: 16 bytes per lane, lane l to `lds` + 16 l. Assembly, so
+// that the compiler does not wait for them before LDS reads it cannot tell
+// apart; the waits are the ones written (wait_dma, then a barrier).
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t lds_address(const void *p) {
+  typedef __attribute__((address_space(3))) const unsigned char lds_byte;
+  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_byte *)p));
+}
+// From `off` bytes into a buffer resource; what lies outside it arrives as zeros.
+__device__ __forceinline__ void dma(v4u32_t desc, uint32_t off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(desc)
+               : "memory", "m0");
+}
+// 4 bytes per lane, lane l to `lds` + 4 l: for sources aligned to no more.
+__device__ __forceinline__ void dma4(v4u32_t desc, uint32_t off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(desc)
+               : "memory", "m0");
+}
+// From a 64-bit address per lane.
+__device__ __forceinline__ void dma(const void *src, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(src)
+               : "memory", "m0");
+}
+__device__ __forceinline__ v4u32_t dma_desc(const void *base, long bytes) {
+  const uint64_t a = reinterpret_cast<uint64_t>(base);
+  return v4u32_t{static_cast<uint32_t>(a), static_cast<uint32_t>(a >> 32) & 0xffffu,
+                 static_cast<uint32_t>(bytes > 0 ? bytes : 0), static_cast<uint32_t>(RSRC_WORD3)};
+}
+__device__ __forceinline__ void wait_dma() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// Every wave has reached this point; its LDS reads have returned.
+__device__ __forceinline__ void block_sync() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// x and its other lane half's (lane ^ 32).
+__device__ __forceinline__ float max_xor32(float x) {
+  float a = x, b = x;
+  swap32(a, b);
+  return fmaxf(a, b);
+}
+
+// A wave-uniform value in a scalar register.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// ---------------------------------------------------------------------------
+// Which keys a query sees: position p sees key j when j <= p and
+// (j > p - window or j < sinks). Without branches, and used to select, never to
+// guard the write of one element of a matrix accumulator: hipcc (ROCm 7.2) has
+// dropped such a guarded write.
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ bool sees(int p, int j, int window, int sinks) {
+  return (j <= p) & ((j > p - window) | (j < sinks));
+}
+
+// One sequence of a call.
+struct Seq {
+  int q0, nq;  // its first query token and how many
+  int k0, nk;  // its first key token and how many
+};
+
+// Sequence b's bounds, clamped into the tensors whatever the boundaries hold.
+// b == nseq: what a packed call's last boundaries leave over; KEYS says whether
+// the caller walks keys (the leftover has no queries) or queries (no keys).
+__device__ __forceinline__ int boundary(const int32_t *cu, int i, int total) {
+  const int x = cu[i];
+  return x < 0 ? 0 : x > total ? total : x;
+}
+template <bool KEYS>
+__device__ __forceinline__ Seq sequence(const int32_t *cu_q, const int32_t *cu_k, int b, int nseq, int Tq, int Tk) {
+  if (!cu_q) return Seq{0, Tq, 0, Tk};
+  Seq s;
+  s.q0 = boundary(cu_q, b, Tq);
+  s.nq = (b < nseq ? boundary(cu_q, b + 1, Tq) : KEYS ? s.q0 : Tq) - s.q0;
+  const int32_t *cu = cu_k ? cu_k : cu_q;
+  s.k0 = boundary(cu, b, Tk);
+  s.nk = (b < nseq ? boundary(cu, b + 1, Tk) : KEYS ? Tk : s.k0) - s.k0;
+  return s;
+}
+
+// Tiles of a packed call without a list of them: sequence b's tiles start at
+// slot floor(first[b] rows / TILE) + b, which leaves each of them at least the
+// ceil(rows / TILE) slots it needs, whatever the lengths; slots past that are
+// empty. What the boundaries leave over counts as sequence n. Returns the
+// sequence of `slot` by bisection.
+__device__ __forceinline__ int slot_start(const int32_t *cu, int b, int total, int rows, int tile) {
+  return static_cast<int>(static_cast<long>(boundary(cu, b, total)) * rows / tile) + b;
+}
+__device__ __forceinline__ int slot_sequence(const int32_t *cu, int n, int total, int rows, int tile, int slot) {
+  int lo = 0, hi = n;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (slot_start(cu, mid, total, rows, tile) <= slot)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  return lo;
+}
+
+// ---------------------------------------------------------------------------
+// The keys a block of rows sees, in order: the sinks [0, sinks), then from
+// `lo` on. Index u is key u below `sinks`, key u + delta from there.
+struct KeyRange {
+  int sinks, delta, count;
+};
+__device__ __forceinline__ KeyRange key_range(int p_first, int p_last, int window, int sinks) {
+  KeyRange r;
+  const int low = p_first - window + 1;
+  const int lo = low > 0 ? low : 0;
+  r.sinks = sinks < lo ? sinks : lo;
+  r.delta = lo - r.sinks;
+  r.count = p_last < 0 ? 0 : r.sinks + p_last - lo + 1;
+  return r;
+}
+
+// Stages rows u0 .. of a key range into a tile: wave w of NW fills its share.
+template <int DT, int D, int BN, int NW>
+struct KeyStage {
+  using L = Tile<DT, D>;
+  static constexpr int LOADS = BN / L::PER_DMA / NW;
+  static_assert(LOADS * L::PER_DMA * NW == BN, "whole loads");
+
+  __device__ static __forceinline__ void tile(const unsigned char *base, long stride, const KeyRange &r, int u0,
+                                              unsigned char *lds, int wave, int lane) {
+    const uint32_t at = uniform(lds_address(lds) + wave * 1024);
+    if (u0 >= r.sinks) {  // one run of keys: a scalar base, fixed lane offsets
+      const int left = r.count - u0, rows = left < BN ? left : BN;
+      const v4u32_t desc = dma_desc(base + (u0 + r.delta) * stride, (rows - 1) * stride + L::ROW);
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        const int row = (wave + NW * i) * L::PER_DMA + lane / L::UNITS;
+        dma(desc, static_cast<uint32_t>(row) * static_cast<uint32_t>(stride) + ((lane % L::UNITS) ^ L::swz(row)) * 16,
+            at + i * NW * 1024);
+      }
+    } else {  // sinks and the window's start in one tile; rows past the end repeat the last key
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        const int row = (wave + NW * i) * L::PER_DMA + lane / L::UNITS;
+        int u = u0 + row;
+        u = u < r.count ? u : r.count - 1;
+        const long j = u < r.sinks ? u : u + r.delta;
+        dma(base + j * stride + ((lane % L::UNITS) ^ L::swz(row)) * 16, at + i * NW * 1024);
+      }
+    }
+  }
+};
+
+// Position of a workgroup in the call: the (batch, key head) `group` and its
+// tile `slot`. Workgroups go to the XCDs in turn, and each XCD has its own L2:
+// the tiles of a group, which share keys, stay on one XCD (or on as few as
+// there are groups for), the longest of a causal call first.
+__device__ __forceinline__ void place(int id, int groups, int slots, int &group, int &slot) {
+  if (groups % 8 == 0) {
+    const int x = id & 7, i = id >> 3;
+    group = x + 8 * (i / slots);
+    slot = i % slots;
+  } else {
+    group = id % groups;
+    slot = id / groups;
+  }
+  slot = slots - 1 - slot;
+}
+
+}  // namespace pbgdn

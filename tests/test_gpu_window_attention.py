@@ -1,0 +1,259 @@
+"""window_attention and its backward on the device against the float64 oracle
+(oracle/attention.py), element by element within its error bounds: head layouts,
+widths, windows and sinks, lengths around the tiles, rows that see nothing,
+packed sequences, strided and broadcast inputs, dtypes."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import attention as oa
+from pseudobrain_amd import attention as at
+from pseudobrain_amd.workloads import to_numpy
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+NAMES = {torch.float32: "float32", torch.bfloat16: "bfloat16", torch.float16: "float16"}
+
+
+def make(batch, tq, tk, hq, hk, d, dtype, seed, go_scale=0.5):
+    gen = torch.Generator().manual_seed(seed)
+    q, k, v, go = (torch.randn(s, generator=gen) for s in
+                   ((batch, tq, hq, d), (batch, tk, hk, d), (batch, tk, hk, d), (batch, tq, hq, d)))
+    glse = torch.randn(batch, tq, hq, generator=gen)
+    return [x.to(dtype).to(DEV) for x in (q, k, v, go * go_scale)] + [glse.to(DEV) * go_scale]
+
+
+def f64(x):
+    return to_numpy(x).astype(np.float64)
+
+
+def compare(where, got, ref, tol):
+    got = f64(got)
+    assert got.shape == ref.shape, where
+    np.testing.assert_array_equal(np.isneginf(got), np.isneginf(ref), err_msg=where)
+    ok = np.isfinite(ref)
+    got, ref, tol = got[ok], ref[ok], tol[ok]
+    assert np.isfinite(got).all(), f"{where}: not finite"
+    error = np.abs(got - ref)
+    print(f"[{where}] max error {error.max(initial=0):.3e}, largest share of its bound "
+          f"{(error / np.maximum(tol, 1e-300)).max(initial=0):.3f}", flush=True)
+    assert (error <= tol).all(), f"{where}: beyond the bound by {(error - tol).max():.3e}"
+
+
+def check(where, q, k, v, go, glse, scale, window=None, sinks=0, cu=None, cu_k=None, grads=True):
+    """Forward, and backward through autograd, of o and lse."""
+    print(f"[{where}] q {tuple(q.shape)} k {tuple(k.shape)} window {window} sinks {sinks} {q.dtype}", flush=True)
+    leaves = [x.detach().requires_grad_(grads) for x in (q, k, v)]
+    o, lse = at.window_attention(*leaves, scale, window, sinks, cu, cu_k, return_lse=True)
+    got = dict(o=o, lse=lse)
+    if grads:
+        got.update(zip(("dq", "dk", "dv"), torch.autograd.grad((o, lse), leaves, (go, glse))))
+    torch.cuda.synchronize()
+    args = [f64(x) for x in (q, k, v)]
+    go64, glse64 = (f64(go), f64(glse)) if grads else (None, None)
+    if cu is not None:
+        cq = cu.tolist()
+        ck = cq if cu_k is None else cu_k.tolist()
+        refs = [oa.packed(args[0][0], args[1][0], args[2][0], scale, window, sinks, cq, ck,
+                          None if go64 is None else go64[0], None if glse64 is None else glse64[0], NAMES[q.dtype])]
+    else:
+        refs = [oa.attention(*(x[b] for x in args), scale, window, sinks, None if go64 is None else go64[b],
+                             None if glse64 is None else glse64[b], NAMES[q.dtype]) for b in range(q.shape[0])]
+    for n, x in got.items():
+        compare(f"{where} {n}", x, np.stack([r[n] for r in refs]), np.stack([r[n + "_tol"] for r in refs]))
+    return got
+
+
+# lengths around the tiles (32 queries or keys, 64 keys, 128 rows), windows around them
+@pytest.mark.parametrize("length,window,sinks", [
+    (1, None, 0), (2, 1, 0), (5, 2, 1), (31, 7, 2), (32, 32, 0), (33, 16, 40), (64, None, 0), (65, 64, 1), (127, 33, 4),
+    (128, 128, 4), (130, 1, 3), (200, 100, 70), (257, 64, 0), (300, 299, 5), (321, 1000, 4)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_lengths_windows_and_sinks(length, window, sinks, dtype):
+    x = make(2, length, length, 4, 2, 64, dtype, length)
+    check("lengths", *x, 64 ** -0.5, window, sinks)
+
+
+@pytest.mark.parametrize("hq,hk", [(1, 1), (3, 3), (2, 1), (6, 2), (7, 1), (10, 2), (8, 1), (24, 2), (40, 1), (64, 1)])
+def test_head_groups(hq, hk):
+    """Groups that divide the tiles' rows, do not, and exceed them."""
+    x = make(1, 150, 150, hq, hk, 128, torch.bfloat16, hq)
+    check("groups", *x, 128 ** -0.5, 60, 3)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_widths_and_types(d, dtype):
+    x = make(1, 203, 203, 6, 2, d, dtype, d)
+    check("widths", *x, d ** -0.5, 90, 5)
+    check("widths, no window", *x, d ** -0.5)
+
+
+@pytest.mark.parametrize("d", [1, 40, 80, 200])
+def test_padded_widths(d):
+    x = make(1, 70, 70, 4, 2, d, torch.bfloat16, d)
+    check("padded", *x, max(d, 4) ** -0.5, 20, 2)
+
+
+@pytest.mark.parametrize("tq,tk", [(1, 200), (5, 133), (64, 300), (100, 101), (90, 40), (3, 0), (130, 1)])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (50, 4)])
+def test_queries_and_keys_of_different_lengths(tq, tk, window, sinks):
+    """Continued prompts, and queries before the first key, which see nothing."""
+    x = make(2, tq, tk, 4, 2, 64, torch.bfloat16, tq)
+    got = check("different", *x, 0.125, window, sinks)
+    if tk < tq:
+        assert torch.equal(got["o"][:, : tq - tk], torch.zeros_like(got["o"][:, : tq - tk]))
+        assert torch.equal(got["dq"][:, : tq - tk], torch.zeros_like(got["dq"][:, : tq - tk]))
+
+
+@pytest.mark.parametrize("dtype,d", [(torch.bfloat16, 128), (torch.float16, 64), (torch.float32, 64)])
+def test_packed_sequences(dtype, d):
+    """Uneven sequences with empty ones, tokens past the last boundary, sinks beyond the window."""
+    lengths = [1, 0, 77, 200, 0, 3, 130]
+    cu = torch.tensor(np.cumsum([0] + lengths), dtype=torch.int32, device=DEV)
+    x = make(1, sum(lengths) + 19, sum(lengths) + 19, 6, 2, d, dtype, 3)
+    check("packed", *x, d ** -0.5, 40, 4, cu)
+    check("packed, no window", *x, d ** -0.5, None, 0, cu)
+
+
+def test_packed_queries_and_keys():
+    """Packed continuations: each sequence's queries against more (or fewer) keys."""
+    nq, nk = [5, 64, 0, 40, 9], [70, 64, 12, 10, 0]
+    cq, ck = (torch.tensor(np.cumsum([0] + n), dtype=torch.int32, device=DEV) for n in (nq, nk))
+    x = make(1, sum(nq), sum(nk) + 6, 4, 2, 64, torch.bfloat16, 4)
+    check("packed continuations", *x, 0.125, 30, 2, cq, ck)
+    check("packed continuations, no window", *x, 0.125, None, 0, cq, ck)
+
+
+def test_many_short_sequences_equal_the_batched_call():
+    """300 packed sequences of 9 tokens are the batched call, bit for bit."""
+    q, k, v, go, _ = make(300, 9, 9, 4, 2, 64, torch.bfloat16, 5)
+    cu = torch.arange(301, dtype=torch.int32, device=DEV) * 9
+    with torch.no_grad():
+        o = at.window_attention(q, k, v, 0.125, 4, 1)
+        flat = at.window_attention(*(x.reshape(1, 2700, -1, 64) for x in (q, k, v)), 0.125, 4, 1, cu)
+    assert torch.equal(o.view(-1), flat.view(-1))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_long_walks_are_split(dtype):
+    """One key head and no window: a key tile's queries are walked in parts; with
+    sinks: their later queries in parts of their own."""
+    x = make(1, 1500, 1500, 3, 1, 64, dtype, 6)
+    check("split", *x, 0.125)
+    check("split, sinks", *x, 0.125, 100, 33)
+
+
+def test_strided_inputs():
+    """q, k and v cut out of one projection, heads before tokens, and odd offsets (copied)."""
+    torch.manual_seed(7)
+    z = torch.randn(2, 100, (4 + 2 + 2) * 64, device=DEV).to(torch.bfloat16)
+    q, k, v = (x.view(2, 100, -1, 64) for x in z.split([256, 128, 128], -1))
+    _, _, _, go, glse = make(2, 100, 100, 4, 2, 64, torch.bfloat16, 7)
+    assert not q.is_contiguous()
+    check("projection", q, k, v, go, glse, 0.125, 30, 2)
+    t = [x.transpose(1, 2).contiguous().transpose(1, 2) for x in (q, k, v)]
+    check("heads first", *t, go, glse, 0.125, 30, 2)
+    flat = torch.randn(2 * 100 * 128 + 1, device=DEV).to(torch.bfloat16)[1:].view(2, 100, 2, 64)
+    check("odd offset", q, flat, v, go, glse, 0.125, 30, 2)
+
+
+def test_broadcast_inputs():
+    """Keys and values shared by the batch: the gradient is the sum over it."""
+    q, k, v, go, glse = make(3, 70, 70, 4, 2, 64, torch.float32, 8)
+    k1, v1 = k[:1].detach().requires_grad_(True), v[:1].detach().requires_grad_(True)
+    o = at.window_attention(q, k1.expand(3, -1, -1, -1), v1.expand(3, -1, -1, -1), 0.125, 20, 1)
+    dk, dv = torch.autograd.grad(o, (k1, v1), go)
+    parts = [at.window_attention_bwd(q[b:b + 1], k[:1], v[:1], *at.window_attention_fwd(
+        q[b:b + 1], k[:1], v[:1], 0.125, 20, 1), go[b:b + 1], 0.125, 20, 1) for b in range(3)]
+    torch.testing.assert_close(dk, sum(p[1] for p in parts), rtol=1e-5, atol=1e-5)
+    torch.testing.assert_close(dv, sum(p[2] for p in parts), rtol=1e-5, atol=1e-5)
+
+
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 1.5])
+def test_scales(scale):
+    x = make(1, 90, 90, 4, 2, 64, torch.float32, 9)
+    check("scale", *x, scale, 30, 2)
+
+
+@pytest.mark.parametrize("go_scale", [1e-6, 300.0])
+def test_float16_gradients_of_any_size(go_scale):
+    """ds leaves float16's range at both ends unless it is scaled."""
+    x = make(1, 200, 200, 4, 2, 64, torch.float16, 10, go_scale)
+    x[4].zero_()
+    if go_scale < 1:  # (dq itself stays above float16's smallest numbers)
+        x[1] = x[1] * 64
+    check("float16 range", *x, 0.125 / (64 if go_scale < 1 else 1), 100, 2)
+
+
+def test_what_no_query_sees_is_never_used():
+    """NaN and infinite keys and values left of every window, and past the last boundary."""
+    q, k, v, go, glse = make(1, 40, 300, 4, 2, 64, torch.bfloat16, 11)
+    k[:, 3:200], v[:, 3:200] = float("nan"), float("inf")
+    check("unseen", q, k, v, go, glse, 0.125, 50, 3)
+    cu = torch.tensor([0, 100], dtype=torch.int32, device=DEV)
+    q, k, v, go, glse = make(1, 130, 130, 4, 2, 64, torch.bfloat16, 12)
+    k[:, 100:], v[:, 100:] = float("nan"), float("nan")
+    check("past the last boundary", q, k, v, go, glse, 0.125, None, 0, cu)
+
+
+def test_lowest_scores_and_visible_nan():
+    """Scores at the type's lowest value still weigh; a NaN key spoils only rows that see it."""
+    q, k, v, go, glse = make(1, 50, 50, 1, 1, 64, torch.float32, 13)
+    q[0, :, 0, 0], k[0, :, 0, 0] = 1e19, -1e19
+    q[..., 1:] = 0
+    with torch.no_grad():
+        o, lse = at.window_attention(q, k, v, 1.0, return_lse=True)
+    mean = torch.cumsum(v.double(), 1) / torch.arange(1, 51, device=DEV, dtype=torch.float64).view(1, 50, 1, 1)
+    torch.testing.assert_close(o.double(), mean, rtol=1e-5, atol=1e-6)
+    assert torch.isfinite(lse).all()
+    q, k, v, *_ = make(1, 100, 100, 2, 1, 64, torch.bfloat16, 14)
+    k[0, 70, 0, 5] = float("nan")
+    with torch.no_grad():
+        o = at.window_attention(q, k, v, 0.125, 20, 0)
+    bad = torch.isnan(o).all(-1)[0, :, 0]
+    assert bad[70:90].all() and not bad[:70].any() and not bad[90:].any()
+
+
+def test_runs_are_equal_and_follow_the_stream():
+    """Equal inputs give equal bits, on another stream too."""
+    q, k, v, go, _ = make(2, 700, 700, 8, 2, 128, torch.bfloat16, 15)
+    o, lse = at.window_attention_fwd(q, k, v, 0.09, 200, 4)
+    g = at.window_attention_bwd(q, k, v, o, lse, go, 0.09, 200, 4)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        o2, lse2 = at.window_attention_fwd(q, k, v, 0.09, 200, 4)
+        g2 = at.window_attention_bwd(q, k, v, o2, lse2, go, 0.09, 200, 4)
+    torch.cuda.current_stream().wait_stream(side)
+    for a, b in zip((o, lse, *g), (o2, lse2, *g2)):
+        assert torch.equal(a, b)
+
+
+def test_gradients_against_differences():
+    """Central differences of the device's own forward, float32, along random directions."""
+    q, k, v, go, _ = make(1, 90, 90, 4, 2, 64, torch.float32, 16)
+    leaves = [x.detach().requires_grad_(True) for x in (q, k, v)]
+    o = at.window_attention(*leaves, 0.125, 30, 2)
+    grads = torch.autograd.grad(o, leaves, go)
+    gen = torch.Generator(device=DEV).manual_seed(17)
+    step = 2.0 ** -6
+    for i, g in enumerate(grads):
+        x = torch.randn(g.shape, generator=gen, device=DEV)
+        ends = []
+        for sign in (1, -1):
+            args = [q, k, v]
+            args[i] = args[i] + sign * step * x
+            with torch.no_grad():
+                ends.append((at.window_attention(*args, 0.125, 30, 2).double() * go.double()).sum())
+        diff, want = (ends[0] - ends[1]) / (2 * step), (g.double() * x.double()).sum()
+        # third derivatives times step^2 / 6, and the forward's 2^-22 relative error over the step
+        size = (o.detach().double().abs() * go.double().abs()).sum()
+        assert abs(diff - want) <= 2e-4 * g.double().norm() * x.double().norm() + size * 2.0 ** -22 / step
+
+
+def test_compiled_ops_pass_the_opcheck():
+    q, k, v, *_ = make(1, 20, 20, 2, 1, 64, torch.float32, 18)
+    args = tuple(x.requires_grad_(True) for x in (q, k, v))
+    torch.library.opcheck(at.window_attention_op, (*args, 0.125, 8, 1, None, None),
+                          test_utils=("test_schema", "test_faketensor", "test_autograd_registration"))
