@@ -10,20 +10,20 @@ from tests import test_gpu_window_attention as window
 pytestmark = pytest.mark.gpu
 
 CASES = {
-    "lengths": lambda: window.test_lengths_windows_and_sinks(torch.bfloat16, 200, 100, 70),
+    "lengths": lambda: window.test_lengths_windows_and_sinks(200, 100, 70, torch.bfloat16),
     "groups": lambda: window.test_head_groups(7, 1),
     "groups beyond a tile": lambda: window.test_head_groups(40, 1),
-    "256 wide": lambda: window.test_widths_and_types(torch.bfloat16, 256),
-    "256 wide, float32": lambda: window.test_widths_and_types(torch.float32, 256),
-    "float16": lambda: window.test_widths_and_types(torch.float16, 128),
-    "rows that see nothing": lambda: window.test_queries_and_keys_of_different_lengths(50, 4, 90, 40),
+    "256 wide": lambda: window.test_widths_and_types(256, torch.bfloat16),
+    "256 wide, float32": lambda: window.test_widths_and_types(256, torch.float32),
+    "float16": lambda: window.test_widths_and_types(128, torch.float16),
+    "rows that see nothing": lambda: window.test_queries_and_keys_of_different_lengths(90, 40, 50, 4),
     "packed": lambda: window.test_packed_sequences(torch.bfloat16, 128),
     "packed queries and keys": window.test_packed_queries_and_keys,
     "split walks": lambda: window.test_long_walks_are_split(torch.bfloat16),
     "pages": lambda: paged.test_pages_windows_and_lengths(40, 5, 7),
     "drafts": lambda: paged.test_head_groups_and_drafts(24, 8, 4),
     "joined parts": paged.test_long_contexts_are_split_and_joined,
-    "decode, 256 wide": lambda: paged.test_widths_and_types(torch.bfloat16, 256),
+    "decode, 256 wide": lambda: paged.test_widths_and_types(256, torch.bfloat16),
 }
 
 
