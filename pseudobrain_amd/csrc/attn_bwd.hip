@@ -24,7 +24,7 @@
 namespace pbgdn {
 
 constexpr int QR = 32;            // rows of a query tile of dkdv_kernel
-constexpr int TAIL_TOKENS = 512;  // query tokens of one part of the sinks' walk
+constexpr int TAIL_ROWS = 512;    // rows, or a token's heads if more, of one part of the sinks' walk
 constexpr int MAX_PARTS = 16;     // parts of an ordinary key tile's walk
 
 struct BwdParams {
@@ -41,18 +41,19 @@ struct BwdParams {
   int parts;          // parts of a key tile's walk
   int key_slots;      // key tiles of a (batch, key head)
   int sink_tiles;     // 32-key tiles that hold sinks, 0 when no query is beyond their window
+  int tail_tokens;    // query tokens of one part of the sinks' walk
   int tail_slots;     // parts of the sinks' walk over all sequences, and slot 0 of each: the window's own part
   // query tiles: `heads` heads of `tokens` tokens each, `splits` tiles for the heads of a token
   int heads, tokens, splits;
 };
 
-// Sequence n's slots in the parts of the sinks: the window's part, then one per TAIL_TOKENS tokens.
+// Sequence n's slots in the parts of the sinks: the window's part, then one per tail_tokens tokens.
 __device__ __forceinline__ int tail_start(const BwdParams &p, int seq) {
-  if (!p.f.cu_q) return seq * ((p.f.Tq + TAIL_TOKENS - 1) / TAIL_TOKENS + 1);
-  return boundary(p.f.cu_q, seq, p.f.Tq) / TAIL_TOKENS + 2 * seq;
+  if (!p.f.cu_q) return seq * ((p.f.Tq + p.tail_tokens - 1) / p.tail_tokens + 1);
+  return boundary(p.f.cu_q, seq, p.f.Tq) / p.tail_tokens + 2 * seq;
 }
-inline long tail_slot_count(int Tq, int nseq, bool packed) {
-  return packed ? Tq / TAIL_TOKENS + 2L * nseq : nseq * ((Tq + TAIL_TOKENS - 1L) / TAIL_TOKENS + 1);
+inline long tail_slot_count(int Tq, int nseq, int tokens, bool packed) {
+  return packed ? Tq / tokens + 2L * nseq : nseq * ((Tq + tokens - 1L) / tokens + 1);
 }
 
 // ---------------------------------------------------------------------------
@@ -75,21 +76,35 @@ __global__ void range_zero_kernel(uint32_t *range) {
   if (threadIdx.x < 4) range[threadIdx.x] = 0;
 }
 
-// max |v| over rows of D elements (float16).
+// A workgroup's maximum into a word of `range`: one atomic, and none when the
+// word holds as much (maxima do not depend on their order).
+__device__ __forceinline__ void range_max(float x, uint32_t *word) {
+  __shared__ float top[4];
+  x = wave_max(x);
+  if ((threadIdx.x & 63) == 0) top[threadIdx.x >> 6] = x;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const uint32_t bits = __float_as_uint(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
+    if (bits > __hip_atomic_load(word, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) atomicMax(word, bits);
+  }
+  __syncthreads();
+}
+
+// max |v| over rows of D elements (float16): workgroup `block` of `blocks`.
 template <int D>
-__global__ __launch_bounds__(256) void range_v_kernel(View v, int B, int Tk, int Hk, uint32_t *range) {
+__device__ __forceinline__ void range_v(const BwdParams &p, int block, int blocks) {
   constexpr int LPR = D / 8;  // lanes of a row
-  const long rows = static_cast<long>(B) * Tk * Hk;
+  const View &v = p.f.v;
+  const long rows = static_cast<long>(p.B) * p.f.Tk * p.f.Hk;
   float top = 0.0f;
-  for (long r = blockIdx.x * (256L / LPR) + threadIdx.x / LPR; r < rows; r += gridDim.x * (256L / LPR)) {
-    const long b = r / (static_cast<long>(Tk) * Hk), t = r / Hk % Tk, h = r % Hk;
-    const half8_t x = *reinterpret_cast<const half8_t *>(v.base + b * v.batch + t * v.token + h * v.head +
-                                                         (threadIdx.x % LPR) * 16);
+  for (long r = block * (256L / LPR) + threadIdx.x / LPR; r < rows; r += blocks * (256L / LPR)) {
+    const long bt = r / p.f.Hk, b = bt / p.f.Tk;
+    const half8_t x = *reinterpret_cast<const half8_t *>(
+        v.base + b * v.batch + (bt - b * p.f.Tk) * v.token + (r - bt * p.f.Hk) * v.head + (threadIdx.x % LPR) * 16);
 #pragma unroll
     for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(static_cast<float>(x[i])));
   }
-  top = wave_max(top);
-  if ((threadIdx.x & 63) == 0) atomicMax(range + 1, __float_as_uint(top));
+  range_max(top, p.range + 1);
 }
 
 template <int DT, int D>
@@ -97,9 +112,16 @@ __global__ __launch_bounds__(256) void stat_kernel(const BwdParams p) {
   using E = Elem<DT>;
   constexpr int PER = 16 / E::BYTES, LPR = D / PER < 64 ? D / PER : 64, RPB = 256 / LPR;  // lanes a row, rows a block
   constexpr int UNITS = D / PER / LPR;
+  const int blocks = DT == PBGDN_F16 ? gridDim.x * 3 / 4 : gridDim.x;  // float16: the last quarter reads v
+  if constexpr (DT == PBGDN_F16) {
+    if (blockIdx.x >= blocks) {
+      range_v<D>(p, blockIdx.x - blocks, gridDim.x - blocks);
+      return;
+    }
+  }
   const long rows = static_cast<long>(p.B) * p.f.Tq * p.f.Hq;
   float top_do = 0.0f, top_delta = 0.0f;
-  for (long r = blockIdx.x * static_cast<long>(RPB) + threadIdx.x / LPR; r < rows; r += gridDim.x * static_cast<long>(RPB)) {
+  for (long r = blockIdx.x * static_cast<long>(RPB) + threadIdx.x / LPR; r < rows; r += blocks * static_cast<long>(RPB)) {
     float sum = 0.0f;
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) {
@@ -129,12 +151,8 @@ __global__ __launch_bounds__(256) void stat_kernel(const BwdParams p) {
     }
   }
   if constexpr (DT == PBGDN_F16) {
-    top_do = wave_max(top_do);
-    top_delta = wave_max(top_delta);
-    if ((threadIdx.x & 63) == 0) {
-      atomicMax(p.range, __float_as_uint(top_do));
-      atomicMax(p.range + 2, __float_as_uint(top_delta));
-    }
+    range_max(top_do, p.range);
+    range_max(top_delta, p.range + 2);
   }
 }
 
@@ -165,9 +183,9 @@ struct Dkdv {
   using L = Tile<DT, D>;
   static constexpr int BN = 32 * NW, TILE = QR * L::ROW, STAT = QR * 8, BUF = 2 * TILE + STAT, LDS = 2 * BUF;
   static constexpr int LOADS = QR / L::PER_DMA;  // of one tensor, all waves
-  // float32 rows of 256: K and V rows are read from LDS instead of registers
-  static constexpr bool HELD = L::STEPS <= 32;
-  static constexpr int KV = HELD ? 0 : 2 * BN * L::ROW, BUFS = HELD ? 2 : 1;
+  // wide rows: K and V rows are read from LDS, registers hold the sums alone
+  static constexpr bool HELD = D < 256;
+  static constexpr int KV = HELD ? 0 : 2 * BN * L::ROW, BUFS = KV + 2 * BUF <= 160 * 1024 ? 2 : 1;
   static constexpr int BYTES = KV + BUFS * BUF;
 };
 
@@ -231,9 +249,10 @@ __global__ __launch_bounds__(NW * 64, WAVES) void dkdv_kernel(const BwdParams p)
   if constexpr (TAIL) {
     t0 = j0 + f.window - off;  // the first beyond the window of the tile's first key
     t0 = t0 > 0 ? t0 : 0;
-    t0 = t0 > part * TAIL_TOKENS ? t0 : part * TAIL_TOKENS;
-    t1 = (part + 1) * TAIL_TOKENS < sq.nq ? (part + 1) * TAIL_TOKENS : sq.nq;
-    if (part * TAIL_TOKENS >= sq.nq) return;
+    const int from = part * p.tail_tokens;
+    if (from >= sq.nq) return;
+    t0 = t0 > from ? t0 : from;
+    t1 = sq.nq - from > p.tail_tokens ? from + p.tail_tokens : sq.nq;
   } else {
     const int jl = (j0 + K::BN < sq.nk ? j0 + K::BN : sq.nk) - 1;
     t0 = j0 - off > 0 ? j0 - off : 0;
@@ -255,7 +274,7 @@ __global__ __launch_bounds__(NW * 64, WAVES) void dkdv_kernel(const BwdParams p)
   const unsigned char *vrow = f.v.base + b * f.v.batch + hk * f.v.head + (sq.k0 + kc) * f.v.token;
   v4u32_t kf[K::HELD ? S : 1], vf[K::HELD ? S : 1];
   unsigned char *const kl = lds + wave * 32 * L::ROW, *const vl = kl + K::BN * L::ROW;
-  const uint32_t rbase = L::rows_base(n, h), cbase = L::cols_base(lane);
+  uint32_t rbase = L::rows_base(n, h), cbase = L::cols_base(lane);
 #pragma unroll
   for (int s = 0; s < S; ++s) {
     const v4u32_t x = *reinterpret_cast<const v4u32_t *>(krow + (2 * s + h) * 16);
@@ -269,8 +288,6 @@ __global__ __launch_bounds__(NW * 64, WAVES) void dkdv_kernel(const BwdParams p)
       *reinterpret_cast<v4u32_t *>(vl + at) = y;
     }
   }
-  const auto k_unit = [&](int s) { return K::HELD ? kf[K::HELD ? s : 0] : L::rows(kl, rbase, 0, s); };
-  const auto v_unit = [&](int s) { return K::HELD ? vf[K::HELD ? s : 0] : L::rows(vl, rbase, 0, s); };
 
   float16_t dk[MB], dv[MB];
 #pragma unroll
@@ -284,7 +301,9 @@ __global__ __launch_bounds__(NW * 64, WAVES) void dkdv_kernel(const BwdParams p)
   const long g_token = static_cast<long>(f.Hq) * L::ROW;
   const float2 *sb = p.stat + ((static_cast<long>(b) * f.Hk + hk) * f.Tq + sq.q0) * G;
   unsigned char *const bufs = lds + K::KV;
-  const auto stage = [&](int i) {
+  const uint32_t inv = 65536 / p.heads + 1;  // row / heads = row inv >> 16 for rows below 32
+  const auto stage = [&](int i) __attribute__((always_inline)) {
+    const int lane = opaque(threadIdx.x & 63);
     const int group = p.splits == 1 ? i : i / p.splits, split = p.splits == 1 ? 0 : i % p.splits;
     const int t = t0 + group * p.tokens, g0 = split * QR;
     const int tn = t1 - t < p.tokens ? t1 - t : p.tokens, hn = G - g0 < p.heads ? G - g0 : p.heads;
@@ -296,7 +315,7 @@ __global__ __launch_bounds__(NW * 64, WAVES) void dkdv_kernel(const BwdParams p)
     for (int w = 0; w < (K::LOADS + NW - 1) / NW; ++w) {
       const int inst = wave + NW * w;
       const int row = inst * L::PER_DMA + lane / L::UNITS;
-      const int tt = row / p.heads, gg = row - tt * p.heads;
+      const int tt = static_cast<int>((row * inv) >> 16), gg = row - tt * p.heads;
       const uint32_t unit = ((lane % L::UNITS) ^ L::swz(row)) * 16;
       const bool in = tt < tn && gg < hn;
       dma(dq_, in ? tt * static_cast<uint32_t>(f.q.token) + gg * static_cast<uint32_t>(f.q.head) + unit : OUT_OF_RANGE,
@@ -309,9 +328,24 @@ __global__ __launch_bounds__(NW * 64, WAVES) void dkdv_kernel(const BwdParams p)
     }
   };
 
+  // Each wave computes with the tiles [lead, mine) whose queries see any of its
+  // keys, in a loop without a way around the products (around one, the compiler
+  // moves every accumulator between register files), and keeps step with the
+  // others' staging before and after.
   const int w_lo = j0 + wave * 32, w_hi = w_lo + 31;
+  int lead = 0, mine = tiles;
+  if constexpr (TAIL) {
+    if (w_lo >= f.sinks) mine = 0;
+  } else {
+    const int before = w_lo - off - t0, after = w_hi - t0 - off;  // tokens before the first that sees w_lo
+    lead = before > 0 ? before / p.tokens * p.splits : 0;
+    if (after < t1 - t0 - f.window) {  // tokens from after + window on see none
+      const int n = (after + f.window + p.tokens - 1) / p.tokens * p.splits;
+      mine = n < 0 ? 0 : n < tiles ? n : tiles;
+    }
+  }
   if (tiles > 0 && K::BUFS == 2) stage(0);
-  for (int i = 0; i < tiles; ++i) {
+  const auto advance = [&](int i) __attribute__((always_inline)) {
     if constexpr (K::BUFS == 2) {
       wait_dma();
       block_sync();
@@ -322,27 +356,28 @@ __global__ __launch_bounds__(NW * 64, WAVES) void dkdv_kernel(const BwdParams p)
       wait_dma();
       block_sync();
     }
+  };
+  int i = 0;
+  for (; i < lead && i < tiles; ++i) advance(i);
+  for (; i < mine; ++i) {
+    advance(i);
     const unsigned char *qt = bufs + (K::BUFS == 2 ? (i & 1) * K::BUF : 0), *gt = qt + K::TILE;
     const float4_t *st = reinterpret_cast<const float4_t *>(qt + 2 * K::TILE);
     const int tok = t0 + (p.splits == 1 ? i : i / p.splits) * p.tokens;
     const int p_lo = tok + off, p_hi = (tok + p.tokens < t1 ? tok + p.tokens : t1) - 1 + off;
-    bool whole, none;
-    if constexpr (TAIL) {
-      whole = w_hi < f.sinks && w_hi <= p_lo - f.window;
-      none = w_lo >= f.sinks || w_lo > p_hi - f.window;
-    } else {
-      whole = w_hi <= p_lo && w_lo > p_hi - f.window;
-      none = w_lo > p_hi || w_hi <= p_lo - f.window;
-    }
-    if (none) continue;
+    const bool whole = TAIL ? w_hi < f.sinks && w_hi <= p_lo - f.window : w_hi <= p_lo && w_lo > p_hi - f.window;
 
-    float16_t x = zero16(), y = zero16();
-#pragma unroll
-    for (int s = 0; s < S; ++s) x = E::mma(L::rows(qt, rbase, 0, s), k_unit(s), x);
-#pragma unroll
-    for (int s = 0; s < S; ++s) y = E::mma(L::rows(gt, rbase, 0, s), v_unit(s), y);
+    rbase = opaque(rbase);
+    cbase = opaque(cbase);
+    float16_t x, y;
+    if constexpr (K::HELD) {
+      x = L::rows_product(qt, rbase, 0, kf);
+      y = L::rows_product(gt, rbase, 0, vf);
+    } else {
+      x = L::rows_product_lds(qt, kl, rbase);
+      y = L::rows_product_lds(gt, vl, rbase);
+    }
     if (!whole) {
-      const uint32_t inv = 65536 / p.heads + 1;
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         const int pos = p_lo + static_cast<int>((acc_row(e, h) * inv) >> 16);
@@ -364,9 +399,16 @@ __global__ __launch_bounds__(NW * 64, WAVES) void dkdv_kernel(const BwdParams p)
         y[e + r] = w == 0.0f ? 0.0f : w * d;
       }
     }
-    L::cols_product(gt, cbase, 0, L::operand(x), dv);
-    L::cols_product(qt, cbase, 0, L::operand(y), dk);
+    if constexpr (K::HELD) {
+      L::cols_product(gt, cbase, 0, L::operand(x), dv);
+      L::cols_product(qt, cbase, 0, L::operand(y), dk);
+    } else {
+      const typename L::Operand xo = L::operand(x), yo = L::operand(y);
+      L::cols_product_ahead(gt, cbase, xo, dv);
+      L::cols_product_ahead(qt, cbase, yo, dk);
+    }
   }
+  for (; i < tiles; ++i) advance(i);
 
   if (key >= sq.nk) return;
   const float fk = p.scale / range;
@@ -437,7 +479,7 @@ __global__ __launch_bounds__(256) void join_kernel(const BwdParams p, long rows,
       if (f.cu_q) key -= sq.k0;
     }
     const bool inside = key >= 0 && key < sq.nk;
-    const int tails = (sq.nq + TAIL_TOKENS - 1) / TAIL_TOKENS;
+    const int tails = (sq.nq + p.tail_tokens - 1) / p.tail_tokens;
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
       float4_t sum = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -495,19 +537,16 @@ __global__ __launch_bounds__(NW * 64, WAVES) void dq_kernel(const BwdParams p) {
   const long total = static_cast<long>(sq.nq) * G, row0 = static_cast<long>(slot) * F::BM;
   if (slot < 0 || row0 >= total) return;
   const int off = sq.nk - sq.nq;
-  const auto position = [&](long row) { return static_cast<int>((row < total ? row : total - 1) / G) + off; };
+  const auto position = [&](long row) __attribute__((always_inline)) { return static_cast<int>((row < total ? row : total - 1) / G) + off; };
   const KeyRange range = key_range(position(row0), position(row0 + F::BM - 1), f.window, f.sinks);
   const long wrow = row0 + wave * 32;
   const int w_first = position(wrow), w_last = position(wrow + 31);
 
   const unsigned char *kb_ = f.k.base + b * f.k.batch + hk * f.k.head + sq.k0 * f.k.token;
   const unsigned char *vb_ = f.v.base + b * f.v.batch + hk * f.v.head + sq.k0 * f.v.token;
-  using Stage = KeyStage<DT, D, BN, NW>;
+  const KeyStage<DT, D, BN, NW> stage(kb_, f.k.token, vb_, f.v.token, range, wave, lane);
   const int tiles = (range.count + BN - 1) / BN;
-  if (tiles > 0) {
-    Stage::tile(kb_, f.k.token, range, 0, lds, wave, lane);
-    Stage::tile(vb_, f.v.token, range, 0, lds + 2 * F::TILE, wave, lane);
-  }
+  if (tiles > 0) stage.tile(0, lds, wave);
 
   const long row = wrow + n, r = row < total ? row : total - 1;
   const int t = static_cast<int>(r / G), head = hk * G + static_cast<int>(r % G), pos = t + off;
@@ -527,19 +566,18 @@ __global__ __launch_bounds__(NW * 64, WAVES) void dq_kernel(const BwdParams p) {
   for (int m = 0; m < MB; ++m) dq[m] = zero16();
 
   const uint32_t rbase = L::rows_base(n, h), cbase = L::cols_base(lane);
-  for (int it = 0; it < tiles; ++it) {
+  const auto advance = [&](int it) __attribute__((always_inline)) {
     wait_dma();
     block_sync();
+    if (it + 1 < tiles) stage.tile(it + 1, lds + ((it + 1) & 1) * F::TILE, wave);
+  };
+  const int mine = wave_tiles(range, tiles, w_last, BN);
+  int it = 0;
+  for (; it < mine; ++it) {
+    advance(it);
     const unsigned char *kt = lds + (it & 1) * F::TILE, *vt = kt + 2 * F::TILE;
-    if (it + 1 < tiles) {
-      unsigned char *next = lds + ((it + 1) & 1) * F::TILE;
-      Stage::tile(kb_, f.k.token, range, (it + 1) * BN, next, wave, lane);
-      Stage::tile(vb_, f.v.token, range, (it + 1) * BN, next + 2 * F::TILE, wave, lane);
-    }
     const int u0 = it * BN;
-    const int first = u0 < range.sinks ? u0 : u0 + range.delta, last = u0 + BN - 1 + range.delta;
-    const bool whole = u0 >= range.sinks && last <= w_first && first > w_last - f.window;
-    if (first > w_last) continue;
+    const bool whole = whole_tile(range, u0, BN, w_first, w_last, f.window);
 #pragma unroll
     for (int kb = 0; kb < BN / 32; ++kb) {
       float16_t x = L::rows_product(kt, rbase, 32 * kb, qf), y = L::rows_product(vt, rbase, 32 * kb, gf);
@@ -560,6 +598,7 @@ __global__ __launch_bounds__(NW * 64, WAVES) void dq_kernel(const BwdParams p) {
       L::cols_product(kt, cbase, 32 * kb, L::operand(x), dq);
     }
   }
+  for (; it < tiles; ++it) advance(it);
   if (row < total) store_row<DT, D>(static_cast<unsigned char *>(p.dq) + out * L::ROW, dq, h, p.scale / scale16);
 }
 
@@ -593,18 +632,14 @@ static int launch_bwd(BwdParams &p, hipStream_t stream) {
   const int nb = f.cu_q ? 1 : p.B;
   DeviceShape shape;
   if (!device_shape(shape)) return PBGDN_ERR_LAUNCH;
-  if constexpr (DT == PBGDN_F16) {
-    hipLaunchKernelGGL(range_zero_kernel, dim3(1), dim3(64), 0, stream, p.range);
-    if (f.Tk > 0)
-      hipLaunchKernelGGL(range_v_kernel<D>, dim3(shape.cus * 4), dim3(256), 0, stream, f.v, p.B, f.Tk, f.Hk, p.range);
-  }
+  if constexpr (DT == PBGDN_F16) hipLaunchKernelGGL(range_zero_kernel, dim3(1), dim3(64), 0, stream, p.range);
   hipLaunchKernelGGL((stat_kernel<DT, D>), dim3(shape.cus * 8), dim3(256), 0, stream, p);
 
   constexpr int NW = dkdv_waves<DT, D>(), BN = 32 * NW;
   if (f.Tk > 0) {
     {
       using K = Dkdv<DT, D, NW>;
-      constexpr int W = 1;
+      constexpr int W = DT != PBGDN_F32 && D <= 128 ? 2 : 1;
       static std::atomic<bool> flags[MAX_DEVICES];
       const auto kernel = dkdv_kernel<DT, D, NW, false, W>;
       if (!smem_configured(reinterpret_cast<const void *>(kernel), K::BYTES, flags)) return PBGDN_ERR_LAUNCH;
@@ -617,7 +652,7 @@ static int launch_bwd(BwdParams &p, hipStream_t stream) {
     if (p.sink_tiles) {
       using K = Dkdv<DT, D, 1>;
       static std::atomic<bool> flags[MAX_DEVICES];
-      const auto kernel = dkdv_kernel<DT, D, 1, true, 1>;
+      const auto kernel = dkdv_kernel<DT, D, 1, true, DT != PBGDN_F32 && D <= 128 ? 2 : 1>;
       if (!smem_configured(reinterpret_cast<const void *>(kernel), K::BYTES, flags)) return PBGDN_ERR_LAUNCH;
       const long blocks = static_cast<long>(p.tail_slots) * f.Hk * p.sink_tiles;
       if (blocks > 0x7fffffffL) return PBGDN_ERR_UNSUPPORTED;
@@ -650,7 +685,7 @@ static int launch_bwd(BwdParams &p, hipStream_t stream) {
 // The workspace: statistics, the float16 range, the parts.
 struct Plan {
   size_t stat, range, part, tail, bytes;
-  int parts, sink_tiles, tail_slots;
+  int parts, sink_tiles, tail_tokens, tail_slots;
 };
 static int key_tile(int dtype, int D) {
   return 32 * (dtype == PBGDN_F32 ? (D == 256 ? 1 : 2) : D == 256 ? 2 : 4);
@@ -660,7 +695,8 @@ static bool plan(Plan &w, const WindowParams &f, int dtype, int B, int D) {
   if (!device_shape(shape)) shape.cus = 256;  // sizes are asked for without a device too
   w.parts = walk_parts(f, B, key_tile(dtype, D), shape.cus);
   w.sink_tiles = sink_tiles(f);
-  const long slots = w.sink_tiles ? tail_slot_count(f.Tq, f.nseq, f.cu_q != nullptr) : 0;
+  w.tail_tokens = (TAIL_ROWS + f.group - 1) / f.group;
+  const long slots = w.sink_tiles ? tail_slot_count(f.Tq, f.nseq, w.tail_tokens, f.cu_q != nullptr) : 0;
   if (slots > 0x7fffffffL) return false;
   w.tail_slots = static_cast<int>(slots);
   const auto round = [](size_t x) { return (x + 255) & ~static_cast<size_t>(255); };
@@ -732,6 +768,7 @@ extern "C" int pbattn_window_bwd(const void *q, const void *k, const void *v, in
   p.D = D;
   p.parts = w.parts;
   p.sink_tiles = w.sink_tiles;
+  p.tail_tokens = w.tail_tokens;
   p.tail_slots = w.tail_slots;
   p.heads = p.f.group < QR ? p.f.group : QR;
   p.tokens = QR / p.heads;

@@ -198,7 +198,7 @@ __global__ __launch_bounds__(DEC_WAVES * 64, OCC) void decode_kernel(const Decod
   const unsigned char *kbase = p.k + hk * p.head, *vbase = p.v + hk * p.head;
   const int32_t *table = p.table + static_cast<long>(b) * p.max_pages;
   // the cache row of key `lane & 31` of a block, -1 where there is none
-  const auto lookup = [&](int blk) {
+  const auto lookup = [&](int blk) __attribute__((always_inline)) {
     const int u = blk * DEC_KEYS + (lane & 31);
     if (u >= range.count) return -1;
     const int j = u < range.sinks ? u : u + range.delta;

@@ -15,6 +15,8 @@
 
 namespace pbgdn {
 
+constexpr float LAG = 8.0f;  // weights stay below 2^8
+
 template <int DT, int D, int CB, int NW, int BN>
 struct Fwd {
   using L = Tile<DT, D>;
@@ -50,19 +52,16 @@ __global__ __launch_bounds__(NW * 64, WAVES) void window_fwd_kernel(const Window
 
   // positions of the workgroup's first and last row, and of this wave's
   const int off = sq.nk - sq.nq;
-  const auto position = [&](long row) { return static_cast<int>((row < total ? row : total - 1) / G) + off; };
+  const auto position = [&](long row) __attribute__((always_inline)) { return static_cast<int>((row < total ? row : total - 1) / G) + off; };
   const KeyRange range = key_range(position(row0), position(row0 + F::BM - 1), p.window, p.sinks);
   const long wrow = row0 + wave * 32 * CB;
   const int w_first = position(wrow), w_last = position(wrow + 32 * CB - 1);
 
   const unsigned char *kb_ = p.k.base + b * p.k.batch + hk * p.k.head + sq.k0 * p.k.token;
   const unsigned char *vb_ = p.v.base + b * p.v.batch + hk * p.v.head + sq.k0 * p.v.token;
-  using Stage = KeyStage<DT, D, BN, NW>;
+  const KeyStage<DT, D, BN, NW> stage(kb_, p.k.token, vb_, p.v.token, range, wave, lane);
   const int tiles = (range.count + BN - 1) / BN;
-  if (tiles > 0) {
-    Stage::tile(kb_, p.k.token, range, 0, lds, wave, lane);
-    Stage::tile(vb_, p.v.token, range, 0, lds + 2 * F::TILE, wave, lane);
-  }
+  if (tiles > 0) stage.tile(0, lds, wave);
 
   // this lane's columns: their query rows
   v4u32_t qf[CB][S];
@@ -90,20 +89,18 @@ __global__ __launch_bounds__(NW * 64, WAVES) void window_fwd_kernel(const Window
   }
 
   const uint32_t rbase = L::rows_base(n, h), cbase = L::cols_base(lane);
-  for (int it = 0; it < tiles; ++it) {
+  const auto advance = [&](int it) __attribute__((always_inline)) {
     wait_dma();
     block_sync();
+    if (it + 1 < tiles) stage.tile(it + 1, lds + ((it + 1) & 1) * F::TILE, wave);
+  };
+  const int mine = wave_tiles(range, tiles, w_last, BN);
+  int it = 0;
+  for (; it < mine; ++it) {
+    advance(it);
     const unsigned char *kt = lds + (it & 1) * F::TILE, *vt = kt + 2 * F::TILE;
-    if (it + 1 < tiles) {
-      unsigned char *next = lds + ((it + 1) & 1) * F::TILE;
-      Stage::tile(kb_, p.k.token, range, (it + 1) * BN, next, wave, lane);
-      Stage::tile(vb_, p.v.token, range, (it + 1) * BN, next + 2 * F::TILE, wave, lane);
-    }
-    // the tile's keys: all seen by all of the wave's rows, or masked
     const int u0 = it * BN;
-    const int first = u0 < range.sinks ? u0 : u0 + range.delta, last = u0 + BN - 1 + range.delta;
-    const bool whole = u0 >= range.sinks && last <= w_first && first > w_last - p.window;
-    if (first > w_last) continue;
+    const bool whole = whole_tile(range, u0, BN, w_first, w_last, p.window);
 
     float16_t sc[KB][CB];
 #pragma unroll
@@ -136,9 +133,21 @@ __global__ __launch_bounds__(NW * 64, WAVES) void window_fwd_kernel(const Window
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
         for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[kb][cb][i]);
-      const float top = fmaxf(m[cb], max_xor32(mx)), base = top == -INFINITY ? 0.0f : top, at = base * p.c;
-      const float alpha = __builtin_amdgcn_exp2f((m[cb] - base) * p.c);
-      m[cb] = top;
+      // The reference the weights are taken against moves only when a score
+      // passes it by more than LAG powers of two, so most tiles leave the sums
+      // as they are.
+      mx = max_xor32(mx);
+      if (__any((mx - m[cb]) * p.c > LAG)) {
+        const float top = fmaxf(m[cb], mx);
+        const float alpha = __builtin_amdgcn_exp2f((m[cb] - (top == -INFINITY ? 0.0f : top)) * p.c);
+        m[cb] = top;
+        l[cb] *= alpha;
+#pragma unroll
+        for (int i = 0; i < MB; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[cb][i][e] *= alpha;
+      }
+      const float base = m[cb] == -INFINITY ? 0.0f : m[cb], at = base * p.c;
       float sum = 0.0f;
       if (__any(fabsf(at) > EXACT_SCORES)) {
 #pragma unroll
@@ -156,15 +165,12 @@ __global__ __launch_bounds__(NW * 64, WAVES) void window_fwd_kernel(const Window
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
         for (int i = 0; i < 16; ++i) sum += sc[kb][cb][i];
-      l[cb] = l[cb] * alpha + sum;
-#pragma unroll
-      for (int i = 0; i < MB; ++i)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) o[cb][i][e] *= alpha;
+      l[cb] += sum;
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) L::cols_product(vt, cbase, 32 * kb, L::operand(sc[kb][cb]), o[cb]);
     }
   }
+  for (; it < tiles; ++it) advance(it);
 
 #pragma unroll
   for (int cb = 0; cb < CB; ++cb) {
@@ -209,7 +215,7 @@ static int dispatch_fwd(WindowParams &p, int B, int D, hipStream_t stream) {
   switch (D) {
     case 64: return launch_fwd<DT, 64, 1, 4, 64, 2>(p, B, stream);
     case 128: return launch_fwd<DT, 128, 1, 4, wide ? 32 : 64, wide ? 1 : 2>(p, B, stream);
-    case 256: return launch_fwd<DT, 256, 1, 4, 32, 1>(p, B, stream);
+    case 256: return launch_fwd<DT, 256, 1, 4, 32, wide ? 1 : 2>(p, B, stream);
     default: return PBGDN_ERR_UNSUPPORTED;
   }
 }

@@ -167,6 +167,32 @@ struct Tile {
     return x;
   }
 
+  // The same with both sides in LDS, GROUP steps read ahead of the ones that are
+  // multiplied: bounds the registers that reads in flight take.
+  static constexpr int GROUP = 4;
+  __device__ static __forceinline__ float16_t rows_product_lds(const unsigned char *tile, const unsigned char *other,
+                                                               uint32_t base) {
+    v4u32_t a[2][GROUP], b[2][GROUP];
+    float16_t x = zero16();
+#pragma unroll
+    for (int s = 0; s < STEPS + GROUP; s += GROUP) {
+      if (s < STEPS) {
+#pragma unroll
+        for (int i = 0; i < GROUP; ++i) {
+          a[s / GROUP % 2][i] = rows(tile, base, 0, s + i);
+          b[s / GROUP % 2][i] = rows(other, base, 0, s + i);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if (s > 0) {
+#pragma unroll
+        for (int i = 0; i < GROUP; ++i) x = E::mma(a[(s / GROUP + 1) % 2][i], b[(s / GROUP + 1) % 2][i], x);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    return x;
+  }
+
   // X as the B operand of a cols product.
   struct Operand {
     v4u32_t w[E::BYTES == 2 ? 2 : 4];
@@ -183,6 +209,39 @@ struct Tile {
       for (int i = 0; i < 16; ++i) o.w[i / 4][i % 4] = __float_as_uint(x[i]);
     }
     return o;
+  }
+  // z[m] += columns 32 m .. of M[r0 .. r0 + 31] times X, every m, GROUP reads ahead.
+  __device__ static __forceinline__ void cols_product_ahead(const unsigned char *tile, uint32_t base, const Operand &x,
+                                                            float16_t *z) {
+    constexpr int N = (E::BYTES == 2 ? 2 : 16) * MB;
+    v4u32_t a[2][GROUP];
+#pragma unroll
+    for (int j = 0; j < N + GROUP; j += GROUP) {
+      if (j < N) {
+#pragma unroll
+        for (int i = 0; i < GROUP; ++i) {
+          const int at = (j + i) / MB, m = (j + i) % MB;
+          if constexpr (E::BYTES == 2)
+            a[j / GROUP % 2][i] = cols(tile, base, 0, at, m);
+          else
+            a[j / GROUP % 2][i][0] = __float_as_uint(col1(tile, base, 0, at, m));
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if (j > 0) {
+#pragma unroll
+        for (int i = 0; i < GROUP; ++i) {
+          const int at = (j - GROUP + i) / MB, m = (j - GROUP + i) % MB;
+          const v4u32_t y = a[(j / GROUP + 1) % 2][i];
+          if constexpr (E::BYTES == 2)
+            z[m] = E::mma(y, x.w[at], z[m]);
+          else
+            z[m] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(y[0]), __uint_as_float(x.w[at / 4][at % 4]), z[m],
+                                                        0, 0, 0);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
   }
   // z[m] += columns 32 m .. of M[r0 .. r0 + 31] times X, every m.
   __device__ static __forceinline__ void cols_product(const unsigned char *tile, uint32_t base, int r0,
@@ -215,17 +274,17 @@ __device__ __forceinline__ uint32_t lds_address(const void *p) {
 // From `off` bytes into a buffer resource; what lies outside it arrives as zeros.
 __device__ __forceinline__ void dma(v4u32_t desc, uint32_t off, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(desc)
-               : "memory", "m0");
+               : "memory");
 }
 // 4 bytes per lane, lane l to `lds` + 4 l: for sources aligned to no more.
 __device__ __forceinline__ void dma4(v4u32_t desc, uint32_t off, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(desc)
-               : "memory", "m0");
+               : "memory");
 }
 // From a 64-bit address per lane.
 __device__ __forceinline__ void dma(const void *src, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(src)
-               : "memory", "m0");
+               : "memory");
 }
 __device__ __forceinline__ v4u32_t dma_desc(const void *base, long bytes) {
   const uint64_t a = reinterpret_cast<uint64_t>(base);
@@ -245,6 +304,13 @@ __device__ __forceinline__ float max_xor32(float x) {
   float a = x, b = x;
   swap32(a, b);
   return fmaxf(a, b);
+}
+
+// x, of which the compiler knows nothing more: what is computed from it inside a
+// loop is computed there instead of being kept in registers across it.
+__device__ __forceinline__ uint32_t opaque(uint32_t x) {
+  asm volatile("" : "+v"(x));
+  return x;
 }
 
 // A wave-uniform value in a scalar register.
@@ -321,35 +387,65 @@ __device__ __forceinline__ KeyRange key_range(int p_first, int p_last, int windo
   return r;
 }
 
-// Stages rows u0 .. of a key range into a tile: wave w of NW fills its share.
+// How many of a workgroup's key tiles a wave whose last row stands at w_last
+// looks at: those up to the one that holds the key there. (The rest of the tiles
+// are a loop of their own, in which it only keeps step with the staging: around
+// a way past the products inside one loop, the compiler moves every accumulator
+// between register files.)
+__device__ __forceinline__ int wave_tiles(const KeyRange &r, int tiles, int w_last, int bn) {
+  const int n = w_last < 0 ? 0 : (w_last - r.delta) / bn + 1;
+  return n < tiles ? n : tiles;
+}
+// Every row of the wave sees every key of the tile from u0 on.
+__device__ __forceinline__ bool whole_tile(const KeyRange &r, int u0, int bn, int w_first, int w_last, int window) {
+  return u0 >= r.sinks && u0 + bn - 1 + r.delta <= w_first && u0 + r.delta > w_last - window;
+}
+
+// Stages rows u0 .. of a key range into tiles of K and V: wave w of NW fills its
+// share of the loads, load i rows NW PER_DMA i further on. A load's lane offsets
+// are those of the first, but for the permutation of its units.
 template <int DT, int D, int BN, int NW>
 struct KeyStage {
   using L = Tile<DT, D>;
-  static constexpr int LOADS = BN / L::PER_DMA / NW;
-  static_assert(LOADS * L::PER_DMA * NW == BN, "whole loads");
+  static constexpr int STEP = NW * L::PER_DMA, LOADS = BN / STEP, TILE = BN * L::ROW;
+  static_assert(LOADS * STEP == BN, "whole loads");
+  const unsigned char *k, *v;
+  long k_stride, v_stride;
+  KeyRange range;
+  int row;       // this lane's row of the first load
+  uint32_t unit;  // and its unit
 
-  __device__ static __forceinline__ void tile(const unsigned char *base, long stride, const KeyRange &r, int u0,
-                                              unsigned char *lds, int wave, int lane) {
-    const uint32_t at = uniform(lds_address(lds) + wave * 1024);
-    if (u0 >= r.sinks) {  // one run of keys: a scalar base, fixed lane offsets
-      const int left = r.count - u0, rows = left < BN ? left : BN;
-      const v4u32_t desc = dma_desc(base + (u0 + r.delta) * stride, (rows - 1) * stride + L::ROW);
+  __device__ __forceinline__ KeyStage(const unsigned char *k_, long ks, const unsigned char *v_, long vs,
+                                      const KeyRange &r, int wave, int lane)
+      : k(k_), v(v_), k_stride(ks), v_stride(vs), range(r), row(wave * L::PER_DMA + lane / L::UNITS),
+        unit((lane % L::UNITS) ^ L::swz(row)) {}
+
+  __device__ __forceinline__ void one(const unsigned char *base, long stride, int u0, unsigned char *lds,
+                                      int wave) const {
+    const uint32_t to = uniform(lds_address(lds) + wave * 1024);
+    if (u0 >= range.sinks) {  // one run of keys: a scalar base, fixed lane offsets
+      const int left = range.count - u0, rows = left < BN ? left : BN;
+      const unsigned char *from = base + (u0 + range.delta) * stride;
+      const uint32_t at = static_cast<uint32_t>(row) * static_cast<uint32_t>(stride);
+      const long step = STEP * stride;
 #pragma unroll
-      for (int i = 0; i < LOADS; ++i) {
-        const int row = (wave + NW * i) * L::PER_DMA + lane / L::UNITS;
-        dma(desc, static_cast<uint32_t>(row) * static_cast<uint32_t>(stride) + ((lane % L::UNITS) ^ L::swz(row)) * 16,
-            at + i * NW * 1024);
-      }
+      for (int i = 0; i < LOADS; ++i)
+        dma(dma_desc(from + i * step, (rows - 1) * stride + L::ROW - i * step), at + (unit ^ L::swz(i * STEP % 16)) * 16,
+            to + i * NW * 1024);
     } else {  // sinks and the window's start in one tile; rows past the end repeat the last key
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
-        const int row = (wave + NW * i) * L::PER_DMA + lane / L::UNITS;
-        int u = u0 + row;
-        u = u < r.count ? u : r.count - 1;
-        const long j = u < r.sinks ? u : u + r.delta;
-        dma(base + j * stride + ((lane % L::UNITS) ^ L::swz(row)) * 16, at + i * NW * 1024);
+        int u = u0 + row + i * STEP;
+        u = u < range.count ? u : range.count - 1;
+        const long j = u < range.sinks ? u : u + range.delta;
+        dma(base + j * stride + (unit ^ L::swz(i * STEP % 16)) * 16, to + i * NW * 1024);
       }
     }
+  }
+  // Tile `it` into `buffer`: K, and V two tiles further on.
+  __device__ __forceinline__ void tile(int it, unsigned char *buffer, int wave) const {
+    one(k, k_stride, it * BN, buffer, wave);
+    one(v, v_stride, it * BN, buffer + 2 * TILE, wave);
   }
 };
 
