@@ -25,8 +25,8 @@ only; a missing library or a CPU tensor raises.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
+import functools
 
 import torch
 
@@ -36,12 +36,33 @@ from .gated_deltanet import _aligned, _pad_last, _require_device, _width_at_leas
 ATTENTION_HEAD_DIMS = (64, 128, 256)  # widths the kernels are built for
 MAX_DRAFT = 16                        # query tokens a sequence may have in paged_decode_attention
 _MAX_TOKEN_STRIDE = 1 << 24           # bytes (pbattn_window_fwd)
-_NO_GUARD = contextlib.nullcontext()
 
 
-def _guard(dev: torch.device):
-    """The launch goes to the current device: make it the tensors'."""
-    return _NO_GUARD if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+# What follows from shapes, strides and types alone (checks, stride arrays,
+# workspace sizes) is kept by them: a decode step's calls repeat them, and are
+# short enough that working it out again would be most of their time.
+_plan = functools.lru_cache(maxsize=1024)
+
+
+def _launch(where: str, fn, dev: torch.device, *args) -> None:
+    """fn(*args, stream) on the tensors' device, which need not be the current one."""
+    if torch.cuda.current_device() == dev.index:
+        status = fn(*args, _lib.stream_handle(dev))
+    else:
+        with torch.cuda.device(dev):
+            status = fn(*args, _lib.stream_handle(dev))
+    if status:
+        _lib.check(status, where)
+
+
+def _one_device(*tensors) -> torch.device:
+    """The tensors' device, by _require_device's rules and errors."""
+    first = tensors[0]
+    index = first.get_device()
+    for t in tensors:
+        if t is not None and (index < 0 or t.get_device() != index):
+            return _require_device(*tensors)
+    return first.device
 
 
 def _dtype_code(dtype: torch.dtype) -> int:
@@ -52,40 +73,41 @@ def _dtype_code(dtype: torch.dtype) -> int:
 
 def _window_args(window, sinks) -> tuple[int, int]:
     """(window, 0 for none; sinks) as the C ABI takes them."""
-    if window is not None and int(window) < 1:
+    if window is not None and window < 1:
         raise ValueError(f"window must be at least 1 (None for no window), got {window}")
-    if int(sinks) < 0:
+    if sinks < 0:
         raise ValueError(f"sinks must not be negative, got {sinks}")
-    return (0 if window is None else min(int(window), 2**31 - 1)), min(int(sinks), 2**31 - 1)
+    return (0 if window is None else min(window, 2**31 - 1)), min(sinks, 2**31 - 1)
 
 
-def _strided(x: torch.Tensor) -> torch.Tensor:
-    """x, or a copy, as the kernels read it: a dense last axis, the other
-    strides and the address multiples of 16 bytes."""
-    size = x.element_size()
-    steps = [s for n, s in zip(x.shape[:-1], x.stride()) if n > 1]
-    if (x.shape[-1] > 1 and x.stride(-1) != 1) or any(s * size % 16 for s in steps) or (
-            x.ndim > 2 and x.stride(-3) * size >= _MAX_TOKEN_STRIDE and x.shape[-3] > 1):
-        x = x.contiguous()
-    return _aligned(x, 16)
+def _readable(shape, stride, size: int) -> bool:
+    """The kernels read a tensor of these strides in place: a dense last axis, the
+    other strides multiples of 16 bytes, token rows less than 16 MiB apart."""
+    if shape[-1] > 1 and stride[-1] != 1:
+        return False
+    if len(shape) > 2 and shape[-3] > 1 and stride[-3] * size >= _MAX_TOKEN_STRIDE:
+        return False
+    return all(n <= 1 or st * size % 16 == 0 for n, st in zip(shape[:-1], stride))
 
 
-def _strides(*tensors) -> ctypes.Array:
+def _steps(*views) -> ctypes.Array:
     """Element strides of every axis but the last (0 for axes of one element)."""
-    out = [s if n > 1 else 0 for x in tensors for n, s in zip(x.shape[:-1], x.stride())]
+    out = [st if n > 1 else 0 for shape, stride in views for n, st in zip(shape[:-1], stride)]
     return (ctypes.c_int64 * len(out))(*out)
 
 
 # ----------------------------------------------------------------------------
 # Prefill and training.
 # ----------------------------------------------------------------------------
-def _window_shapes(q, k, v, cu_q, cu_k):
-    """Checked sizes (B, Tq, Tk, Hq, Hk, D) and the number of sequences."""
-    if q.ndim != 4 or k.ndim != 4 or v.shape != k.shape:
+@_plan
+def _window_plan(q, k, v, dtype, cu_q, cu_k, window, sinks):
+    """Checked sizes (B, Tq, Tk, Hq, Hk, D) and number of sequences of a call with
+    q, k, v, boundaries of these shapes, its dtype code, window and sinks."""
+    if len(q) != 4 or len(k) != 4 or v != k:
         raise ValueError("expected q [B,Tq,Hq,D] and k, v [B,Tk,Hk,D] of one shape")
-    batch, tq, hq, d = q.shape
-    tk, hk = k.shape[1], k.shape[2]
-    if k.shape[0] != batch or k.shape[3] != d:
+    batch, tq, hq, d = q
+    tk, hk = k[1], k[2]
+    if k[0] != batch or k[3] != d:
         raise ValueError("k and v must share q's batch axis and head width")
     if hk < 1 or hq < 1 or hq % hk:
         raise ValueError("query heads must be a multiple of the key heads")
@@ -98,18 +120,61 @@ def _window_shapes(q, k, v, cu_q, cu_k):
     else:
         if batch != 1:
             raise ValueError("cu_seqlens needs B == 1 (sequences packed along T)")
-        if cu_q.ndim != 1 or cu_q.numel() < 1:
+        if len(cu_q) != 1 or cu_q[0] < 1:
             raise ValueError("cu_seqlens must be a 1-D tensor [N+1]")
         if cu_k is None and tk != tq:
             raise ValueError("q and k of different lengths need cu_seqlens_k beside cu_seqlens")
-        if cu_k is not None and cu_k.shape != cu_q.shape:
+        if cu_k is not None and cu_k != cu_q:
             raise ValueError("cu_seqlens_k must have cu_seqlens' shape")
-        nseq = cu_q.numel() - 1
-    return (batch, tq, tk, hq, hk, d), nseq
+        nseq = cu_q[0] - 1
+    return ((batch, tq, tk, hq, hk, d), nseq, _dtype_code(dtype), *_window_args(window, sinks))
+
+
+def _shape(x):
+    return None if x is None else x.shape
+
+
+def _window_check(q, k, v, cu_q, cu_k, window, sinks):
+    return _window_plan(q.shape, k.shape, v.shape, q.dtype, _shape(cu_q), _shape(cu_k),
+                        None if window is None else int(window), int(sinks))
+
+
+@_plan
+def _window_steps(q, k, v, size):
+    """The stride array of q, k, v by their (shape, stride), None if one is not readable in place."""
+    return _steps(q, k, v) if all(_readable(*x, size) for x in (q, k, v)) else None
+
+
+def _window_operands(q, k, v):
+    """q, k, v in q's dtype as the kernels read them, and their stride array."""
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        k, v = k.to(q.dtype), v.to(q.dtype)
+    steps = _window_steps((q.shape, q.stride()), (k.shape, k.stride()), (v.shape, v.stride()), q.element_size())
+    if steps is None:
+        q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
+    q, k, v = _aligned(q, 16), _aligned(k, 16), _aligned(v, 16)
+    if steps is None:
+        steps = _steps(*((x.shape, x.stride()) for x in (q, k, v)))
+    return q, k, v, steps
 
 
 def _boundaries(cu):
-    return None if cu is None else cu.to(torch.int32).contiguous()
+    if cu is None or (cu.dtype == torch.int32 and cu.is_contiguous()):
+        return cu
+    return cu.to(torch.int32).contiguous()
+
+
+def _output(out, q):
+    if out is None:
+        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or out.data_ptr() % 16:
+        raise ValueError("out must be a contiguous, 16-byte aligned tensor of q's shape and dtype")
+    return out
+
+
+def _built_width(d: int) -> None:
+    if d not in ATTENTION_HEAD_DIMS:
+        raise ValueError(f"attention kernels are built for head widths {ATTENTION_HEAD_DIMS}")
 
 
 def window_attention_fwd(q, k, v, scale: float, window=None, sinks: int = 0, cu_seqlens=None, cu_seqlens_k=None, *,
@@ -117,29 +182,19 @@ def window_attention_fwd(q, k, v, scale: float, window=None, sinks: int = 0, cu_
     """Launch pbattn_window_fwd at one of the built widths. Returns (o [B,Tq,Hq,D]
     in q's dtype, lse [B,Tq,Hq] float32 or None). k and v are cast to q's dtype;
     `out` may supply o. No backward (window_attention has one)."""
-    (batch, tq, tk, hq, hk, d), nseq = _window_shapes(q, k, v, cu_seqlens, cu_seqlens_k)
-    dev = _require_device(q, k, v, cu_seqlens, cu_seqlens_k)
-    code = _dtype_code(q.dtype)
-    if d not in ATTENTION_HEAD_DIMS:
-        raise ValueError(f"attention kernels are built for head widths {ATTENTION_HEAD_DIMS}")
-    window, sinks = _window_args(window, sinks)
-    q, k, v = _strided(q), _strided(k.to(q.dtype)), _strided(v.to(q.dtype))
+    sizes, nseq, code, window, sinks = _window_check(q, k, v, cu_seqlens, cu_seqlens_k, window, sinks)
+    dev = _one_device(q, k, v, cu_seqlens, cu_seqlens_k)
+    _built_width(sizes[-1])
+    q, k, v, steps = _window_operands(q, k, v)
     cu_q, cu_k = _boundaries(cu_seqlens), _boundaries(cu_seqlens_k)
-    if out is None:
-        out = torch.empty(batch, tq, hq, d, dtype=q.dtype, device=dev)
-    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or out.data_ptr() % 16:
-        raise ValueError("out must be a contiguous, 16-byte aligned tensor of q's shape and dtype")
+    out = _output(out, q)
+    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=dev) if return_lse else None
     if nseq == 0:
         out.zero_()
-    lse = torch.empty(batch, tq, hq, dtype=torch.float32, device=dev) if return_lse else None
-    if nseq == 0 and return_lse:
-        lse.fill_(-torch.inf)
-    with _guard(dev):
-        status = _lib.attn_lib().pbattn_window_fwd(
-            _lib.ptr(q), _lib.ptr(k), _lib.ptr(v), code, _strides(q, k, v), _lib.ptr(cu_q), _lib.ptr(cu_k), nseq,
-            _lib.ptr(out), _lib.ptr(lse), batch, tq, tk, hq, hk, d, float(scale), window, sinks,
-            _lib.stream_handle(dev))
-    _lib.check(status, "pbattn_window_fwd")
+        if return_lse:
+            lse.fill_(-torch.inf)
+    _launch("pbattn_window_fwd", _lib.attn_lib().pbattn_window_fwd, dev, q.data_ptr(), k.data_ptr(), v.data_ptr(), code,
+            steps, _lib.ptr(cu_q), _lib.ptr(cu_k), nseq, out.data_ptr(), _lib.ptr(lse), *sizes, float(scale), window, sinks)
     return out, lse
 
 
@@ -147,37 +202,30 @@ def window_attention_bwd(q, k, v, o, lse, grad_o, scale: float, window=None, sin
                          cu_seqlens_k=None, grad_lse=None):
     """Launch pbattn_window_bwd: (dq, dk, dv) in q's dtype from the forward call's
     inputs and results and the gradients of o and (optionally) lse."""
-    (batch, tq, tk, hq, hk, d), nseq = _window_shapes(q, k, v, cu_seqlens, cu_seqlens_k)
-    dev = _require_device(q, k, v, o, lse, grad_o, grad_lse, cu_seqlens, cu_seqlens_k)
-    code = _dtype_code(q.dtype)
-    if d not in ATTENTION_HEAD_DIMS:
-        raise ValueError(f"attention kernels are built for head widths {ATTENTION_HEAD_DIMS}")
+    sizes, nseq, code, window, sinks = _window_check(q, k, v, cu_seqlens, cu_seqlens_k, window, sinks)
+    dev = _one_device(q, k, v, o, lse, grad_o, grad_lse, cu_seqlens, cu_seqlens_k)
+    _built_width(sizes[-1])
     if o.shape != q.shape or grad_o.shape != q.shape or lse.shape != q.shape[:3] or (
             grad_lse is not None and grad_lse.shape != q.shape[:3]):
         raise ValueError("o and grad_o must have q's shape, lse and grad_lse [B,Tq,Hq]")
-    window, sinks = _window_args(window, sinks)
-    q, k, v = _strided(q), _strided(k.to(q.dtype)), _strided(v.to(q.dtype))
+    q, k, v, steps = _window_operands(q, k, v)
     o, grad_o = (_aligned(x.to(q.dtype).contiguous(), 16) for x in (o, grad_o))
     lse = lse.to(torch.float32).contiguous()
     grad_lse = None if grad_lse is None else grad_lse.to(torch.float32).contiguous()
     cu_q, cu_k = _boundaries(cu_seqlens), _boundaries(cu_seqlens_k)
-    dq = torch.empty(batch, tq, hq, d, dtype=q.dtype, device=dev)
-    dk, dv = (torch.empty(batch, tk, hk, d, dtype=q.dtype, device=dev) for _ in range(2))
-    if nseq == 0 or tq == 0:
+    dq = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    dk, dv = (torch.empty(k.shape, dtype=q.dtype, device=dev) for _ in range(2))
+    if nseq == 0 or sizes[1] == 0:
         for x in (dq, dk, dv):
             x.zero_()
         return dq, dk, dv
-    with _guard(dev):
-        lib = _lib.attn_lib()
-        nbytes = lib.pbattn_window_bwd_workspace_size(batch, tq, tk, hq, hk, d, nseq, code, int(cu_q is not None),
-                                                      window, sinks)
-        workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        status = lib.pbattn_window_bwd(
-            _lib.ptr(q), _lib.ptr(k), _lib.ptr(v), code, _strides(q, k, v), _lib.ptr(cu_q), _lib.ptr(cu_k), nseq,
-            _lib.ptr(o), _lib.ptr(lse), _lib.ptr(grad_o), _lib.ptr(grad_lse), _lib.ptr(dq), _lib.ptr(dk), _lib.ptr(dv),
-            batch, tq, tk, hq, hk, d, float(scale), window, sinks, _lib.ptr(workspace), nbytes,
-            _lib.stream_handle(dev))
-    _lib.check(status, "pbattn_window_bwd")
+    lib = _lib.attn_lib()
+    with torch.cuda.device(dev):  # (the size depends on the device's compute units)
+        nbytes = lib.pbattn_window_bwd_workspace_size(*sizes, nseq, code, int(cu_q is not None), window, sinks)
+    workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    _launch("pbattn_window_bwd", lib.pbattn_window_bwd, dev, q.data_ptr(), k.data_ptr(), v.data_ptr(), code, steps,
+            _lib.ptr(cu_q), _lib.ptr(cu_k), nseq, o.data_ptr(), lse.data_ptr(), grad_o.data_ptr(), _lib.ptr(grad_lse),
+            dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *sizes, float(scale), window, sinks, workspace.data_ptr(), nbytes)
     return dq, dk, dv
 
 
@@ -238,20 +286,16 @@ def window_attention(q, k, v, scale: float, window=None, sinks: int = 0, cu_seql
     in number) packs sequences. Returns o [B,Tq,Hq,D] in q's dtype, with
     return_lse (o, lse [B,Tq,Hq] float32); differentiable in q, k and v, also
     through lse."""
-    shapes, _ = _window_shapes(q, k, v, cu_seqlens, cu_seqlens_k)
-    _require_device(q, k, v, cu_seqlens, cu_seqlens_k)
-    _dtype_code(q.dtype)
-    _window_args(window, sinks)
-    d = shapes[-1]
-    width = _width_at_least(d, ATTENTION_HEAD_DIMS)
-    if width != d:
-        q, k, v = (_pad_last(x, width) for x in (q, k, v))
+    d = _window_check(q, k, v, cu_seqlens, cu_seqlens_k, window, sinks)[0][-1]
+    _one_device(q, k, v, cu_seqlens, cu_seqlens_k)
+    if d not in ATTENTION_HEAD_DIMS:
+        q, k, v = (_pad_last(x, _width_at_least(d, ATTENTION_HEAD_DIMS)) for x in (q, k, v))
     if grad_needed(q, k, v) or torch.compiler.is_compiling():
         window = None if window is None else int(window)
         o, lse = window_attention_op(q, k, v, float(scale), window, int(sinks), cu_seqlens, cu_seqlens_k)
     else:
         o, lse = window_attention_fwd(q, k, v, scale, window, sinks, cu_seqlens, cu_seqlens_k, return_lse=return_lse)
-    if width != d:
+    if d not in ATTENTION_HEAD_DIMS:
         o = o[..., :d].contiguous()
     return (o, lse) if return_lse else o
 
@@ -265,60 +309,71 @@ def _inference_only(where: str, *tensors) -> None:
                            "window_attention, which has one")
 
 
-def _caches(k_cache, v_cache):
-    """Checked caches [pages, page, Hk, D] of equal strides (any axis order with
-    the token rows of a page evenly spaced): (pages, page, Hk, D) and the strides."""
-    if k_cache.ndim != 4 or v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype:
+@_plan
+def _cache_plan(shape, stride, v_shape, v_stride, dtype, v_dtype):
+    """Checked sizes (pages, page, Hk, D) of caches of these shapes and strides, the
+    stride array and the dtype code."""
+    if len(shape) != 4 or v_shape != shape or v_dtype != dtype:
         raise ValueError("expected k_cache and v_cache [pages, page, Hk, D] of one shape and dtype")
-    pages, page, hk, d = k_cache.shape
-    if page < 1 or hk < 1:
+    if shape[1] < 1 or shape[2] < 1:
         raise ValueError("a cache has at least one token a page and one head")
-    size = k_cache.element_size()
-    strides = k_cache.stride()
-    if (strides != v_cache.stride() or strides[3] != 1 or any(s * size % 16 for s in strides[:3])
-            or strides[1] < 1 or strides[0] % strides[1] or k_cache.data_ptr() % 16 or v_cache.data_ptr() % 16):
+    code = _dtype_code(dtype)
+    if (stride != v_stride or stride[3] != 1 or any(s * dtype.itemsize % 16 for s in stride[:3]) or stride[1] < 1
+            or stride[0] % stride[1]):
         raise ValueError("caches must have equal strides, a dense last axis, page strides that are multiples of the "
-                         "token stride, and strides and addresses that are multiples of 16 bytes")
-    return (pages, page, hk, d), (ctypes.c_int64 * 3)(*strides[:3])
+                         "token stride, and strides that are multiples of 16 bytes")
+    return tuple(shape), (ctypes.c_int64 * 3)(*stride[:3]), code
 
 
-def _decode(q, k_cache, v_cache, page_table, lengths, scale, window, sinks, out=None, return_lse=False):
-    if q.ndim != 4:
+def _caches(k_cache, v_cache):
+    """_cache_plan of two caches, and their addresses."""
+    plan = _cache_plan(k_cache.shape, k_cache.stride(), v_cache.shape, v_cache.stride(), k_cache.dtype, v_cache.dtype)
+    at = k_cache.data_ptr(), v_cache.data_ptr()
+    if (at[0] | at[1]) % 16:
+        raise ValueError("caches must be aligned to 16 bytes")
+    return (*plan, at)
+
+
+@_plan
+def _decode_plan(q, cache, table, lengths, window, sinks):
+    """Checked sizes (B, T, Hq, Hk, D) of a decode call with tensors of these shapes, window and sinks."""
+    if len(q) != 4:
         raise ValueError("expected q [B,T,Hq,D]")
-    batch, length, hq, d = q.shape
-    dev = _require_device(q, k_cache, v_cache, page_table, lengths)
-    (pages, page, hk, dc), strides = _caches(k_cache, v_cache)
-    code = _dtype_code(k_cache.dtype)
-    if q.dtype != k_cache.dtype:
-        raise ValueError(f"q ({q.dtype}) and the caches ({k_cache.dtype}) must have one dtype")
-    if d != dc or hq < 1 or hq % hk:
+    batch, length, hq, d = q
+    hk = cache[2]
+    if d != cache[3] or hq < 1 or hq % hk:
         raise ValueError("q must have the caches' head width and a multiple of their heads")
     if d not in ATTENTION_HEAD_DIMS:
         raise ValueError(f"cached heads must have a width in {ATTENTION_HEAD_DIMS}")
     if not 1 <= length <= MAX_DRAFT:
         raise ValueError(f"paged decoding takes 1 to {MAX_DRAFT} query tokens a sequence, got {length}")
-    if page_table.ndim != 2 or page_table.shape[0] != batch or lengths.shape != (batch,):
+    if len(table) != 2 or table[0] != batch or lengths != (batch,):
         raise ValueError("expected page_table [B, max_pages] and lengths [B]")
-    window, sinks = _window_args(window, sinks)
+    return ((batch, length, hq, hk, d), *_window_args(window, sinks))
+
+
+@_plan
+def _decode_workspace(device_index: int, *sizes) -> int:
+    with torch.cuda.device(device_index):  # (it depends on the device's compute units)
+        return _lib.attn_lib().pbattn_paged_decode_workspace_size(*sizes)
+
+
+def _decode(q, k_cache, v_cache, page_table, lengths, scale, window, sinks, out=None, return_lse=False):
+    dev = _one_device(q, k_cache, v_cache, page_table, lengths)
+    cache, steps, code, at = _caches(k_cache, v_cache)
+    sizes, window, sinks = _decode_plan(q.shape, cache, page_table.shape, lengths.shape,
+                                        None if window is None else int(window), int(sinks))
+    if q.dtype != k_cache.dtype:
+        raise ValueError(f"q ({q.dtype}) and the caches ({k_cache.dtype}) must have one dtype")
     q = _aligned(q.contiguous(), 16)
-    if page_table.dtype != torch.int32 or not page_table.is_contiguous():
-        page_table = page_table.to(torch.int32).contiguous()
-    if lengths.dtype != torch.int32 or not lengths.is_contiguous():
-        lengths = lengths.to(torch.int32).contiguous()
-    if out is None:
-        out = torch.empty(batch, length, hq, d, dtype=q.dtype, device=dev)
-    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or out.data_ptr() % 16:
-        raise ValueError("out must be a contiguous, 16-byte aligned tensor of q's shape and dtype")
-    lse = torch.empty(batch, length, hq, dtype=torch.float32, device=dev) if return_lse else None
-    with _guard(dev):
-        lib = _lib.attn_lib()
-        nbytes = lib.pbattn_paged_decode_workspace_size(batch, length, hq, hk, d)
-        workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        status = lib.pbattn_paged_decode(
-            _lib.ptr(q), _lib.ptr(k_cache), _lib.ptr(v_cache), code, strides, page, pages, _lib.ptr(page_table),
-            page_table.shape[1], _lib.ptr(lengths), _lib.ptr(out), _lib.ptr(lse), batch, length, hq, hk, d,
-            float(scale), window, sinks, _lib.ptr(workspace), nbytes, _lib.stream_handle(dev))
-    _lib.check(status, "pbattn_paged_decode")
+    page_table, lengths = _boundaries(page_table), _boundaries(lengths)
+    out = _output(out, q)
+    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=dev) if return_lse else None
+    nbytes = _decode_workspace(dev.index, *sizes)
+    workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    _launch("pbattn_paged_decode", _lib.attn_lib().pbattn_paged_decode, dev, q.data_ptr(), *at, code, steps, cache[1],
+            cache[0], page_table.data_ptr(), page_table.shape[1], lengths.data_ptr(), out.data_ptr(), _lib.ptr(lse),
+            *sizes, float(scale), window, sinks, workspace.data_ptr(), nbytes)
     return out, lse
 
 
@@ -356,21 +411,31 @@ def paged_decode_attention(q, k_cache, v_cache, page_table, lengths, scale: floa
     return (o, lse) if return_lse else o
 
 
-def _write(k, v, k_cache, v_cache, slots):
-    dev = _require_device(k, v, k_cache, v_cache, slots)
-    (pages, page, hk, d), strides = _caches(k_cache, v_cache)
-    code = _dtype_code(k_cache.dtype)
-    if k.ndim < 3 or v.shape != k.shape or k.shape[-2:] != (hk, d) or slots.shape != k.shape[:-2]:
+@_plan
+def _write_steps(cache, k, k_stride, v, v_stride, slots, size):
+    """The stride array of new rows of these shapes, None if they are not readable
+    as [N, Hk, D] in place."""
+    if len(k) < 3 or v != k or k[-2:] != cache[2:] or slots != k[:-2]:
         raise ValueError("expected k, v [..., Hk, D] with the caches' heads and slots [...]")
+    if len(k) != 3 or not (_readable(k, k_stride, size) and _readable(v, v_stride, size)):
+        return None
+    return _steps((k, k_stride), (v, v_stride))
+
+
+def _write(k, v, k_cache, v_cache, slots):
+    dev = _one_device(k, v, k_cache, v_cache, slots)
+    cache, cache_steps, code, at = _caches(k_cache, v_cache)
+    steps = _write_steps(cache, k.shape, k.stride(), v.shape, v.stride(), slots.shape, k_cache.element_size())
     if slots.dtype not in (torch.int32, torch.int64):
         raise ValueError("slots must be int32 or int64")
-    k, v = (_strided(x.to(k_cache.dtype).reshape(-1, hk, d)) for x in (k, v))
-    slots = slots.reshape(-1).to(torch.int64).contiguous()
-    with _guard(dev):
-        status = _lib.attn_lib().pbattn_paged_write(
-            _lib.ptr(k), _lib.ptr(v), code, _strides(k, v), _lib.ptr(k_cache), _lib.ptr(v_cache), strides, page, pages,
-            _lib.ptr(slots), slots.numel(), hk, d, _lib.stream_handle(dev))
-    _lib.check(status, "pbattn_paged_write")
+    if steps is None or k.dtype != k_cache.dtype or v.dtype != k_cache.dtype:
+        k, v = (x.to(k_cache.dtype).reshape(-1, *cache[2:]).contiguous() for x in (k, v))
+        steps = _steps((k.shape, k.stride()), (v.shape, v.stride()))
+    k, v = _aligned(k, 16), _aligned(v, 16)
+    if slots.dtype != torch.int64 or slots.ndim != 1 or not slots.is_contiguous():
+        slots = slots.reshape(-1).to(torch.int64).contiguous()
+    _launch("pbattn_paged_write", _lib.attn_lib().pbattn_paged_write, dev, k.data_ptr(), v.data_ptr(), code, steps, *at,
+            cache_steps, cache[1], cache[0], slots.data_ptr(), slots.shape[0], cache[2], cache[3])
 
 
 @torch.library.custom_op("pbgdn::paged_cache_write_", mutates_args=("k_cache", "v_cache"),

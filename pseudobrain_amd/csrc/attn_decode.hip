@@ -22,6 +22,7 @@ constexpr int DEC_WAVES = 4;         // waves of a workgroup
 constexpr int DEC_KEYS = 32;         // keys of a block
 constexpr int DEC_MIN = DEC_WAVES;   // fewest blocks of a part: one a wave
 constexpr int DEC_ROWS = 16;         // rows of a matrix tile
+constexpr int JOIN_SPLIT_ROWS = 2048;  // up to here four waves join a row's parts
 
 struct DecodeParams {
   const unsigned char *q, *k, *v;
@@ -392,62 +393,76 @@ __global__ __launch_bounds__(DEC_WAVES * 64, OCC) void decode_kernel(const Decod
   }
 }
 
-// Joins a sequence's parts: a workgroup per (sequence, query row and head),
-// a quarter of the parts to a wave.
-template <int DT, int D>
+// Joins a sequence's parts, SPLIT waves to a (sequence, query row and head):
+// the weights of 64 parts at a time, one a lane, then their outputs, whose loads
+// wait for nothing but each other. Four waves a row where there are few rows,
+// one where there are many.
+template <int DT, int D, int SPLIT>
 __global__ __launch_bounds__(256) void decode_join_kernel(const DecodeParams p) {
-  using E = Elem<DT>;
-  constexpr int VEC = D / 64;
-  __shared__ float acc[4][D], stat[4][2];
+  constexpr int VEC = D / 64, ROWS = 4 / SPLIT;  // rows of a workgroup
+  __shared__ float acc[SPLIT > 1 ? 4 : 1][D], stat[4][2];
   PBGDN_POISON_LDS(acc, sizeof(acc));
   PBGDN_POISON_SYNC();
-  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), w = wave % SPLIT;
+  const int tiles = (p.rows + ROWS - 1) / ROWS;
   int id = blockIdx.x;
-  const int row = id % p.rows;
-  id /= p.rows;
+  const int row = id % tiles * ROWS + wave / SPLIT;
+  id /= tiles;
   const int hk = id % p.Hk, b = id / p.Hk;
   const int per = uniform(share_size(p, lane));
   const int parts = uniform(seq_parts(p, b, per));
   if (parts == 1) return;  // written by the first kernel
+  if (SPLIT == 1 && row >= p.rows) return;
   const int first = uniform(first_slot(p, b, per, lane));
   float m = -INFINITY, l = 0.0f, o[VEC];
 #pragma unroll
   for (int e = 0; e < VEC; ++e) o[e] = 0.0f;
-  for (int i = wave; i < parts; i += 4) {
-    const long at = (static_cast<long>(first + i) * p.Hk + hk) * p.rows + row;
-    const float2 s = p.stat[at];
-    const float top = fmaxf(m, s.x), base = top == -INFINITY ? 0.0f : top;
-    const float f1 = __builtin_amdgcn_exp2f(m - base), f2 = __builtin_amdgcn_exp2f(s.x - base);
+  for (int i0 = w; i0 < parts; i0 += 64 * SPLIT) {  // this wave's parts: i0, i0 + SPLIT, ...
+    const int mine = i0 + lane * SPLIT, count = (parts - i0 + SPLIT - 1) / SPLIT, n = count < 64 ? count : 64;
+    const long at0 = (static_cast<long>(first + i0) * p.Hk + hk) * p.rows + row;
+    const long step = static_cast<long>(SPLIT) * p.Hk * p.rows;
+    const float2 s = mine < parts ? p.stat[at0 + lane * step] : make_float2(-INFINITY, 0.0f);
+    const float top = fmaxf(m, wave_max(s.x)), base = top == -INFINITY ? 0.0f : top;
+    const float f = __builtin_amdgcn_exp2f(s.x - base), keep = __builtin_amdgcn_exp2f(m - base);
     m = top;
-    l = l * f1 + s.y * f2;
+    l = l * keep + wave_sum(s.y * f);
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) o[e] = o[e] * f1 + p.part[at * D + lane * VEC + e] * f2;
-  }
+    for (int e = 0; e < VEC; ++e) o[e] *= keep;
+#pragma unroll 8
+    for (int i = 0; i < n; ++i) {
+      const float fi = __shfl(f, i, 64);
 #pragma unroll
-  for (int e = 0; e < VEC; ++e) acc[wave][lane * VEC + e] = o[e];
-  if (lane == 0) {
-    stat[wave][0] = m;
-    stat[wave][1] = l;
+      for (int e = 0; e < VEC; ++e) o[e] += p.part[(at0 + i * step) * D + lane * VEC + e] * fi;
+    }
   }
-  __syncthreads();
-  const float top = fmaxf(fmaxf(stat[0][0], stat[1][0]), fmaxf(stat[2][0], stat[3][0]));
-  const float base = top == -INFINITY ? 0.0f : top;
-  float f[4], sum = 0.0f;
+  if constexpr (SPLIT > 1) {
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    f[w] = __builtin_amdgcn_exp2f(stat[w][0] - base);
-    sum += stat[w][1] * f[w];
+    for (int e = 0; e < VEC; ++e) acc[wave][lane * VEC + e] = o[e];
+    if (lane == 0) {
+      stat[wave][0] = m;
+      stat[wave][1] = l;
+    }
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
+    for (int i = 1; i < SPLIT; ++i) m = fmaxf(m, stat[i][0]);
+    const float base = m == -INFINITY ? 0.0f : m;
+    l = 0.0f;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) o[e] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < SPLIT; ++i) {
+      const float f = __builtin_amdgcn_exp2f(stat[i][0] - base);
+      l += stat[i][1] * f;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) o[e] += acc[i][lane * VEC + e] * f;
+    }
   }
-  const float inv = sum > 0.0f ? 1.0f / sum : sum;
+  const float inv = l > 0.0f ? 1.0f / l : l;
   const long at = (static_cast<long>(b) * p.T + row / p.group) * p.Hq + hk * p.group + row % p.group;
-  if (threadIdx.x < D) {
-    float x = 0.0f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) x += acc[w][threadIdx.x] * f[w];
-    store_elem(p.o, at * D + threadIdx.x, DT, x * inv);
-  }
-  if (p.lse && threadIdx.x == 0)
-    p.lse[at] = sum > 0.0f ? (top + __builtin_amdgcn_logf(sum)) * LN2 : sum == 0.0f ? -INFINITY : sum;
+  for (int e = 0; e < VEC; ++e) store_elem(p.o, at * D + lane * VEC + e, DT, o[e] * inv);
+  if (p.lse && lane == 0) p.lse[at] = l > 0.0f ? (m + __builtin_amdgcn_logf(l)) * LN2 : l == 0.0f ? -INFINITY : l;
 }
 
 // ---------------------------------------------------------------------------
@@ -493,8 +508,13 @@ static int launch_decode(DecodeParams &p, hipStream_t stream) {
   const bool ok = p.rows <= DEC_ROWS ? run(decode_kernel<DT, D, 1, WIDE <= 256 ? 2 : 1>, 1)
                                      : run(decode_kernel<DT, D, 2, WIDE <= 256 ? 2 : 1>, 2);
   if (!ok) return PBGDN_ERR_UNSUPPORTED;
-  hipLaunchKernelGGL((decode_join_kernel<DT, D>), dim3(static_cast<unsigned>(p.B * p.Hk * p.rows)), dim3(256), 0,
-                     stream, p);
+  const long rows = static_cast<long>(p.B) * p.Hk * p.rows;
+  if (rows <= JOIN_SPLIT_ROWS) {
+    hipLaunchKernelGGL((decode_join_kernel<DT, D, 4>), dim3(static_cast<unsigned>(rows)), dim3(256), 0, stream, p);
+  } else {
+    const unsigned blocks = static_cast<unsigned>(p.B * p.Hk * ((p.rows + 3) / 4));
+    hipLaunchKernelGGL((decode_join_kernel<DT, D, 1>), dim3(blocks), dim3(256), 0, stream, p);
+  }
   return hipGetLastError() == hipSuccess ? PBGDN_OK : PBGDN_ERR_LAUNCH;
 }
 

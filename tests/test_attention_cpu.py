@@ -203,7 +203,7 @@ def test_window_attention_refuses_cpu_tensors_and_bad_values():
         at._dtype_code(torch.float64)
     with pytest.raises(ValueError, match="one shape"):
         q, k, v = tensors()
-        at._window_shapes(q, k, v[:, :4], None, None)
+        at.window_attention(q, k, v[:, :4], 1.0)
 
 
 def test_paged_calls_refuse():
@@ -223,7 +223,8 @@ def test_paged_calls_refuse():
         at._caches(cache, torch.zeros(5, 2, 16, 64).transpose(1, 2))
     with pytest.raises(ValueError, match="one shape"):
         at._caches(cache, cache[:4])
-    sizes, steps = at._caches(cache.transpose(1, 2).contiguous().transpose(1, 2), cache.transpose(1, 2).contiguous().transpose(1, 2))
+    heads_first = cache.transpose(1, 2).contiguous().transpose(1, 2)
+    sizes, steps, *_ = at._caches(heads_first, heads_first)
     assert sizes == (5, 16, 2, 64) and list(steps) == [2048, 64, 1024]
 
 
