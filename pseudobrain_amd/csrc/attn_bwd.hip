@@ -36,7 +36,7 @@ struct BwdParams {
   uint32_t *range;    // float16: bits of max |do|, |v|, |delta|
   float *part;        // [2][parts][B][Hk][Tk][D] when parts > 1
   float *tail;        // [2][tail slots][Hk][sink tiles 32][D]
-  float scale, c;     // signed
+  float scale;
   int B, D;
   int parts;          // parts of a key tile's walk
   int key_slots;      // key tiles of a (batch, key head)
@@ -156,25 +156,6 @@ __global__ __launch_bounds__(256) void stat_kernel(const BwdParams p) {
   }
 }
 
-// A row of transposed accumulators: column d of z[d / 32], times f, as DT.
-template <int DT, int D>
-__device__ __forceinline__ void store_row(void *dst, const float16_t *z, int h, float f) {
-  using E = Elem<DT>;
-#pragma unroll
-  for (int m = 0; m < D / 32; ++m)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float4_t x = {z[m][4 * e] * f, z[m][4 * e + 1] * f, z[m][4 * e + 2] * f, z[m][4 * e + 3] * f};
-      const int d = 32 * m + 8 * e + 4 * h;
-      if constexpr (E::BYTES == 2) {
-        *reinterpret_cast<v2u32_t *>(static_cast<unsigned char *>(dst) + 2 * d) =
-            v2u32_t{E::pack(x[0], x[1]), E::pack(x[2], x[3])};
-      } else {
-        *reinterpret_cast<float4_t *>(static_cast<unsigned char *>(dst) + 4 * d) = x;
-      }
-    }
-}
-
 // ---------------------------------------------------------------------------
 // dK and dV. TAIL: the sinks' keys against the queries beyond their window.
 // ---------------------------------------------------------------------------
@@ -183,9 +164,11 @@ struct Dkdv {
   using L = Tile<DT, D>;
   static constexpr int BN = 32 * NW, TILE = QR * L::ROW, STAT = QR * 8, BUF = 2 * TILE + STAT, LDS = 2 * BUF;
   static constexpr int LOADS = QR / L::PER_DMA;  // of one tensor, all waves
-  // wide rows: K and V rows are read from LDS, registers hold the sums alone
-  static constexpr bool HELD = D < 256;
-  static constexpr int KV = HELD ? 0 : 2 * BN * L::ROW, BUFS = KV + 2 * BUF <= 160 * 1024 ? 2 : 1;
+  // Registers hold the sums, and K and V rows where they find room beside them
+  // (two waves a SIMD up to D = 128 in 16 bits): otherwise LDS does.
+  static constexpr bool HELD = D < 256, V_HELD = HELD && (D == 64 || L::E::BYTES == 4);
+  static constexpr int VS = HELD ? 0 : BN * L::ROW, KV = VS + (V_HELD ? 0 : BN * L::ROW);  // V's place, both sizes
+  static constexpr int BUFS = KV + 2 * BUF <= 160 * 1024 ? 2 : 1;
   static constexpr int BYTES = KV + BUFS * BUF;
 };
 
@@ -207,10 +190,10 @@ __global__ __launch_bounds__(NW * 64, WAVES) void dkdv_kernel(const BwdParams p)
   int b, hk, seq, tile, part, slot = 0;
   if constexpr (TAIL) {
     int id = blockIdx.x;
-    tile = id % p.sink_tiles;
+    tile = uniform(id % p.sink_tiles);
     id /= p.sink_tiles;
-    hk = id % f.Hk;
-    slot = id / f.Hk;
+    hk = uniform(id % f.Hk);
+    slot = uniform(id / f.Hk);
     // bisection over the sequences' first slots
     int lo = 0, hi = f.nseq - 1;
     while (lo < hi) {
@@ -220,7 +203,7 @@ __global__ __launch_bounds__(NW * 64, WAVES) void dkdv_kernel(const BwdParams p)
       else
         hi = mid - 1;
     }
-    seq = lo;
+    seq = uniform(lo);
     b = f.cu_q ? 0 : seq;
     part = slot - tail_start(p, seq) - 1;
   } else {
@@ -228,15 +211,15 @@ __global__ __launch_bounds__(NW * 64, WAVES) void dkdv_kernel(const BwdParams p)
     int grp, s;
     place(blockIdx.x, groups, p.key_slots * p.parts, grp, s);
     s = p.key_slots * p.parts - 1 - s;  // the first keys, which most queries see, first
-    b = grp / f.Hk;
-    hk = grp % f.Hk;
-    part = s % p.parts;
-    tile = s / p.parts;
+    b = uniform(grp / f.Hk);
+    hk = grp - b * f.Hk;
+    tile = uniform(s / p.parts);
+    part = s - tile * p.parts;
     seq = b;
     const int32_t *cu = f.cu_k ? f.cu_k : f.cu_q;
     if (f.cu_q) {
       seq = slot_sequence(cu, f.nseq, f.Tk, 1, K::BN, tile);
-      tile -= slot_start(cu, seq, f.Tk, 1, K::BN);
+      tile = uniform(tile - slot_start(cu, seq, f.Tk, 1, K::BN));
     }
   }
   const Seq sq = sequence<true>(f.cu_q, f.cu_k, seq, f.nseq, f.Tq, f.Tk);
@@ -260,33 +243,35 @@ __global__ __launch_bounds__(NW * 64, WAVES) void dkdv_kernel(const BwdParams p)
     t1 = t1 < 0 ? 0 : t1;
     if (p.parts > 1) {
       int step = (t1 - t0 + p.parts - 1) / p.parts;
-      step = (step + p.tokens - 1) / p.tokens * p.tokens;
+      step = uniform((step + p.tokens - 1) / p.tokens * p.tokens);
       t0 = t0 + part * step;
       t1 = t1 < t0 + step ? t1 : t0 + step;
     }
   }
-  const int tiles = t1 > t0 ? (t1 - t0 + p.tokens - 1) / p.tokens * p.splits : 0;
+  const int tiles = uniform(t1 > t0 ? (t1 - t0 + p.tokens - 1) / p.tokens * p.splits : 0);
 
   // this wave's keys
   const int key = j0 + wave * 32 + n;
   const int kc = key < sq.nk ? key : sq.nk - 1;
   const unsigned char *krow = f.k.base + b * f.k.batch + hk * f.k.head + (sq.k0 + kc) * f.k.token;
   const unsigned char *vrow = f.v.base + b * f.v.batch + hk * f.v.head + (sq.k0 + kc) * f.v.token;
-  v4u32_t kf[K::HELD ? S : 1], vf[K::HELD ? S : 1];
-  unsigned char *const kl = lds + wave * 32 * L::ROW, *const vl = kl + K::BN * L::ROW;
+  v4u32_t kf[K::HELD ? S : 1], vf[K::V_HELD ? S : 1];
+  unsigned char *const kl = lds + wave * 32 * L::ROW, *const vl = kl + K::VS;
   uint32_t rbase = L::rows_base(n, h), cbase = L::cols_base(lane);
 #pragma unroll
   for (int s = 0; s < S; ++s) {
-    const v4u32_t x = *reinterpret_cast<const v4u32_t *>(krow + (2 * s + h) * 16);
+    v4u32_t x = *reinterpret_cast<const v4u32_t *>(krow + (2 * s + h) * 16);
+    if (f.negate) x ^= E::BYTES == 2 ? 0x80008000u : 0x80000000u;  // (K here serves the scores alone)
     const v4u32_t y = *reinterpret_cast<const v4u32_t *>(vrow + (2 * s + h) * 16);
-    if constexpr (K::HELD) {
+    const uint32_t at = (rbase ^ ((2 * s) % 16 * 16)) + (2 * s) / 16 * 256;
+    if constexpr (K::HELD)
       kf[s] = x;
-      vf[s] = y;
-    } else {
-      const uint32_t at = (rbase ^ ((2 * s) % 16 * 16)) + (2 * s) / 16 * 256;
+    else
       *reinterpret_cast<v4u32_t *>(kl + at) = x;
+    if constexpr (K::V_HELD)
+      vf[s] = y;
+    else
       *reinterpret_cast<v4u32_t *>(vl + at) = y;
-    }
   }
 
   float16_t dk[MB], dv[MB];
@@ -294,37 +279,65 @@ __global__ __launch_bounds__(NW * 64, WAVES) void dkdv_kernel(const BwdParams p)
   for (int m = 0; m < MB; ++m) dk[m] = dv[m] = zero16();
   const float range = range_scale<DT, D>(p.range);
 
-  // staging of query tile i: `tokens` tokens from its first, `heads` heads
-  const unsigned char *qb = f.q.base + b * f.q.batch + sq.q0 * f.q.token + hk * G * f.q.head;
-  const unsigned char *gb = static_cast<const unsigned char *>(p.grad_o) +
-                            ((static_cast<long>(b) * f.Tq + sq.q0) * f.Hq + hk * G) * static_cast<long>(L::ROW);
-  const long g_token = static_cast<long>(f.Hq) * L::ROW;
-  const float2 *sb = p.stat + ((static_cast<long>(b) * f.Hk + hk) * f.Tq + sq.q0) * G;
-  unsigned char *const bufs = lds + K::KV;
+  // Staging of the query tiles in turn: `tokens` tokens of `heads` heads, or the
+  // heads of a token in `splits` tiles. A lane's offsets into a tile do not change;
+  // a lane past the tile's tokens (or heads, where they are split) stages zeros.
   const uint32_t inv = 65536 / p.heads + 1;  // row / heads = row inv >> 16 for rows below 32
-  const auto stage = [&](int i) __attribute__((always_inline)) {
-    const int lane = opaque(threadIdx.x & 63);
-    const int group = p.splits == 1 ? i : i / p.splits, split = p.splits == 1 ? 0 : i % p.splits;
-    const int t = t0 + group * p.tokens, g0 = split * QR;
-    const int tn = t1 - t < p.tokens ? t1 - t : p.tokens, hn = G - g0 < p.heads ? G - g0 : p.heads;
-    const uint32_t to = uniform(lds_address(bufs + (K::BUFS == 2 ? (i & 1) * K::BUF : 0)));
-    const v4u32_t dq_ = dma_desc(qb + t * f.q.token + g0 * f.q.head,
-                                 (tn - 1) * f.q.token + (hn - 1) * f.q.head + L::ROW);
-    const v4u32_t dg_ = dma_desc(gb + t * g_token + g0 * L::ROW, (tn - 1) * g_token + (hn - 1) * L::ROW + L::ROW);
+  const long g_token = static_cast<long>(f.Hq) * L::ROW;
+  constexpr int PER_WAVE = (K::LOADS + NW - 1) / NW;
+  const auto offsets = [&](int lane, int w, uint32_t &q_at, uint32_t &g_at, int &index) __attribute__((always_inline)) {
+    const int row = (wave + NW * w) * L::PER_DMA + lane / L::UNITS;
+    const int tt = static_cast<int>((row * inv) >> 16), gg = row - tt * p.heads;
+    const uint32_t unit = ((lane % L::UNITS) ^ L::swz(row)) * 16;
+    q_at = tt * static_cast<uint32_t>(f.q.token) + gg * static_cast<uint32_t>(f.q.head) + unit;
+    g_at = tt * static_cast<uint32_t>(g_token) + gg * L::ROW + unit;
+    index = p.splits == 1 ? tt : gg;
+  };
+  uint32_t q_at[K::HELD ? PER_WAVE : 1], g_at[K::HELD ? PER_WAVE : 1];
+  int index[K::HELD ? PER_WAVE : 1];
+  if constexpr (K::HELD) {
 #pragma unroll
-    for (int w = 0; w < (K::LOADS + NW - 1) / NW; ++w) {
+    for (int w = 0; w < PER_WAVE; ++w) offsets(lane, w, q_at[w], g_at[w], index[w]);
+  }
+  const unsigned char *qp = f.q.base + b * f.q.batch + (sq.q0 + t0) * f.q.token + hk * G * f.q.head;
+  const unsigned char *gp = static_cast<const unsigned char *>(p.grad_o) +
+                            ((static_cast<long>(b) * f.Tq + sq.q0 + t0) * f.Hq + hk * G) * static_cast<long>(L::ROW);
+  const float2 *sp = p.stat + ((static_cast<long>(b) * f.Hk + hk) * f.Tq + sq.q0 + t0) * G;
+  const long q_size = (p.tokens - 1) * f.q.token + (p.heads - 1) * f.q.head + L::ROW;
+  const long g_size = (p.tokens - 1) * g_token + p.heads * L::ROW;
+  int st = t0, split = 0;  // of the tile to stage next
+  unsigned char *const bufs = lds + K::KV;
+  const auto stage = [&](int i) __attribute__((always_inline)) {
+    const uint32_t to = uniform(lds_address(bufs + (K::BUFS == 2 ? (i & 1) * K::BUF : 0)));
+    const int left = p.splits == 1 ? t1 - st : G - split * QR, most = p.splits == 1 ? p.tokens : QR;
+    const int limit = left < most ? left : most;
+    const v4u32_t dq_ = dma_desc(qp, q_size), dg_ = dma_desc(gp, g_size);
+    const int lane_ = K::HELD ? 0 : opaque(threadIdx.x & 63);
+#pragma unroll
+    for (int w = 0; w < PER_WAVE; ++w) {
       const int inst = wave + NW * w;
-      const int row = inst * L::PER_DMA + lane / L::UNITS;
-      const int tt = static_cast<int>((row * inv) >> 16), gg = row - tt * p.heads;
-      const uint32_t unit = ((lane % L::UNITS) ^ L::swz(row)) * 16;
-      const bool in = tt < tn && gg < hn;
-      dma(dq_, in ? tt * static_cast<uint32_t>(f.q.token) + gg * static_cast<uint32_t>(f.q.head) + unit : OUT_OF_RANGE,
-          to + inst * 1024);
-      dma(dg_, in ? tt * static_cast<uint32_t>(g_token) + gg * L::ROW + unit : OUT_OF_RANGE, to + K::TILE + inst * 1024);
+      uint32_t qa, ga;
+      int x;
+      if constexpr (K::HELD)
+        qa = q_at[w], ga = g_at[w], x = index[w];
+      else
+        offsets(lane_, w, qa, ga, x);
+      const bool in = x < limit;
+      dma(dq_, in ? qa : OUT_OF_RANGE, to + inst * 1024);
+      dma(dg_, in ? ga : OUT_OF_RANGE, to + K::TILE + inst * 1024);
     }
-    if (wave == 0) {
-      const int rows = p.splits == 1 ? tn * G : hn;
-      dma4(dma_desc(sb + static_cast<long>(t) * G + g0, rows * 8L), lane * 4, to + 2 * K::TILE);
+    if (wave == 0) dma4(dma_desc(sp, limit * (p.splits == 1 ? G * 8L : 8L)), lane * 4, to + 2 * K::TILE);
+    // on to the next
+    if (++split == p.splits) {
+      split = 0;
+      st += p.tokens;
+      qp += p.tokens * f.q.token - (p.splits - 1) * QR * f.q.head;
+      gp += p.tokens * g_token - (p.splits - 1) * QR * L::ROW;
+      sp += p.tokens * G - (p.splits - 1) * QR;
+    } else {
+      qp += QR * f.q.head;
+      gp += QR * L::ROW;
+      sp += QR;
     }
   };
 
@@ -338,22 +351,22 @@ __global__ __launch_bounds__(NW * 64, WAVES) void dkdv_kernel(const BwdParams p)
     if (w_lo >= f.sinks) mine = 0;
   } else {
     const int before = w_lo - off - t0, after = w_hi - t0 - off;  // tokens before the first that sees w_lo
-    lead = before > 0 ? before / p.tokens * p.splits : 0;
+    lead = uniform(before > 0 ? before / p.tokens * p.splits : 0);
     if (after < t1 - t0 - f.window) {  // tokens from after + window on see none
       const int n = (after + f.window + p.tokens - 1) / p.tokens * p.splits;
-      mine = n < 0 ? 0 : n < tiles ? n : tiles;
+      mine = uniform(n < 0 ? 0 : n < tiles ? n : tiles);
     }
   }
   if (tiles > 0 && K::BUFS == 2) stage(0);
   const auto advance = [&](int i) __attribute__((always_inline)) {
     if constexpr (K::BUFS == 2) {
-      wait_dma();
+      wait_dma<0>();
       block_sync();
       if (i + 1 < tiles) stage(i + 1);
     } else {
       block_sync();
       stage(i);
-      wait_dma();
+      wait_dma<0>();
       block_sync();
     }
   };
@@ -362,19 +375,25 @@ __global__ __launch_bounds__(NW * 64, WAVES) void dkdv_kernel(const BwdParams p)
   for (; i < mine; ++i) {
     advance(i);
     const unsigned char *qt = bufs + (K::BUFS == 2 ? (i & 1) * K::BUF : 0), *gt = qt + K::TILE;
-    const float4_t *st = reinterpret_cast<const float4_t *>(qt + 2 * K::TILE);
-    const int tok = t0 + (p.splits == 1 ? i : i / p.splits) * p.tokens;
+    const float4_t *stat = reinterpret_cast<const float4_t *>(qt + 2 * K::TILE);
+    const int tok = t0 + (p.splits == 1 ? i : uniform(i / p.splits)) * p.tokens;
     const int p_lo = tok + off, p_hi = (tok + p.tokens < t1 ? tok + p.tokens : t1) - 1 + off;
     const bool whole = TAIL ? w_hi < f.sinks && w_hi <= p_lo - f.window : w_hi <= p_lo && w_lo > p_hi - f.window;
 
     rbase = opaque(rbase);
     cbase = opaque(cbase);
     float16_t x, y;
-    if constexpr (K::HELD) {
+    if constexpr (K::HELD)
       x = L::rows_product(qt, rbase, 0, kf);
-      y = L::rows_product(gt, rbase, 0, vf);
-    } else {
+    else
       x = L::rows_product_lds(qt, kl, rbase);
+    if constexpr (K::V_HELD) {
+      y = L::rows_product(gt, rbase, 0, vf);
+    } else if constexpr (K::HELD) {
+      y = zero16();
+#pragma unroll
+      for (int s = 0; s < S; ++s) y = E::mma(L::rows(gt, rbase, 0, s), L::rows(vl, rbase, 0, s), y);
+    } else {
       y = L::rows_product_lds(gt, vl, rbase);
     }
     if (!whole) {
@@ -383,20 +402,20 @@ __global__ __launch_bounds__(NW * 64, WAVES) void dkdv_kernel(const BwdParams p)
         const int pos = p_lo + static_cast<int>((acc_row(e, h) * inv) >> 16);
         const bool seen = TAIL ? (key < f.sinks) & (key <= pos - f.window) : (key <= pos) & (key > pos - f.window);
         x[e] = seen ? x[e] : -INFINITY;
+        y[e] = seen ? y[e] : 0.0f;
       }
     }
 #pragma unroll
     for (int e = 0; e < 16; e += 4) {
       // rows 2 e + 4 h .. + 3: (lse, delta) pairs
-      const float4_t a = st[e + 2 * h], c = st[e + 2 * h + 1];
+      const float4_t a = stat[e + 2 * h], c = stat[e + 2 * h + 1];
       const float lse[4] = {a[0], a[2], c[0], c[2]}, delta[4] = {a[1], a[3], c[1], c[3]};
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const float w = __builtin_amdgcn_exp2f(x[e + r] == -INFINITY ? x[e + r] : __builtin_fmaf(x[e + r], p.c, -lse[r]));
-        x[e + r] = w;
+        x[e + r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e + r], f.c, -lse[r]));
         float d = y[e + r] - delta[r];
         if constexpr (DT == PBGDN_F16) d *= range;
-        y[e + r] = w == 0.0f ? 0.0f : w * d;
+        y[e + r] = x[e + r] * d;
       }
     }
     if constexpr (K::HELD) {
@@ -527,29 +546,31 @@ __global__ __launch_bounds__(NW * 64, WAVES) void dq_kernel(const BwdParams p) {
   const int groups = gridDim.x / f.slots;
   int grp, slot;
   place(blockIdx.x, groups, f.slots, grp, slot);
-  const int b = grp / f.Hk, hk = grp % f.Hk;
+  const int b = uniform(grp / f.Hk), hk = grp - b * f.Hk;
   int seq = b;
   if (f.cu_q) {
     seq = slot_sequence(f.cu_q, f.nseq, f.Tq, G, F::BM, slot);
-    slot -= slot_start(f.cu_q, seq, f.Tq, G, F::BM);
+    slot = uniform(slot - slot_start(f.cu_q, seq, f.Tq, G, F::BM));
   }
   const Seq sq = sequence<false>(f.cu_q, f.cu_k, seq, f.nseq, f.Tq, f.Tk);
-  const long total = static_cast<long>(sq.nq) * G, row0 = static_cast<long>(slot) * F::BM;
+  const int total = sq.nq * G, row0 = slot * F::BM;
   if (slot < 0 || row0 >= total) return;
   const int off = sq.nk - sq.nq;
-  const auto position = [&](long row) __attribute__((always_inline)) { return static_cast<int>((row < total ? row : total - 1) / G) + off; };
+  const auto position = [&](int row) __attribute__((always_inline)) {
+    return uniform((row < total ? row : total - 1) / G) + off;
+  };
   const KeyRange range = key_range(position(row0), position(row0 + F::BM - 1), f.window, f.sinks);
-  const long wrow = row0 + wave * 32;
+  const int wrow = row0 + wave * 32;
   const int w_first = position(wrow), w_last = position(wrow + 31);
 
   const unsigned char *kb_ = f.k.base + b * f.k.batch + hk * f.k.head + sq.k0 * f.k.token;
   const unsigned char *vb_ = f.v.base + b * f.v.batch + hk * f.v.head + sq.k0 * f.v.token;
   const KeyStage<DT, D, BN, NW> stage(kb_, f.k.token, vb_, f.v.token, range, wave, lane);
   const int tiles = (range.count + BN - 1) / BN;
-  if (tiles > 0) stage.tile(0, lds, wave);
+  if (tiles > 0) stage.tile(0, lds);
 
-  const long row = wrow + n, r = row < total ? row : total - 1;
-  const int t = static_cast<int>(r / G), head = hk * G + static_cast<int>(r % G), pos = t + off;
+  const int row = wrow + n, r = row < total ? row : total - 1;
+  const int t = r / G, head = hk * G + (r - t * G), pos = t + off;
   const long out = (static_cast<long>(b) * f.Tq + sq.q0 + t) * f.Hq + head;
   const unsigned char *qrow = f.q.base + b * f.q.batch + (sq.q0 + t) * f.q.token + head * f.q.head;
   const unsigned char *grow = static_cast<const unsigned char *>(p.grad_o) + out * L::ROW;
@@ -558,6 +579,7 @@ __global__ __launch_bounds__(NW * 64, WAVES) void dq_kernel(const BwdParams p) {
   for (int s = 0; s < S; ++s) {
     qf[s] = *reinterpret_cast<const v4u32_t *>(qrow + (2 * s + h) * 16);
     gf[s] = *reinterpret_cast<const v4u32_t *>(grow + (2 * s + h) * 16);
+    if (f.negate) qf[s] ^= E::BYTES == 2 ? 0x80008000u : 0x80000000u;
   }
   const float2 st = p.stat[((static_cast<long>(b) * f.Hk + hk) * f.Tq + sq.q0) * G + r];
   const float scale16 = range_scale<DT, D>(p.range);
@@ -567,9 +589,9 @@ __global__ __launch_bounds__(NW * 64, WAVES) void dq_kernel(const BwdParams p) {
 
   const uint32_t rbase = L::rows_base(n, h), cbase = L::cols_base(lane);
   const auto advance = [&](int it) __attribute__((always_inline)) {
-    wait_dma();
+    wait_dma<0>();
     block_sync();
-    if (it + 1 < tiles) stage.tile(it + 1, lds + ((it + 1) & 1) * F::TILE, wave);
+    if (it + 1 < tiles) stage.tile(it + 1, lds + ((it + 1) & 1) * F::TILE);
   };
   const int mine = wave_tiles(range, tiles, w_last, BN);
   int it = 0;
@@ -585,15 +607,16 @@ __global__ __launch_bounds__(NW * 64, WAVES) void dq_kernel(const BwdParams p) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int u = u0 + 32 * kb + acc_row(i, h);
-          x[i] = sees(pos, u < range.sinks ? u : u + range.delta, f.window, f.sinks) ? x[i] : -INFINITY;
+          const bool seen = sees(pos, u < range.sinks ? u : u + range.delta, f.window, f.sinks);
+          x[i] = seen ? x[i] : -INFINITY;
+          y[i] = seen ? y[i] : 0.0f;
         }
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const float w = __builtin_amdgcn_exp2f(x[i] == -INFINITY ? x[i] : __builtin_fmaf(x[i], p.c, -st.x));
         float d = y[i] - st.y;
         if constexpr (DT == PBGDN_F16) d *= scale16;
-        x[i] = w == 0.0f ? 0.0f : w * d;
+        x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], f.c, -st.x)) * d;
       }
       L::cols_product(kt, cbase, 32 * kb, L::operand(x), dq);
     }
@@ -763,7 +786,6 @@ extern "C" int pbattn_window_bwd(const void *q, const void *k, const void *v, in
   p.part = reinterpret_cast<float *>(ws + w.part);
   p.tail = reinterpret_cast<float *>(ws + w.tail);
   p.scale = scale;
-  p.c = scale * LOG2E;
   p.B = B;
   p.D = D;
   p.parts = w.parts;

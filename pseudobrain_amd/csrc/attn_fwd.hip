@@ -15,207 +15,320 @@
 
 namespace pbgdn {
 
+// Workgroups of 128 rows per CU below which the waves of a workgroup share 32
+// rows instead.
+constexpr int SPLIT_BELOW = 2;
 constexpr float LAG = 8.0f;  // weights stay below 2^8
 
-template <int DT, int D, int CB, int NW, int BN>
-struct Fwd {
-  using L = Tile<DT, D>;
-  using E = Elem<DT>;
-  static constexpr int BM = 32 * CB * NW, KB = BN / 32, TILE = BN * L::ROW;
-  static constexpr int LDS = 4 * TILE;
+// Where a workgroup's BM rows lie: their sequence, its keys, and a run of rows'
+// positions.
+struct Place {
+  int b, hk, off;
+  int total, row0;
+  Seq sq;
+  bool empty;
+  const unsigned char *k, *v;
 };
-
-template <int DT, int D, int CB, int NW, int BN, int WAVES>
-__global__ __launch_bounds__(NW * 64, WAVES) void window_fwd_kernel(const WindowParams p) {
-  using F = Fwd<DT, D, CB, NW, BN>;
-  using L = typename F::L;
-  using E = typename F::E;
-  constexpr int KB = F::KB, S = L::STEPS, MB = L::MB;
-  extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
-  PBGDN_POISON_LDS(lds, F::LDS);
-  PBGDN_POISON_SYNC();
-
-  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
-  const int n = lane & 31, h = lane >> 5, G = p.group;
-  const int groups = gridDim.x / p.slots;
+template <int BM>
+__device__ __forceinline__ Place place_rows(const WindowParams &p) {
+  Place w;
   int grp, slot;
-  place(blockIdx.x, groups, p.slots, grp, slot);
-  const int b = grp / p.Hk, hk = grp % p.Hk;
-  int seq = b;
+  place(blockIdx.x, gridDim.x / p.slots, p.slots, grp, slot);
+  w.b = uniform(grp / p.Hk);
+  w.hk = grp - w.b * p.Hk;
+  int seq = w.b;
   if (p.cu_q) {
-    seq = slot_sequence(p.cu_q, p.nseq, p.Tq, G, F::BM, slot);
-    slot -= slot_start(p.cu_q, seq, p.Tq, G, F::BM);
+    seq = slot_sequence(p.cu_q, p.nseq, p.Tq, p.group, BM, slot);
+    slot = uniform(slot - slot_start(p.cu_q, seq, p.Tq, p.group, BM));
   }
-  const Seq sq = sequence<false>(p.cu_q, p.cu_k, seq, p.nseq, p.Tq, p.Tk);
-  const long total = static_cast<long>(sq.nq) * G, row0 = static_cast<long>(slot) * F::BM;
-  if (slot < 0 || row0 >= total) return;
+  w.sq = sequence<false>(p.cu_q, p.cu_k, seq, p.nseq, p.Tq, p.Tk);
+  w.total = w.sq.nq * p.group;
+  w.row0 = slot * BM;
+  w.empty = slot < 0 || w.row0 >= w.total;
+  w.off = w.sq.nk - w.sq.nq;
+  w.k = p.k.base + w.b * p.k.batch + w.hk * p.k.head + w.sq.k0 * p.k.token;
+  w.v = p.v.base + w.b * p.v.batch + w.hk * p.v.head + w.sq.k0 * p.v.token;
+  return w;
+}
+__device__ __forceinline__ int position(const Place &w, int row, int group) {
+  return uniform((row < w.total ? row : w.total - 1) / group) + w.off;
+}
 
-  // positions of the workgroup's first and last row, and of this wave's
-  const int off = sq.nk - sq.nq;
-  const auto position = [&](long row) __attribute__((always_inline)) { return static_cast<int>((row < total ? row : total - 1) / G) + off; };
-  const KeyRange range = key_range(position(row0), position(row0 + F::BM - 1), p.window, p.sinks);
-  const long wrow = row0 + wave * 32 * CB;
-  const int w_first = position(wrow), w_last = position(wrow + 32 * CB - 1);
+// The 32 rows of a wave: lane (n, h) has row n's query units 2 s + h, its softmax
+// state and the rows 8 (i / 4) + 4 h + i % 4 of every 32 of its output.
+template <int DT, int D>
+struct WaveRows {
+  using L = Tile<DT, D>;
+  using E = typename L::E;
+  static constexpr int S = L::STEPS, MB = L::MB;
+  v4u32_t q[S];
+  int pos;
+  long out;  // (token, head) index of the row, or -1
+  float m, l;
+  float16_t o[MB];
+  uint32_t rbase, cbase;
+  int h;
 
-  const unsigned char *kb_ = p.k.base + b * p.k.batch + hk * p.k.head + sq.k0 * p.k.token;
-  const unsigned char *vb_ = p.v.base + b * p.v.batch + hk * p.v.head + sq.k0 * p.v.token;
-  const KeyStage<DT, D, BN, NW> stage(kb_, p.k.token, vb_, p.v.token, range, wave, lane);
-  const int tiles = (range.count + BN - 1) / BN;
-  if (tiles > 0) stage.tile(0, lds, wave);
-
-  // this lane's columns: their query rows
-  v4u32_t qf[CB][S];
-  int pos[CB];
-  long out[CB];  // (token, head) index of the row, or -1
-  float m[CB], l[CB];
-  float16_t o[CB][MB];
-#pragma unroll
-  for (int cb = 0; cb < CB; ++cb) {
-    const long row = wrow + 32 * cb + n;
-    const long r = row < total ? row : total - 1;
-    const int t = static_cast<int>(r / G), head = hk * G + static_cast<int>(r % G);
-    pos[cb] = t + off;
-    out[cb] = row < total ? (static_cast<long>(b) * p.Tq + sq.q0 + t) * p.Hq + head : -1;
-    const unsigned char *src = p.q.base + b * p.q.batch + (sq.q0 + t) * p.q.token + head * p.q.head;
+  __device__ __forceinline__ void load(const WindowParams &p, const Place &w, int row, int lane) {
+    h = lane >> 5;
+    row += lane & 31;
+    const int r = row < w.total ? row : w.total - 1;
+    const int t = r / p.group, head = w.hk * p.group + (r - t * p.group);
+    pos = t + w.off;
+    out = row < w.total ? (static_cast<long>(w.b) * p.Tq + w.sq.q0 + t) * p.Hq + head : -1;
+    const unsigned char *src = p.q.base + w.b * p.q.batch + (w.sq.q0 + t) * p.q.token + head * p.q.head;
 #pragma unroll
     for (int s = 0; s < S; ++s) {
-      qf[cb][s] = *reinterpret_cast<const v4u32_t *>(src + (2 * s + h) * 16);
-      if (p.negate) qf[cb][s] ^= E::BYTES == 2 ? 0x80008000u : 0x80000000u;
+      q[s] = *reinterpret_cast<const v4u32_t *>(src + (2 * s + h) * 16);
+      if (p.negate) q[s] ^= E::BYTES == 2 ? 0x80008000u : 0x80000000u;
     }
-    m[cb] = -INFINITY;
-    l[cb] = 0.0f;
+    m = -INFINITY;
+    l = 0.0f;
 #pragma unroll
-    for (int i = 0; i < MB; ++i) o[cb][i] = zero16();
+    for (int i = 0; i < MB; ++i) o[i] = zero16();
+    rbase = L::rows_base(lane & 31, h);
+    cbase = L::cols_base(lane);
   }
 
-  const uint32_t rbase = L::rows_base(n, h), cbase = L::cols_base(lane);
-  const auto advance = [&](int it) __attribute__((always_inline)) {
-    wait_dma();
-    block_sync();
-    if (it + 1 < tiles) stage.tile(it + 1, lds + ((it + 1) & 1) * F::TILE, wave);
-  };
-  const int mine = wave_tiles(range, tiles, w_last, BN);
-  int it = 0;
-  for (; it < mine; ++it) {
-    advance(it);
-    const unsigned char *kt = lds + (it & 1) * F::TILE, *vt = kt + 2 * F::TILE;
-    const int u0 = it * BN;
-    const bool whole = whole_tile(range, u0, BN, w_first, w_last, p.window);
-
-    float16_t sc[KB][CB];
+  // Scores of a tile's KB x 32 keys, those from u0 on of the range; `whole`: every
+  // row sees all of them.
+  template <int KB>
+  __device__ __forceinline__ void scores(const WindowParams &p, const KeyRange &range, const unsigned char *tile, int u0,
+                                         bool whole, float16_t *sc) const {
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) {
-#pragma unroll
-      for (int cb = 0; cb < CB; ++cb) sc[kb][cb] = zero16();
-#pragma unroll
-      for (int s = 0; s < S; ++s) {
-        const v4u32_t a = L::rows(kt, rbase, 32 * kb, s);
-#pragma unroll
-        for (int cb = 0; cb < CB; ++cb) sc[kb][cb] = E::mma(a, qf[cb][s], sc[kb][cb]);
-      }
-    }
+    for (int kb = 0; kb < KB; ++kb) sc[kb] = L::rows_product(tile, L::ROW < 512 ? rbase : opaque(rbase), 32 * kb, q);
     if (!whole) {
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int u = u0 + 32 * kb + acc_row(i, h);
-          const int j = u < range.sinks ? u : u + range.delta;
-#pragma unroll
-          for (int cb = 0; cb < CB; ++cb)
-            sc[kb][cb][i] = sees(pos[cb], j, p.window, p.sinks) ? sc[kb][cb][i] : -INFINITY;
+          sc[kb][i] = sees(pos, u < range.sinks ? u : u + range.delta, p.window, p.sinks) ? sc[kb][i] : -INFINITY;
         }
     }
+  }
+
+  // Scores to weights, against a reference m that moves only when a score passes
+  // it by more than LAG powers of two: most tiles leave the sums as they are.
+  template <int KB>
+  __device__ __forceinline__ void weights(float c, float16_t *sc) {
+    float mx = sc[0][0];
 #pragma unroll
-    for (int cb = 0; cb < CB; ++cb) {
-      float mx = sc[0][cb][0];
+    for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
+      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[kb][i]);
+    mx = max_xor32(mx);
+    if (__any((mx - m) * c > LAG)) {
+      const float top = fmaxf(m, mx);
+      const float alpha = __builtin_amdgcn_exp2f((m - (top == -INFINITY ? 0.0f : top)) * c);
+      m = top;
+      l *= alpha;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[kb][cb][i]);
-      // The reference the weights are taken against moves only when a score
-      // passes it by more than LAG powers of two, so most tiles leave the sums
-      // as they are.
-      mx = max_xor32(mx);
-      if (__any((mx - m[cb]) * p.c > LAG)) {
-        const float top = fmaxf(m[cb], mx);
-        const float alpha = __builtin_amdgcn_exp2f((m[cb] - (top == -INFINITY ? 0.0f : top)) * p.c);
-        m[cb] = top;
-        l[cb] *= alpha;
+      for (int i = 0; i < MB; ++i)
 #pragma unroll
-        for (int i = 0; i < MB; ++i)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) o[cb][i][e] *= alpha;
-      }
-      const float base = m[cb] == -INFINITY ? 0.0f : m[cb], at = base * p.c;
-      float sum = 0.0f;
-      if (__any(fabsf(at) > EXACT_SCORES)) {
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) sc[kb][cb][i] = __builtin_amdgcn_exp2f((sc[kb][cb][i] - base) * p.c);
-      } else {
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            sc[kb][cb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[kb][cb][i], p.c, -at));
-      }
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) sum += sc[kb][cb][i];
-      l[cb] += sum;
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb) L::cols_product(vt, cbase, 32 * kb, L::operand(sc[kb][cb]), o[cb]);
+        for (int e = 0; e < 16; ++e) o[i][e] *= alpha;
     }
+    const float base = m == -INFINITY ? 0.0f : m, at = base * c;
+    if (__any(fabsf(at) > EXACT_SCORES)) {
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sc[kb][i] = __builtin_amdgcn_exp2f((sc[kb][i] - base) * c);
+    } else {
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sc[kb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[kb][i], c, -at));
+    }
+    float sum = 0.0f;
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sum += sc[kb][i];
+    l += sum;
+  }
+
+  template <int KB>
+  __device__ __forceinline__ void values(const unsigned char *tile, const float16_t *sc) {
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) L::cols_product(tile, L::ROW < 512 ? cbase : opaque(cbase), 32 * kb, L::operand(sc[kb]), o);
+  }
+
+  // o and lse of the wave's rows; l summed over the lane halves.
+  __device__ __forceinline__ void store(const WindowParams &p) const {
+    const float inv = l > 0.0f ? 1.0f / l : l;  // no key seen: zeros (a NaN stays)
+    if (out < 0) return;
+    if (p.lse && h == 0)
+      p.lse[out] = l > 0.0f ? (m * p.c + __builtin_amdgcn_logf(l)) * LN2 : l == 0.0f ? -INFINITY : l;
+    store_row<DT, D>(static_cast<unsigned char *>(p.o) + out * L::ROW, o, h, inv);
+  }
+};
+
+template <int DT, int D, int NW, int BN>
+struct Fwd {
+  static constexpr int BM = 32 * NW, KB = BN / 32, TILE = BN * Tile<DT, D>::ROW, LDS = 4 * TILE;
+};
+
+template <int DT, int D, int NW, int BN, int WAVES>
+__global__ __launch_bounds__(NW * 64, WAVES) void window_fwd_kernel(const WindowParams p) {
+  using F = Fwd<DT, D, NW, BN>;
+  extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
+  PBGDN_POISON_LDS(lds, F::LDS);
+  PBGDN_POISON_SYNC();
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const Place w = place_rows<F::BM>(p);
+  if (w.empty) return;
+  // the keys of the workgroup's rows, and this wave's first and last position
+  const KeyRange range =
+      key_range(position(w, w.row0, p.group), position(w, w.row0 + F::BM - 1, p.group), p.window, p.sinks);
+  const int row = w.row0 + wave * 32;
+  const int w_first = position(w, row, p.group), w_last = position(w, row + 31, p.group);
+  const KeyStage<DT, D, BN, NW, (Tile<DT, D>::ROW < 512)> stage(w.k, p.k.token, w.v, p.v.token, range, wave, lane);
+  const int tiles = (range.count + BN - 1) / BN;
+  if (tiles > 0) stage.tile(0, lds);
+  WaveRows<DT, D> r;
+  r.load(p, w, row, lane);
+
+  const auto advance = [&](int it) __attribute__((always_inline)) {
+    wait_dma<0>();
+    block_sync();
+    if (it + 1 < tiles) stage.tile(it + 1, lds + ((it + 1) & 1) * F::TILE);
+  };
+  const int mine = wave_tiles(range, tiles, w_last, BN);
+  int it = 0;
+  for (; it < mine; ++it) {
+    advance(it);
+    const unsigned char *kt = lds + (it & 1) * F::TILE, *vt = kt + 2 * F::TILE;
+    float16_t sc[F::KB];
+    r.template scores<F::KB>(p, range, kt, it * BN, whole_tile(range, it * BN, BN, w_first, w_last, p.window), sc);
+    r.template weights<F::KB>(p.c, sc);
+    r.template values<F::KB>(vt, sc);
   }
   for (; it < tiles; ++it) advance(it);
-
-#pragma unroll
-  for (int cb = 0; cb < CB; ++cb) {
-    const float sum = add_xor32(l[cb]);
-    const float inv = sum > 0.0f ? 1.0f / sum : sum;  // no key seen: zeros (a NaN stays)
-    if (out[cb] < 0) continue;
-    if (p.lse && h == 0) p.lse[out[cb]] = sum > 0.0f ? (m[cb] * p.c + __builtin_amdgcn_logf(sum)) * LN2 : sum == 0.0f ? -INFINITY : sum;
-    unsigned char *dst = static_cast<unsigned char *>(p.o) + out[cb] * L::ROW;
-#pragma unroll
-    for (int i = 0; i < MB; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float4_t x;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) x[c] = o[cb][i][4 * e + c] * inv;
-        const int d = 32 * i + 8 * e + 4 * h;
-        if constexpr (E::BYTES == 2) {
-          *reinterpret_cast<v2u32_t *>(dst + 2 * d) = v2u32_t{E::pack(x[0], x[1]), E::pack(x[2], x[3])};
-        } else {
-          *reinterpret_cast<float4_t *>(dst + 4 * d) = x;
-        }
-      }
-  }
+  r.l = add_xor32(r.l);
+  r.store(p);
 }
 
-template <int DT, int D, int CB, int NW, int BN, int WAVES>
-static int launch_fwd(WindowParams &p, int B, hipStream_t stream) {
-  using F = Fwd<DT, D, CB, NW, BN>;
-  static std::atomic<bool> flags[MAX_DEVICES];
-  const auto kernel = window_fwd_kernel<DT, D, CB, NW, BN, WAVES>;
-  if (!smem_configured(reinterpret_cast<const void *>(kernel), F::LDS, flags)) return PBGDN_ERR_LAUNCH;
-  const long slots = window_slots(p, F::BM), blocks = slots * (p.cu_q ? 1 : B) * p.Hk;
+// The same for calls with too few rows to fill the GPU: the waves of a workgroup
+// share its 32 rows and take their key tiles in turn, each through tiles of its
+// own with no barrier, and join their sums at the end.
+template <int DT, int D>
+struct Split {
+  using L = Tile<DT, D>;
+  static constexpr int BN = 32, TILE = BN * L::ROW;
+  static constexpr int NW = L::ROW <= 512 ? 4 : 2;    // as many as the tiles leave room for
+  static constexpr int SUMS = 64 * (L::MB * 16 + 2) * 4;  // a wave's sums
+  static constexpr int LDS = NW * 2 * TILE > NW / 2 * SUMS ? NW * 2 * TILE : NW / 2 * SUMS;
+};
+
+template <int DT, int D, int NW, int WAVES>
+__global__ __launch_bounds__(NW * 64, WAVES) void window_split_kernel(const WindowParams p) {
+  using F = Split<DT, D>;
+  using L = typename F::L;
+  constexpr int BN = F::BN, MB = L::MB;
+  static_assert(NW == F::NW, "the waves the LDS is laid out for");
+  using Stage = KeyStage<DT, D, BN, 1, (L::ROW < 512)>;
+  extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
+  PBGDN_POISON_LDS(lds, F::LDS);
+  PBGDN_POISON_SYNC();
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const Place w = place_rows<32>(p);
+  if (w.empty) return;
+  const int w_first = position(w, w.row0, p.group), w_last = position(w, w.row0 + 31, p.group);
+  const KeyRange range = key_range(w_first, w_last, p.window, p.sinks);
+  const Stage stage(w.k, p.k.token, w.v, p.v.token, range, 0, lane);
+  const int tiles = (range.count + BN - 1) / BN;
+  unsigned char *const kt = lds + wave * 2 * F::TILE, *const vt = kt + F::TILE;
+  WaveRows<DT, D> r;
+  r.load(p, w, w.row0, lane);
+  if (wave < tiles) {
+    stage.keys(wave, kt);
+    stage.values(wave, vt);
+  }
+  // K of the next tile is fetched while this one's weights and values are worked
+  // on, V while the next one's scores are.
+  for (int it = wave; it < tiles; it += NW) {
+    const bool more = it + NW < tiles;
+    float16_t sc[1];
+    wait_dma<Stage::LOADS>();
+    r.template scores<1>(p, range, kt, it * BN, whole_tile(range, it * BN, BN, w_first, w_last, p.window), sc);
+    wait_lds();
+    if (more) stage.keys(it + NW, kt);
+    r.template weights<1>(p.c, sc);
+    if (more)
+      wait_dma<Stage::LOADS>();
+    else
+      wait_dma<0>();
+    r.template values<1>(vt, sc);
+    wait_lds();
+    if (more) stage.values(it + NW, vt);
+  }
+  r.l = add_xor32(r.l);
+
+  // the waves' sums into wave 0, the upper half into the lower
+#pragma unroll
+  for (int half = NW / 2; half > 0; half >>= 1) {
+    __syncthreads();
+    float *const at = reinterpret_cast<float *>(lds + (wave % half) * F::SUMS);
+    if (wave >= half && wave < 2 * half) {
+#pragma unroll
+      for (int i = 0; i < MB; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          *reinterpret_cast<float4_t *>(at + ((4 * i + e) * 64 + lane) * 4) =
+              float4_t{r.o[i][4 * e], r.o[i][4 * e + 1], r.o[i][4 * e + 2], r.o[i][4 * e + 3]};
+      at[MB * 1024 + lane] = r.m;
+      at[MB * 1024 + 64 + lane] = r.l;
+    }
+    __syncthreads();
+    if (wave < half) {
+      const float m2 = at[MB * 1024 + lane], top = fmaxf(r.m, m2), base = top == -INFINITY ? 0.0f : top;
+      const float f1 = __builtin_amdgcn_exp2f((r.m - base) * p.c), f2 = __builtin_amdgcn_exp2f((m2 - base) * p.c);
+      r.m = top;
+      r.l = r.l * f1 + at[MB * 1024 + 64 + lane] * f2;
+#pragma unroll
+      for (int i = 0; i < MB; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float4_t x = *reinterpret_cast<const float4_t *>(at + ((4 * i + e) * 64 + lane) * 4);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) r.o[i][4 * e + c] = r.o[i][4 * e + c] * f1 + x[c] * f2;
+        }
+    }
+  }
+  if (wave == 0) r.store(p);
+}
+
+template <typename Kernel>
+static int launch_rows(WindowParams &p, int B, Kernel kernel, int bm, int nw, int lds, std::atomic<bool> *flags,
+                       hipStream_t stream) {
+  if (!smem_configured(reinterpret_cast<const void *>(kernel), lds, flags)) return PBGDN_ERR_LAUNCH;
+  const long slots = window_slots(p, bm), blocks = slots * (p.cu_q ? 1 : B) * p.Hk;
   if (blocks > 0x7fffffffL) return PBGDN_ERR_UNSUPPORTED;
   p.slots = static_cast<int>(slots);
-  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(NW * 64), F::LDS, stream, p);
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(nw * 64), lds, stream, p);
   return hipGetLastError() == hipSuccess ? PBGDN_OK : PBGDN_ERR_LAUNCH;
+}
+
+template <int DT, int D, int BN, int WAVES>
+static int launch_fwd(WindowParams &p, int B, hipStream_t stream) {
+  static std::atomic<bool> flags[MAX_DEVICES], split_flags[MAX_DEVICES];
+  using F = Fwd<DT, D, 4, BN>;
+  using S = Split<DT, D>;
+  DeviceShape shape;
+  if (!device_shape(shape)) return PBGDN_ERR_LAUNCH;
+  if (window_slots(p, F::BM) * (p.cu_q ? 1 : B) * p.Hk < SPLIT_BELOW * shape.cus)
+    return launch_rows(p, B, window_split_kernel<DT, D, S::NW, WAVES>, 32, S::NW, S::LDS, split_flags, stream);
+  return launch_rows(p, B, window_fwd_kernel<DT, D, 4, BN, WAVES>, F::BM, 4, F::LDS, flags, stream);
 }
 
 template <int DT>
 static int dispatch_fwd(WindowParams &p, int B, int D, hipStream_t stream) {
   constexpr bool wide = DT == PBGDN_F32;
   switch (D) {
-    case 64: return launch_fwd<DT, 64, 1, 4, 64, 2>(p, B, stream);
-    case 128: return launch_fwd<DT, 128, 1, 4, wide ? 32 : 64, wide ? 1 : 2>(p, B, stream);
-    case 256: return launch_fwd<DT, 256, 1, 4, 32, wide ? 1 : 2>(p, B, stream);
+    case 64: return launch_fwd<DT, 64, 64, 2>(p, B, stream);
+    case 128: return launch_fwd<DT, 128, wide ? 32 : 64, wide ? 1 : 2>(p, B, stream);
+    case 256: return launch_fwd<DT, 256, 32, wide ? 1 : 2>(p, B, stream);
     default: return PBGDN_ERR_UNSUPPORTED;
   }
 }
@@ -235,6 +348,7 @@ int window_params(WindowParams &p, const void *q, const void *k, const void *v, 
   if (!aligned16(q) || !aligned16(k) || !aligned16(v)) return PBGDN_ERR_INVALID_ARGUMENT;
   if (D != 64 && D != 128 && D != 256) return PBGDN_ERR_UNSUPPORTED;
   if (Tq >= NO_WINDOW || Tk >= NO_WINDOW) return PBGDN_ERR_UNSUPPORTED;
+  if (static_cast<long>(Tq) * (Hq / Hk) > 0x7fffffffL - 1024) return PBGDN_ERR_UNSUPPORTED;  // rows of a key head
   const int bytes = attn_bytes(dtype);
   View *views[3] = {&p.q, &p.k, &p.v};
   const void *bases[3] = {q, k, v};

@@ -262,6 +262,35 @@ struct Tile {
   }
 };
 
+// A row of transposed accumulators: column d of z[d / 32], times f, as DT.
+template <int DT, int D>
+__device__ __forceinline__ void store_row(void *dst, const float16_t *z, int h, float f) {
+  using E = Elem<DT>;
+#pragma unroll
+  for (int m = 0; m < D / 32; ++m)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float4_t x = {z[m][4 * e] * f, z[m][4 * e + 1] * f, z[m][4 * e + 2] * f, z[m][4 * e + 3] * f};
+      const int d = 32 * m + 8 * e + 4 * h;
+      if constexpr (E::BYTES == 2) {
+        *reinterpret_cast<v2u32_t *>(static_cast<unsigned char *>(dst) + 2 * d) =
+            v2u32_t{E::pack(x[0], x[1]), E::pack(x[2], x[3])};
+      } else {
+        *reinterpret_cast<float4_t *>(static_cast<unsigned char *>(dst) + 4 * d) = x;
+      }
+    }
+}
+
+// x, of which the compiler knows nothing more: what is computed from it inside a
+// loop is computed there instead of being kept in registers across it.
+__device__ __forceinline__ uint32_t opaque(uint32_t x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
+// A wave-uniform value in a scalar register.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
 // ---------------------------------------------------------------------------
 // Direct-to-LDS loads: 16 bytes per lane, lane l to `lds` + 16 l. Assembly, so
 // that the compiler does not wait for them before LDS reads it cannot tell
@@ -286,15 +315,24 @@ __device__ __forceinline__ void dma(const void *src, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(src)
                : "memory");
 }
+// (the words in scalar registers whatever unit the compiler worked them out on)
 __device__ __forceinline__ v4u32_t dma_desc(const void *base, long bytes) {
   const uint64_t a = reinterpret_cast<uint64_t>(base);
-  return v4u32_t{static_cast<uint32_t>(a), static_cast<uint32_t>(a >> 32) & 0xffffu,
-                 static_cast<uint32_t>(bytes > 0 ? bytes : 0), static_cast<uint32_t>(RSRC_WORD3)};
+  return v4u32_t{static_cast<uint32_t>(uniform(static_cast<int>(a))),
+                 static_cast<uint32_t>(uniform(static_cast<int>(a >> 32))) & 0xffffu,
+                 static_cast<uint32_t>(uniform(static_cast<int>(bytes > 0 ? bytes : 0))),
+                 static_cast<uint32_t>(RSRC_WORD3)};
 }
-__device__ __forceinline__ void wait_dma() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// All but the last N loads of this wave have arrived.
+template <int N>
+__device__ __forceinline__ void wait_dma() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+// This wave's LDS reads have returned.
+__device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 // Every wave has reached this point; its LDS reads have returned.
 __device__ __forceinline__ void block_sync() {
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  wait_lds();
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
@@ -305,16 +343,6 @@ __device__ __forceinline__ float max_xor32(float x) {
   swap32(a, b);
   return fmaxf(a, b);
 }
-
-// x, of which the compiler knows nothing more: what is computed from it inside a
-// loop is computed there instead of being kept in registers across it.
-__device__ __forceinline__ uint32_t opaque(uint32_t x) {
-  asm volatile("" : "+v"(x));
-  return x;
-}
-
-// A wave-uniform value in a scalar register.
-__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
 // ---------------------------------------------------------------------------
 // Which keys a query sees: position p sees key j when j <= p and
@@ -368,7 +396,7 @@ __device__ __forceinline__ int slot_sequence(const int32_t *cu, int n, int total
     else
       hi = mid - 1;
   }
-  return lo;
+  return uniform(lo);
 }
 
 // ---------------------------------------------------------------------------
@@ -402,50 +430,74 @@ __device__ __forceinline__ bool whole_tile(const KeyRange &r, int u0, int bn, in
 }
 
 // Stages rows u0 .. of a key range into tiles of K and V: wave w of NW fills its
-// share of the loads, load i rows NW PER_DMA i further on. A load's lane offsets
-// are those of the first, but for the permutation of its units.
-template <int DT, int D, int BN, int NW>
+// share of the loads, load i STEP rows further on. A lane's offset changes from
+// load to load by whole rows and by the permutation of the row's units, which
+// repeats every 16 rows: VARS offsets, kept in registers, serve all loads. With
+// HELD false they are worked out at each tile, where registers are scarce (a
+// spilled one would be read back through the loads' own counter, and so wait for
+// all of them).
+template <int DT, int D, int BN, int NW, bool HELD = true>
 struct KeyStage {
   using L = Tile<DT, D>;
   static constexpr int STEP = NW * L::PER_DMA, LOADS = BN / STEP, TILE = BN * L::ROW;
+  static constexpr int VARS = STEP >= 16 || LOADS == 1 ? 1 : 16 / STEP < LOADS ? 16 / STEP : LOADS;
   static_assert(LOADS * STEP == BN, "whole loads");
   const unsigned char *k, *v;
   long k_stride, v_stride;
   KeyRange range;
-  int row;       // this lane's row of the first load
-  uint32_t unit;  // and its unit
+  int wave;
+  uint32_t k_at[VARS], v_at[VARS];
+
+  // this lane's row of the first load, and its unit of load i
+  __device__ __forceinline__ static int row_of(int wave, int lane) { return wave * L::PER_DMA + lane / L::UNITS; }
+  __device__ __forceinline__ static uint32_t unit_of(int row, int lane, int i) {
+    return ((lane % L::UNITS) ^ L::swz(row) ^ L::swz(i * STEP % 16)) * 16;
+  }
+  __device__ __forceinline__ static void offsets(int wave, int lane, long stride, uint32_t *at) {
+    const int row = row_of(wave, lane);
+#pragma unroll
+    for (int i = 0; i < VARS; ++i)
+      at[i] = (row + i * STEP) * static_cast<uint32_t>(stride) + unit_of(row, lane, i);
+  }
 
   __device__ __forceinline__ KeyStage(const unsigned char *k_, long ks, const unsigned char *v_, long vs,
-                                      const KeyRange &r, int wave, int lane)
-      : k(k_), v(v_), k_stride(ks), v_stride(vs), range(r), row(wave * L::PER_DMA + lane / L::UNITS),
-        unit((lane % L::UNITS) ^ L::swz(row)) {}
+                                      const KeyRange &r, int wave_, int lane)
+      : k(k_), v(v_), k_stride(ks), v_stride(vs), range(r), wave(wave_) {
+    if constexpr (HELD) {
+      offsets(wave, lane, ks, k_at);
+      offsets(wave, lane, vs, v_at);
+    }
+  }
 
-  __device__ __forceinline__ void one(const unsigned char *base, long stride, int u0, unsigned char *lds,
-                                      int wave) const {
+  __device__ __forceinline__ void one(const unsigned char *base, long stride, const uint32_t *held, int u0,
+                                      unsigned char *lds) const {
     const uint32_t to = uniform(lds_address(lds) + wave * 1024);
-    if (u0 >= range.sinks) {  // one run of keys: a scalar base, fixed lane offsets
+    if (u0 >= range.sinks) {  // one run of keys
       const int left = range.count - u0, rows = left < BN ? left : BN;
-      const unsigned char *from = base + (u0 + range.delta) * stride;
-      const uint32_t at = static_cast<uint32_t>(row) * static_cast<uint32_t>(stride);
-      const long step = STEP * stride;
+      const v4u32_t desc = dma_desc(base + (u0 + range.delta) * stride, (rows - 1) * stride + L::ROW);
+      uint32_t at[VARS];
+      if constexpr (!HELD) offsets(wave, opaque(threadIdx.x & 63), stride, at);
 #pragma unroll
       for (int i = 0; i < LOADS; ++i)
-        dma(dma_desc(from + i * step, (rows - 1) * stride + L::ROW - i * step), at + (unit ^ L::swz(i * STEP % 16)) * 16,
+        dma(desc, (HELD ? held : at)[i % VARS] + static_cast<uint32_t>(i / VARS * VARS * STEP) * static_cast<uint32_t>(stride),
             to + i * NW * 1024);
     } else {  // sinks and the window's start in one tile; rows past the end repeat the last key
+      const int lane = opaque(threadIdx.x & 63), row = row_of(wave, lane);
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
         int u = u0 + row + i * STEP;
         u = u < range.count ? u : range.count - 1;
         const long j = u < range.sinks ? u : u + range.delta;
-        dma(base + j * stride + (unit ^ L::swz(i * STEP % 16)) * 16, to + i * NW * 1024);
+        dma(base + j * stride + unit_of(row, lane, i), to + i * NW * 1024);
       }
     }
   }
+  __device__ __forceinline__ void keys(int it, unsigned char *tile) const { one(k, k_stride, k_at, it * BN, tile); }
+  __device__ __forceinline__ void values(int it, unsigned char *tile) const { one(v, v_stride, v_at, it * BN, tile); }
   // Tile `it` into `buffer`: K, and V two tiles further on.
-  __device__ __forceinline__ void tile(int it, unsigned char *buffer, int wave) const {
-    one(k, k_stride, it * BN, buffer, wave);
-    one(v, v_stride, it * BN, buffer + 2 * TILE, wave);
+  __device__ __forceinline__ void tile(int it, unsigned char *buffer) const {
+    keys(it, buffer);
+    values(it, buffer + 2 * TILE);
   }
 };
 
@@ -462,7 +514,9 @@ __device__ __forceinline__ void place(int id, int groups, int slots, int &group,
     group = id % groups;
     slot = id / groups;
   }
-  slot = slots - 1 - slot;
+  // (divisions are done in vector registers: say that the results are uniform)
+  group = uniform(group);
+  slot = uniform(slots - 1 - slot);
 }
 
 }  // namespace pbgdn
