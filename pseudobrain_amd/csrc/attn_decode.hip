@@ -12,6 +12,8 @@
 // The visible blocks of all sequences are shared out evenly from the lengths:
 // every workgroup derives the same shares, so a batch of uneven contexts needs
 // neither a host's knowledge of the lengths nor a list made by another kernel.
+#include <type_traits>
+
 #include "attn.hpp"
 #include "attn_tile.hpp"
 #include "device.hpp"
@@ -53,36 +55,48 @@ __device__ __forceinline__ int seq_blocks(const DecodeParams &p, int b) {
 }
 
 // The shares: every part takes `per` blocks (the last of a sequence what is
-// left), a sequence at least one part.
-struct Share {
-  int seq, part, parts, per, first;  // first: the sequence's first slot
-};
+// left), a sequence at least one part. Every wave works them out for itself: the
+// first 256 sequences' blocks, four a lane, are read once and together.
+__device__ __forceinline__ int wave_sum_int(int x) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off, 64);
+  return x;
+}
 __device__ __forceinline__ long wave_sum_long(long x) {
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off, 64);
   return x;
 }
-// Blocks per part, the same in every workgroup.
-__device__ __forceinline__ int share_size(const DecodeParams &p, int lane) {
-  long total = 0;
-  for (int b = lane; b < p.B; b += 64) total += seq_blocks(p, b);
-  total = wave_sum_long(total);
-  const int per = static_cast<int>((total + p.target - 1) / p.target);
-  const int whole = (per + DEC_MIN - 1) / DEC_MIN * DEC_MIN;
-  return whole > DEC_MIN ? whole : DEC_MIN;
-}
-__device__ __forceinline__ int seq_parts(const DecodeParams &p, int b, int per) {
-  const int n = (seq_blocks(p, b) + per - 1) / per;
-  return n > 0 ? n : 1;
-}
+struct Shares {
+  static constexpr int HELD = 4;
+  int held[HELD];  // blocks of sequences 64 i + lane
+  int per;
+
+  __device__ __forceinline__ Shares(const DecodeParams &p, int lane) {
+    long total = 0;
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) {
+      held[i] = 64 * i + lane < p.B ? seq_blocks(p, 64 * i + lane) : 0;
+      total += held[i];
+    }
+    for (int b = 64 * HELD + lane; b < p.B; b += 64) total += seq_blocks(p, b);
+    total = wave_sum_long(total);
+    const int even = static_cast<int>((total + p.target - 1) / p.target);
+    const int whole = (even + DEC_MIN - 1) / DEC_MIN * DEC_MIN;
+    per = uniform(whole > DEC_MIN ? whole : DEC_MIN);
+  }
+  __device__ __forceinline__ int parts(int blocks) const { return blocks > per ? (blocks + per - 1) / per : 1; }
+};
 // Whose slot it is: a scan over the sequences, 64 at a time. seq = -1 past the last.
+struct Share {
+  int seq, part, parts, per;
+};
 __device__ __forceinline__ Share share_of_slot(const DecodeParams &p, int slot, int lane) {
-  Share s;
-  s.per = share_size(p, lane);
-  s.seq = -1;
+  const Shares all(p, lane);
+  Share s{-1, 0, 0, all.per};
   int base = 0;
-  for (int b0 = 0; b0 < p.B; b0 += 64) {
-    const int mine = b0 + lane < p.B ? seq_parts(p, b0 + lane, s.per) : 0;
+  const auto look = [&](int b0, int blocks) __attribute__((always_inline)) {
+    const int mine = b0 + lane < p.B ? all.parts(blocks) : 0;
     int scan = mine;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
@@ -94,19 +108,18 @@ __device__ __forceinline__ Share share_of_slot(const DecodeParams &p, int slot, 
       const int l = __builtin_ctzll(past);
       s.seq = b0 + l;
       s.parts = __shfl(mine, l, 64);
-      s.first = base + __shfl(scan, l, 64) - s.parts;
-      s.part = slot - s.first;
-      return s;
+      s.part = slot - (base + __shfl(scan, l, 64) - s.parts);
     }
     base += __shfl(scan, 63, 64);
+    return past != 0;
+  };
+#pragma unroll
+  for (int i = 0; i < Shares::HELD; ++i) {
+    if (64 * i >= p.B || look(64 * i, all.held[i])) return s;
   }
+  for (int b0 = 64 * Shares::HELD; b0 < p.B; b0 += 64)
+    if (look(b0, b0 + lane < p.B ? seq_blocks(p, b0 + lane) : 0)) break;
   return s;
-}
-// The first slot of sequence b.
-__device__ __forceinline__ int first_slot(const DecodeParams &p, int b, int per, int lane) {
-  long before = 0;
-  for (int i = lane; i < b; i += 64) before += seq_parts(p, i, per);
-  return static_cast<int>(wave_sum_long(before));
 }
 
 template <int DT, int D>
@@ -119,6 +132,12 @@ struct Dec {
   static constexpr int VLOADS = ROW / 16 / VB;      // times it does
   static constexpr int VE = VB / E::BYTES;          // elements of one such read
   static constexpr int OT = D / 16;                 // 16-wide output tiles: VLOADS * VE
+  // Rows up to 256 bytes: 32 keys at a time. Wider ones 16, and Q in LDS where a
+  // wave has two row blocks of it (its registers hold the sums, 16 keys and their
+  // values): two waves a SIMD up to 512 bytes.
+  static constexpr int KG = ROW <= 256 ? 2 : 1;     // 16-key groups at a time
+  static constexpr bool q_in_lds(int rb) { return ROW > 512 || (ROW == 512 && rb == 2); }
+  static constexpr int OCC = ROW <= 512 ? 2 : 1;
 };
 
 // Scores of 16 keys: x += K rows (a lane's units) times Q rows.
@@ -144,11 +163,12 @@ __device__ __forceinline__ float max_rows(float x) {
   return fmaxf(a, b);
 }
 
-template <int DT, int D, int RB, int OCC>
-__global__ __launch_bounds__(DEC_WAVES * 64, OCC) void decode_kernel(const DecodeParams p) {
+template <int DT, int D, int RB>
+__global__ __launch_bounds__(DEC_WAVES * 64, (Dec<DT, D>::OCC)) void decode_kernel(const DecodeParams p) {
   using K = Dec<DT, D>;
   using E = typename K::E;
-  constexpr int KS = K::KSTEPS, OT = K::OT;
+  constexpr int KS = K::KSTEPS, OT = K::OT, KG = K::KG, KEYS = 16 * KG;
+  constexpr bool Q_LDS = K::q_in_lds(RB);
   // waves joined at a time: pairs, or one after the other where two would not fit
   constexpr int JOINS = RB * D <= 256 ? 2 : 1;
   __shared__ __attribute__((aligned(16))) float merge[JOINS][RB * DEC_ROWS * (D + 2)];
@@ -157,21 +177,21 @@ __global__ __launch_bounds__(DEC_WAVES * 64, OCC) void decode_kernel(const Decod
 
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
-  int id = blockIdx.x;
-  const int hk = id % p.Hk;
-  id /= p.Hk;
-  const int row0 = id % p.row_tiles * (RB * DEC_ROWS);
-  const int slot = id / p.row_tiles;
+  const int slots = p.target + p.B, id = uniform(blockIdx.x / slots), slot = blockIdx.x - id * slots;
+  const int row0 = uniform(id / p.Hk) * (RB * DEC_ROWS), hk = uniform(id % p.Hk);
   const Share share = share_of_slot(p, slot, lane);
   if (share.seq < 0) return;
   const int b = uniform(share.seq), len = uniform(seq_length(p, b));
   const KeyRange range = seq_keys(p, len);
-  const int blocks = (range.count + DEC_KEYS - 1) / DEC_KEYS;
-  const int begin = uniform(share.part * share.per);
-  const int end = uniform(begin + share.per < blocks ? begin + share.per : blocks);
+  // this wave's KEYS-wide blocks of the part: begin + wave, then every DEC_WAVES-th
+  const int blocks = (range.count + KEYS - 1) / KEYS;
+  const int begin = uniform(share.part * share.per * (DEC_KEYS / KEYS));
+  const int end_ = begin + share.per * (DEC_KEYS / KEYS);
+  const int end = uniform(end_ < blocks ? end_ : blocks);
 
   // this lane's rows of Q (column c of every row block)
-  v4u32_t qf[RB][KS];
+  unsigned char *const ql = reinterpret_cast<unsigned char *>(&merge[0][0]);
+  v4u32_t qf[Q_LDS ? 1 : RB][KS];
   int pos[RB];
 #pragma unroll
   for (int r = 0; r < RB; ++r) {
@@ -179,13 +199,19 @@ __global__ __launch_bounds__(DEC_WAVES * 64, OCC) void decode_kernel(const Decod
     const int rr = row < p.rows ? row : p.rows - 1;
     const int t = rr / p.group;
     pos[r] = len - p.T + t;
-    const unsigned char *src = p.q + ((static_cast<long>(b) * p.T + t) * p.Hq + hk * p.group + rr % p.group) * K::ROW;
+    const unsigned char *src = p.q + ((static_cast<long>(b) * p.T + t) * p.Hq + hk * p.group + rr - t * p.group) * K::ROW;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-      qf[r][s] = *reinterpret_cast<const v4u32_t *>(src + (4 * s + g) * 16);
-      if (p.negate) qf[r][s] ^= K::SHORT ? 0x80008000u : 0x80000000u;
+      if (Q_LDS && s % DEC_WAVES != wave) continue;  // each wave brings in a share
+      v4u32_t x = *reinterpret_cast<const v4u32_t *>(src + (4 * s + g) * 16);
+      if (p.negate) x ^= K::SHORT ? 0x80008000u : 0x80000000u;
+      if constexpr (Q_LDS)
+        *reinterpret_cast<v4u32_t *>(ql + (r * DEC_ROWS + c) * K::ROW + ((4 * s + g) ^ c) * 16) = x;
+      else
+        qf[r][s] = x;
     }
   }
+  if constexpr (Q_LDS) __syncthreads();
   float m[RB], l[RB];
   float4_t o[RB][OT];
 #pragma unroll
@@ -198,123 +224,166 @@ __global__ __launch_bounds__(DEC_WAVES * 64, OCC) void decode_kernel(const Decod
 
   const unsigned char *kbase = p.k + hk * p.head, *vbase = p.v + hk * p.head;
   const int32_t *table = p.table + static_cast<long>(b) * p.max_pages;
-  // the cache row of key `lane & 31` of a block, -1 where there is none
+  // the cache row of key `lane` (modulo KEYS) of a block, -1 where there is none
   const auto lookup = [&](int blk) __attribute__((always_inline)) {
-    const int u = blk * DEC_KEYS + (lane & 31);
+    const int u = blk * KEYS + lane % KEYS;
     if (u >= range.count) return -1;
     const int j = u < range.sinks ? u : u + range.delta;
     const int pg = j / p.page;
     const int at = pg < p.max_pages ? table[pg] : -1;
     return at >= 0 && at < p.num_pages ? at * p.page_rows + (j - pg * p.page) : -1;
   };
-  int rows = begin + wave < end ? lookup(begin + wave) : -1;
-  for (int blk = begin + wave; blk < end; blk += DEC_WAVES) {
-    const bool all = __ballot(rows >= 0) == ~0ull;
+  // The cache is read once: past the caches (non-temporal), 4 to 9% faster where
+  // it is larger than they are.
+  v4u32_t kf[KG][KS];
+  uint32_t vf[4 * KG][K::VLOADS][K::VB / 4];
+  const auto load_keys = [&](int rows) __attribute__((always_inline)) {
     const int safe = rows >= 0 ? rows : 0;
-    v4u32_t kf[2][KS];
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
+    for (int kb = 0; kb < KG; ++kb) {
       const unsigned char *src = kbase + static_cast<long>(__shfl(safe, 16 * kb + c, 64)) * p.token;
 #pragma unroll
-      for (int s = 0; s < KS; ++s) kf[kb][s] = *reinterpret_cast<const v4u32_t *>(src + (4 * s + g) * 16);
+      for (int s = 0; s < KS; ++s)
+        kf[kb][s] = __builtin_nontemporal_load(reinterpret_cast<const v4u32_t *>(src + (4 * s + g) * 16));
     }
-    uint32_t vf[8][K::VLOADS][K::VB / 4];
+  };
+  const auto load_values = [&](int rows) __attribute__((always_inline)) {
+    const int safe = rows >= 0 ? rows : 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int key = (i < 4 ? 0 : 16) + 4 * g + i % 4;
-      const unsigned char *src = vbase + static_cast<long>(__shfl(safe, key, 64)) * p.token;
+    for (int i = 0; i < 4 * KG; ++i) {
+      const unsigned char *src = vbase + static_cast<long>(__shfl(safe, i / 4 * 16 + 4 * g + i % 4, 64)) * p.token;
 #pragma unroll
       for (int x = 0; x < K::VLOADS; ++x) {
         if constexpr (K::VB == 16) {
-          const v4u32_t w = *reinterpret_cast<const v4u32_t *>(src + x * 16 * K::VB + c * K::VB);
+          const v4u32_t w = __builtin_nontemporal_load(reinterpret_cast<const v4u32_t *>(src + x * 16 * K::VB + c * K::VB));
 #pragma unroll
           for (int e = 0; e < 4; ++e) vf[i][x][e] = w[e];
         } else {
-          const v2u32_t w = *reinterpret_cast<const v2u32_t *>(src + x * 16 * K::VB + c * K::VB);
+          const v2u32_t w = __builtin_nontemporal_load(reinterpret_cast<const v2u32_t *>(src + x * 16 * K::VB + c * K::VB));
 #pragma unroll
           for (int e = 0; e < 2; ++e) vf[i][x][e] = w[e];
         }
       }
     }
-    const int valid = rows;
-    if (blk + DEC_WAVES < end) rows = lookup(blk + DEC_WAVES);
-
+  };
+  // A block's keys are fetched while the one before is weighed, its values while
+  // the scores are formed: the registers of either are free again by then.
+  int valid = -1, next = -1;
+  if (begin + wave < end) {
+    valid = lookup(begin + wave);
+    load_keys(valid);
+    load_values(valid);
+    if (begin + wave + DEC_WAVES < end) next = lookup(begin + wave + DEC_WAVES);
+  }
+  for (int blk = begin + wave; blk < end; blk += DEC_WAVES) {
+    const bool more = blk + DEC_WAVES < end, all = __ballot(valid >= 0) == ~0ull;
+    float4_t sc[RB][KG];
+#pragma unroll
+    for (int r = 0; r < RB; ++r)
+#pragma unroll
+      for (int kb = 0; kb < KG; ++kb) sc[r][kb] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    const uint32_t qat = opaque(c * K::ROW + (g ^ c) * 16);  // unit g of row c: unit 4 s + g is 64 s from it, by exclusive or
+#pragma unroll
+    for (int k = 0; k < KS; ++k)
+#pragma unroll
+      for (int r = 0; r < RB; ++r) {
+        v4u32_t q;
+        if constexpr (Q_LDS) {
+          const uint32_t lo = (4 * k) % 16 * 16, hi = (4 * k) / 16 * 256;
+          q = *reinterpret_cast<const v4u32_t *>(ql + r * DEC_ROWS * K::ROW + (qat ^ lo) + hi);
+        } else {
+          q = qf[r][k];
+        }
+#pragma unroll
+        for (int kb = 0; kb < KG; ++kb) sc[r][kb] = key_mma<DT>(kf[kb][k], q, sc[r][kb]);
+      }
+    if (more) load_keys(next);
     if (!all) {  // values of absent keys: zeros, whatever the row they were read from holds
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const bool in = __shfl(valid, (i < 4 ? 0 : 16) + 4 * g + i % 4, 64) >= 0;
+      for (int i = 0; i < 4 * KG; ++i) {
+        const bool in = __shfl(valid, i / 4 * 16 + 4 * g + i % 4, 64) >= 0;
 #pragma unroll
         for (int x = 0; x < K::VLOADS; ++x)
 #pragma unroll
           for (int e = 0; e < K::VB / 4; ++e) vf[i][x][e] = in ? vf[i][x][e] : 0u;
       }
     }
-    const int u0 = blk * DEC_KEYS;
-    const int j0 = u0 < range.sinks ? u0 : u0 + range.delta, j1 = u0 + DEC_KEYS - 1 + range.delta;
+    const int u0 = blk * KEYS;
+    const int j0 = u0 < range.sinks ? u0 : u0 + range.delta, j1 = u0 + KEYS - 1 + range.delta;
     const bool whole = all && u0 >= range.sinks && j1 <= len - p.T && j0 > len - 1 - p.window;
 #pragma unroll
     for (int r = 0; r < RB; ++r) {
-      float4_t s[2];
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {
-        s[kb] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int k = 0; k < KS; ++k) s[kb] = key_mma<DT>(kf[kb][k], qf[r][k], s[kb]);
-      }
+      float4_t (&s)[KG] = sc[r];
       if (!whole) {
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int key = 16 * kb + 4 * g + i, u = u0 + key;
-            const int j = u < range.sinks ? u : u + range.delta;
-            const bool seen = (__shfl(valid, key, 64) >= 0) & sees(pos[r], j, p.window, p.sinks);
-            s[kb][i] = seen ? s[kb][i] : -INFINITY;
-          }
+        for (int i = 0; i < 4 * KG; ++i) {
+          const int key = i / 4 * 16 + 4 * g + i % 4, u = u0 + key;
+          const int j = u < range.sinks ? u : u + range.delta;
+          const bool seen = (__shfl(valid, key, 64) >= 0) & sees(pos[r], j, p.window, p.sinks);
+          s[i / 4][i % 4] = seen ? s[i / 4][i % 4] : -INFINITY;
+        }
       }
       float mx = s[0][0];
 #pragma unroll
-      for (int i = 1; i < 8; ++i) mx = fmaxf(mx, s[i / 4][i % 4]);
-      const float top = fmaxf(m[r], max_rows(mx)), base = top == -INFINITY ? 0.0f : top, at = base * p.c;
-      const float alpha = __builtin_amdgcn_exp2f((m[r] - base) * p.c);
-      m[r] = top;
-      float sum = 0.0f;
-      const bool far = __any(fabsf(at) > EXACT_SCORES);
+      for (int i = 1; i < 4 * KG; ++i) mx = fmaxf(mx, s[i / 4][i % 4]);
+      mx = max_rows(mx);
+      if (__any((mx - m[r]) * p.c > LAG)) {
+        const float top = fmaxf(m[r], mx);
+        const float alpha = __builtin_amdgcn_exp2f((m[r] - (top == -INFINITY ? 0.0f : top)) * p.c);
+        m[r] = top;
+        l[r] *= alpha;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+        for (int j = 0; j < OT; ++j) o[r][j] *= alpha;
+      }
+      const float base = m[r] == -INFINITY ? 0.0f : m[r], at = base * p.c;
+      const bool far = __any(fabsf(at) > EXACT_SCORES);
+      float sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 4 * KG; ++i) {
         const float x = s[i / 4][i % 4];
         s[i / 4][i % 4] = __builtin_amdgcn_exp2f(far ? (x - base) * p.c : __builtin_fmaf(x, p.c, -at));
         sum += s[i / 4][i % 4];
       }
-      l[r] = l[r] * alpha + sum;
+      l[r] += sum;
+    }
+    // O^T += V^T P; element e of the lane's value rows makes output tile x VE + e
+    if constexpr (K::SHORT) {
+      using Half = std::conditional_t<KG == 2, v4u32_t, v2u32_t>;
+      Half w[RB];
 #pragma unroll
-      for (int j = 0; j < OT; ++j) o[r][j] *= alpha;
-      if constexpr (K::SHORT) {
-        const v4u32_t w = {E::pack(s[0][0], s[0][1]), E::pack(s[0][2], s[0][3]), E::pack(s[1][0], s[1][1]),
-                           E::pack(s[1][2], s[1][3])};
+      for (int r = 0; r < RB; ++r)
+#pragma unroll
+        for (int i = 0; i < 2 * KG; ++i) w[r][i] = E::pack(sc[r][i / 2][2 * (i % 2)], sc[r][i / 2][2 * (i % 2) + 1]);
+#pragma unroll
+      for (int x = 0; x < K::VLOADS; ++x)
+#pragma unroll
+        for (int e = 0; e < K::VE; ++e) {
+          Half a;
+#pragma unroll
+          for (int i = 0; i < 2 * KG; ++i)
+            a[i] = __builtin_amdgcn_perm(vf[2 * i + 1][x][e / 2], vf[2 * i][x][e / 2], e % 2 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+          for (int r = 0; r < RB; ++r) o[r][x * K::VE + e] = E::mma16(a, w[r], o[r][x * K::VE + e]);
+        }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4 * KG; ++i)
 #pragma unroll
         for (int x = 0; x < K::VLOADS; ++x)
 #pragma unroll
-          for (int e = 0; e < K::VE; ++e) {
-            v4u32_t a;  // element e of the lane's eight value rows
+          for (int e = 0; e < K::VE; ++e)
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              a[i] = __builtin_amdgcn_perm(vf[2 * i + 1][x][e / 2], vf[2 * i][x][e / 2],
-                                           e % 2 ? 0x07060302u : 0x05040100u);
-            o[r][x * K::VE + e] = E::mma16(a, w, o[r][x * K::VE + e]);
-          }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-#pragma unroll
-          for (int x = 0; x < K::VLOADS; ++x)
-#pragma unroll
-            for (int e = 0; e < K::VE; ++e)
+            for (int r = 0; r < RB; ++r)
               o[r][x * K::VE + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                  __uint_as_float(vf[i][x][e]), s[i / 4][i % 4], o[r][x * K::VE + e], 0, 0, 0);
-      }
+                  __uint_as_float(vf[i][x][e]), sc[r][i / 4][i % 4], o[r][x * K::VE + e], 0, 0, 0);
+    }
+    if (more) {
+      load_values(next);
+      valid = next;
+      if (blk + 2 * DEC_WAVES < end) next = lookup(blk + 2 * DEC_WAVES);
     }
   }
+  if constexpr (Q_LDS) __syncthreads();  // Q's place is the joins'
 
 #pragma unroll
   for (int r = 0; r < RB; ++r) l[r] = add_xor32(add_xor16(l[r]));
@@ -409,11 +478,16 @@ __global__ __launch_bounds__(256) void decode_join_kernel(const DecodeParams p) 
   const int row = id % tiles * ROWS + wave / SPLIT;
   id /= tiles;
   const int hk = id % p.Hk, b = id / p.Hk;
-  const int per = uniform(share_size(p, lane));
-  const int parts = uniform(seq_parts(p, b, per));
+  const Shares all(p, lane);
+  const int parts = uniform(all.parts(seq_blocks(p, b)));
   if (parts == 1) return;  // written by the first kernel
   if (SPLIT == 1 && row >= p.rows) return;
-  const int first = uniform(first_slot(p, b, per, lane));
+  int before = 0;  // the slots of the sequences before b
+#pragma unroll
+  for (int i = 0; i < Shares::HELD; ++i)
+    if (64 * i + lane < b) before += all.parts(all.held[i]);
+  for (int i = 64 * Shares::HELD + lane; i < b; i += 64) before += all.parts(seq_blocks(p, i));
+  const int first = uniform(wave_sum_int(before));
   float m = -INFINITY, l = 0.0f, o[VEC];
 #pragma unroll
   for (int e = 0; e < VEC; ++e) o[e] = 0.0f;
@@ -504,9 +578,7 @@ static int launch_decode(DecodeParams &p, hipStream_t stream) {
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(DEC_WAVES * 64), 0, stream, p);
     return true;
   };
-  constexpr int WIDE = D * Elem<DT>::BYTES;
-  const bool ok = p.rows <= DEC_ROWS ? run(decode_kernel<DT, D, 1, WIDE <= 256 ? 2 : 1>, 1)
-                                     : run(decode_kernel<DT, D, 2, WIDE <= 256 ? 2 : 1>, 2);
+  const bool ok = p.rows <= DEC_ROWS ? run(decode_kernel<DT, D, 1>, 1) : run(decode_kernel<DT, D, 2>, 2);
   if (!ok) return PBGDN_ERR_UNSUPPORTED;
   const long rows = static_cast<long>(p.B) * p.Hk * p.rows;
   if (rows <= JOIN_SPLIT_ROWS) {
@@ -528,12 +600,16 @@ static int dispatch_decode(DecodeParams &p, int D, hipStream_t stream) {
   }
 }
 
-// Parts wanted over all sequences: workgroups for every CU a few times over.
-static int decode_target(int Hk, int rows) {
+// Parts wanted over all sequences: enough workgroups to even out the GPU, few
+// enough that the parts' sums stay small beside the cache. Eight a CU for rows up
+// to 256 bytes (three at a time; 64 contexts up to 16,384 tokens, 128 wide: 364 us,
+// with four 400, with two 459), four for wider ones (two at a time; 233 contexts,
+// 256 wide, 32 query rows: 337 us, with eight 349, with two 343).
+static int decode_target(int Hk, int rows, int row_bytes) {
   DeviceShape shape;
   if (!device_shape(shape)) shape.cus = 256;
   const int tiles = (rows + 2 * DEC_ROWS - 1) / (2 * DEC_ROWS);
-  const int t = 4 * shape.cus / (Hk * tiles);
+  const int t = (row_bytes <= 256 ? 8 : 4) * shape.cus / (Hk * tiles);
   return t > 1 ? t : 1;
 }
 static bool decode_sizes_ok(int B, int T, int Hq, int Hk, int D) {
@@ -555,7 +631,7 @@ extern "C" size_t pbattn_paged_decode_workspace_size(int B, int T, int Hq, int H
   using namespace pbgdn;
   if (!decode_sizes_ok(B, T, Hq, Hk, D)) return 0;
   const int rows = Hq / Hk * T;
-  const size_t slots = static_cast<size_t>(decode_target(Hk, rows)) + B;
+  const size_t slots = static_cast<size_t>(decode_target(Hk, rows, 0)) + B;  // the most of any type
   return slots * Hk * rows * (D * sizeof(float) + sizeof(float2));
 }
 
@@ -604,7 +680,12 @@ extern "C" int pbattn_paged_decode(const void *q, const void *k_cache, const voi
   p.rows = p.group * T;
   p.window = window <= 0 || window > NO_WINDOW ? NO_WINDOW : window;
   p.sinks = sinks < NO_WINDOW ? sinks : NO_WINDOW;
-  p.target = decode_target(Hk, p.rows);
+  // (no more parts than the table's pages, or the window, can need)
+  long most = static_cast<long>(max_pages) * page_size;
+  if (most > static_cast<long>(p.window) + T + p.sinks) most = static_cast<long>(p.window) + T + p.sinks;
+  most = (most + DEC_MIN * DEC_KEYS - 1) / (DEC_MIN * DEC_KEYS) * B;
+  const int wanted = decode_target(Hk, p.rows, D * attn_bytes(dtype));
+  p.target = most < wanted ? static_cast<int>(most > 1 ? most : 1) : wanted;
   const float c = __builtin_fabsf(scale) * LOG2E;
   p.c = c > 1.17549435e-38f ? c : 1.17549435e-38f;
   p.negate = scale < 0.0f;

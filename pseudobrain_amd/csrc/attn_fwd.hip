@@ -18,7 +18,6 @@ namespace pbgdn {
 // Workgroups of 128 rows per CU below which the waves of a workgroup share 32
 // rows instead.
 constexpr int SPLIT_BELOW = 2;
-constexpr float LAG = 8.0f;  // weights stay below 2^8
 
 // Where a workgroup's BM rows lie: their sequence, its keys, and a run of rows'
 // positions.
@@ -108,8 +107,7 @@ struct WaveRows {
     }
   }
 
-  // Scores to weights, against a reference m that moves only when a score passes
-  // it by more than LAG powers of two: most tiles leave the sums as they are.
+  // Scores to weights, against a reference m that lags behind the maximum.
   template <int KB>
   __device__ __forceinline__ void weights(float c, float16_t *sc) {
     float mx = sc[0][0];

@@ -38,6 +38,11 @@ constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 // it would no longer stay near 1 (2^-24 of it), and the kernels subtract first.
 constexpr float EXACT_SCORES = 65536.0f;
 
+// The reference the weights are taken against moves only when a score passes it
+// by more than LAG powers of two: most tiles leave the sums as they are. Weights
+// stay below 2^8.
+constexpr float LAG = 8.0f;
+
 // Element types: bytes, one matrix step of the rows product (a 16-byte unit per
 // lane and side) and the packing of two float32 values.
 template <int DT>
@@ -54,6 +59,10 @@ struct Elem<PBGDN_BF16> {
   __device__ static float4_t mma16(v4u32_t a, v4u32_t b, float4_t c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c,
                                                    0, 0, 0);
+  }
+  __device__ static float4_t mma16(v2u32_t a, v2u32_t b, float4_t c) {  // 16 wide in the contraction
+    return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(i16x4_t, a), __builtin_bit_cast(i16x4_t, b), c,
+                                                     0, 0, 0);
   }
   __device__ static uint32_t pack(float x, float y) {
     return __builtin_bit_cast(uint32_t, bf16x2_t{static_cast<__bf16>(x), static_cast<__bf16>(y)});
@@ -73,6 +82,9 @@ struct Elem<PBGDN_F16> {
   __device__ static float4_t mma16(v4u32_t a, v4u32_t b, float4_t c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0,
                                                   0, 0);
+  }
+  __device__ static float4_t mma16(v2u32_t a, v2u32_t b, float4_t c) {
+    return mfma16(__builtin_bit_cast(half4_t, a), __builtin_bit_cast(half4_t, b), c);
   }
   __device__ static uint32_t pack(float x, float y) {
     return __builtin_bit_cast(uint32_t, half2_t{static_cast<half_t>(x), static_cast<half_t>(y)});
