@@ -639,12 +639,16 @@ static int sink_tiles(const WindowParams &f) {
   return (s + 31) / 32;
 }
 
-// Parts of a key tile's walk: enough workgroups for every CU several times
-// over, none shorter than about 16 query tiles.
+// Parts of a key tile's walk, none shorter than about 16 query tiles: enough
+// workgroups to fill the GPU twice over within a window, whose walks are equal
+// (4 x 2,048 tokens, window 1,024: 650 us in all, with twice as many 690, the
+// join's), twice that without one, where the first keys' walks are the longest
+// (8,192 tokens: 2,565 us, with half as many 3,145).
 static int walk_parts(const WindowParams &f, int B, int bn, int cus) {
   const long tiles = (static_cast<long>(f.Tk) * (f.cu_q ? 1 : B) + bn - 1) / bn * f.Hk;
   const long walk = (f.window < f.Tq ? static_cast<long>(f.window) + bn : f.Tq) * f.group / QR;
-  long parts = tiles > 0 ? (4L * cus + tiles - 1) / tiles : 1;
+  const long want = (f.window < f.Tq ? 2L : 4L) * cus;
+  long parts = tiles > 0 ? (want + tiles - 1) / tiles : 1;
   if (parts > walk / 16) parts = walk / 16;
   return parts < 2 ? 1 : parts > MAX_PARTS ? MAX_PARTS : static_cast<int>(parts);
 }

@@ -15,10 +15,6 @@
 
 namespace pbgdn {
 
-// Workgroups of 128 rows per CU below which the waves of a workgroup share 32
-// rows instead.
-constexpr int SPLIT_BELOW = 2;
-
 // Where a workgroup's BM rows lie: their sequence, its keys, and a run of rows'
 // positions.
 struct Place {
@@ -210,21 +206,19 @@ __global__ __launch_bounds__(NW * 64, WAVES) void window_fwd_kernel(const Window
 // The same for calls with too few rows to fill the GPU: the waves of a workgroup
 // share its 32 rows and take their key tiles in turn, each through tiles of its
 // own with no barrier, and join their sums at the end.
-template <int DT, int D>
+template <int DT, int D, int NW>
 struct Split {
   using L = Tile<DT, D>;
   static constexpr int BN = 32, TILE = BN * L::ROW;
-  static constexpr int NW = L::ROW <= 512 ? 4 : 2;    // as many as the tiles leave room for
   static constexpr int SUMS = 64 * (L::MB * 16 + 2) * 4;  // a wave's sums
   static constexpr int LDS = NW * 2 * TILE > NW / 2 * SUMS ? NW * 2 * TILE : NW / 2 * SUMS;
 };
 
 template <int DT, int D, int NW, int WAVES>
 __global__ __launch_bounds__(NW * 64, WAVES) void window_split_kernel(const WindowParams p) {
-  using F = Split<DT, D>;
+  using F = Split<DT, D, NW>;
   using L = typename F::L;
   constexpr int BN = F::BN, MB = L::MB;
-  static_assert(NW == F::NW, "the waves the LDS is laid out for");
   using Stage = KeyStage<DT, D, BN, 1, (L::ROW < 512)>;
   extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
   PBGDN_POISON_LDS(lds, F::LDS);
@@ -308,15 +302,32 @@ static int launch_rows(WindowParams &p, int B, Kernel kernel, int bm, int nw, in
   return hipGetLastError() == hipSuccess ? PBGDN_OK : PBGDN_ERR_LAUNCH;
 }
 
+template <int DT, int D, int NW, int WAVES>
+static int launch_split(WindowParams &p, int B, hipStream_t stream) {
+  static std::atomic<bool> flags[MAX_DEVICES];
+  return launch_rows(p, B, window_split_kernel<DT, D, NW, WAVES>, 32, NW, Split<DT, D, NW>::LDS, flags, stream);
+}
+
+// Which of the two, by how far the rows fill the GPU: below two workgroups of
+// 128 rows a CU (what its registers hold) the waves share rows, four of them to
+// 32, and eight where even those workgroups number no more than the CUs, as far
+// as their tiles have room. (777 tokens of 32 heads, bf16, 128 wide: 22 us, in
+// workgroups of 128 rows 25; 2,048 tokens of 4 heads, float32, 64 wide: 8 waves
+// 42 us, 4 waves 45, in workgroups of 128 rows 141.)
 template <int DT, int D, int BN, int WAVES>
 static int launch_fwd(WindowParams &p, int B, hipStream_t stream) {
-  static std::atomic<bool> flags[MAX_DEVICES], split_flags[MAX_DEVICES];
+  static std::atomic<bool> flags[MAX_DEVICES];
   using F = Fwd<DT, D, 4, BN>;
-  using S = Split<DT, D>;
+  constexpr int ROW = Tile<DT, D>::ROW;
   DeviceShape shape;
   if (!device_shape(shape)) return PBGDN_ERR_LAUNCH;
-  if (window_slots(p, F::BM) * (p.cu_q ? 1 : B) * p.Hk < SPLIT_BELOW * shape.cus)
-    return launch_rows(p, B, window_split_kernel<DT, D, S::NW, WAVES>, 32, S::NW, S::LDS, split_flags, stream);
+  const long groups = static_cast<long>(p.cu_q ? 1 : B) * p.Hk;
+  if (window_slots(p, F::BM) * groups < 2 * shape.cus) {
+    if constexpr (ROW <= 256) {
+      if (window_slots(p, 32) * groups <= shape.cus) return launch_split<DT, D, 8, WAVES>(p, B, stream);
+    }
+    return launch_split<DT, D, ROW <= 512 ? 4 : 2, WAVES>(p, B, stream);
+  }
   return launch_rows(p, B, window_fwd_kernel<DT, D, 4, BN, WAVES>, F::BM, 4, F::LDS, flags, stream);
 }
 
