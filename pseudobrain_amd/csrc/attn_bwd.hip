@@ -274,6 +274,14 @@ __global__ __launch_bounds__(NW * 64, WAVES) void dkdv_kernel(const BwdParams p)
       *reinterpret_cast<v4u32_t *>(vl + at) = y;
   }
 
+  if constexpr (K::HELD) {
+#pragma unroll
+    for (int s = 0; s < S; ++s) settle(kf[s]);
+  }
+  if constexpr (K::V_HELD) {
+#pragma unroll
+    for (int s = 0; s < S; ++s) settle(vf[s]);
+  }
   float16_t dk[MB], dv[MB];
 #pragma unroll
   for (int m = 0; m < MB; ++m) dk[m] = dv[m] = zero16();
@@ -293,9 +301,10 @@ __global__ __launch_bounds__(NW * 64, WAVES) void dkdv_kernel(const BwdParams p)
     g_at = tt * static_cast<uint32_t>(g_token) + gg * L::ROW + unit;
     index = p.splits == 1 ? tt : gg;
   };
-  uint32_t q_at[K::HELD ? PER_WAVE : 1], g_at[K::HELD ? PER_WAVE : 1];
-  int index[K::HELD ? PER_WAVE : 1];
-  if constexpr (K::HELD) {
+  constexpr bool AT_HELD = K::HELD && PER_WAVE <= 2;  // kept in registers, or worked out at each tile
+  uint32_t q_at[AT_HELD ? PER_WAVE : 1], g_at[AT_HELD ? PER_WAVE : 1];
+  int index[AT_HELD ? PER_WAVE : 1];
+  if constexpr (AT_HELD) {
 #pragma unroll
     for (int w = 0; w < PER_WAVE; ++w) offsets(lane, w, q_at[w], g_at[w], index[w]);
   }
@@ -312,13 +321,13 @@ __global__ __launch_bounds__(NW * 64, WAVES) void dkdv_kernel(const BwdParams p)
     const int left = p.splits == 1 ? t1 - st : G - split * QR, most = p.splits == 1 ? p.tokens : QR;
     const int limit = left < most ? left : most;
     const v4u32_t dq_ = dma_desc(qp, q_size), dg_ = dma_desc(gp, g_size);
-    const int lane_ = K::HELD ? 0 : opaque(threadIdx.x & 63);
+    const int lane_ = AT_HELD ? 0 : opaque(threadIdx.x & 63);
 #pragma unroll
     for (int w = 0; w < PER_WAVE; ++w) {
       const int inst = wave + NW * w;
       uint32_t qa, ga;
       int x;
-      if constexpr (K::HELD)
+      if constexpr (AT_HELD)
         qa = q_at[w], ga = g_at[w], x = index[w];
       else
         offsets(lane_, w, qa, ga, x);
@@ -384,18 +393,13 @@ __global__ __launch_bounds__(NW * 64, WAVES) void dkdv_kernel(const BwdParams p)
     cbase = opaque(cbase);
     float16_t x, y;
     if constexpr (K::HELD)
-      x = L::rows_product(qt, rbase, 0, kf);
+      L::template rows_product<1>(qt, rbase, kf, &x);
     else
       x = L::rows_product_lds(qt, kl, rbase);
-    if constexpr (K::V_HELD) {
-      y = L::rows_product(gt, rbase, 0, vf);
-    } else if constexpr (K::HELD) {
-      y = zero16();
-#pragma unroll
-      for (int s = 0; s < S; ++s) y = E::mma(L::rows(gt, rbase, 0, s), L::rows(vl, rbase, 0, s), y);
-    } else {
+    if constexpr (K::V_HELD)
+      L::template rows_product<1>(gt, rbase, vf, &y);
+    else
       y = L::rows_product_lds(gt, vl, rbase);
-    }
     if (!whole) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
@@ -418,14 +422,9 @@ __global__ __launch_bounds__(NW * 64, WAVES) void dkdv_kernel(const BwdParams p)
         y[e + r] = x[e + r] * d;
       }
     }
-    if constexpr (K::HELD) {
-      L::cols_product(gt, cbase, 0, L::operand(x), dv);
-      L::cols_product(qt, cbase, 0, L::operand(y), dk);
-    } else {
-      const typename L::Operand xo = L::operand(x), yo = L::operand(y);
-      L::cols_product_ahead(gt, cbase, xo, dv);
-      L::cols_product_ahead(qt, cbase, yo, dk);
-    }
+    const typename L::Operand xo = L::operand(x), yo = L::operand(y);
+    L::template cols_product<1>(gt, cbase, &xo, dv);
+    L::template cols_product<1>(qt, cbase, &yo, dk);
   }
   for (; i < tiles; ++i) advance(i);
 
@@ -581,7 +580,14 @@ __global__ __launch_bounds__(NW * 64, WAVES) void dq_kernel(const BwdParams p) {
     gf[s] = *reinterpret_cast<const v4u32_t *>(grow + (2 * s + h) * 16);
     if (f.negate) qf[s] ^= E::BYTES == 2 ? 0x80008000u : 0x80000000u;
   }
-  const float2 st = p.stat[((static_cast<long>(b) * f.Hk + hk) * f.Tq + sq.q0) * G + r];
+#pragma unroll
+  for (int s = 0; s < S; ++s) {
+    settle(qf[s]);
+    settle(gf[s]);
+  }
+  float2 st = p.stat[((static_cast<long>(b) * f.Hk + hk) * f.Tq + sq.q0) * G + r];
+  settle(st.x);
+  settle(st.y);
   const float scale16 = range_scale<DT, D>(p.range);
   float16_t dq[MB];
 #pragma unroll
@@ -602,7 +608,9 @@ __global__ __launch_bounds__(NW * 64, WAVES) void dq_kernel(const BwdParams p) {
     const bool whole = whole_tile(range, u0, BN, w_first, w_last, f.window);
 #pragma unroll
     for (int kb = 0; kb < BN / 32; ++kb) {
-      float16_t x = L::rows_product(kt, rbase, 32 * kb, qf), y = L::rows_product(vt, rbase, 32 * kb, gf);
+      float16_t x, y;
+      L::template rows_product<1>(kt + 32 * kb * L::ROW, rbase, qf, &x);
+      L::template rows_product<1>(vt + 32 * kb * L::ROW, rbase, gf, &y);
       if (!whole) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
@@ -618,7 +626,8 @@ __global__ __launch_bounds__(NW * 64, WAVES) void dq_kernel(const BwdParams p) {
         if constexpr (DT == PBGDN_F16) d *= scale16;
         x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], f.c, -st.x)) * d;
       }
-      L::cols_product(kt, cbase, 32 * kb, L::operand(x), dq);
+      const typename L::Operand w = L::operand(x);
+      L::template cols_product<1>(kt + 32 * kb * L::ROW, cbase, &w, dq);
     }
   }
   for (; it < tiles; ++it) advance(it);

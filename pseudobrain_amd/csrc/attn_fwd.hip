@@ -77,6 +77,8 @@ struct WaveRows {
       q[s] = *reinterpret_cast<const v4u32_t *>(src + (2 * s + h) * 16);
       if (p.negate) q[s] ^= E::BYTES == 2 ? 0x80008000u : 0x80000000u;
     }
+#pragma unroll
+    for (int s = 0; s < S; ++s) settle(q[s]);
     m = -INFINITY;
     l = 0.0f;
 #pragma unroll
@@ -90,8 +92,7 @@ struct WaveRows {
   template <int KB>
   __device__ __forceinline__ void scores(const WindowParams &p, const KeyRange &range, const unsigned char *tile, int u0,
                                          bool whole, float16_t *sc) const {
-#pragma unroll
-    for (int kb = 0; kb < KB; ++kb) sc[kb] = L::rows_product(tile, L::ROW < 512 ? rbase : opaque(rbase), 32 * kb, q);
+    L::template rows_product<KB>(tile, L::ROW < 512 ? rbase : opaque(rbase), q, sc);
     if (!whole) {
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
@@ -144,8 +145,10 @@ struct WaveRows {
 
   template <int KB>
   __device__ __forceinline__ void values(const unsigned char *tile, const float16_t *sc) {
+    typename L::Operand w[KB];
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) L::cols_product(tile, L::ROW < 512 ? cbase : opaque(cbase), 32 * kb, L::operand(sc[kb]), o);
+    for (int kb = 0; kb < KB; ++kb) w[kb] = L::operand(sc[kb]);
+    L::template cols_product<KB>(tile, L::ROW < 512 ? cbase : opaque(cbase), w, o);
   }
 
   // o and lse of the wave's rows; l summed over the lane halves.

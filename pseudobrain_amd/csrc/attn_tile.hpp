@@ -170,36 +170,43 @@ struct Tile {
     return *reinterpret_cast<const float *>(tile + ((base ^ (k * 16)) + hi * 256 + (r0 + 8 * (i / 4) + i % 4) * ROW));
   }
 
-  // X = M[r0 .. r0 + 31] Y^T; y: STEPS units a lane.
-  __device__ static __forceinline__ float16_t rows_product(const unsigned char *tile, uint32_t base, int r0,
-                                                           const v4u32_t *y) {
-    float16_t x = zero16();
-#pragma unroll
-    for (int s = 0; s < STEPS; ++s) x = E::mma(rows(tile, base, r0, s), y[s], x);
-    return x;
-  }
+  // The products, KB x 32 rows of a tile at once. Reads run AHEAD steps before
+  // the matrix instruction that takes them, and nothing is moved across a step:
+  // left to itself the compiler reads one step ahead, and every instruction waits
+  // for LDS (three to four of them, 32 cycles each, cover its latency).
+  static constexpr int AHEAD = 3;
 
-  // The same with both sides in LDS, GROUP steps read ahead of the ones that are
-  // multiplied: bounds the registers that reads in flight take.
-  static constexpr int GROUP = 4;
+  // x[kb] = M[32 kb ..] Y^T; y: STEPS units a lane.
+  template <int KB>
+  __device__ static __forceinline__ void rows_product(const unsigned char *tile, uint32_t base, const v4u32_t *y,
+                                                      float16_t *x) {
+    v4u32_t a[AHEAD + 1];
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) x[kb] = zero16();
+#pragma unroll
+    for (int j = -AHEAD; j < KB * STEPS; ++j) {
+      if (j + AHEAD < KB * STEPS)
+        a[(j + AHEAD) % (AHEAD + 1)] = rows(tile, base, 32 * ((j + AHEAD) % KB), (j + AHEAD) / KB);
+      __builtin_amdgcn_sched_barrier(0);
+      if (j >= 0) x[j % KB] = E::mma(a[j % (AHEAD + 1)], y[j / KB], x[j % KB]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+  // The same for 32 rows with Y's rows in LDS too (two reads a step, of which two
+  // are as much ahead).
   __device__ static __forceinline__ float16_t rows_product_lds(const unsigned char *tile, const unsigned char *other,
                                                                uint32_t base) {
-    v4u32_t a[2][GROUP], b[2][GROUP];
+    constexpr int LDS_AHEAD = 2;
+    v4u32_t a[LDS_AHEAD + 1], b[LDS_AHEAD + 1];
     float16_t x = zero16();
 #pragma unroll
-    for (int s = 0; s < STEPS + GROUP; s += GROUP) {
-      if (s < STEPS) {
-#pragma unroll
-        for (int i = 0; i < GROUP; ++i) {
-          a[s / GROUP % 2][i] = rows(tile, base, 0, s + i);
-          b[s / GROUP % 2][i] = rows(other, base, 0, s + i);
-        }
+    for (int j = -LDS_AHEAD; j < STEPS; ++j) {
+      if (j + LDS_AHEAD < STEPS) {
+        a[(j + LDS_AHEAD) % (LDS_AHEAD + 1)] = rows(tile, base, 0, j + LDS_AHEAD);
+        b[(j + LDS_AHEAD) % (LDS_AHEAD + 1)] = rows(other, base, 0, j + LDS_AHEAD);
       }
       __builtin_amdgcn_sched_barrier(0);
-      if (s > 0) {
-#pragma unroll
-        for (int i = 0; i < GROUP; ++i) x = E::mma(a[(s / GROUP + 1) % 2][i], b[(s / GROUP + 1) % 2][i], x);
-      }
+      if (j >= 0) x = E::mma(a[j % (LDS_AHEAD + 1)], b[j % (LDS_AHEAD + 1)], x);
       __builtin_amdgcn_sched_barrier(0);
     }
     return x;
@@ -222,54 +229,33 @@ struct Tile {
     }
     return o;
   }
-  // z[m] += columns 32 m .. of M[r0 .. r0 + 31] times X, every m, GROUP reads ahead.
-  __device__ static __forceinline__ void cols_product_ahead(const unsigned char *tile, uint32_t base, const Operand &x,
-                                                            float16_t *z) {
-    constexpr int N = (E::BYTES == 2 ? 2 : 16) * MB;
-    v4u32_t a[2][GROUP];
+  // z[m] += columns 32 m .. of M[32 kb ..] times x[kb], every m and kb.
+  template <int KB>
+  __device__ static __forceinline__ void cols_product(const unsigned char *tile, uint32_t base, const Operand *x,
+                                                      float16_t *z) {
+    constexpr int PER = (E::BYTES == 2 ? 2 : 16) * MB, N = KB * PER;  // instructions of 32 rows
+    v4u32_t a[AHEAD + 1];
 #pragma unroll
-    for (int j = 0; j < N + GROUP; j += GROUP) {
-      if (j < N) {
-#pragma unroll
-        for (int i = 0; i < GROUP; ++i) {
-          const int at = (j + i) / MB, m = (j + i) % MB;
-          if constexpr (E::BYTES == 2)
-            a[j / GROUP % 2][i] = cols(tile, base, 0, at, m);
-          else
-            a[j / GROUP % 2][i][0] = __float_as_uint(col1(tile, base, 0, at, m));
-        }
+    for (int j = -AHEAD; j < N; ++j) {
+      const int r = j + AHEAD;
+      if (r < N) {
+        if constexpr (E::BYTES == 2)
+          a[r % (AHEAD + 1)] = cols(tile, base, 32 * (r / PER), r % PER / MB, r % MB);
+        else
+          a[r % (AHEAD + 1)][0] = __float_as_uint(col1(tile, base, 32 * (r / PER), r % PER / MB, r % MB));
       }
       __builtin_amdgcn_sched_barrier(0);
-      if (j > 0) {
-#pragma unroll
-        for (int i = 0; i < GROUP; ++i) {
-          const int at = (j - GROUP + i) / MB, m = (j - GROUP + i) % MB;
-          const v4u32_t y = a[(j / GROUP + 1) % 2][i];
-          if constexpr (E::BYTES == 2)
-            z[m] = E::mma(y, x.w[at], z[m]);
-          else
-            z[m] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(y[0]), __uint_as_float(x.w[at / 4][at % 4]), z[m],
-                                                        0, 0, 0);
-        }
+      if (j >= 0) {
+        const v4u32_t y = a[j % (AHEAD + 1)];
+        const Operand &o = x[j / PER];
+        const int t = j % PER / MB, m = j % MB;
+        if constexpr (E::BYTES == 2)
+          z[m] = E::mma(y, o.w[t], z[m]);
+        else
+          z[m] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(y[0]), __uint_as_float(o.w[t / 4][t % 4]), z[m], 0,
+                                                      0, 0);
       }
       __builtin_amdgcn_sched_barrier(0);
-    }
-  }
-  // z[m] += columns 32 m .. of M[r0 .. r0 + 31] times X, every m.
-  __device__ static __forceinline__ void cols_product(const unsigned char *tile, uint32_t base, int r0,
-                                                      const Operand &x, float16_t *z) {
-    if constexpr (E::BYTES == 2) {
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int m = 0; m < MB; ++m) z[m] = E::mma(cols(tile, base, r0, t, m), x.w[t], z[m]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-#pragma unroll
-        for (int m = 0; m < MB; ++m)
-          z[m] = __builtin_amdgcn_mfma_f32_32x32x2f32(col1(tile, base, r0, i, m), __uint_as_float(x.w[i / 4][i % 4]),
-                                                      z[m], 0, 0, 0);
     }
   }
 };
@@ -291,6 +277,14 @@ __device__ __forceinline__ void store_row(void *dst, const float16_t *z, int h, 
         *reinterpret_cast<float4_t *>(static_cast<unsigned char *>(dst) + 4 * d) = x;
       }
     }
+}
+
+// Loads of x have returned when the code after this runs. (Registers loaded
+// before a loop and first used in it are otherwise waited for inside it, by a
+// counter that the loop's own loads share.)
+template <typename T>
+__device__ __forceinline__ void settle(T &x) {
+  asm volatile("" : "+v"(x));
 }
 
 // x, of which the compiler knows nothing more: what is computed from it inside a
