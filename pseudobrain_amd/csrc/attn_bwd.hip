@@ -24,7 +24,10 @@
 namespace pbgdn {
 
 constexpr int QR = 32;            // rows of a query tile of dkdv_kernel
-constexpr int TAIL_ROWS = 512;    // rows, or a token's heads if more, of one part of the sinks' walk
+// Rows (or a token's heads if more) of one part of the sinks' walk, by how many
+// sinks there are: a part's sums are as many float32 values as there are sinks,
+// for rows of 16 bits read twice, and stay a quarter of that.
+constexpr int tail_rows(int sinks) { return sinks < 8 ? 128 : sinks < 256 ? 16 * sinks : 4096; }
 constexpr int MAX_PARTS = 16;     // parts of an ordinary key tile's walk
 
 struct BwdParams {
@@ -35,12 +38,12 @@ struct BwdParams {
   float2 *stat;       // [B][Hk][Tq G]: (lse log2(e), delta); +inf for a row that sees nothing
   uint32_t *range;    // float16: bits of max |do|, |v|, |delta|
   float *part;        // [2][parts][B][Hk][Tk][D] when parts > 1
-  float *tail;        // [2][tail slots][Hk][sink tiles 32][D]
+  float *tail;        // [2][tail slots][Hk][sinks][D]
   float scale;
   int B, D;
   int parts;          // parts of a key tile's walk
   int key_slots;      // key tiles of a (batch, key head)
-  int sink_tiles;     // 32-key tiles that hold sinks, 0 when no query is beyond their window
+  int sinks;          // keys that stay visible, 0 when no query is beyond their window
   int tail_tokens;    // query tokens of one part of the sinks' walk
   int tail_slots;     // parts of the sinks' walk over all sequences, and slot 0 of each: the window's own part
   // query tiles: `heads` heads of `tokens` tokens each, `splits` tiles for the heads of a token
@@ -166,7 +169,7 @@ struct Dkdv {
   static constexpr int LOADS = QR / L::PER_DMA;  // of one tensor, all waves
   // Registers hold the sums, and K and V rows where they find room beside them
   // (two waves a SIMD up to D = 128 in 16 bits): otherwise LDS does.
-  static constexpr bool HELD = D < 256, V_HELD = HELD && (D == 64 || L::E::BYTES == 4);
+  static constexpr bool HELD = L::ROW <= 512, V_HELD = HELD && (D != 128 || L::E::BYTES == 4);
   static constexpr int VS = HELD ? 0 : BN * L::ROW, KV = VS + (V_HELD ? 0 : BN * L::ROW);  // V's place, both sizes
   static constexpr int BUFS = KV + 2 * BUF <= 160 * 1024 ? 2 : 1;
   static constexpr int BYTES = KV + BUFS * BUF;
@@ -190,8 +193,9 @@ __global__ __launch_bounds__(NW * 64, WAVES) void dkdv_kernel(const BwdParams p)
   int b, hk, seq, tile, part, slot = 0;
   if constexpr (TAIL) {
     int id = blockIdx.x;
-    tile = uniform(id % p.sink_tiles);
-    id /= p.sink_tiles;
+    const int sink_tiles = (p.sinks + 31) / 32;
+    tile = uniform(id % sink_tiles);
+    id /= sink_tiles;
     hk = uniform(id % f.Hk);
     slot = uniform(id / f.Hk);
     // bisection over the sequences' first slots
@@ -428,21 +432,21 @@ __global__ __launch_bounds__(NW * 64, WAVES) void dkdv_kernel(const BwdParams p)
   }
   for (; i < tiles; ++i) advance(i);
 
-  if (key >= sq.nk) return;
+  if (key >= sq.nk || (TAIL && key >= p.sinks)) return;
   const float fk = p.scale / range;
   const long row = (static_cast<long>(b) * f.Tk + sq.k0 + key) * f.Hk + hk;
   if constexpr (TAIL) {
-    const long at = ((static_cast<long>(slot) * f.Hk + hk) * p.sink_tiles * 32 + key) * D;
-    const long half = static_cast<long>(p.tail_slots) * f.Hk * p.sink_tiles * 32 * D;
+    const long at = ((static_cast<long>(slot) * f.Hk + hk) * p.sinks + key) * D;
+    const long half = static_cast<long>(p.tail_slots) * f.Hk * p.sinks * D;
     store_row<PBGDN_F32, D>(p.tail + at, dk, h, fk);
     store_row<PBGDN_F32, D>(p.tail + half + at, dv, h, 1.0f);
   } else if (p.parts > 1) {
     const long half = static_cast<long>(p.B) * f.Tk * f.Hk * D;
     store_row<PBGDN_F32, D>(p.part + part * half + row * D, dk, h, fk);
     store_row<PBGDN_F32, D>(p.part + (p.parts + part) * half + row * D, dv, h, 1.0f);
-  } else if (key < p.sink_tiles * 32 && seq < f.nseq) {
-    const long at = ((static_cast<long>(tail_start(p, seq)) * f.Hk + hk) * p.sink_tiles * 32 + key) * D;
-    const long half = static_cast<long>(p.tail_slots) * f.Hk * p.sink_tiles * 32 * D;
+  } else if (key < p.sinks && seq < f.nseq) {
+    const long at = ((static_cast<long>(tail_start(p, seq)) * f.Hk + hk) * p.sinks + key) * D;
+    const long half = static_cast<long>(p.tail_slots) * f.Hk * p.sinks * D;
     store_row<PBGDN_F32, D>(p.tail + at, dk, h, fk);
     store_row<PBGDN_F32, D>(p.tail + half + at, dv, h, 1.0f);
   } else {
@@ -451,33 +455,67 @@ __global__ __launch_bounds__(NW * 64, WAVES) void dkdv_kernel(const BwdParams p)
   }
 }
 
-// Sums the parts of dk and dv, in order: the window's parts of every key when
-// p.parts > 1, and the sinks' parts. Each thread four elements of a key's row.
-template <int DT, int D>
-__global__ __launch_bounds__(256) void join_kernel(const BwdParams p, long rows, bool sinks_only) {
+// Sums the parts of dk and dv, in a fixed order. The first `sink_blocks`
+// workgroups take a sink each (of a sequence and key head): its threads, four
+// elements of the row each, split the many parts and join through LDS. The rest
+// take the other keys where p.parts > 1, four elements a thread.
+template <int DT>
+__device__ __forceinline__ void store4(void *dst, long at, float4_t x) {
   using E = Elem<DT>;
+  if constexpr (E::BYTES == 2)
+    reinterpret_cast<v2u32_t *>(dst)[at / 4] = v2u32_t{E::pack(x[0], x[1]), E::pack(x[2], x[3])};
+  else
+    reinterpret_cast<float4_t *>(dst)[at / 4] = x;
+}
+template <int DT, int D>
+__global__ __launch_bounds__(256) void join_kernel(const BwdParams p, int sink_blocks) {
   const WindowParams &f = p.f;
-  constexpr int TPR = D / 4;
+  constexpr int TPR = D / 4, GROUPS = 256 / TPR;
+  __shared__ __attribute__((aligned(16))) float sums[GROUPS][D];
   const long half = static_cast<long>(p.B) * f.Tk * f.Hk * D;
-  const int sinkpad = p.sink_tiles * 32;
-  const long tail_half = static_cast<long>(p.tail_slots) * f.Hk * sinkpad * D;
-  for (long i = blockIdx.x * 256L + threadIdx.x; i < rows * TPR; i += gridDim.x * 256L) {
-    const long r = i / TPR;
-    const int d = static_cast<int>(i % TPR) * 4;
-    int seq, hk, key;
-    long row;  // of dk and dv
-    if (sinks_only) {
-      key = static_cast<int>(r % sinkpad);
-      hk = static_cast<int>(r / sinkpad % f.Hk);
-      seq = static_cast<int>(r / sinkpad / f.Hk);
-    } else {
-      hk = static_cast<int>(r % f.Hk);
-      const long token = r / f.Hk;
-      seq = static_cast<int>(token / f.Tk);
-      key = static_cast<int>(token % f.Tk);
+  if (static_cast<int>(blockIdx.x) < sink_blocks) {
+    int id = blockIdx.x;
+    const int key = id % p.sinks;
+    id /= p.sinks;
+    const int hk = id % f.Hk, seq = id / f.Hk;
+    const Seq sq = sequence<true>(f.cu_q, f.cu_k, seq, f.nseq, f.Tq, f.Tk);
+    if (key >= sq.nk) return;
+    const long row = ((f.cu_q ? 0 : static_cast<long>(seq) * f.Tk) + sq.k0 + key) * f.Hk + hk;
+    const int tails = (sq.nq + p.tail_tokens - 1) / p.tail_tokens;
+    const int d = threadIdx.x % TPR * 4, group = threadIdx.x / TPR;
+    const long tail_half = static_cast<long>(p.tail_slots) * f.Hk * p.sinks * D;
+    const long tail = ((static_cast<long>(tail_start(p, seq)) * f.Hk + hk) * p.sinks + key) * D + d;
+    const long step = static_cast<long>(f.Hk) * p.sinks * D;
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      float4_t sum = {0.0f, 0.0f, 0.0f, 0.0f};
+      if (p.parts > 1)
+        for (int a = group; a < p.parts; a += GROUPS)
+          sum += *reinterpret_cast<const float4_t *>(p.part + (which * p.parts + a) * half + row * D + d);
+#pragma unroll 4
+      for (int a = group + (p.parts > 1); a <= tails; a += GROUPS)  // (slot 0: the window's, where it has no parts)
+        sum += *reinterpret_cast<const float4_t *>(p.tail + which * tail_half + tail + a * step);
+      __syncthreads();
+      *reinterpret_cast<float4_t *>(&sums[group][d]) = sum;
+      __syncthreads();
+      if (group == 0) {
+#pragma unroll
+        for (int g = 1; g < GROUPS; ++g) sum += *reinterpret_cast<const float4_t *>(&sums[g][d]);
+        store4<DT>(which ? p.dv : p.dk, row * D + d, sum);
+      }
+    }
+    return;
+  }
+  const long n = static_cast<long>(p.B) * f.Tk * f.Hk * TPR, blocks = gridDim.x - sink_blocks;
+  for (long i = (blockIdx.x - sink_blocks) * 256L + threadIdx.x; i < n; i += blocks * 256L) {
+    const long row = i / TPR;
+    const int d = static_cast<int>(i - row * TPR) * 4;
+    if (p.sinks) {  // the sinks are taken above
+      const long token = row / f.Hk;
+      int seq = static_cast<int>(token / f.Tk), key = static_cast<int>(token - static_cast<long>(seq) * f.Tk);
       if (f.cu_q) {
         const int32_t *cu = f.cu_k ? f.cu_k : f.cu_q;
-        int lo = 0, hi = f.nseq - 1;
+        int lo = 0, hi = f.nseq;
         while (lo < hi) {
           const int mid = (lo + hi + 1) >> 1;
           if (boundary(cu, mid, f.Tk) <= key)
@@ -486,36 +524,17 @@ __global__ __launch_bounds__(256) void join_kernel(const BwdParams p, long rows,
             hi = mid - 1;
         }
         seq = lo;
+        key -= boundary(cu, lo, f.Tk);
       }
+      if (key < p.sinks && seq < f.nseq) continue;
     }
-    const Seq sq = sequence<true>(f.cu_q, f.cu_k, seq, f.nseq, f.Tq, f.Tk);
-    if (sinks_only) {
-      if (key >= sq.nk) continue;
-      row = ((f.cu_q ? 0 : static_cast<long>(seq) * f.Tk) + sq.k0 + key) * f.Hk + hk;
-    } else {
-      row = r;
-      if (f.cu_q) key -= sq.k0;
-    }
-    const bool inside = key >= 0 && key < sq.nk;
-    const int tails = (sq.nq + p.tail_tokens - 1) / p.tail_tokens;
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
       float4_t sum = {0.0f, 0.0f, 0.0f, 0.0f};
-      if (!sinks_only && inside)
-        for (int a = 0; a < p.parts; ++a)
-          sum += *reinterpret_cast<const float4_t *>(p.part + (which * p.parts + a) * half + row * D + d);
-      if (inside && key < sinkpad) {
-        const long slot = tail_start(p, seq);
-        for (int a = sinks_only ? 0 : 1; a <= tails; ++a)
-          sum += *reinterpret_cast<const float4_t *>(p.tail + which * tail_half +
-                                                     (((slot + a) * f.Hk + hk) * sinkpad + key) * D + d);
-      }
-      void *dst = which ? p.dv : p.dk;
-      if constexpr (E::BYTES == 2) {
-        reinterpret_cast<v2u32_t *>(dst)[(row * D + d) / 4] = v2u32_t{E::pack(sum[0], sum[1]), E::pack(sum[2], sum[3])};
-      } else {
-        reinterpret_cast<float4_t *>(dst)[(row * D + d) / 4] = sum;
-      }
+#pragma unroll 4
+      for (int a = 0; a < p.parts; ++a)
+        sum += *reinterpret_cast<const float4_t *>(p.part + (which * p.parts + a) * half + row * D + d);
+      store4<DT>(which ? p.dv : p.dk, row * D + d, sum);
     }
   }
 }
@@ -639,14 +658,10 @@ __global__ __launch_bounds__(NW * 64, WAVES) void dq_kernel(const BwdParams p) {
 // ---------------------------------------------------------------------------
 // Waves (of 32 keys) of a workgroup of dkdv_kernel.
 template <int DT, int D>
-constexpr int dkdv_waves() { return DT == PBGDN_F32 && D == 256 ? 1 : DT == PBGDN_F32 || D == 256 ? 2 : 4; }
+constexpr int dkdv_waves() { return DT != PBGDN_F32 ? 4 : D == 256 ? 1 : 2; }
 
 static bool sinks_beyond(const WindowParams &f) { return f.sinks > 0 && f.window < f.Tk; }
-static int sink_tiles(const WindowParams &f) {
-  if (!sinks_beyond(f)) return 0;
-  const int s = f.sinks < f.Tk ? f.sinks : f.Tk;
-  return (s + 31) / 32;
-}
+static int sink_count(const WindowParams &f) { return !sinks_beyond(f) ? 0 : f.sinks < f.Tk ? f.sinks : f.Tk; }
 
 // Parts of a key tile's walk, none shorter than about 16 query tiles: enough
 // workgroups to fill the GPU twice over within a window, whose walks are equal
@@ -685,22 +700,22 @@ static int launch_bwd(BwdParams &p, hipStream_t stream) {
       p.key_slots = static_cast<int>(slots);
       hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(NW * 64), K::BYTES, stream, p);
     }
-    if (p.sink_tiles) {
+    if (p.sinks) {
       using K = Dkdv<DT, D, 1>;
       static std::atomic<bool> flags[MAX_DEVICES];
       const auto kernel = dkdv_kernel<DT, D, 1, true, DT != PBGDN_F32 && D <= 128 ? 2 : 1>;
       if (!smem_configured(reinterpret_cast<const void *>(kernel), K::BYTES, flags)) return PBGDN_ERR_LAUNCH;
-      const long blocks = static_cast<long>(p.tail_slots) * f.Hk * p.sink_tiles;
+      const long blocks = static_cast<long>(p.tail_slots) * f.Hk * ((p.sinks + 31) / 32);
       if (blocks > 0x7fffffffL) return PBGDN_ERR_UNSUPPORTED;
       hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(64), K::BYTES, stream, p);
     }
-    if (p.parts > 1 || p.sink_tiles) {
-      const bool sinks_only = p.parts == 1;
-      const long rows = sinks_only ? static_cast<long>(f.nseq) * f.Hk * p.sink_tiles * 32
-                                   : static_cast<long>(p.B) * f.Tk * f.Hk;
-      const long want = (rows * (D / 4) + 255) / 256;
-      hipLaunchKernelGGL((join_kernel<DT, D>), dim3(static_cast<unsigned>(want < 65536 ? want : 65536)), dim3(256), 0,
-                         stream, p, rows, sinks_only);
+    if (p.parts > 1 || p.sinks) {
+      const long sinks = static_cast<long>(f.nseq) * f.Hk * p.sinks;
+      const long want = p.parts > 1 ? (static_cast<long>(p.B) * f.Tk * f.Hk * (D / 4) + 255) / 256 : 0;
+      const long blocks = sinks + (want < 65536 ? want : 65536);
+      if (blocks > 0x7fffffffL) return PBGDN_ERR_UNSUPPORTED;
+      hipLaunchKernelGGL((join_kernel<DT, D>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, p,
+                         static_cast<int>(sinks));
     }
   }
   {
@@ -721,18 +736,18 @@ static int launch_bwd(BwdParams &p, hipStream_t stream) {
 // The workspace: statistics, the float16 range, the parts.
 struct Plan {
   size_t stat, range, part, tail, bytes;
-  int parts, sink_tiles, tail_tokens, tail_slots;
+  int parts, sinks, tail_tokens, tail_slots;
 };
 static int key_tile(int dtype, int D) {
-  return 32 * (dtype == PBGDN_F32 ? (D == 256 ? 1 : 2) : D == 256 ? 2 : 4);
+  return 32 * (dtype != PBGDN_F32 ? 4 : D == 256 ? 1 : 2);
 }
 static bool plan(Plan &w, const WindowParams &f, int dtype, int B, int D) {
   DeviceShape shape;
   if (!device_shape(shape)) shape.cus = 256;  // sizes are asked for without a device too
   w.parts = walk_parts(f, B, key_tile(dtype, D), shape.cus);
-  w.sink_tiles = sink_tiles(f);
-  w.tail_tokens = (TAIL_ROWS + f.group - 1) / f.group;
-  const long slots = w.sink_tiles ? tail_slot_count(f.Tq, f.nseq, w.tail_tokens, f.cu_q != nullptr) : 0;
+  w.sinks = sink_count(f);
+  w.tail_tokens = (tail_rows(w.sinks) + f.group - 1) / f.group;
+  const long slots = w.sinks ? tail_slot_count(f.Tq, f.nseq, w.tail_tokens, f.cu_q != nullptr) : 0;
   if (slots > 0x7fffffffL) return false;
   w.tail_slots = static_cast<int>(slots);
   const auto round = [](size_t x) { return (x + 255) & ~static_cast<size_t>(255); };
@@ -740,7 +755,7 @@ static bool plan(Plan &w, const WindowParams &f, int dtype, int B, int D) {
   w.range = round(static_cast<size_t>(B) * f.Tq * f.Hq * sizeof(float2));
   w.part = w.range + 256;
   w.tail = w.part + round(w.parts > 1 ? 2 * sizeof(float) * w.parts * B * f.Tk * f.Hk * static_cast<size_t>(D) : 0);
-  w.bytes = w.tail + round(2 * sizeof(float) * slots * f.Hk * w.sink_tiles * 32 * static_cast<size_t>(D));
+  w.bytes = w.tail + round(2 * sizeof(float) * slots * f.Hk * w.sinks * static_cast<size_t>(D));
   return true;
 }
 
@@ -802,7 +817,7 @@ extern "C" int pbattn_window_bwd(const void *q, const void *k, const void *v, in
   p.B = B;
   p.D = D;
   p.parts = w.parts;
-  p.sink_tiles = w.sink_tiles;
+  p.sinks = w.sinks;
   p.tail_tokens = w.tail_tokens;
   p.tail_slots = w.tail_slots;
   p.heads = p.f.group < QR ? p.f.group : QR;
