@@ -311,12 +311,23 @@ static int launch_split(WindowParams &p, int B, hipStream_t stream) {
   return launch_rows(p, B, window_split_kernel<DT, D, NW, WAVES>, 32, NW, Split<DT, D, NW>::LDS, flags, stream);
 }
 
-// Which of the two, by how far the rows fill the GPU: below two workgroups of
-// 128 rows a CU (what its registers hold) the waves share rows, four of them to
-// 32, and eight where even those workgroups number no more than the CUs, as far
-// as their tiles have room. (777 tokens of 32 heads, bf16, 128 wide: 22 us, in
-// workgroups of 128 rows 25; 2,048 tokens of 4 heads, float32, 64 wide: 8 waves
-// 42 us, 4 waves 45, in workgroups of 128 rows 141.)
+// Which of the two, by how far the rows fill the GPU. n workgroups of 32 rows,
+// whose waves share the keys, up to five a CU (three with rows of 512 bytes and
+// more); of more rows, 128 to a workgroup.
+// Waves of a workgroup: two where a row's walk is no longer than five tiles or
+// workgroups of four would number more than a CU's LDS and registers hold (or two
+// a CU), else four, or eight for narrow heads where the workgroups number no more
+// than the CUs. Measured,
+// us, window 1,024, one sequence (128 rows to a workgroup / 2 / 4 / 8 waves to 32):
+//   32 heads of 128 on 8, bf16      64 tokens   7.8 /  5.7 /  6.8 /  7.9
+//                                  500 tokens  16.5 / 12.3 / 10.9 / 17.2
+//                                  777 tokens  21.6 / 18.5 / 20.5 / 32.5
+//                                1,300 tokens  29.8 / 28.0 / 34.4 / 53.2
+//                                1,700 tokens  32.8 / 39.6 / 46.6 / 67.9
+//   16 heads of 256 on 2, bf16     500 tokens  27.7 / 18.0 / 14.3
+//                                1,300 tokens  48.5 / 36.5 / 44.6
+//                                1,700 tokens  49.4 / 52.8 / 61.7
+//   4 heads of 64, float32       1,300 tokens  90.1 / 44.0 / 27.2 / 25.5
 template <int DT, int D, int BN, int WAVES>
 static int launch_fwd(WindowParams &p, int B, hipStream_t stream) {
   static std::atomic<bool> flags[MAX_DEVICES];
@@ -324,12 +335,17 @@ static int launch_fwd(WindowParams &p, int B, hipStream_t stream) {
   constexpr int ROW = Tile<DT, D>::ROW;
   DeviceShape shape;
   if (!device_shape(shape)) return PBGDN_ERR_LAUNCH;
-  const long groups = static_cast<long>(p.cu_q ? 1 : B) * p.Hk;
-  if (window_slots(p, F::BM) * groups < 2 * shape.cus) {
-    if constexpr (ROW <= 256) {
-      if (window_slots(p, 32) * groups <= shape.cus) return launch_split<DT, D, 8, WAVES>(p, B, stream);
+  const long n = window_slots(p, 32) * (p.cu_q ? 1 : B) * p.Hk;
+  const long keys = p.window < p.Tk ? static_cast<long>(p.window) + p.sinks : p.Tk, walk = (keys + 31) / 32;
+  if (n <= (ROW <= 256 ? 5L : 3L) * shape.cus) {
+    if constexpr (D == 64) {
+      if (n <= shape.cus && walk > 20) return launch_split<DT, D, 8, WAVES>(p, B, stream);
     }
-    return launch_split<DT, D, ROW <= 512 ? 4 : 2, WAVES>(p, B, stream);
+    if constexpr (ROW <= 512) {
+      constexpr int RESIDENT = ROW <= 128 ? 4 : 2;
+      if (n <= RESIDENT * shape.cus && walk > 5) return launch_split<DT, D, 4, WAVES>(p, B, stream);
+    }
+    return launch_split<DT, D, 2, WAVES>(p, B, stream);
   }
   return launch_rows(p, B, window_fwd_kernel<DT, D, 4, BN, WAVES>, F::BM, 4, F::LDS, flags, stream);
 }
