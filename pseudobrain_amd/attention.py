@@ -55,13 +55,14 @@ def _launch(where: str, fn, dev: torch.device, *args) -> None:
         _lib.check(status, where)
 
 
-def _one_device(*tensors) -> torch.device:
+def _one_device(first, *rest) -> torch.device:
     """The tensors' device, by _require_device's rules and errors."""
-    first = tensors[0]
     index = first.get_device()
-    for t in tensors:
-        if t is not None and (index < 0 or t.get_device() != index):
-            return _require_device(*tensors)
+    if index < 0:
+        return _require_device(first, *rest)
+    for t in rest:
+        if t is not None and t.get_device() != index:
+            return _require_device(first, *rest)
     return first.device
 
 
@@ -165,8 +166,9 @@ def _boundaries(cu):
 
 
 def _output(out, q):
+    """The output tensor of a call with these q: `out`, or a new dense one."""
     if out is None:
-        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        return torch.empty_like(q, memory_format=torch.contiguous_format)
     if out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or out.data_ptr() % 16:
         raise ValueError("out must be a contiguous, 16-byte aligned tensor of q's shape and dtype")
     return out
@@ -304,7 +306,7 @@ def window_attention(q, k, v, scale: float, window=None, sinks: int = 0, cu_seql
 # The paged cache.
 # ----------------------------------------------------------------------------
 def _inference_only(where: str, *tensors) -> None:
-    if grad_needed(*tensors):
+    if torch.is_grad_enabled() and any([t.requires_grad for t in tensors]):
         raise RuntimeError(f"{where} has no backward: call it under torch.no_grad() (inference), or use "
                            "window_attention, which has one")
 
@@ -335,13 +337,16 @@ def _caches(k_cache, v_cache):
 
 
 @_plan
-def _decode_plan(q, cache, table, lengths, window, sinks):
-    """Checked sizes (B, T, Hq, Hk, D) of a decode call with tensors of these shapes, window and sinks."""
+def _decode_plan(q, q_dtype, cache, table, lengths, window, sinks, device_index: int):
+    """What a decode call with tensors of these shapes passes on: its checked sizes
+    (B, T, Hq, Hk, D), window, sinks, and the workspace's bytes on the device."""
+    (_, _, hk, dc), dtype = cache
+    if q_dtype != dtype:
+        raise ValueError(f"q ({q_dtype}) and the caches ({dtype}) must have one dtype")
     if len(q) != 4:
         raise ValueError("expected q [B,T,Hq,D]")
     batch, length, hq, d = q
-    hk = cache[2]
-    if d != cache[3] or hq < 1 or hq % hk:
+    if d != dc or hq < 1 or hq % hk:
         raise ValueError("q must have the caches' head width and a multiple of their heads")
     if d not in ATTENTION_HEAD_DIMS:
         raise ValueError(f"cached heads must have a width in {ATTENTION_HEAD_DIMS}")
@@ -349,27 +354,22 @@ def _decode_plan(q, cache, table, lengths, window, sinks):
         raise ValueError(f"paged decoding takes 1 to {MAX_DRAFT} query tokens a sequence, got {length}")
     if len(table) != 2 or table[0] != batch or lengths != (batch,):
         raise ValueError("expected page_table [B, max_pages] and lengths [B]")
-    return ((batch, length, hq, hk, d), *_window_args(window, sinks))
-
-
-@_plan
-def _decode_workspace(device_index: int, *sizes) -> int:
-    with torch.cuda.device(device_index):  # (it depends on the device's compute units)
-        return _lib.attn_lib().pbattn_paged_decode_workspace_size(*sizes)
+    sizes = (batch, length, hq, hk, d)
+    with torch.cuda.device(device_index):  # (the workspace depends on the device's compute units)
+        nbytes = _lib.attn_lib().pbattn_paged_decode_workspace_size(*sizes)
+    return sizes, *_window_args(window, sinks), nbytes
 
 
 def _decode(q, k_cache, v_cache, page_table, lengths, scale, window, sinks, out=None, return_lse=False):
     dev = _one_device(q, k_cache, v_cache, page_table, lengths)
     cache, steps, code, at = _caches(k_cache, v_cache)
-    sizes, window, sinks = _decode_plan(q.shape, cache, page_table.shape, lengths.shape,
-                                        None if window is None else int(window), int(sinks))
-    if q.dtype != k_cache.dtype:
-        raise ValueError(f"q ({q.dtype}) and the caches ({k_cache.dtype}) must have one dtype")
+    sizes, window, sinks, nbytes = _decode_plan(
+        q.shape, q.dtype, (cache, k_cache.dtype), page_table.shape, lengths.shape,
+        None if window is None else int(window), int(sinks), dev.index)
     q = _aligned(q.contiguous(), 16)
     page_table, lengths = _boundaries(page_table), _boundaries(lengths)
     out = _output(out, q)
     lse = torch.empty(q.shape[:3], dtype=torch.float32, device=dev) if return_lse else None
-    nbytes = _decode_workspace(dev.index, *sizes)
     workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     _launch("pbattn_paged_decode", _lib.attn_lib().pbattn_paged_decode, dev, q.data_ptr(), *at, code, steps, cache[1],
             cache[0], page_table.data_ptr(), page_table.shape[1], lengths.data_ptr(), out.data_ptr(), _lib.ptr(lse),

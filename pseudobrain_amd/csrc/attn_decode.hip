@@ -73,6 +73,11 @@ struct Shares {
   int per;
 
   __device__ __forceinline__ Shares(const DecodeParams &p, int lane) {
+    if (p.B == 1) {  // one request: nothing to add up over the lanes
+      held[0] = seq_blocks(p, 0);
+      share(p, held[0]);
+      return;
+    }
     long total = 0;
 #pragma unroll
     for (int i = 0; i < HELD; ++i) {
@@ -80,8 +85,12 @@ struct Shares {
       total += held[i];
     }
     for (int b = 64 * HELD + lane; b < p.B; b += 64) total += seq_blocks(p, b);
-    total = wave_sum_long(total);
-    const int even = static_cast<int>((total + p.target - 1) / p.target);
+    share(p, wave_sum_long(total));
+  }
+  __device__ __forceinline__ void share(const DecodeParams &p, long total) {
+    const int even = total <= 0x7fffffff - p.target
+                         ? (static_cast<int>(total) + p.target - 1) / p.target
+                         : static_cast<int>((total + p.target - 1) / p.target);
     const int whole = (even + DEC_MIN - 1) / DEC_MIN * DEC_MIN;
     per = uniform(whole > DEC_MIN ? whole : DEC_MIN);
   }
@@ -94,6 +103,12 @@ struct Share {
 __device__ __forceinline__ Share share_of_slot(const DecodeParams &p, int slot, int lane) {
   const Shares all(p, lane);
   Share s{-1, 0, 0, all.per};
+  if (p.B == 1) {
+    s.parts = all.parts(all.held[0]);
+    s.part = slot;
+    s.seq = slot < s.parts ? 0 : -1;
+    return s;
+  }
   int base = 0;
   const auto look = [&](int b0, int blocks) __attribute__((always_inline)) {
     const int mine = b0 + lane < p.B ? all.parts(blocks) : 0;
@@ -462,13 +477,13 @@ __global__ __launch_bounds__(DEC_WAVES * 64, (Dec<DT, D>::OCC)) void decode_kern
   }
 }
 
-// Joins a sequence's parts, SPLIT waves to a (sequence, query row and head):
-// the weights of 64 parts at a time, one a lane, then their outputs, whose loads
-// wait for nothing but each other. Four waves a row where there are few rows,
+// Joins a sequence's parts, SPLIT waves to a (sequence, query row and head),
+// eight parts of a wave at a time: their outputs and their weights' statistics,
+// one a lane, are fetched together. Four waves a row where there are few rows,
 // one where there are many.
 template <int DT, int D, int SPLIT>
 __global__ __launch_bounds__(256) void decode_join_kernel(const DecodeParams p) {
-  constexpr int VEC = D / 64, ROWS = 4 / SPLIT;  // rows of a workgroup
+  constexpr int VEC = D / 64, ROWS = 4 / SPLIT, AT_ONCE = 8;  // ROWS: rows of a workgroup
   __shared__ float acc[SPLIT > 1 ? 4 : 1][D], stat[4][2];
   PBGDN_POISON_LDS(acc, sizeof(acc));
   PBGDN_POISON_SYNC();
@@ -482,31 +497,40 @@ __global__ __launch_bounds__(256) void decode_join_kernel(const DecodeParams p) 
   const int parts = uniform(all.parts(seq_blocks(p, b)));
   if (parts == 1) return;  // written by the first kernel
   if (SPLIT == 1 && row >= p.rows) return;
-  int before = 0;  // the slots of the sequences before b
+  int first = 0;  // the sequence's first slot
+  if (b > 0) {
 #pragma unroll
-  for (int i = 0; i < Shares::HELD; ++i)
-    if (64 * i + lane < b) before += all.parts(all.held[i]);
-  for (int i = 64 * Shares::HELD + lane; i < b; i += 64) before += all.parts(seq_blocks(p, i));
-  const int first = uniform(wave_sum_int(before));
+    for (int i = 0; i < Shares::HELD; ++i)
+      if (64 * i + lane < b) first += all.parts(all.held[i]);
+    for (int i = 64 * Shares::HELD + lane; i < b; i += 64) first += all.parts(seq_blocks(p, i));
+    first = uniform(wave_sum_int(first));
+  }
   float m = -INFINITY, l = 0.0f, o[VEC];
 #pragma unroll
   for (int e = 0; e < VEC; ++e) o[e] = 0.0f;
-  for (int i0 = w; i0 < parts; i0 += 64 * SPLIT) {  // this wave's parts: i0, i0 + SPLIT, ...
-    const int mine = i0 + lane * SPLIT, count = (parts - i0 + SPLIT - 1) / SPLIT, n = count < 64 ? count : 64;
+  for (int i0 = w; i0 < parts; i0 += AT_ONCE * SPLIT) {  // this wave's parts: i0, i0 + SPLIT, ...
+    const int count = (parts - i0 + SPLIT - 1) / SPLIT, n = count < AT_ONCE ? count : AT_ONCE;
     const long at0 = (static_cast<long>(first + i0) * p.Hk + hk) * p.rows + row;
     const long step = static_cast<long>(SPLIT) * p.Hk * p.rows;
-    const float2 s = mine < parts ? p.stat[at0 + lane * step] : make_float2(-INFINITY, 0.0f);
+    float x[AT_ONCE][VEC];
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i) {
+      const float *src = p.part + (at0 + (i < n ? i : 0) * step) * D + lane * VEC;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) x[i][e] = src[e];
+    }
+    const float2 s = lane < n ? p.stat[at0 + lane * step] : make_float2(-INFINITY, 0.0f);
     const float top = fmaxf(m, wave_max(s.x)), base = top == -INFINITY ? 0.0f : top;
     const float f = __builtin_amdgcn_exp2f(s.x - base), keep = __builtin_amdgcn_exp2f(m - base);
     m = top;
     l = l * keep + wave_sum(s.y * f);
 #pragma unroll
     for (int e = 0; e < VEC; ++e) o[e] *= keep;
-#pragma unroll 8
-    for (int i = 0; i < n; ++i) {
-      const float fi = __shfl(f, i, 64);
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) o[e] += p.part[(at0 + i * step) * D + lane * VEC + e] * fi;
+    for (int i = 0; i < AT_ONCE; ++i) {
+      const float fi = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), i));
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) o[e] += i < n ? x[i][e] * fi : 0.0f;
     }
   }
   if constexpr (SPLIT > 1) {
