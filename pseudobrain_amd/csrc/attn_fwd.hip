@@ -151,6 +151,56 @@ struct WaveRows {
     L::template cols_product<KB>(tile, L::ROW < 512 ? cbase : opaque(cbase), w, o);
   }
 
+  // A value that some rows of a tile see and others do not (a later token's, one
+  // the window has passed) enters the products of them all, with weight zero where
+  // it is not seen: harmless unless it is infinite or NaN. Rows that end so are
+  // worked out again, key by key, from what they see alone. Uniform over the wave.
+  __device__ __forceinline__ bool spoiled() const {
+    float x = 0.0f;
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) x = __builtin_fmaf(o[i][e], 0.0f, x);  // zero, or NaN
+    return __any(x != 0.0f);
+  }
+  __device__ __forceinline__ void redo(const WindowParams &p, const KeyRange &range, const unsigned char *k,
+                                                 const unsigned char *v) {
+    m = -INFINITY;
+    l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < MB; ++i) o[i] = zero16();
+    for (int u = 0; u < range.count; ++u) {
+      const long j = u < range.sinks ? u : u + range.delta;
+      const unsigned char *kr = k + j * p.k.token, *vr = v + j * p.v.token;
+      float dot = 0.0f;
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        const v4u32_t x = *reinterpret_cast<const v4u32_t *>(kr + (2 * s + h) * 16);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if constexpr (E::BYTES == 2)
+            dot += E::low(x[i]) * E::low(q[s][i]) + E::high(x[i]) * E::high(q[s][i]);
+          else
+            dot += __uint_as_float(x[i]) * __uint_as_float(q[s][i]);
+        }
+      }
+      dot = add_xor32(dot);
+      if (!sees(pos, static_cast<int>(j), p.window, p.sinks)) continue;
+      const float top = fmaxf(m, dot), base = top == -INFINITY ? 0.0f : top;
+      const float keep = __builtin_amdgcn_exp2f((m - base) * p.c), w = __builtin_amdgcn_exp2f((dot - base) * p.c);
+      m = top;
+      l = l * keep + w;
+#pragma unroll
+      for (int i = 0; i < MB; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int d = 32 * i + acc_row(e, h);
+          const float x = load_elem(vr, d, DT);
+          o[i][e] = o[i][e] * keep + w * x;
+        }
+    }
+  }
+
   // o and lse of the wave's rows; l summed over the lane halves.
   __device__ __forceinline__ void store(const WindowParams &p) const {
     const float inv = l > 0.0f ? 1.0f / l : l;  // no key seen: zeros (a NaN stays)
@@ -203,6 +253,7 @@ __global__ __launch_bounds__(NW * 64, WAVES) void window_fwd_kernel(const Window
   }
   for (; it < tiles; ++it) advance(it);
   r.l = add_xor32(r.l);
+  if (r.spoiled()) r.redo(p, range, w.k, w.v);
   r.store(p);
 }
 
@@ -291,7 +342,9 @@ __global__ __launch_bounds__(NW * 64, WAVES) void window_split_kernel(const Wind
         }
     }
   }
-  if (wave == 0) r.store(p);
+  if (wave != 0) return;
+  if (r.spoiled()) r.redo(p, range, w.k, w.v);
+  r.store(p);
 }
 
 template <typename Kernel>

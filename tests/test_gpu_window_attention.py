@@ -215,6 +215,34 @@ def test_lowest_scores_and_visible_nan():
     assert bad[70:90].all() and not bad[:70].any() and not bad[90:].any()
 
 
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("heads,length", [((4, 2), 150), ((32, 8), 1400)])
+def test_a_bad_value_reaches_only_the_rows_that_see_it(d, dtype, heads, length):
+    """NaN and infinite values (and a NaN key) in tiles that also hold seen keys: rows
+    before them and past their window come out as without them, rows that see them
+    do not. Both forward kernels (the longer call fills the GPU)."""
+    window, sinks = 40, 2
+    q, k, v, *_ = make(1, length, length, *heads, d, dtype, 30)
+    bad = {5: float("nan"), 70: float("inf"), length - 2: float("nan")}
+    with torch.no_grad():
+        clean = at.window_attention(q, k, v, d ** -0.5, window, sinks)
+        for j, x in bad.items():
+            v[0, j, :, 3] = x
+        k[0, 100] = float("nan")
+        got, lse = at.window_attention(q, k, v, d ** -0.5, window, sinks, return_lse=True)
+    pos = torch.arange(length, device=DEV)
+    sees = [(pos >= j) & (pos - j < window) for j in (*bad, 100)]
+    hit = torch.stack(sees).any(0)
+    assert torch.isfinite(got[0, ~hit]).all() and torch.isfinite(lse[0, ~sees[-1]]).all()
+    # both sides within a bound of u (|o| + sum p |v|) of the truth, values up to 6
+    bound = 4 * 6 * oa.UNIT[NAMES[dtype]] + 1e-4
+    assert (got[0, ~hit].float() - clean[0, ~hit].float()).abs().max() <= bound
+    for seen in sees[:-1]:
+        assert not torch.isfinite(got[0, seen, :, 3]).any()
+    assert torch.isnan(got[0, sees[-1]]).all()
+
+
 def test_runs_are_equal_and_follow_the_stream():
     """Equal inputs give equal bits, on another stream too."""
     q, k, v, go, _ = make(2, 700, 700, 8, 2, 128, torch.bfloat16, 15)
