@@ -5,13 +5,14 @@
 //                 delta = do . o - dlse, stored by (batch, key head) in the
 //                 row order of the tiles below; float16 also takes the maxima
 //                 that bound ds
+//   dq_kernel     the forward's walk over keys: S^T, dP^T, dS^T, dQ^T += K^T dS^T
+//                 (first where rows see few keys: delta made exact)
 //   dkdv_kernel   a wave owns 32 keys, with K and V rows and the sums of dK^T
 //                 and dV^T in registers, and walks the queries that see them
 //                 (all heads of the group): S = Q K^T, P, dV^T += dO^T P,
 //                 dP = dO V^T, dS, dK^T += Q^T dS. Long or few walks are split
 //                 into parts; the sinks, which every later query sees, are
 //                 always walked in parts beyond their window
-//   dq_kernel     the forward's walk over keys: S^T, dP^T, dS^T, dQ^T += K^T dS^T
 //   join_kernel   sums of parts, in a fixed order
 // Recomputing S and dP on both sides costs two products of seven, and saves
 // float32 sums of dQ in memory and their atomics.
@@ -61,7 +62,8 @@ inline long tail_slot_count(int Tq, int nseq, int tokens, bool packed) {
 
 // ---------------------------------------------------------------------------
 // float16's range: ds is bounded by max |do| max |v| D + max |delta|; a power
-// of two brings that bound to 2^14.
+// of two brings that bound to 2^14 (a corrected delta, see dq_kernel, passes it
+// by its correction, far less than what 2^16 leaves).
 // ---------------------------------------------------------------------------
 template <int DT, int D>
 __device__ __forceinline__ float range_scale(const uint32_t *range) {
@@ -541,11 +543,20 @@ __global__ __launch_bounds__(256) void join_kernel(const BwdParams p, int sink_b
 
 // ---------------------------------------------------------------------------
 // dQ: the forward's rows and walk.
+//
+// delta = do . o is taken from an o that the forward rounded to 16 bits, after
+// weights of 16 bits: with few keys, whose weights are large, that is as much as
+// the rounding of dS itself (17 keys, bf16: dq 0.0029 of its norm off, with an
+// exact delta 0.0024; 1,024 keys 0.0025 and 0.0024). As the sum of dS over a
+// row's keys is dlse, what it comes to instead is delta's error. Where a walk is
+// of 128 keys at most, the rows walk once for that sum, and again with the delta
+// corrected by it, which is kept for dkdv_kernel, so this kernel comes first.
 // ---------------------------------------------------------------------------
 template <int DT, int D, int NW, int BN>
 struct Dq {
   using L = Tile<DT, D>;
   static constexpr int BM = 32 * NW, TILE = BN * L::ROW, LDS = 4 * TILE;
+  static constexpr int EXACT_TILES = DT == PBGDN_F32 ? 0 : 128 / BN;  // walks whose delta is corrected
 };
 
 template <int DT, int D, int NW, int BN, int WAVES>
@@ -604,7 +615,8 @@ __global__ __launch_bounds__(NW * 64, WAVES) void dq_kernel(const BwdParams p) {
     settle(qf[s]);
     settle(gf[s]);
   }
-  float2 st = p.stat[((static_cast<long>(b) * f.Hk + hk) * f.Tq + sq.q0) * G + r];
+  float2 *stat = p.stat + ((static_cast<long>(b) * f.Hk + hk) * f.Tq + sq.q0) * G + r;
+  float2 st = *stat;
   settle(st.x);
   settle(st.y);
   const float scale16 = range_scale<DT, D>(p.range);
@@ -618,8 +630,52 @@ __global__ __launch_bounds__(NW * 64, WAVES) void dq_kernel(const BwdParams p) {
     block_sync();
     if (it + 1 < tiles) stage.tile(it + 1, lds + ((it + 1) & 1) * F::TILE);
   };
+  // Scores and dP of 32 keys, those from u0 on of the range; `whole`: every row sees all of them.
+  const auto products = [&](const unsigned char *kt, const unsigned char *vt, int u0, bool whole, float16_t &x,
+                            float16_t &y) __attribute__((always_inline)) {
+    L::template rows_product<1>(kt, rbase, qf, &x);
+    L::template rows_product<1>(vt, rbase, gf, &y);
+    if (!whole) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int u = u0 + acc_row(i, h);
+        const bool seen = sees(pos, u < range.sinks ? u : u + range.delta, f.window, f.sinks);
+        x[i] = seen ? x[i] : -INFINITY;
+        y[i] = seen ? y[i] : 0.0f;
+      }
+    }
+  };
   const int mine = wave_tiles(range, tiles, w_last, BN);
   int it = 0;
+  if constexpr (F::EXACT_TILES > 0) {
+    if (tiles > 0 && tiles <= F::EXACT_TILES) {
+      float sum = 0.0f;
+      for (; it < mine; ++it) {
+        advance(it);
+        const unsigned char *kt = lds + (it & 1) * F::TILE, *vt = kt + 2 * F::TILE;
+        const bool whole = whole_tile(range, it * BN, BN, w_first, w_last, f.window);
+#pragma unroll 1
+        for (int kb = 0; kb < BN / 32; ++kb) {
+          float16_t x, y;
+          products(kt + 32 * kb * L::ROW, vt + 32 * kb * L::ROW, it * BN + 32 * kb, whole, x, y);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            sum = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(x[i], f.c, -st.x)), y[i] - st.y, sum);
+          }
+        }
+      }
+      for (; it < tiles; ++it) advance(it);
+      sum += __shfl_xor(sum, 32, 64);
+      if (st.x != INFINITY) {
+        st.y += p.grad_lse ? sum - p.grad_lse[out] : sum;
+        if (h == 0 && row < total) stat->y = st.y;
+      }
+      settle(st.y);
+      it = 0;
+      block_sync();
+      stage.tile(0, lds);
+    }
+  }
   for (; it < mine; ++it) {
     advance(it);
     const unsigned char *kt = lds + (it & 1) * F::TILE, *vt = kt + 2 * F::TILE;
@@ -628,17 +684,7 @@ __global__ __launch_bounds__(NW * 64, WAVES) void dq_kernel(const BwdParams p) {
 #pragma unroll
     for (int kb = 0; kb < BN / 32; ++kb) {
       float16_t x, y;
-      L::template rows_product<1>(kt + 32 * kb * L::ROW, rbase, qf, &x);
-      L::template rows_product<1>(vt + 32 * kb * L::ROW, rbase, gf, &y);
-      if (!whole) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int u = u0 + 32 * kb + acc_row(i, h);
-          const bool seen = sees(pos, u < range.sinks ? u : u + range.delta, f.window, f.sinks);
-          x[i] = seen ? x[i] : -INFINITY;
-          y[i] = seen ? y[i] : 0.0f;
-        }
-      }
+      products(kt + 32 * kb * L::ROW, vt + 32 * kb * L::ROW, u0 + 32 * kb, whole, x, y);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         float d = y[i] - st.y;
@@ -685,6 +731,18 @@ static int launch_bwd(BwdParams &p, hipStream_t stream) {
   if (!device_shape(shape)) return PBGDN_ERR_LAUNCH;
   if constexpr (DT == PBGDN_F16) hipLaunchKernelGGL(range_zero_kernel, dim3(1), dim3(64), 0, stream, p.range);
   hipLaunchKernelGGL((stat_kernel<DT, D>), dim3(shape.cus * 8), dim3(256), 0, stream, p);
+  {
+    constexpr int DQ_NW = 4, DQ_BN = DT == PBGDN_F32 ? (D == 64 ? 64 : 32) : D == 256 ? 32 : 64;
+    constexpr int W = DT != PBGDN_F32 && D <= 128 ? 2 : 1;
+    using F = Dq<DT, D, DQ_NW, DQ_BN>;
+    static std::atomic<bool> flags[MAX_DEVICES];
+    const auto kernel = dq_kernel<DT, D, DQ_NW, DQ_BN, W>;
+    if (!smem_configured(reinterpret_cast<const void *>(kernel), F::LDS, flags)) return PBGDN_ERR_LAUNCH;
+    const long slots = window_slots(f, F::BM), blocks = slots * nb * f.Hk;
+    if (blocks > 0x7fffffffL) return PBGDN_ERR_UNSUPPORTED;
+    f.slots = static_cast<int>(slots);
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(DQ_NW * 64), F::LDS, stream, p);
+  }
 
   constexpr int NW = dkdv_waves<DT, D>(), BN = 32 * NW;
   if (f.Tk > 0) {
@@ -717,18 +775,6 @@ static int launch_bwd(BwdParams &p, hipStream_t stream) {
       hipLaunchKernelGGL((join_kernel<DT, D>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, p,
                          static_cast<int>(sinks));
     }
-  }
-  {
-    constexpr int DQ_NW = 4, DQ_BN = DT == PBGDN_F32 ? (D == 64 ? 64 : 32) : D == 256 ? 32 : 64;
-    constexpr int W = DT != PBGDN_F32 && D <= 128 ? 2 : 1;
-    using F = Dq<DT, D, DQ_NW, DQ_BN>;
-    static std::atomic<bool> flags[MAX_DEVICES];
-    const auto kernel = dq_kernel<DT, D, DQ_NW, DQ_BN, W>;
-    if (!smem_configured(reinterpret_cast<const void *>(kernel), F::LDS, flags)) return PBGDN_ERR_LAUNCH;
-    const long slots = window_slots(f, F::BM), blocks = slots * nb * f.Hk;
-    if (blocks > 0x7fffffffL) return PBGDN_ERR_UNSUPPORTED;
-    f.slots = static_cast<int>(slots);
-    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(DQ_NW * 64), F::LDS, stream, p);
   }
   return hipGetLastError() == hipSuccess ? PBGDN_OK : PBGDN_ERR_LAUNCH;
 }

@@ -258,6 +258,26 @@ def test_runs_are_equal_and_follow_the_stream():
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("length,window,sinks", [(17, None, 0), (60, None, 0), (100, 40, 3)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("hq,hk,d", [(8, 2, 128), (2, 2, 64), (8, 1, 256)])
+def test_gradients_of_rows_with_few_keys(length, window, sinks, dtype, hq, hk, d):
+    """dq and dk carry two roundings to 16 bits, of dS and of the result, independent and alike in size:
+    sqrt(2) times what the result's alone costs, in norm, and 6% for the sample. delta's own error, from an
+    output of few large rounded weights, is no third one."""
+    q, k, v, go, glse = make(8, length, length, hq, hk, d, dtype, 19)
+    o, lse = at.window_attention_fwd(q, k, v, d ** -0.5, window, sinks)
+    got = at.window_attention_bwd(q, k, v, o, lse, go, d ** -0.5, window, sinks, grad_lse=glse)
+    args = [f64(x) for x in (q, k, v)]
+    refs = [oa.attention(*(x[b] for x in args), d ** -0.5, window, sinks, f64(go)[b], f64(glse)[b]) for b in range(8)]
+    for n, x in zip(("dq", "dk"), got):
+        want = np.stack([r[n] for r in refs])
+        rounded = f64(torch.from_numpy(want).to(dtype))
+        error, unit = (np.linalg.norm(y - want) / np.linalg.norm(want) for y in (f64(x), rounded))
+        print(f"[few keys {n}] {error:.3e}, the rounding's {unit:.3e}, {error / unit:.3f} of it", flush=True)
+        assert error <= 1.5 * unit, n
+
+
 def test_gradients_against_differences():
     """Central differences of the device's own forward, float32, along random directions."""
     q, k, v, go, _ = make(1, 90, 90, 4, 2, 64, torch.float32, 16)
