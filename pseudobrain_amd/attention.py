@@ -29,6 +29,8 @@ import ctypes
 import functools
 
 import torch
+from torch.autograd.function import once_differentiable
+from torch.utils._python_dispatch import _get_current_dispatch_mode
 
 from . import _lib
 from .gated_deltanet import _aligned, _pad_last, _require_device, _width_at_least, grad_needed
@@ -244,13 +246,17 @@ def _(q, k, v, scale, window, sinks, cu_seqlens, cu_seqlens_k):
     return q.new_empty(q.shape), q.new_empty(q.shape[:3], dtype=torch.float32)
 
 
+def _backward_launch(q, k, v, o, lse, grad_o, grad_lse, scale, window, sinks, cu_seqlens, cu_seqlens_k):
+    return window_attention_bwd(q, k, v, o, lse, grad_o, scale, window, sinks, cu_seqlens, cu_seqlens_k, grad_lse)
+
+
 @torch.library.custom_op("pbgdn::window_attention_backward", mutates_args=(),
                          schema="(Tensor q, Tensor k, Tensor v, Tensor o, Tensor lse, Tensor grad_o, "
                                 "Tensor? grad_lse, float scale, int? window, int sinks, Tensor? cu_seqlens, "
                                 "Tensor? cu_seqlens_k) -> (Tensor, Tensor, Tensor)")
 def window_attention_backward_op(q, k, v, o, lse, grad_o, grad_lse, scale, window, sinks, cu_seqlens, cu_seqlens_k):
     """(dq, dk, dv) in q's dtype (window_attention_bwd)."""
-    return window_attention_bwd(q, k, v, o, lse, grad_o, scale, window, sinks, cu_seqlens, cu_seqlens_k, grad_lse)
+    return _backward_launch(q, k, v, o, lse, grad_o, grad_lse, scale, window, sinks, cu_seqlens, cu_seqlens_k)
 
 
 @window_attention_backward_op.register_fake
@@ -266,17 +272,44 @@ def _attention_setup(ctx, inputs, output):
     ctx.set_materialize_grads(False)
 
 
-def _attention_grad(ctx, grad_o, grad_lse):
-    if grad_o is None and grad_lse is None:
-        return (None,) * 8
-    q, k, v, o, lse, cu_seqlens, cu_seqlens_k = ctx.saved_tensors
-    grad_o = torch.zeros_like(o) if grad_o is None else grad_o
-    dq, dk, dv = window_attention_backward_op(q, k, v, o, lse, grad_o, grad_lse, ctx.scale, ctx.window, ctx.sinks,
-                                              cu_seqlens, cu_seqlens_k)
-    return dq, dk.to(k.dtype), dv.to(v.dtype), None, None, None, None, None
+def _gradients(backward):
+    """The backward formula, by `backward`: the op, or its launch itself."""
+    def formula(ctx, grad_o, grad_lse):
+        if grad_o is None and grad_lse is None:
+            return (None,) * 8
+        q, k, v, o, lse, cu_seqlens, cu_seqlens_k = ctx.saved_tensors
+        grad_o = torch.zeros_like(o) if grad_o is None else grad_o
+        dq, dk, dv = backward(q, k, v, o, lse, grad_o, grad_lse, ctx.scale, ctx.window, ctx.sinks, cu_seqlens,
+                              cu_seqlens_k)
+        return dq, dk.to(k.dtype), dv.to(v.dtype), None, None, None, None, None
+    return formula
 
 
-window_attention_op.register_autograd(_attention_grad, setup_context=_attention_setup)
+window_attention_op.register_autograd(_gradients(window_attention_backward_op), setup_context=_attention_setup)
+
+
+def _untraced(*tensors) -> bool:
+    """Ordinary tensors that nothing compiles, traces or transforms."""
+    return (not torch.compiler.is_compiling() and _get_current_dispatch_mode() is None
+            and not torch._C._are_functorch_transforms_active() and all(type(t) in (torch.Tensor, torch.nn.Parameter) for t in tensors))
+
+
+class _WindowAttention(torch.autograd.Function):
+    """The op and its gradients without the op's dispatch, which costs more than a short call."""
+    _launched = staticmethod(_gradients(_backward_launch))
+    _traced = staticmethod(_gradients(window_attention_backward_op))
+
+    @staticmethod
+    def forward(ctx, *inputs):
+        output = window_attention_fwd(*inputs)
+        _attention_setup(ctx, inputs, output)
+        return output
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_o, grad_lse):
+        tensors = [t for t in (grad_o, grad_lse) if t is not None]
+        return (_WindowAttention._launched if _untraced(*tensors) else _WindowAttention._traced)(ctx, grad_o, grad_lse)
 
 
 def window_attention(q, k, v, scale: float, window=None, sinks: int = 0, cu_seqlens=None, cu_seqlens_k=None, *,
@@ -292,9 +325,10 @@ def window_attention(q, k, v, scale: float, window=None, sinks: int = 0, cu_seql
     _one_device(q, k, v, cu_seqlens, cu_seqlens_k)
     if d not in ATTENTION_HEAD_DIMS:
         q, k, v = (_pad_last(x, _width_at_least(d, ATTENTION_HEAD_DIMS)) for x in (q, k, v))
-    if grad_needed(q, k, v) or torch.compiler.is_compiling():
+    traced = not _untraced(q, k, v)
+    if traced or grad_needed(q, k, v):
         window = None if window is None else int(window)
-        o, lse = window_attention_op(q, k, v, float(scale), window, int(sinks), cu_seqlens, cu_seqlens_k)
+        o, lse = (window_attention_op if traced else _WindowAttention.apply)(q, k, v, float(scale), window, int(sinks), cu_seqlens, cu_seqlens_k)
     else:
         o, lse = window_attention_fwd(q, k, v, scale, window, sinks, cu_seqlens, cu_seqlens_k, return_lse=return_lse)
     if d not in ATTENTION_HEAD_DIMS:
