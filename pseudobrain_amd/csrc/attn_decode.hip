@@ -49,10 +49,10 @@ __device__ __forceinline__ int seq_length(const DecodeParams &p, int b) {
 __device__ __forceinline__ KeyRange seq_keys(const DecodeParams &p, int len) {
   return key_range(len - p.T, len - 1, p.window, p.sinks);
 }
-__device__ __forceinline__ int seq_blocks(const DecodeParams &p, int b) {
-  const int len = seq_length(p, b);
+__device__ __forceinline__ int len_blocks(const DecodeParams &p, int len) {
   return (seq_keys(p, len).count + DEC_KEYS - 1) / DEC_KEYS;
 }
+__device__ __forceinline__ int seq_blocks(const DecodeParams &p, int b) { return len_blocks(p, seq_length(p, b)); }
 
 // The shares: every part takes `per` blocks (the last of a sequence what is
 // left), a sequence at least one part. Every wave works them out for itself: the
@@ -79,9 +79,15 @@ struct Shares {
       return;
     }
     long total = 0;
+    int len[HELD];  // (read by every lane, so that the four reads are in flight together)
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) len[i] = p.lengths[64 * i + lane < p.B ? 64 * i + lane : p.B - 1];
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) settle(len[i]);
 #pragma unroll
     for (int i = 0; i < HELD; ++i) {
-      held[i] = 64 * i + lane < p.B ? seq_blocks(p, 64 * i + lane) : 0;
+      const bool any = (64 * i + lane < p.B) & (p.num_pages > 0) & (len[i] > 0);
+      held[i] = any ? len_blocks(p, len[i]) : 0;
       total += held[i];
     }
     for (int b = 64 * HELD + lane; b < p.B; b += 64) total += seq_blocks(p, b);
@@ -204,10 +210,13 @@ __global__ __launch_bounds__(DEC_WAVES * 64, (Dec<DT, D>::OCC)) void decode_kern
   const int end_ = begin + share.per * (DEC_KEYS / KEYS);
   const int end = uniform(end_ < blocks ? end_ : blocks);
 
-  // this lane's rows of Q (column c of every row block)
+  // this lane's rows of Q (column c of every row block); in LDS, each wave brings in a share
   unsigned char *const ql = reinterpret_cast<unsigned char *>(&merge[0][0]);
   v4u32_t qf[Q_LDS ? 1 : RB][KS];
   int pos[RB];
+  constexpr int QS = Q_LDS ? KS / DEC_WAVES : KS;  // steps of Q that a wave brings in
+  const int q0 = Q_LDS ? wave * QS : 0;
+  v4u32_t qs[Q_LDS ? RB : 1][QS];
 #pragma unroll
   for (int r = 0; r < RB; ++r) {
     const int row = row0 + r * DEC_ROWS + c;
@@ -215,15 +224,18 @@ __global__ __launch_bounds__(DEC_WAVES * 64, (Dec<DT, D>::OCC)) void decode_kern
     const int t = rr / p.group;
     pos[r] = len - p.T + t;
     const unsigned char *src = p.q + ((static_cast<long>(b) * p.T + t) * p.Hq + hk * p.group + rr - t * p.group) * K::ROW;
+    v4u32_t *x = Q_LDS ? qs[r] : qf[r];
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      if (Q_LDS && s % DEC_WAVES != wave) continue;  // each wave brings in a share
-      v4u32_t x = *reinterpret_cast<const v4u32_t *>(src + (4 * s + g) * 16);
-      if (p.negate) x ^= K::SHORT ? 0x80008000u : 0x80000000u;
+    for (int s = 0; s < QS; ++s) x[s] = *reinterpret_cast<const v4u32_t *>(src + (4 * (q0 + s) + g) * 16);
+  }
+#pragma unroll
+  for (int r = 0; r < RB; ++r) {
+    v4u32_t *x = Q_LDS ? qs[r] : qf[r];
+#pragma unroll
+    for (int s = 0; s < QS; ++s) {
+      if (p.negate) x[s] ^= K::SHORT ? 0x80008000u : 0x80000000u;
       if constexpr (Q_LDS)
-        *reinterpret_cast<v4u32_t *>(ql + (r * DEC_ROWS + c) * K::ROW + ((4 * s + g) ^ c) * 16) = x;
-      else
-        qf[r][s] = x;
+        *reinterpret_cast<v4u32_t *>(ql + (r * DEC_ROWS + c) * K::ROW + ((4 * (q0 + s) + g) ^ c) * 16) = x[s];
     }
   }
   if constexpr (Q_LDS) __syncthreads();
@@ -239,14 +251,16 @@ __global__ __launch_bounds__(DEC_WAVES * 64, (Dec<DT, D>::OCC)) void decode_kern
 
   const unsigned char *kbase = p.k + hk * p.head, *vbase = p.v + hk * p.head;
   const int32_t *table = p.table + static_cast<long>(b) * p.max_pages;
-  // the cache row of key `lane` (modulo KEYS) of a block, -1 where there is none
-  const auto lookup = [&](int blk) __attribute__((always_inline)) {
-    const int u = blk * KEYS + lane % KEYS;
-    if (u >= range.count) return -1;
-    const int j = u < range.sinks ? u : u + range.delta;
+  // Key `lane` (modulo KEYS) of a block: its page, and its place there (-1: there is none); then its row in the cache.
+  const auto lookup = [&](int blk, int &page, int &place) __attribute__((always_inline)) {
+    const uint32_t u = static_cast<uint32_t>(blk) * KEYS + lane % KEYS, last = range.count - 1;  // (past a range's end too)
+    const int v = static_cast<int>(u < last ? u : last), j = v < range.sinks ? v : v + range.delta;
     const int pg = j / p.page;
-    const int at = pg < p.max_pages ? table[pg] : -1;
-    return at >= 0 && at < p.num_pages ? at * p.page_rows + (j - pg * p.page) : -1;
+    page = table[pg < p.max_pages ? pg : p.max_pages - 1];
+    place = ((u <= last) & (pg < p.max_pages)) ? j - pg * p.page : -1;
+  };
+  const auto cache_row = [&](int page, int place) __attribute__((always_inline)) {
+    return ((place >= 0) & (page >= 0) & (page < p.num_pages)) ? page * p.page_rows + place : -1;
   };
   // The cache is read once: past the caches (non-temporal), 4 to 9% faster where
   // it is larger than they are.
@@ -282,16 +296,20 @@ __global__ __launch_bounds__(DEC_WAVES * 64, (Dec<DT, D>::OCC)) void decode_kern
     }
   };
   // A block's keys are fetched while the one before is weighed, its values while
-  // the scores are formed: the registers of either are free again by then.
-  int valid = -1, next = -1;
+  // the scores are formed: the registers of either are free again by then. The
+  // pages of the block after are asked for before those values: loads come back
+  // in order, and the next keys' addresses would otherwise wait for them all.
+  int valid = -1, page = -1, place = -1;
   if (begin + wave < end) {
-    valid = lookup(begin + wave);
+    lookup(begin + wave, page, place);
+    valid = cache_row(page, place);
+    lookup(begin + wave + DEC_WAVES, page, place);
     load_keys(valid);
     load_values(valid);
-    if (begin + wave + DEC_WAVES < end) next = lookup(begin + wave + DEC_WAVES);
   }
-  for (int blk = begin + wave; blk < end; blk += DEC_WAVES) {
-    const bool more = blk + DEC_WAVES < end, all = __ballot(valid >= 0) == ~0ull;
+  const auto step = [&](int blk, auto last) __attribute__((always_inline)) {
+    constexpr bool more = !decltype(last)::value;
+    const bool all = __ballot(valid >= 0) == ~0ull;
     float4_t sc[RB][KG];
 #pragma unroll
     for (int r = 0; r < RB; ++r)
@@ -312,7 +330,8 @@ __global__ __launch_bounds__(DEC_WAVES * 64, (Dec<DT, D>::OCC)) void decode_kern
 #pragma unroll
         for (int kb = 0; kb < KG; ++kb) sc[r][kb] = key_mma<DT>(kf[kb][k], q, sc[r][kb]);
       }
-    if (more) load_keys(next);
+    const int next = more ? cache_row(page, place) : -1;
+    if constexpr (more) load_keys(next);
     if (!all) {  // values of absent keys: zeros, whatever the row they were read from holds
 #pragma unroll
       for (int i = 0; i < 4 * KG; ++i) {
@@ -392,12 +411,17 @@ __global__ __launch_bounds__(DEC_WAVES * 64, (Dec<DT, D>::OCC)) void decode_kern
               o[r][x * K::VE + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(
                   __uint_as_float(vf[i][x][e]), sc[r][i / 4][i % 4], o[r][x * K::VE + e], 0, 0, 0);
     }
-    if (more) {
+    if constexpr (more) {
+      lookup(blk + 2 * DEC_WAVES, page, place);
       load_values(next);
       valid = next;
-      if (blk + 2 * DEC_WAVES < end) next = lookup(blk + 2 * DEC_WAVES);
     }
-  }
+  };
+  // The last block apart: loads on some ways through the loop only would have its
+  // values wait for the next keys.
+  int blk = begin + wave;
+  for (; blk + DEC_WAVES < end; blk += DEC_WAVES) step(blk, std::false_type{});
+  if (blk < end) step(blk, std::true_type{});
   if constexpr (Q_LDS) __syncthreads();  // Q's place is the joins'
 
 #pragma unroll
@@ -690,7 +714,7 @@ extern "C" int pbattn_paged_decode(const void *q, const void *k_cache, const voi
   p.head = st[2];
   p.page_rows = static_cast<int>(page_rows);
   p.page = page_size;
-  p.num_pages = num_pages;
+  p.num_pages = max_pages > 0 ? num_pages : 0;  // (no table: no keys)
   p.max_pages = max_pages;
   p.table = page_table;
   p.lengths = lengths;
