@@ -330,6 +330,12 @@ __global__ __launch_bounds__(DEC_WAVES * 64, (Dec<DT, D>::OCC)) void decode_kern
 #pragma unroll
         for (int kb = 0; kb < KG; ++kb) sc[r][kb] = key_mma<DT>(kf[kb][k], q, sc[r][kb]);
       }
+    if constexpr (!K::SHORT && !more) {
+      // nothing stands between the last products and the reads of their results, which the
+      // compiler may put closer than the ten cycles they take to be there
+      __builtin_amdgcn_sched_barrier(0);
+      asm volatile("s_nop 1");
+    }
     const int next = more ? cache_row(page, place) : -1;
     if constexpr (more) load_keys(next);
     if (!all) {  // values of absent keys: zeros, whatever the row they were read from holds
