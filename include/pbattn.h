@@ -31,6 +31,13 @@
  * operands, with float32 inputs nothing is rounded below float32. Strides are
  * in elements; the innermost axis (the head width) is dense. Results do not
  * depend on scheduling: no sum is taken by atomics.
+ *
+ * Infinities and NaN. What no query of the call sees (keys past a sequence's
+ * length, absent pages, tokens of no sequence) is never used, whatever it
+ * holds. The forward and the decoding call also keep a key's or value's infinity
+ * or NaN from the queries that do not see that key. The backward call does not: a key,
+ * value, query or grad_o that is not finite may reach the gradients of its
+ * neighbours (within 128 positions) that it has no part in.
  */
 #ifndef PBATTN_H_
 #define PBATTN_H_

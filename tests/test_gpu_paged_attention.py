@@ -137,6 +137,36 @@ def test_absent_pages_and_stale_rows():
     assert torch.count_nonzero(none) == 0
 
 
+@pytest.mark.parametrize("d,dtype", [(64, torch.float32), (64, torch.float16), (128, torch.bfloat16), (256, torch.bfloat16),
+                                     (256, torch.float32)])
+@pytest.mark.parametrize("group", [1, 3, 8])
+def test_a_bad_value_reaches_only_the_tokens_that_see_it(d, dtype, group):
+    """Infinities and NaN among the drafts and at the window's edge, in values and keys."""
+    draft, window, lengths = 4, 50, [200, 131]
+    q, kc, vc, table, lens = make(lengths, 16, 2 * group, 2, d, draft, dtype, 31)
+    clean = at.paged_decode_attention(q, kc, vc, table, lens, d ** -0.5, window, 3)
+    bad = {0: (200 - 1, 200 - 4 - window + 1, 200 - 2), 1: (131 - 2, 131 - 4 - window + 2, 131 - 1)}
+    for b, (x, y, key) in bad.items():
+        vc[table[b, x // 16].long(), x % 16, :, 3] = float("inf")
+        vc[table[b, y // 16].long(), y % 16, :, 5] = float("nan")
+        kc[table[b, key // 16].long(), key % 16] = float("nan")
+    got, lse = at.paged_decode_attention(q, kc, vc, table, lens, d ** -0.5, window, 3, return_lse=True)
+    # both sides within a bound of u (|o| + sum p |v|) of the truth, values up to 6
+    bound = 4 * 6 * oa.UNIT[NAMES[dtype]] + 1e-4
+    for b, (x, y, key) in bad.items():
+        for t in range(draft):
+            pos = lengths[b] - draft + t
+            sees_x, sees_y, sees_key = (pos - window < j <= pos for j in (x, y, key))
+            if sees_key:
+                assert torch.isnan(got[b, t]).all()
+                continue
+            assert torch.isfinite(lse[b, t]).all()
+            hit = torch.zeros(d, dtype=torch.bool, device=DEV)
+            hit[3], hit[5] = sees_x, sees_y
+            assert not torch.isfinite(got[b, t][:, hit]).any()
+            assert (got[b, t][:, ~hit].float() - clean[b, t][:, ~hit].float()).abs().max() <= bound
+
+
 def test_offsets_past_32_bits():
     """Rows of a cache beyond 4 GiB (keys and values each)."""
     if torch.cuda.mem_get_info()[0] < 14 << 30:
