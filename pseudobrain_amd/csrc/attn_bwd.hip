@@ -731,16 +731,18 @@ constexpr int dkdv_waves() { return DT != PBGDN_F32 ? 4 : D == 256 ? 1 : 2; }
 static bool sinks_beyond(const WindowParams &f) { return f.sinks > 0 && f.window < f.Tk; }
 static int sink_count(const WindowParams &f) { return !sinks_beyond(f) ? 0 : f.sinks < f.Tk ? f.sinks : f.Tk; }
 
-// Parts of a key tile's walk, none shorter than about 16 query tiles: enough
-// workgroups to fill the GPU twice over within a window, whose walks are equal
-// (4 x 2,048 tokens, window 1,024: 650 us in all, with twice as many 690, the
-// join's), twice that without one, where the first keys' walks are the longest
-// (8,192 tokens: 2,565 us, with half as many 3,145).
+// Parts of a key tile's walk, none shorter than about 16 query tiles. Within a
+// window, whose walks are equal: as many as keep the workgroups to twice the CUs,
+// for every further part costs its sums' way through memory (8,000 tokens, window
+// 1,000, 2 key heads: 359 us with four parts, with five 391; 8,028 tokens, window
+// 128, 8 key heads: 293 us with one, with two 343; 4 x 2,048 tokens, window 1,024:
+// with one 650 us, with two 690). Without one, where the first keys' walks are
+// the longest: at least four workgroups a CU (8,192 tokens: 2,565 us, with half as many 3,145).
 static int walk_parts(const WindowParams &f, int B, int bn, int cus) {
   const long tiles = (static_cast<long>(f.Tk) * (f.cu_q ? 1 : B) + bn - 1) / bn * f.Hk;
   const long walk = (f.window < f.Tq ? static_cast<long>(f.window) + bn : f.Tq) * f.group / QR;
   const long want = (f.window < f.Tq ? 2L : 4L) * cus;
-  long parts = tiles > 0 ? (want + tiles - 1) / tiles : 1;
+  long parts = tiles > 0 ? (f.window < f.Tq ? want : want + tiles - 1) / tiles : 1;
   if (parts > walk / 16) parts = walk / 16;
   return parts < 2 ? 1 : parts > MAX_PARTS ? MAX_PARTS : static_cast<int>(parts);
 }
