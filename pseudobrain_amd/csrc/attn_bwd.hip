@@ -1,12 +1,11 @@
 // Windowed attention, backward (pbattn_window_bwd).
 //
 // Four kernels, none with an atomic sum:
-//   stat_kernel   per (token, head): lse in powers of two and
-//                 delta = do . o - dlse, stored by (batch, key head) in the
-//                 row order of the tiles below; float16 also takes the maxima
-//                 that bound ds
-//   dq_kernel     the forward's walk over keys: S^T, dP^T, dS^T, dQ^T += K^T dS^T
-//                 (first where rows see few keys: delta made exact)
+//   range_kernel  float16: the maxima that bound ds
+//   dq_kernel     the forward's walk over keys: S^T, dP^T, dS^T, dQ^T += K^T dS^T;
+//                 before it, per row, lse in powers of two and delta = do . o - dlse
+//                 (made exact where rows see few keys), which it keeps for
+//                 dkdv_kernel by (batch, key head) in the row order of the tiles
 //   dkdv_kernel   a wave owns 32 keys, with K and V rows and the sums of dK^T
 //                 and dV^T in registers, and walks the queries that see them
 //                 (all heads of the group): S = Q K^T, P, dV^T += dO^T P,
@@ -43,7 +42,7 @@ struct BwdParams {
   const float *lse, *grad_lse;
   void *dq, *dk, *dv;
   float2 *stat;       // [B][Hk][Tq G]: (lse log2(e), delta); +inf for a row that sees nothing
-  uint32_t *range;    // float16: bits of max |do|, |v|, |delta|
+  uint32_t *range;    // float16: bits of max |do|, |v|, |dlse|
   float *part;        // [2][parts][B][Hk][Tk][D] when parts > 1
   float *tail;        // [2][tail slots][Hk][sinks][D]
   float scale;
@@ -67,14 +66,14 @@ inline long tail_slot_count(int Tq, int nseq, int tokens, bool packed) {
 }
 
 // ---------------------------------------------------------------------------
-// float16's range: ds is bounded by max |do| max |v| D + max |delta|; a power
-// of two brings that bound to 2^14 (a corrected delta, see dq_kernel, passes it
-// by its correction, far less than what 2^16 leaves).
+// float16's range: o is a mean of the values its row sees, so |delta| and |dp| are
+// at most D max |do| max |v| (and max |dlse|), and ds their sum; a power of two
+// brings that bound to 2^14.
 // ---------------------------------------------------------------------------
 template <int DT, int D>
 __device__ __forceinline__ float range_scale(const uint32_t *range) {
   if constexpr (DT != PBGDN_F16) return 1.0f;
-  const float bound = __uint_as_float(range[0]) * __uint_as_float(range[1]) * D + __uint_as_float(range[2]);
+  const float bound = 2.0f * D * __uint_as_float(range[0]) * __uint_as_float(range[1]) + __uint_as_float(range[2]);
   if (!(bound > 0.0f && bound < 1e30f)) return 1.0f;
   int e;
   frexpf(bound, &e);
@@ -101,72 +100,27 @@ __device__ __forceinline__ void range_max(float x, uint32_t *word) {
   __syncthreads();
 }
 
-// max |v| over rows of D elements (float16): workgroup `block` of `blocks`.
+// max |do|, |dlse| and |v|: three quarters of the workgroups read grad_o, the rest v.
 template <int D>
-__device__ __forceinline__ void range_v(const BwdParams &p, int block, int blocks) {
-  constexpr int LPR = D / 8;  // lanes of a row
-  const View &v = p.f.v;
-  const long rows = static_cast<long>(p.B) * p.f.Tk * p.f.Hk;
-  float top = 0.0f;
-  for (long r = block * (256L / LPR) + threadIdx.x / LPR; r < rows; r += blocks * (256L / LPR)) {
-    const long bt = r / p.f.Hk, b = bt / p.f.Tk;
-    const half8_t x = *reinterpret_cast<const half8_t *>(
-        v.base + b * v.batch + (bt - b * p.f.Tk) * v.token + (r - bt * p.f.Hk) * v.head + (threadIdx.x % LPR) * 16);
+__global__ __launch_bounds__(256) void range_kernel(const BwdParams p) {
+  constexpr int LPR = D / 8, RPB = 256 / LPR;  // lanes of a row, rows of a workgroup
+  const int split = gridDim.x * 3 / 4;
+  const bool of_v = blockIdx.x >= split;
+  const int block = of_v ? blockIdx.x - split : blockIdx.x, blocks = of_v ? gridDim.x - split : split;
+  const int heads = of_v ? p.f.Hk : p.f.Hq, tokens = of_v ? p.f.Tk : p.f.Tq, unit = threadIdx.x % LPR * 16;
+  const long rows = static_cast<long>(p.B) * tokens * heads;
+  float top = 0.0f, top_dlse = 0.0f;
+  for (long r = block * static_cast<long>(RPB) + threadIdx.x / LPR; r < rows; r += blocks * static_cast<long>(RPB)) {
+    const long bt = r / heads, b = bt / tokens;
+    const unsigned char *src = of_v ? p.f.v.base + b * p.f.v.batch + (bt - b * tokens) * p.f.v.token + (r - bt * heads) * p.f.v.head
+                                    : static_cast<const unsigned char *>(p.grad_o) + r * D * 2;
+    const half8_t x = *reinterpret_cast<const half8_t *>(src + unit);
 #pragma unroll
     for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(static_cast<float>(x[i])));
+    if (!of_v && p.grad_lse && unit == 0 && p.lse[r] != -INFINITY) top_dlse = fmaxf(top_dlse, fabsf(p.grad_lse[r]));
   }
-  range_max(top, p.range + 1);
-}
-
-// One read of o and grad_o, as many rows to a workgroup as its lanes can hold 16
-// bytes each of: 4 x 2,048 tokens, 32 heads of 128: 24 us for 134 MB (5.6 TB/s).
-template <int DT, int D>
-__global__ __launch_bounds__(256) void stat_kernel(const BwdParams p) {
-  using E = Elem<DT>;
-  constexpr int PER = 16 / E::BYTES, LPR = D / PER < 64 ? D / PER : 64, RPB = 256 / LPR;  // lanes a row, rows a block
-  constexpr int UNITS = D / PER / LPR;
-  const int blocks = DT == PBGDN_F16 ? gridDim.x * 3 / 4 : gridDim.x;  // float16: the last quarter reads v
-  if constexpr (DT == PBGDN_F16) {
-    if (blockIdx.x >= blocks) {
-      range_v<D>(p, blockIdx.x - blocks, gridDim.x - blocks);
-      return;
-    }
-  }
-  const long rows = static_cast<long>(p.B) * p.f.Tq * p.f.Hq;
-  float top_do = 0.0f, top_delta = 0.0f;
-  for (long r = blockIdx.x * static_cast<long>(RPB) + threadIdx.x / LPR; r < rows; r += blocks * static_cast<long>(RPB)) {
-    float sum = 0.0f;
-#pragma unroll
-    for (int u = 0; u < UNITS; ++u) {
-      const long at = r * D * E::BYTES + (u * LPR + threadIdx.x % LPR) * 16;
-      const v4u32_t x = *reinterpret_cast<const v4u32_t *>(static_cast<const unsigned char *>(p.o) + at);
-      const v4u32_t y = *reinterpret_cast<const v4u32_t *>(static_cast<const unsigned char *>(p.grad_o) + at);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (E::BYTES == 2) {
-          sum += E::low(x[i]) * E::low(y[i]) + E::high(x[i]) * E::high(y[i]);
-          if constexpr (DT == PBGDN_F16) top_do = fmaxf(top_do, fmaxf(fabsf(E::low(y[i])), fabsf(E::high(y[i]))));
-        } else {
-          sum += __uint_as_float(x[i]) * __uint_as_float(y[i]);
-        }
-      }
-    }
-#pragma unroll
-    for (int w = LPR / 2; w > 0; w >>= 1) sum += __shfl_xor(sum, w, 64);
-    if (threadIdx.x % LPR == 0) {
-      const float lse = p.lse[r];
-      const bool empty = lse == -INFINITY;
-      const float delta = empty ? 0.0f : p.grad_lse ? sum - p.grad_lse[r] : sum;
-      const int h = static_cast<int>(r % p.f.Hq), G = p.f.group;
-      const long bt = r / p.f.Hq, b = bt / p.f.Tq, t = bt % p.f.Tq;
-      p.stat[((b * p.f.Hk + h / G) * p.f.Tq + t) * G + h % G] = make_float2(empty ? INFINITY : lse * LOG2E, delta);
-      top_delta = fmaxf(top_delta, fabsf(delta));
-    }
-  }
-  if constexpr (DT == PBGDN_F16) {
-    range_max(top_do, p.range);
-    range_max(top_delta, p.range + 2);
-  }
+  range_max(top, p.range + (of_v ? 1 : 0));
+  if (!of_v && p.grad_lse) range_max(top_dlse, p.range + 2);
 }
 
 // ---------------------------------------------------------------------------
@@ -637,8 +591,26 @@ __global__ __launch_bounds__(NW * 64, WAVES) void dq_kernel(const BwdParams p) {
     settle(qf[s]);
     settle(gf[s]);
   }
-  float2 *stat = p.stat + ((static_cast<long>(b) * f.Hk + hk) * f.Tq + sq.q0) * G + r;
-  float2 st = *stat;
+  float2 st;
+  {
+    const unsigned char *orow = static_cast<const unsigned char *>(p.o) + out * L::ROW;
+    float sum = 0.0f;
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      const v4u32_t x = *reinterpret_cast<const v4u32_t *>(orow + (2 * s + h) * 16);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (E::BYTES == 2)
+          sum += E::low(x[i]) * E::low(gf[s][i]) + E::high(x[i]) * E::high(gf[s][i]);
+        else
+          sum += __uint_as_float(x[i]) * __uint_as_float(gf[s][i]);
+      }
+    }
+    sum = add_xor32(sum);
+    const float lse = p.lse[out], dlse = p.grad_lse ? p.grad_lse[out] : 0.0f;
+    const bool empty = lse == -INFINITY;
+    st = make_float2(empty ? INFINITY : lse * LOG2E, empty ? 0.0f : sum - dlse);
+  }
   settle(st.x);
   settle(st.y);
   const float scale16 = range_scale<DT, D>(p.range);
@@ -688,16 +660,14 @@ __global__ __launch_bounds__(NW * 64, WAVES) void dq_kernel(const BwdParams p) {
       }
       for (; it < tiles; ++it) advance(it);
       sum += __shfl_xor(sum, 32, 64);
-      if (st.x != INFINITY) {
-        st.y += p.grad_lse ? sum - p.grad_lse[out] : sum;
-        if (h == 0 && row < total) stat->y = st.y;
-      }
+      if (st.x != INFINITY) st.y += p.grad_lse ? sum - p.grad_lse[out] : sum;
       settle(st.y);
       it = 0;
       block_sync();
       stage.tile(0, lds);
     }
   }
+  if (h == 0 && row < total) p.stat[((static_cast<long>(b) * f.Hk + hk) * f.Tq + sq.q0) * G + r] = st;
   for (; it < mine; ++it) {
     advance(it);
     const unsigned char *kt = lds + (it & 1) * F::TILE, *vt = kt + 2 * F::TILE;
@@ -753,8 +723,10 @@ static int launch_bwd(BwdParams &p, hipStream_t stream) {
   const int nb = f.cu_q ? 1 : p.B;
   DeviceShape shape;
   if (!device_shape(shape)) return PBGDN_ERR_LAUNCH;
-  if constexpr (DT == PBGDN_F16) hipLaunchKernelGGL(range_zero_kernel, dim3(1), dim3(64), 0, stream, p.range);
-  hipLaunchKernelGGL((stat_kernel<DT, D>), dim3(shape.cus * 8), dim3(256), 0, stream, p);
+  if constexpr (DT == PBGDN_F16) {
+    hipLaunchKernelGGL(range_zero_kernel, dim3(1), dim3(64), 0, stream, p.range);
+    hipLaunchKernelGGL((range_kernel<D>), dim3(shape.cus * 8), dim3(256), 0, stream, p);
+  }
   {
     constexpr int DQ_NW = 4, DQ_BN = DT == PBGDN_F32 ? (D == 64 ? 64 : 32) : D == 256 ? 32 : 64;
     constexpr int W = DT != PBGDN_F32 && D <= 128 ? 2 : 1;
