@@ -19,8 +19,8 @@
 // Forward and backward of 8,192 tokens, 32 heads of 128 on 8, float16, take 2.46
 // to 2.59 ms: 740 to 780 TFLOP/s of the formulas' flops, 950 to 1,000 with the two
 // products formed twice, where a large product reaches 1,296. In it the forward
-// takes 580 us, stat_kernel 37, dq_kernel 770 (matrix unit busy 65%), dkdv_kernel
-// 1,150 (54%), join_kernel 27.
+// takes 600 us, range_kernel 25, dq_kernel 800 (matrix unit busy 65%), dkdv_kernel
+// 1,180 (54%), join_kernel 27.
 #include <atomic>
 
 #include "attn.hpp"
@@ -100,7 +100,8 @@ __device__ __forceinline__ void range_max(float x, uint32_t *word) {
   __syncthreads();
 }
 
-// max |do|, |dlse| and |v|: three quarters of the workgroups read grad_o, the rest v.
+// max |do|, |dlse| and |v|: three quarters of the workgroups read grad_o, the rest v
+// (8,192 tokens, 32 heads of 128 on 8: 84 MB in 22 to 27 us).
 template <int D>
 __global__ __launch_bounds__(256) void range_kernel(const BwdParams p) {
   constexpr int LPR = D / 8, RPB = 256 / LPR;  // lanes of a row, rows of a workgroup
@@ -432,7 +433,7 @@ __global__ __launch_bounds__(NW * 64, WAVES) void dkdv_kernel(const BwdParams p)
 // workgroups take a sink each (of a sequence and key head): its threads, four
 // elements of the row each, split the many parts and join through LDS. The rest
 // take the other keys where p.parts > 1, four elements a thread. Bound by the
-// parts' reads (6 parts of 6,011 keys, 2 heads of 256: 148 MB in 26 us).
+// parts' reads (5 parts of 6,011 keys, 2 heads of 256: 123 MB in 23 us).
 template <int DT>
 __device__ __forceinline__ void store4(void *dst, long at, float4_t x) {
   using E = Elem<DT>;
@@ -524,9 +525,10 @@ __global__ __launch_bounds__(256) void join_kernel(const BwdParams p, int sink_b
 // of 128 keys at most, the rows walk once for that sum, and again with the delta
 // corrected by it, which is kept for dkdv_kernel, so this kernel comes first.
 //
-// 4 x 2,048 tokens, 32 heads of 128 on 8, window 1,024: 180 to 195 us (800
-// TFLOP/s, the matrix unit busy 47%); 6,011 tokens in 7 sequences, 16 heads of 256
-// on 2, window 512: 117 us at one wave a SIMD (470 TFLOP/s, 22%).
+// 4 x 2,048 tokens, 32 heads of 128 on 8, window 1,024: 192 to 211 us (770
+// TFLOP/s, the matrix unit busy 46%); 6,011 tokens in 7 sequences, 16 heads of 256
+// on 2, window 512: 120 us at one wave a SIMD (450 TFLOP/s, 21%). Reading o for
+// delta takes 4 to 15 us of it; a pass of its own over o and grad_o took 18 to 37.
 // ---------------------------------------------------------------------------
 template <int DT, int D, int NW, int BN>
 struct Dq {

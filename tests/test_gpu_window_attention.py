@@ -158,6 +158,28 @@ def test_strided_inputs():
     check("odd offset", q, flat, v, go, glse, 0.125, 30, 2)
 
 
+def test_offsets_past_32_bits():
+    """Token rows 12 MB apart, so that the last ones lie past 4 GiB: the same bits as dense tensors."""
+    if torch.cuda.mem_get_info()[0] < 14 << 30:
+        pytest.skip("needs 14 GB")
+    tokens, step = 500, 6_000_000
+    far = torch.empty(tokens, step, dtype=torch.bfloat16, device=DEV)
+    dense = make(1, tokens, tokens, 4, 2, 64, torch.bfloat16, 21)[:4]
+    views = []
+    for i, x in enumerate(dense[:3]):
+        view = far[None, :, i * 2_000_000:][:, :, :x[0, 0].numel()].unflatten(2, x.shape[2:])
+        view.copy_(x)
+        views.append(view)
+    for cu in (None, torch.tensor([0, 30, 480], dtype=torch.int32, device=DEV)):
+        got = []
+        for q, k, v in (views, dense[:3]):
+            assert q.stride(1) == (step if q is views[0] else 256)
+            o, lse = at.window_attention_fwd(q, k, v, 0.125, 200, 3, cu)
+            got.append((o, lse, *at.window_attention_bwd(q, k, v, o, lse, dense[3], 0.125, 200, 3, cu)))
+        for x, y in zip(*got):
+            assert torch.equal(x, y)
+
+
 def test_broadcast_inputs():
     """Keys and values shared by the batch: the gradient is the sum over it."""
     q, k, v, go, glse = make(3, 70, 70, 4, 2, 64, torch.float32, 8)
