@@ -99,7 +99,7 @@ int pbattn_window_fwd(const void *q, const void *k, const void *v, int dtype, co
  *              bytes, 16-byte aligned; needs no initialisation
  *
  * With dtype F16, ds is scaled by a power of two found on the device from the
- * largest |do|, |v| and |delta| before it is rounded, and the results scaled
+ * largest |do|, |v| and |dlse| before it is rounded, and the results scaled
  * back, so that neither small nor large gradients leave float16's range there.
  */
 int pbattn_window_bwd(const void *q, const void *k, const void *v, int dtype, const int64_t *strides,
