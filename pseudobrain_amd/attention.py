@@ -152,11 +152,11 @@ def _window_operands(q, k, v):
     """q, k, v in q's dtype as the kernels read them, and their stride array."""
     if k.dtype != q.dtype or v.dtype != q.dtype:
         k, v = k.to(q.dtype), v.to(q.dtype)
+    # (the strides are taken last: a copy for the alignment may have others than its view)
+    q, k, v = _aligned(q, 16), _aligned(k, 16), _aligned(v, 16)
     steps = _window_steps((q.shape, q.stride()), (k.shape, k.stride()), (v.shape, v.stride()), q.element_size())
     if steps is None:
         q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
-    q, k, v = _aligned(q, 16), _aligned(k, 16), _aligned(v, 16)
-    if steps is None:
         steps = _steps(*((x.shape, x.stride()) for x in (q, k, v)))
     return q, k, v, steps
 
@@ -456,16 +456,22 @@ def _write_steps(cache, k, k_stride, v, v_stride, slots, size):
     return _steps((k, k_stride), (v, v_stride))
 
 
+def _write_operands(k, v, cache, dtype, slots_shape):
+    """New rows in the caches' dtype as the kernel reads them, and their stride array."""
+    k, v = _aligned(k, 16), _aligned(v, 16)  # (before the strides are taken: a copy may have others)
+    steps = _write_steps(cache, k.shape, k.stride(), v.shape, v.stride(), slots_shape, dtype.itemsize)
+    if steps is None or k.dtype != dtype or v.dtype != dtype:
+        k, v = (x.to(dtype).reshape(-1, *cache[2:]).contiguous() for x in (k, v))
+        steps = _steps((k.shape, k.stride()), (v.shape, v.stride()))
+    return k, v, steps
+
+
 def _write(k, v, k_cache, v_cache, slots):
     dev = _one_device(k, v, k_cache, v_cache, slots)
     cache, cache_steps, code, at = _caches(k_cache, v_cache)
-    steps = _write_steps(cache, k.shape, k.stride(), v.shape, v.stride(), slots.shape, k_cache.element_size())
     if slots.dtype not in (torch.int32, torch.int64):
         raise ValueError("slots must be int32 or int64")
-    if steps is None or k.dtype != k_cache.dtype or v.dtype != k_cache.dtype:
-        k, v = (x.to(k_cache.dtype).reshape(-1, *cache[2:]).contiguous() for x in (k, v))
-        steps = _steps((k.shape, k.stride()), (v.shape, v.stride()))
-    k, v = _aligned(k, 16), _aligned(v, 16)
+    k, v, steps = _write_operands(k, v, cache, k_cache.dtype, slots.shape)
     if slots.dtype != torch.int64 or slots.ndim != 1 or not slots.is_contiguous():
         slots = slots.reshape(-1).to(torch.int64).contiguous()
     _launch("pbattn_paged_write", _lib.attn_lib().pbattn_paged_write, dev, k.data_ptr(), v.data_ptr(), code, steps, *at,

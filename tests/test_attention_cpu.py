@@ -228,6 +228,43 @@ def test_paged_calls_refuse():
     assert sizes == (5, 16, 2, 64) and list(steps) == [2048, 64, 1024]
 
 
+def misaligned(tokens, heads, d, dtype, lead=()):
+    """Columns of wider rows: strides of whole 16 bytes, a base 8 bytes off."""
+    skip = 8 // dtype.itemsize
+    z = torch.randn(*lead, tokens, heads * d + 16 // dtype.itemsize).to(dtype)
+    x = z[..., skip:skip + heads * d].unflatten(-1, (heads, d))
+    assert x.data_ptr() % 16 == 8 and all(s * dtype.itemsize % 16 == 0 for s in x.stride()[:-1])
+    return x
+
+
+def read_by(tensor, steps):
+    """The tensor's rows as a kernel finds them by its stride array."""
+    return tensor.as_strided(tensor.shape, (*steps, 1))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_strides_are_those_of_the_tensors_passed_on(dtype):
+    """A view copied for its base's alignment gives its rows another distance."""
+    q, k, v = (misaligned(5, h, 64, dtype, (2,)) for h in (4, 2, 2))
+    *got, steps = at._window_operands(q, k, v)
+    for i, (x, y) in enumerate(zip(got, (q, k, v))):
+        assert list(steps)[3 * i:3 * i + 3] == list(x.stride())[:3] and x.data_ptr() % 16 == 0
+        assert torch.equal(read_by(x, list(steps)[3 * i:3 * i + 3]), y)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_written_rows_strides_are_those_of_the_tensors_passed_on(dtype, monkeypatch):
+    calls = []
+    monkeypatch.setattr(at, "_one_device", lambda *t: t[0].device)
+    monkeypatch.setattr(at, "_launch", lambda where, fn, dev, *args: calls.append(args))
+    k, v = (misaligned(5, 2, 64, dtype) for _ in range(2))
+    cache = torch.zeros(3, 16, 2, 64, dtype=dtype)
+    at.paged_cache_write(k, v, cache, cache.clone(), torch.arange(5))
+    (k_at, v_at, code, steps, *_), = calls
+    # (an aligned view's tensor is passed as it is, a copy densely)
+    assert k_at % 16 == 0 and v_at % 16 == 0 and list(steps) == [128, 64, 128, 64]
+
+
 def test_a_stale_attention_library_is_named(tmp_path):
     src = tmp_path / "stub.cpp"
     src.write_text('extern "C" int pbattn_abi_version(void) { return 0; }\n')

@@ -240,6 +240,20 @@ def test_cache_write(dtype, d):
     assert torch.equal(kc[0, :6], k4.view(6, hk, d).to(dtype))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_cache_write_of_column_slices_off_the_alignment(dtype):
+    """New rows as columns of wider rows, 8 bytes off the alignment."""
+    skip, pad, n, hk, d = 8 // dtype.itemsize, 16 // dtype.itemsize, 30, 2, 64
+    torch.manual_seed(30)
+    k, v = (torch.randn(n, hk * d + pad, device=DEV).to(dtype)[:, skip:skip + hk * d].unflatten(-1, (hk, d))
+            for _ in range(2))
+    assert k.data_ptr() % 16 == 8
+    kc, vc = (torch.zeros(4, 8, hk, d, dtype=dtype, device=DEV) for _ in range(2))
+    at.paged_cache_write(k, v, kc, vc, torch.arange(n, device=DEV))
+    for c, x in ((kc, k), (vc, v)):
+        assert torch.equal(c.view(-1, hk, d)[:n], x) and torch.count_nonzero(c.view(-1, hk, d)[n:]) == 0
+
+
 def test_prefill_then_decode_equals_one_pass():
     """A prompt attended and cached, then tokens one at a time, against window_attention over all of it."""
     torch.manual_seed(29)

@@ -158,6 +158,25 @@ def test_strided_inputs():
     check("odd offset", q, flat, v, go, glse, 0.125, 30, 2)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_column_slices_off_the_alignment(dtype):
+    """q, k and v as columns of wider rows, 8 bytes off the alignment: the same bits as dense copies."""
+    skip, pad = 8 // dtype.itemsize, 16 // dtype.itemsize
+    torch.manual_seed(22)
+    x = []
+    for heads in (4, 2, 2):
+        z = torch.randn(2, 150, heads * 64 + pad, device=DEV).to(dtype)
+        x.append(z[..., skip:skip + heads * 64].unflatten(-1, (heads, 64)))
+    assert all(t.data_ptr() % 16 == 8 for t in x)
+    go = torch.randn(2, 150, 4, 64, device=DEV).to(dtype)
+    got = []
+    for q, k, v in (x, [t.contiguous() for t in x]):
+        o, lse = at.window_attention_fwd(q, k, v, 0.125, 40, 3)
+        got.append((o, lse, *at.window_attention_bwd(q, k, v, o, lse, go, 0.125, 40, 3)))
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+
+
 def test_offsets_past_32_bits():
     """Token rows 12 MB apart, so that the last ones lie past 4 GiB: the same bits as dense tensors."""
     if torch.cuda.mem_get_info()[0] < 14 << 30:
