@@ -88,7 +88,9 @@ int pbattn_window_fwd(const void *q, const void *k, const void *v, int dtype, co
  *   dv_j = sum_i p_ij do_i,  dk_j = scale sum_i ds_ij q_i,  dq_i = scale sum_j ds_ij k_j,
  * the sums of dk and dv over every query head of the key head's group.
  *
- *   q .. num_seqs, B .. sinks   as in the forward call
+ *   q .. num_seqs, B .. sinks   as in the forward call; besides, 32 rows of q
+ *              (h = min(Hq / Hk, 32) heads of 32 / h tokens) must lie within
+ *              0x7ffffff0 bytes by its strides, and as many of grad_o
  *   o, lse     the forward call's results (dense)
  *   grad_o     [B, Tq, Hq, D] dense, dtype
  *   grad_lse   [B, Tq, Hq] dense float32, or NULL for zeros

@@ -38,6 +38,7 @@ from .gated_deltanet import _aligned, _pad_last, _require_device, _width_at_leas
 ATTENTION_HEAD_DIMS = (64, 128, 256)  # widths the kernels are built for
 MAX_DRAFT = 16                        # query tokens a sequence may have in paged_decode_attention
 _MAX_TOKEN_STRIDE = 1 << 24           # bytes (pbattn_window_fwd)
+_MAX_TILE_SPAN = 0x7ffffff0           # bytes (pbattn_window_bwd)
 
 
 # What follows from shapes, strides and types alone (checks, stride arrays,
@@ -148,12 +149,24 @@ def _window_steps(q, k, v, size):
     return _steps(q, k, v) if all(_readable(*x, size) for x in (q, k, v)) else None
 
 
-def _window_operands(q, k, v):
-    """q, k, v in q's dtype as the kernels read them, and their stride array."""
+@_plan
+def _tile_span(q, stride, hk: int, size: int) -> int:
+    """Bytes from the first to the last element of a gradient kernel's tile of q: 32
+    rows, the heads of a group (32 at most) of as many tokens as there is room for."""
+    heads = min(q[2] // hk, 32)
+    steps = (32 // heads - 1, stride[1] if q[1] > 1 else 0), (heads - 1, stride[2] if q[2] > 1 else 0), (q[3], 1)
+    return sum(n * step for n, step in steps) * size
+
+
+def _window_operands(q, k, v, gradients: bool = False):
+    """q, k, v in q's dtype as the kernels (those of the gradients too) read them, and
+    their stride array."""
     if k.dtype != q.dtype or v.dtype != q.dtype:
         k, v = k.to(q.dtype), v.to(q.dtype)
     # (the strides are taken last: a copy for the alignment may have others than its view)
     q, k, v = _aligned(q, 16), _aligned(k, 16), _aligned(v, 16)
+    if gradients and _tile_span(q.shape, q.stride(), k.shape[2], q.element_size()) > _MAX_TILE_SPAN:
+        q = q.contiguous()
     steps = _window_steps((q.shape, q.stride()), (k.shape, k.stride()), (v.shape, v.stride()), q.element_size())
     if steps is None:
         q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
@@ -212,7 +225,7 @@ def window_attention_bwd(q, k, v, o, lse, grad_o, scale: float, window=None, sin
     if o.shape != q.shape or grad_o.shape != q.shape or lse.shape != q.shape[:3] or (
             grad_lse is not None and grad_lse.shape != q.shape[:3]):
         raise ValueError("o and grad_o must have q's shape, lse and grad_lse [B,Tq,Hq]")
-    q, k, v, steps = _window_operands(q, k, v)
+    q, k, v, steps = _window_operands(q, k, v, gradients=True)
     o, grad_o = (_aligned(x.to(q.dtype).contiguous(), 16) for x in (o, grad_o))
     lse = lse.to(torch.float32).contiguous()
     grad_lse = None if grad_lse is None else grad_lse.to(torch.float32).contiguous()

@@ -867,6 +867,14 @@ extern "C" int pbattn_window_bwd(const void *q, const void *k, const void *v, in
   p.heads = p.f.group < QR ? p.f.group : QR;
   p.tokens = QR / p.heads;
   p.splits = (p.f.group + QR - 1) / QR;
+  // dkdv_kernel's tiles are staged by 32-bit offsets into a buffer resource, and OUT_OF_RANGE has to be past its end
+  const long row = static_cast<long>(D) * attn_bytes(dtype);
+  const long q_head = p.heads > 1 ? p.f.q.head : 0;
+  const long g_span = (p.tokens - 1L) * Hq * row + p.heads * row;
+  if (q_head > OUT_OF_RANGE || (p.tokens - 1) * p.f.q.token + (p.heads - 1) * q_head + row > OUT_OF_RANGE ||
+      g_span > OUT_OF_RANGE) {
+    return PBGDN_ERR_UNSUPPORTED;
+  }
   hipStream_t st = static_cast<hipStream_t>(stream);
   debug_poison(dq, static_cast<size_t>(B) * Tq * Hq * D * attn_bytes(dtype), st);
   debug_poison(dk, static_cast<size_t>(B) * Tk * Hk * D * attn_bytes(dtype), st);

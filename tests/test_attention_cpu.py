@@ -98,6 +98,35 @@ def test_window_bwd_rejects(over):
     assert bwd(**over) == _lib.ERR_INVALID_ARGUMENT
 
 
+@pytest.mark.parametrize("heads,head", [
+    (32, (0x7ffffff0 - 256) // 2 // 31 // 8 * 8 + 8),  # one step of 16 bytes past the limit
+    (32, 1 << 27),                                     # wraps in 32 bits: 31 of 256 MiB
+    (64, 1 << 27),                                     # a group of more heads than a tile
+    (2, 1 << 31), (2, 1 << 59)])
+def test_rows_of_q_past_32_bits_are_refused_and_copied(heads, head):
+    """The gradient kernels reach 32 rows of q by 32-bit offsets: the C ABI refuses heads farther
+    apart than that, the host API makes q dense. (Only refused calls are made: others would launch.)"""
+    assert bwd(Hq=heads, Hk=1, strides=strides(0, 512, head, *QKV[3:])) == _lib.ERR_UNSUPPORTED
+    k, v = (torch.empty(1, 16, 1, 128, dtype=torch.bfloat16, device="meta") for _ in range(2))
+    for step in (head, head - 8):
+        if step * heads * 2 >= 1 << 62:
+            continue  # no such tensor
+        q = torch.empty_strided((1, 16, heads, 128), (0, 512, step, 1), dtype=torch.bfloat16, device="meta")
+        kept = at._window_operands(q, k, v)
+        assert kept[0] is q and list(kept[3])[:3] == [0, 512, step]  # the forward reads it in place
+        got = at._window_operands(q, k, v, gradients=True)
+        copied = got[0] is not q
+        assert copied == (step == head or head >= 1 << 27)
+        assert list(got[3])[:3] == ([0, heads * 128, 128] if copied else [0, 512, step])
+
+
+def test_a_head_of_its_own_may_lie_anywhere():
+    """One head a group: its stride is no part of a tile."""
+    q = torch.empty_strided((1, 16, 2, 128), (0, 128, 1 << 31, 1), dtype=torch.bfloat16, device="meta")
+    k, v = (torch.empty(1, 16, 2, 128, dtype=torch.bfloat16, device="meta") for _ in range(2))
+    assert at._window_operands(q, k, v, gradients=True)[0] is q
+
+
 def test_empty_window_calls_are_ok():
     for empty in (dict(B=0, nseq=0), dict(Tq=0), dict(cu_q=FAKE, nseq=0)):
         assert fwd(**empty) == _lib.OK and bwd(**empty) == _lib.OK

@@ -199,6 +199,25 @@ def test_offsets_past_32_bits():
             assert torch.equal(x, y)
 
 
+@pytest.mark.parametrize("step", [34_000_000, 80_000_000])
+def test_heads_past_32_bits(step):
+    """Heads of q that lie apart, so that a group's span 2.1 GB (read in place) or 5 GB: the same bits as dense ones."""
+    if torch.cuda.mem_get_info()[0] < 8 << 30:
+        pytest.skip("needs 8 GB")
+    tokens, heads, d = 150, 32, 128
+    far = torch.empty(heads, step, dtype=torch.bfloat16, device=DEV)
+    dense, k, v, go, _ = make(1, tokens, tokens, heads, 1, d, torch.bfloat16, 23)
+    q = far[:, :tokens * d].view(heads, tokens, d).transpose(0, 1)[None]
+    q.copy_(dense)
+    for window, sinks in ((None, 0), (40, 3)):
+        o, lse = at.window_attention_fwd(q, k, v, 0.09, window, sinks)
+        got = (o, lse, *at.window_attention_bwd(q, k, v, o, lse, go, 0.09, window, sinks))
+        o, lse = at.window_attention_fwd(dense, k, v, 0.09, window, sinks)
+        want = (o, lse, *at.window_attention_bwd(dense, k, v, o, lse, go, 0.09, window, sinks))
+        for x, y in zip(got, want):
+            assert torch.equal(x, y)
+
+
 def test_broadcast_inputs():
     """Keys and values shared by the batch: the gradient is the sum over it."""
     q, k, v, go, glse = make(3, 70, 70, 4, 2, 64, torch.float32, 8)
