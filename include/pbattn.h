@@ -101,8 +101,10 @@ int pbattn_window_fwd(const void *q, const void *k, const void *v, int dtype, co
  *              bytes, 16-byte aligned; needs no initialisation
  *
  * With dtype F16, ds is scaled by a power of two found on the device from the
- * largest |do|, |v| and |dlse| before it is rounded, and the results scaled
- * back, so that neither small nor large gradients leave float16's range there.
+ * largest finite |do|, |v| and |dlse| of the queries that see a key and the
+ * keys that a query sees, before it is rounded, and the results scaled back, so
+ * that neither small nor large gradients leave float16's range there. It is one
+ * power of two for the call: the largest of them all sets it.
  */
 int pbattn_window_bwd(const void *q, const void *k, const void *v, int dtype, const int64_t *strides,
                       const int32_t *cu_q, const int32_t *cu_k, int num_seqs, const void *o, const float *lse,

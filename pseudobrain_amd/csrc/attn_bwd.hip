@@ -65,6 +65,19 @@ inline long tail_slot_count(int Tq, int nseq, int tokens, bool packed) {
   return packed ? Tq / tokens + 2L * nseq : nseq * ((Tq + tokens - 1L) / tokens + 1);
 }
 
+// The last of the boundaries 0 .. n that is no further than `token`: its sequence, or n past the last.
+__device__ __forceinline__ int last_at(const int32_t *cu, int n, int total, int token) {
+  int lo = 0, hi = n;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (boundary(cu, mid, total) <= token)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  return lo;
+}
+
 // ---------------------------------------------------------------------------
 // float16's range: o is a mean of the values its row sees, so |delta| and |dp| are
 // at most D max |do| max |v| (and max |dlse|), and ds their sum; a power of two
@@ -100,28 +113,56 @@ __device__ __forceinline__ void range_max(float x, uint32_t *word) {
   __syncthreads();
 }
 
-// max |do|, |dlse| and |v|: three quarters of the workgroups read grad_o, the rest v
-// (8,192 tokens, 32 heads of 128 on 8: 84 MB in 22 to 27 us).
+// max |do|, |dlse| and |v| of what takes part: the queries that see a key and the
+// keys that a query sees. Infinities (and NaN) are left out: what they reach is not
+// finite by any scale, and the rest keeps its own. Three quarters of the workgroups
+// read grad_o, the rest v, a run of tokens each (8,192 tokens, 32 heads of 128 on 8:
+// 84 MB in 22 to 27 us).
 template <int D>
 __global__ __launch_bounds__(256) void range_kernel(const BwdParams p) {
   constexpr int LPR = D / 8, RPB = 256 / LPR;  // lanes of a row, rows of a workgroup
-  const int split = gridDim.x * 3 / 4;
-  const bool of_v = blockIdx.x >= split;
-  const int block = of_v ? blockIdx.x - split : blockIdx.x, blocks = of_v ? gridDim.x - split : split;
-  const int heads = of_v ? p.f.Hk : p.f.Hq, tokens = of_v ? p.f.Tk : p.f.Tq, unit = threadIdx.x % LPR * 16;
-  const long rows = static_cast<long>(p.B) * tokens * heads;
-  float top = 0.0f, top_dlse = 0.0f;
-  for (long r = block * static_cast<long>(RPB) + threadIdx.x / LPR; r < rows; r += blocks * static_cast<long>(RPB)) {
-    const long bt = r / heads, b = bt / tokens;
-    const unsigned char *src = of_v ? p.f.v.base + b * p.f.v.batch + (bt - b * tokens) * p.f.v.token + (r - bt * heads) * p.f.v.head
-                                    : static_cast<const unsigned char *>(p.grad_o) + r * D * 2;
+  const WindowParams &f = p.f;
+  const int split = gridDim.x * 3 / 4, unit = threadIdx.x % LPR * 16, first = threadIdx.x / LPR;
+  const auto finite = [](float x) { return x < INFINITY ? x : 0.0f; };
+  const auto largest = [&](const unsigned char *src, float top) {
     const half8_t x = *reinterpret_cast<const half8_t *>(src + unit);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(static_cast<float>(x[i])));
-    if (!of_v && p.grad_lse && unit == 0 && p.lse[r] != -INFINITY) top_dlse = fmaxf(top_dlse, fabsf(p.grad_lse[r]));
+    for (int i = 0; i < 8; ++i) top = fmaxf(top, finite(fabsf(static_cast<float>(x[i]))));
+    return top;
+  };
+  float top = 0.0f, top_dlse = 0.0f;
+  if (static_cast<int>(blockIdx.x) < split) {
+    const long rows = static_cast<long>(p.B) * f.Tq * f.Hq;
+    for (long r = blockIdx.x * static_cast<long>(RPB) + first; r < rows; r += split * static_cast<long>(RPB)) {
+      if (p.lse[r] == -INFINITY) continue;
+      top = largest(static_cast<const unsigned char *>(p.grad_o) + r * D * 2, top);
+      if (p.grad_lse && unit == 0) top_dlse = fmaxf(top_dlse, finite(fabsf(p.grad_lse[r])));
+    }
+    range_max(top, p.range);
+    if (p.grad_lse) range_max(top_dlse, p.range + 2);
+    return;
   }
-  range_max(top, p.range + (of_v ? 1 : 0));
-  if (!of_v && p.grad_lse) range_max(top_dlse, p.range + 2);
+  const long tokens = static_cast<long>(p.B) * f.Tk, blocks = gridDim.x - split;
+  const long per = (tokens + blocks - 1) / blocks, t0 = (blockIdx.x - split) * per;
+  const long t1 = t0 + per < tokens ? t0 + per : tokens;
+  int seq = 0;
+  for (long r = t0 * f.Hk + first; r < t1 * f.Hk; r += RPB) {
+    const long bt = r / f.Hk, b = bt / f.Tk;
+    int key = static_cast<int>(bt - b * f.Tk);
+    const unsigned char *src = f.v.base + b * f.v.batch + key * f.v.token + (r - bt * f.Hk) * f.v.head;
+    if (f.cu_q) {
+      const int32_t *cu = f.cu_k ? f.cu_k : f.cu_q;
+      if (r < t0 * f.Hk + RPB) seq = last_at(cu, f.nseq, f.Tk, key);
+      while (seq < f.nseq && boundary(cu, seq + 1, f.Tk) <= key) ++seq;
+      if (seq == f.nseq) break;  // this token and those after belong to no sequence
+    } else {
+      seq = static_cast<int>(b);
+    }
+    const Seq sq = sequence<true>(f.cu_q, f.cu_k, seq, f.nseq, f.Tq, f.Tk);
+    key -= sq.k0;
+    if (sq.nq > 0 && (key > sq.nk - sq.nq - f.window || key < f.sinks)) top = largest(src, top);
+  }
+  range_max(top, p.range + 1);
 }
 
 // ---------------------------------------------------------------------------
@@ -490,16 +531,8 @@ __global__ __launch_bounds__(256) void join_kernel(const BwdParams p, int sink_b
       int seq = static_cast<int>(token / f.Tk), key = static_cast<int>(token - static_cast<long>(seq) * f.Tk);
       if (f.cu_q) {
         const int32_t *cu = f.cu_k ? f.cu_k : f.cu_q;
-        int lo = 0, hi = f.nseq;
-        while (lo < hi) {
-          const int mid = (lo + hi + 1) >> 1;
-          if (boundary(cu, mid, f.Tk) <= key)
-            lo = mid;
-          else
-            hi = mid - 1;
-        }
-        seq = lo;
-        key -= boundary(cu, lo, f.Tk);
+        seq = last_at(cu, f.nseq, f.Tk, key);
+        key -= boundary(cu, seq, f.Tk);
       }
       if (key < p.sinks && seq < f.nseq) continue;
     }

@@ -257,6 +257,51 @@ def test_what_no_query_sees_is_never_used():
     check("past the last boundary", q, k, v, go, glse, 0.125, None, 0, cu)
 
 
+@pytest.mark.parametrize("stale", [float("inf"), float("nan"), 6e4])
+@pytest.mark.parametrize("case", ["left of the window", "past the last boundary", "without queries", "before the first key"])
+def test_float16_gradients_are_not_scaled_by_what_no_query_sees(stale, case):
+    """The scale of ds, with gradients so small that it decides whether they are there at all."""
+    tq, tk, window, sinks, cu, cu_k = 120, 120, 40, 3, None, None
+    unseen_k, unseen_q = [], []
+    if case == "left of the window":
+        tq, tk = 40, 300
+        unseen_k = list(range(3, 300 - 40 - 40 + 1))
+    elif case == "before the first key":
+        tq, tk = 120, 70
+        unseen_q = list(range(50))
+    else:
+        lengths = ([30, 0, 50], [30, 0, 50]) if case == "past the last boundary" else ([30, 0, 50], [30, 11, 50])
+        cu, cu_k = (torch.tensor(np.cumsum([0] + n), dtype=torch.int32, device=DEV) for n in lengths)
+        unseen_k, unseen_q = list(range(30, 41)) if case == "without queries" else list(range(80, 120)), list(range(80, 120))
+    x = make(1, tq, tk, 4, 2, 64, torch.float16, 24, 1e-6)
+    x[1] = x[1] * 64  # (dq itself stays above float16's smallest numbers)
+    x[4].zero_()
+    for rows, tensors in ((unseen_k, x[1:3]), (unseen_q, x[3:4])):
+        for t in tensors:
+            t[:, rows] = 0
+    want = check(case, *x, 0.125 / 64, window, sinks, cu, cu_k)
+    for n in ("dq", "dv"):  # (dk, a 64th of dq in size, is below float16's smallest number)
+        assert torch.count_nonzero(want[n]) > 0
+    for rows, tensors in ((unseen_k, x[1:3]), (unseen_q, x[3:4])):
+        for t in tensors:
+            t[:, rows] = stale
+    leaves = [t.detach().requires_grad_(True) for t in x[:3]]
+    o, lse = at.window_attention(*leaves, 0.125 / 64, window, sinks, cu, cu_k, return_lse=True)
+    for n, g in zip(("dq", "dk", "dv"), torch.autograd.grad((o, lse), leaves, x[3:])):
+        assert torch.equal(g, want[n]), n
+
+
+def test_float16_gradients_keep_their_scale_beside_a_visible_infinity():
+    """A value that is infinite spoils its own sequence, not the size of another's gradients."""
+    q, k, v, go, _ = make(2, 90, 90, 4, 2, 64, torch.float16, 25, 1e-6)
+    v[0, 40, 1, 7] = 0.25
+    clean = at.window_attention_bwd(q, k, v, *at.window_attention_fwd(q, k, v, 0.125, 30), go, 0.125, 30)
+    v[0, 40, 1, 7] = float("inf")
+    got = at.window_attention_bwd(q, k, v, *at.window_attention_fwd(q, k, v, 0.125, 30), go, 0.125, 30)
+    for x, y in zip(got, clean):
+        assert torch.equal(x[1], y[1])
+
+
 def test_lowest_scores_and_visible_nan():
     """Scores at the type's lowest value still weigh; a NaN key spoils only rows that see it."""
     q, k, v, go, glse = make(1, 50, 50, 1, 1, 64, torch.float32, 13)
