@@ -29,6 +29,7 @@ import ctypes
 import functools
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 from torch.utils._python_dispatch import _get_current_dispatch_mode
 
@@ -67,6 +68,14 @@ def _one_device(first, *rest) -> torch.device:
         if t is not None and t.get_device() != index:
             return _require_device(first, *rest)
     return first.device
+
+
+def _no_tangents(where: str, *tensors) -> None:
+    """Raise where forward-mode differentiation would lose the tensors' tangents."""
+    if torch.compiler.is_compiling() or forward_ad._current_level < 0:
+        return
+    if any([t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors]):
+        raise RuntimeError(f"{where} has no forward-mode derivative")
 
 
 def _dtype_code(dtype: torch.dtype) -> int:
@@ -304,7 +313,8 @@ window_attention_op.register_autograd(_gradients(window_attention_backward_op), 
 def _untraced(*tensors) -> bool:
     """Ordinary tensors that nothing compiles, traces or transforms."""
     return (not torch.compiler.is_compiling() and _get_current_dispatch_mode() is None
-            and not torch._C._are_functorch_transforms_active() and all(type(t) in (torch.Tensor, torch.nn.Parameter) for t in tensors))
+            and not torch._C._are_functorch_transforms_active() and torch._C._get_tracing_state() is None
+            and all([type(t) in (torch.Tensor, torch.nn.Parameter) for t in tensors]))
 
 
 class _WindowAttention(torch.autograd.Function):
@@ -321,6 +331,7 @@ class _WindowAttention(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_o, grad_lse):
+        _no_tangents("window_attention's backward", grad_o, grad_lse)
         tensors = [t for t in (grad_o, grad_lse) if t is not None]
         return (_WindowAttention._launched if _untraced(*tensors) else _WindowAttention._traced)(ctx, grad_o, grad_lse)
 
@@ -333,7 +344,8 @@ def window_attention(q, k, v, scale: float, window=None, sinks: int = 0, cu_seql
     last Tq positions; cu_seqlens (and cu_seqlens_k, where keys and queries differ
     in number) packs sequences. Returns o [B,Tq,Hq,D] in q's dtype, with
     return_lse (o, lse [B,Tq,Hq] float32); differentiable in q, k and v, also
-    through lse."""
+    through lse, once and in reverse mode (a forward-mode tangent raises)."""
+    _no_tangents("window_attention", q, k, v)
     d = _window_check(q, k, v, cu_seqlens, cu_seqlens_k, window, sinks)[0][-1]
     _one_device(q, k, v, cu_seqlens, cu_seqlens_k)
     if d not in ATTENTION_HEAD_DIMS:
@@ -353,6 +365,7 @@ def window_attention(q, k, v, scale: float, window=None, sinks: int = 0, cu_seql
 # The paged cache.
 # ----------------------------------------------------------------------------
 def _inference_only(where: str, *tensors) -> None:
+    _no_tangents(where, *tensors)
     if torch.is_grad_enabled() and any([t.requires_grad for t in tensors]):
         raise RuntimeError(f"{where} has no backward: call it under torch.no_grad() (inference), or use "
                            "window_attention, which has one")

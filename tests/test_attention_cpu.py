@@ -303,6 +303,41 @@ def test_a_stale_attention_library_is_named(tmp_path):
         _lib._load_attn(str(lib))
 
 
+def test_forward_mode_tangents_are_refused(monkeypatch):
+    """The kernels have no forward-mode derivative: no result without its tangent."""
+    import torch.autograd.forward_ad as forward_ad
+    monkeypatch.setattr(at, "_one_device", lambda *t: t[0].device)
+    monkeypatch.setattr(at, "_launch", lambda *args: None)
+    q, k, v = tensors()
+    cache, slots = torch.zeros(5, 16, 2, 64), torch.arange(8)
+    table, lengths = torch.zeros(1, 3, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    with torch.no_grad():
+        at.window_attention(q, k, v, 1.0)
+    with forward_ad.dual_level():
+        at.window_attention(q, k, v, 1.0)  # no tangent among the inputs
+        for i in range(3):
+            x = [q, k, v]
+            x[i] = forward_ad.make_dual(x[i], torch.ones_like(x[i]))
+            with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                at.window_attention(*x, 1.0)
+        with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+            at.paged_decode_attention(forward_ad.make_dual(q, q)[:, :1], cache, cache, table, lengths, 1.0)
+        with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+            at.paged_cache_write(forward_ad.make_dual(k[0], k[0]), v[0], cache, cache, slots)
+    with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+        torch.func.jvp(lambda t: at.window_attention(t, k, v, 1.0), (q,), (q,))
+
+
+@pytest.mark.filterwarnings("ignore")
+def test_jit_trace_records_the_op(monkeypatch):
+    """Not the empty output that the launch fills."""
+    monkeypatch.setattr(at, "_one_device", lambda *t: t[0].device)
+    monkeypatch.setattr(at, "_launch", lambda *args: None)
+    q, k, v = tensors()
+    graph = torch.jit.trace(lambda q, k, v: at.window_attention(q, k, v, 1.0, 4, 1), (q, k, v), check_trace=False).graph
+    assert "pbgdn::window_attention" in str(graph) and "aten::empty" not in str(graph)
+
+
 def test_ops_infer_shapes():
     from torch._subclasses.fake_tensor import FakeTensorMode
     with FakeTensorMode():
