@@ -31,7 +31,6 @@ import functools
 import torch
 from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
-from torch.utils._python_dispatch import _get_current_dispatch_mode
 
 from . import _lib
 from .gated_deltanet import _aligned, _pad_last, _require_device, _width_at_least, grad_needed
@@ -72,10 +71,20 @@ def _one_device(first, *rest) -> torch.device:
 
 def _no_tangents(where: str, *tensors) -> None:
     """Raise where forward-mode differentiation would lose the tensors' tangents."""
-    if torch.compiler.is_compiling() or forward_ad._current_level < 0:
-        return
-    if any([t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors]):
+    if forward_ad._current_level >= 0 and not _compiling() and any(
+            [t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors]):
         raise RuntimeError(f"{where} has no forward-mode derivative")
+
+
+# (bound once: a short call asks all of them)
+_compiling, _dispatch_modes = torch.compiler.is_compiling, torch._C._len_torch_dispatch_stack
+_transformed, _tracing = torch._C._are_functorch_transforms_active, torch._C._get_tracing_state
+_plain = frozenset((torch.Tensor, torch.nn.Parameter)).issuperset
+
+
+def _untraced(*tensors) -> bool:
+    """Ordinary tensors that nothing compiles, traces or transforms."""
+    return not (_compiling() or _dispatch_modes() or _transformed() or _tracing()) and _plain(map(type, tensors))
 
 
 def _dtype_code(dtype: torch.dtype) -> int:
@@ -310,13 +319,6 @@ def _gradients(backward):
 window_attention_op.register_autograd(_gradients(window_attention_backward_op), setup_context=_attention_setup)
 
 
-def _untraced(*tensors) -> bool:
-    """Ordinary tensors that nothing compiles, traces or transforms."""
-    return (not torch.compiler.is_compiling() and _get_current_dispatch_mode() is None
-            and not torch._C._are_functorch_transforms_active() and torch._C._get_tracing_state() is None
-            and all([type(t) in (torch.Tensor, torch.nn.Parameter) for t in tensors]))
-
-
 class _WindowAttention(torch.autograd.Function):
     """The op and its gradients without the op's dispatch, which costs more than a short call."""
     _launched = staticmethod(_gradients(_backward_launch))
@@ -365,7 +367,8 @@ def window_attention(q, k, v, scale: float, window=None, sinks: int = 0, cu_seql
 # The paged cache.
 # ----------------------------------------------------------------------------
 def _inference_only(where: str, *tensors) -> None:
-    _no_tangents(where, *tensors)
+    if forward_ad._current_level >= 0:
+        _no_tangents(where, *tensors)
     if torch.is_grad_enabled() and any([t.requires_grad for t in tensors]):
         raise RuntimeError(f"{where} has no backward: call it under torch.no_grad() (inference), or use "
                            "window_attention, which has one")
@@ -464,10 +467,15 @@ def paged_decode_attention(q, k_cache, v_cache, page_table, lengths, scale: floa
     window_attention. Returns o [B,T,Hq,D] in q's dtype, with return_lse (o, lse
     [B,T,Hq] float32). Inference only."""
     _inference_only("paged_decode_attention", q, k_cache, v_cache)
-    if torch.compiler.is_compiling() and out is None:
-        o, lse = paged_decode_attention_op(q, k_cache, v_cache, page_table, lengths, float(scale), window, int(sinks))
-    else:
+    if _untraced(q, k_cache, v_cache, page_table, lengths):
         o, lse = _decode(q, k_cache, v_cache, page_table, lengths, scale, window, sinks, out, return_lse)
+    else:
+        window = None if window is None else int(window)
+        o, lse = paged_decode_attention_op(q, k_cache, v_cache, page_table, lengths, float(scale), window, int(sinks))
+        if out is not None:
+            if out.shape != o.shape or out.dtype != o.dtype:
+                raise ValueError("out must have q's shape and dtype")
+            o = out.copy_(o)
     return (o, lse) if return_lse else o
 
 
@@ -484,7 +492,8 @@ def _write_steps(cache, k, k_stride, v, v_stride, slots, size):
 
 def _write_operands(k, v, cache, dtype, slots_shape):
     """New rows in the caches' dtype as the kernel reads them, and their stride array."""
-    k, v = _aligned(k, 16), _aligned(v, 16)  # (before the strides are taken: a copy may have others)
+    if (k.data_ptr() | v.data_ptr()) % 16:  # (before the strides are taken: a copy may have others)
+        k, v = _aligned(k, 16), _aligned(v, 16)
     steps = _write_steps(cache, k.shape, k.stride(), v.shape, v.stride(), slots_shape, dtype.itemsize)
     if steps is None or k.dtype != dtype or v.dtype != dtype:
         k, v = (x.to(dtype).reshape(-1, *cache[2:]).contiguous() for x in (k, v))
@@ -523,7 +532,7 @@ def paged_cache_write(k, v, k_cache, v_cache, slots) -> None:
     the others must be distinct. k and v are cast to the caches' dtype. Inference
     only."""
     _inference_only("paged_cache_write", k, v, k_cache, v_cache)
-    if torch.compiler.is_compiling():
-        paged_cache_write_op(k, v, k_cache, v_cache, slots)
-    else:
+    if _untraced(k, v, k_cache, v_cache, slots):
         _write(k, v, k_cache, v_cache, slots)
+    else:
+        paged_cache_write_op(k, v, k_cache, v_cache, slots)

@@ -338,6 +338,44 @@ def test_jit_trace_records_the_op(monkeypatch):
     assert "pbgdn::window_attention" in str(graph) and "aten::empty" not in str(graph)
 
 
+def paged_inputs(dtype=torch.bfloat16, device=None):
+    q, k, v = (torch.zeros(2, 1, h, 64, dtype=dtype, device=device) for h in (4, 2, 2))
+    kc, vc = (torch.zeros(5, 16, 2, 64, dtype=dtype, device=device) for _ in range(2))
+    table, lengths = torch.zeros(2, 3, dtype=torch.int32, device=device), torch.ones(2, dtype=torch.int32, device=device)
+    return q, k[:, 0], v[:, 0], kc, vc, table, lengths, torch.arange(2, device=device)
+
+
+def paged_step(q, k, v, kc, vc, table, lengths, slots, out=None):
+    at.paged_cache_write(k, v, kc, vc, slots)
+    return at.paged_decode_attention(q, kc, vc, table, lengths, 0.125, 8, 1, return_lse=True, out=out)
+
+
+def test_paged_calls_under_fake_tensors():
+    """Inside the mode, and with fake tensors outside of it."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        x = paged_inputs()
+        o, lse = paged_step(*x)
+        assert o.shape == x[0].shape and o.dtype == x[0].dtype and lse.shape == (2, 1, 4)
+        out = torch.empty_like(x[0])
+        assert paged_step(*x, out=out)[0] is out
+        with pytest.raises(ValueError, match="out must"):
+            paged_step(*x, out=out.float())
+    assert paged_step(*x)[0].shape == x[0].shape
+
+
+def test_paged_calls_are_traced_as_ops(monkeypatch):
+    """make_fx of real tensors: the ops, not the outputs that the launches fill."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    monkeypatch.setattr(at, "_one_device", lambda *t: t[0].device)
+    monkeypatch.setattr(at, "_launch", lambda *args: None)
+    monkeypatch.setattr(at, "_decode_plan", lambda *args: ((2, 1, 4, 2, 64), 8, 1, 256))  # (asks for the device)
+    for mode in ("real", "fake", "symbolic"):
+        code = make_fx(lambda *x: paged_step(*x), tracing_mode=mode)(*paged_inputs()).code
+        assert "pbgdn.paged_cache_write_" in code and "pbgdn.paged_decode_attention" in code
+        assert "empty" not in code
+
+
 def test_ops_infer_shapes():
     from torch._subclasses.fake_tensor import FakeTensorMode
     with FakeTensorMode():

@@ -272,3 +272,32 @@ def test_prefill_then_decode_equals_one_pass():
         # two roundings of p and o to bfloat16 over values of size 4 at most
         torch.testing.assert_close(o.float(), whole[:, t:t + 1].float(), rtol=0, atol=4 * 4 * 2.0 ** -8)
         torch.testing.assert_close(l1, lse[:, t:t + 1], rtol=0, atol=1e-4)
+
+
+def test_compiled_decoding_equals_eager():
+    """A decode step under torch.compile: the caches and outputs of the eager calls, no break in the graph."""
+    q, kc, vc, table, lengths = make([300, 17, 90], 16, 8, 2, 64, 1, torch.bfloat16, 32)
+    k, v = (torch.randn(3, 2, 64, device=DEV).to(torch.bfloat16) for _ in range(2))
+    slots = torch.stack([table[b, (n - 1) // 16] * 16 + (n - 1) % 16 for b, n in enumerate((300, 17, 90))]).long()
+
+    def step(q, k, v, kc, vc, slots, out=None):
+        at.paged_cache_write(k, v, kc, vc, slots)
+        return at.paged_decode_attention(q * 2, kc, vc, table, lengths, 0.125, 50, 3, out=out) + 1
+
+    other = kc.clone(), vc.clone()
+    with torch.no_grad():
+        compiled = torch.compile(step, backend="aot_eager", fullgraph=True)
+        want = step(q, k, v, kc, vc, slots)
+        assert torch.equal(compiled(q, k, v, *other, slots), want)
+        assert torch.equal(other[0], kc) and torch.equal(other[1], vc)
+        outs = [torch.zeros_like(q) for _ in range(2)]
+        assert torch.equal(compiled(q, k, v, *other, slots, outs[0]), step(q, k, v, kc, vc, slots, outs[1]))
+        assert torch.equal(*outs)
+
+
+def test_paged_ops_pass_the_opcheck():
+    q, kc, vc, table, lengths = make([30, 7], 16, 4, 2, 64, 1, torch.float32, 33)
+    k, v = (torch.randn(2, 2, 64, device=DEV) for _ in range(2))
+    utils = ("test_schema", "test_faketensor", "test_autograd_registration")
+    torch.library.opcheck(at.paged_decode_attention_op, (q, kc, vc, table, lengths, 0.125, 8, 1), test_utils=utils)
+    torch.library.opcheck(at.paged_cache_write_op, (k, v, kc, vc, torch.tensor([3, 20], device=DEV)), test_utils=utils)

@@ -410,3 +410,30 @@ def test_compiled_ops_pass_the_opcheck():
     args = tuple(x.requires_grad_(True) for x in (q, k, v))
     torch.library.opcheck(at.window_attention_op, (*args, 0.125, 8, 1, None, None),
                           test_utils=("test_schema", "test_faketensor", "test_autograd_registration"))
+
+
+def test_backward_op_passes_the_opcheck():
+    q, k, v, go, glse = make(1, 20, 20, 2, 1, 64, torch.float32, 26)
+    o, lse = at.window_attention_fwd(q, k, v, 0.125, 8, 1)
+    torch.library.opcheck(at.window_attention_backward_op, (q, k, v, o, lse, go, glse, 0.125, 8, 1, None, None),
+                          test_utils=("test_schema", "test_faketensor", "test_autograd_registration"))
+
+
+@pytest.mark.parametrize("packed,d", [(False, 64), (True, 64), (False, 40)])
+def test_compiled_training_equals_eager(packed, d):
+    """Forward and gradients under torch.compile, without a break in the graph, other lengths after the first."""
+    def loss(q, k, v, cu):
+        o, lse = at.window_attention(q * 2, k, v, 0.125, 20, 2, cu, return_lse=True)
+        return (o.float() * 3).sum() + lse.sum()
+
+    compiled = torch.compile(loss, backend="aot_eager", fullgraph=True)
+    for n in (90, 70, 53):
+        x = make(1, n, n, 4, 2, d, torch.bfloat16, 27)[:3]
+        cu = torch.tensor([0, 30, n], dtype=torch.int32, device=DEV) if packed else None
+        got = []
+        for f in (compiled, loss):
+            leaves = [t.detach().requires_grad_(True) for t in x]
+            y = f(*leaves, cu)
+            got.append((y.detach(), *torch.autograd.grad(y, leaves)))
+        for a, b in zip(*got):
+            assert torch.equal(a, b)
