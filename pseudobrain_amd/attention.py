@@ -79,6 +79,7 @@ def _no_tangents(where: str, *tensors) -> None:
 # (bound once: a short call asks all of them)
 _compiling, _dispatch_modes = torch.compiler.is_compiling, torch._C._len_torch_dispatch_stack
 _transformed, _tracing = torch._C._are_functorch_transforms_active, torch._C._get_tracing_state
+_increment_version = torch.autograd.graph.increment_version
 _plain = frozenset((torch.Tensor, torch.nn.Parameter)).issuperset
 
 
@@ -534,5 +535,6 @@ def paged_cache_write(k, v, k_cache, v_cache, slots) -> None:
     _inference_only("paged_cache_write", k, v, k_cache, v_cache)
     if _untraced(k, v, k_cache, v_cache, slots):
         _write(k, v, k_cache, v_cache, slots)
+        _increment_version((k_cache, v_cache))  # (as the op does)
     else:
         paged_cache_write_op(k, v, k_cache, v_cache, slots)

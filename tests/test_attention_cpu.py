@@ -376,6 +376,23 @@ def test_paged_calls_are_traced_as_ops(monkeypatch):
         assert "empty" not in code
 
 
+def test_a_cache_write_counts_as_one(monkeypatch):
+    """The caches' versions rise, so that autograd notices a cache it has saved."""
+    monkeypatch.setattr(at, "_one_device", lambda *t: t[0].device)
+    monkeypatch.setattr(at, "_launch", lambda *args: None)
+    q, k, v, kc, vc, *_, slots = paged_inputs()
+    w = torch.ones(64, dtype=kc.dtype, requires_grad=True)
+    loss = (kc * w).sum() + (vc * w).sum()
+    before = kc._version, vc._version
+    at.paged_cache_write(k, v, kc, vc, slots)
+    assert kc._version > before[0] and vc._version > before[1]
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with torch.inference_mode():  # (tensors without a version)
+        kc, vc = kc.clone(), vc.clone()
+        at.paged_cache_write(k, v, kc, vc, slots)
+
+
 def test_ops_infer_shapes():
     from torch._subclasses.fake_tensor import FakeTensorMode
     with FakeTensorMode():
