@@ -31,8 +31,11 @@ namespace pbgdn {
 
 constexpr int QR = 32;            // rows of a query tile of dkdv_kernel
 // Rows (or a token's heads if more) of one part of the sinks' walk, by how many
-// sinks there are: a part's sums are as many float32 values as there are sinks,
-// for rows of 16 bits read twice, and stay a quarter of that.
+// sinks there are: a part's sums, two float32 rows a sink, against the rows of Q and
+// dO that each 32 sinks read. 16 rows a sink keep what the sums write to an eighth of
+// one such reading in 16 bits; past 256 sinks, where a part stays 4,096 rows, the sums
+// grow with the sinks (to twice one reading at 4,096), and so does the number of
+// readings.
 constexpr int tail_rows(int sinks) { return sinks < 8 ? 128 : sinks < 256 ? 16 * sinks : 4096; }
 constexpr int MAX_PARTS = 16;     // parts of an ordinary key tile's walk
 
@@ -51,18 +54,32 @@ struct BwdParams {
   int key_slots;      // key tiles of a (batch, key head)
   int sinks;          // keys that stay visible, 0 when no query is beyond their window
   int tail_tokens;    // query tokens of one part of the sinks' walk
-  int tail_slots;     // parts of the sinks' walk over all sequences, and slot 0 of each: the window's own part
+  int tail_slots;     // parts of the sinks' walk over all long sequences, and slot 0 of each: the window's own part
   // query tiles: `heads` heads of `tokens` tokens each, `splits` tiles for the heads of a token
   int heads, tokens, splits;
 };
 
-// Sequence n's slots in the parts of the sinks: the window's part, then one per tail_tokens tokens.
+// The sinks' parts belong to the long sequences, those of more keys than the window
+// (in the others no query is beyond it). In a packed call a long sequence's number is
+// at most its place, and at most the windows' worths of keys before it: it has no
+// other's number, whose sequence would lie a window and a key further on.
+__device__ __forceinline__ bool is_long(const WindowParams &f, const Seq &sq) { return sq.nk > f.window; }
+__device__ __forceinline__ int long_number(const WindowParams &f, int seq) {
+  if (!f.cu_q) return seq;
+  const int before = boundary(f.cu_k ? f.cu_k : f.cu_q, seq, f.Tk) / (f.window + 1);
+  return seq < before ? seq : before;
+}
+inline int long_most(const WindowParams &f) {
+  const int most = f.Tk / (f.window + 1);
+  return f.cu_q && most < f.nseq ? most : f.nseq;
+}
+// A long sequence's slots: the window's part, then one per tail_tokens tokens.
 __device__ __forceinline__ int tail_start(const BwdParams &p, int seq) {
   if (!p.f.cu_q) return seq * ((p.f.Tq + p.tail_tokens - 1) / p.tail_tokens + 1);
-  return boundary(p.f.cu_q, seq, p.f.Tq) / p.tail_tokens + 2 * seq;
+  return boundary(p.f.cu_q, seq, p.f.Tq) / p.tail_tokens + 2 * long_number(p.f, seq);
 }
-inline long tail_slot_count(int Tq, int nseq, int tokens, bool packed) {
-  return packed ? Tq / tokens + 2L * nseq : nseq * ((Tq + tokens - 1L) / tokens + 1);
+inline long tail_slot_count(const WindowParams &f, int tokens) {
+  return f.cu_q ? f.Tq / tokens + 2L * long_most(f) : f.nseq * ((f.Tq + tokens - 1L) / tokens + 1);
 }
 
 // The last of the boundaries 0 .. n that is no further than `token`: its sequence, or n past the last.
@@ -213,7 +230,7 @@ __global__ __launch_bounds__(NW * 64, WAVES) void dkdv_kernel(const BwdParams p)
     id /= sink_tiles;
     hk = uniform(id % f.Hk);
     slot = uniform(id / f.Hk);
-    // bisection over the sequences' first slots
+    // bisection over the sequences' first slots: a long one's are past those of all before it
     int lo = 0, hi = f.nseq - 1;
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
@@ -243,7 +260,7 @@ __global__ __launch_bounds__(NW * 64, WAVES) void dkdv_kernel(const BwdParams p)
   }
   const Seq sq = sequence<true>(f.cu_q, f.cu_k, seq, f.nseq, f.Tq, f.Tk);
   const int j0 = tile * K::BN;
-  if (part < 0 || tile < 0 || j0 >= sq.nk) return;
+  if (part < 0 || tile < 0 || j0 >= sq.nk || (TAIL && !is_long(f, sq))) return;
   const int off = sq.nk - sq.nq;  // position of query token 0
 
   // the query tokens [t0, t1) of this part
@@ -459,7 +476,7 @@ __global__ __launch_bounds__(NW * 64, WAVES) void dkdv_kernel(const BwdParams p)
     const long half = static_cast<long>(p.B) * f.Tk * f.Hk * D;
     store_row<PBGDN_F32, D>(p.part + part * half + row * D, dk, h, fk);
     store_row<PBGDN_F32, D>(p.part + (p.parts + part) * half + row * D, dv, h, 1.0f);
-  } else if (key < p.sinks && seq < f.nseq) {
+  } else if (key < p.sinks && seq < f.nseq && is_long(f, sq)) {
     const long at = ((static_cast<long>(tail_start(p, seq)) * f.Hk + hk) * p.sinks + key) * D;
     const long half = static_cast<long>(p.tail_slots) * f.Hk * p.sinks * D;
     store_row<PBGDN_F32, D>(p.tail + at, dk, h, fk);
@@ -471,7 +488,7 @@ __global__ __launch_bounds__(NW * 64, WAVES) void dkdv_kernel(const BwdParams p)
 }
 
 // Sums the parts of dk and dv, in a fixed order. The first `sink_blocks`
-// workgroups take a sink each (of a sequence and key head): its threads, four
+// workgroups take a sink each (of a long sequence and key head): its threads, four
 // elements of the row each, split the many parts and join through LDS. The rest
 // take the other keys where p.parts > 1, four elements a thread. Bound by the
 // parts' reads (5 parts of 6,011 keys, 2 heads of 256: 123 MB in 23 us).
@@ -493,9 +510,21 @@ __global__ __launch_bounds__(256) void join_kernel(const BwdParams p, int sink_b
     int id = blockIdx.x;
     const int key = id % p.sinks;
     id /= p.sinks;
-    const int hk = id % f.Hk, seq = id / f.Hk;
+    const int hk = id % f.Hk, number = id / f.Hk;
+    int seq = number;
+    if (f.cu_q) {  // the last sequence that has no higher number, if it is the long one of this
+      int lo = 0, hi = f.nseq - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (long_number(f, mid) <= number)
+          lo = mid;
+        else
+          hi = mid - 1;
+      }
+      seq = lo;
+    }
     const Seq sq = sequence<true>(f.cu_q, f.cu_k, seq, f.nseq, f.Tq, f.Tk);
-    if (key >= sq.nk) return;
+    if (key >= sq.nk || !is_long(f, sq) || long_number(f, seq) != number) return;
     const long row = ((f.cu_q ? 0 : static_cast<long>(seq) * f.Tk) + sq.k0 + key) * f.Hk + hk;
     const int tails = (sq.nq + p.tail_tokens - 1) / p.tail_tokens;
     const int d = threadIdx.x % TPR * 4, group = threadIdx.x / TPR;
@@ -534,7 +563,7 @@ __global__ __launch_bounds__(256) void join_kernel(const BwdParams p, int sink_b
         seq = last_at(cu, f.nseq, f.Tk, key);
         key -= boundary(cu, seq, f.Tk);
       }
-      if (key < p.sinks && seq < f.nseq) continue;
+      if (key < p.sinks && seq < f.nseq && is_long(f, sequence<true>(f.cu_q, f.cu_k, seq, f.nseq, f.Tq, f.Tk))) continue;
     }
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
@@ -799,7 +828,7 @@ static int launch_bwd(BwdParams &p, hipStream_t stream) {
       hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(64), K::BYTES, stream, p);
     }
     if (p.parts > 1 || p.sinks) {
-      const long sinks = static_cast<long>(f.nseq) * f.Hk * p.sinks;
+      const long sinks = p.sinks ? static_cast<long>(long_most(f)) * f.Hk * p.sinks : 0;
       const long want = p.parts > 1 ? (static_cast<long>(p.B) * f.Tk * f.Hk * (D / 4) + 255) / 256 : 0;
       const long blocks = sinks + (want < 65536 ? want : 65536);
       if (blocks > 0x7fffffffL) return PBGDN_ERR_UNSUPPORTED;
@@ -824,7 +853,7 @@ static bool plan(Plan &w, const WindowParams &f, int dtype, int B, int D) {
   w.parts = walk_parts(f, B, key_tile(dtype, D), shape.cus);
   w.sinks = sink_count(f);
   w.tail_tokens = (tail_rows(w.sinks) + f.group - 1) / f.group;
-  const long slots = w.sinks ? tail_slot_count(f.Tq, f.nseq, w.tail_tokens, f.cu_q != nullptr) : 0;
+  const long slots = w.sinks ? tail_slot_count(f, w.tail_tokens) : 0;
   if (slots > 0x7fffffffL) return false;
   w.tail_slots = static_cast<int>(slots);
   const auto round = [](size_t x) { return (x + 255) & ~static_cast<size_t>(255); };

@@ -142,6 +142,18 @@ def test_backward_workspace():
     assert size(1, 64, 64, 4, 2, 96, 1, 1, 0, 0, 0) == 0                  # width
 
 
+def test_backward_workspace_of_short_documents():
+    """Sequences no longer than the window have no sinks beyond it: 8,192 tokens in 1,000 documents, window
+    128, 64 sinks, 8 key heads of 128. At most 63 of them are longer, with two parts each beside one per 256
+    tokens, of 2 x 64 x 8 x 128 float32 values: 83 MB."""
+    size = _lib.attn_lib().pbattn_window_bwd_workspace_size
+    plain = size(1, 8192, 8192, 32, 8, 128, 1000, 1, 1, 128, 0)
+    packed = size(1, 8192, 8192, 32, 8, 128, 1000, 1, 1, 128, 64)
+    assert 0 < packed - plain <= (2 * 63 + 32 + 1) * 2 * 64 * 8 * 128 * 4
+    # few long ones: two parts of each beside one per 256 tokens
+    assert size(1, 8192, 8192, 32, 8, 128, 2, 1, 1, 128, 64) - plain <= (2 * 2 + 32 + 1) * 2 * 64 * 8 * 128 * 4
+
+
 def decode(**over):
     args = dict(q=FAKE, k=FAKE, v=FAKE, dtype=1, strides=strides(16 * 256, 256, 128), page=16, pages=8, table=FAKE,
                 max_pages=4, lengths=FAKE, o=FAKE, lse=None, B=2, T=1, Hq=4, Hk=2, D=128, scale=0.1, window=0, sinks=0,

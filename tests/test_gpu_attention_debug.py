@@ -31,3 +31,17 @@ CASES = {
 def test_under_the_debug_build(case):
     with _lib.debug_library():
         CASES[case]()
+
+
+SINKS = {
+    "short and long sequences": lambda: window.test_sinks_of_packed_short_and_long_sequences(2, 4),
+    "short and long sequences, many sinks": lambda: window.test_sinks_of_packed_short_and_long_sequences(1, 70),
+    "parts beside the sinks'": lambda: window.test_sinks_of_a_long_packed_call(1),
+}
+
+
+@pytest.mark.parametrize("case", SINKS)
+def test_sinks_under_the_debug_build(case):
+    """A part of the sinks' that is joined but was not written shows as NaN."""
+    with _lib.debug_library():
+        SINKS[case]()

@@ -116,6 +116,31 @@ def test_packed_sequences(dtype, d):
     check("packed, no window", *x, d ** -0.5, None, 0, cu)
 
 
+@pytest.mark.parametrize("hk,sinks", [(2, 4), (1, 70)])
+def test_sinks_of_packed_short_and_long_sequences(hk, sinks):
+    """Sequences around the window's length among many shorter ones; few key heads: walks in parts too."""
+    window = 60
+    lengths = [3] * 25 + [200, 5, 0, 59, 60, 61, 61, 1, 0, 62, 60] + [7] * 30 + [500, 61, 2]
+    cu = torch.tensor(np.cumsum([0] + lengths), dtype=torch.int32, device=DEV)
+    x = make(1, sum(lengths) + 9, sum(lengths) + 9, 4, hk, 64, torch.bfloat16, 28)
+    check("short and long", *x, 0.125, window, sinks, cu)
+    # continuations: queries fewer than keys, more than keys, none
+    nq = [1, 61, 5, 0, 130, 3, 62, 400, 9]
+    nk = [61, 61, 200, 80, 20, 60, 300, 430, 0]
+    cq, ck = (torch.tensor(np.cumsum([0] + n), dtype=torch.int32, device=DEV) for n in (nq, nk))
+    x = make(1, sum(nq), sum(nk) + 4, 4, hk, 64, torch.bfloat16, 29)
+    check("short and long continuations", *x, 0.125, window, sinks, cq, ck)
+
+
+@pytest.mark.parametrize("hk", [1, 2])
+def test_sinks_of_a_long_packed_call(hk):
+    """Long enough for parts of ordinary walks beside the sinks' (a row's sums over both), float32."""
+    lengths = [1500, 3, 90, 1200] + [11] * 20
+    cu = torch.tensor(np.cumsum([0] + lengths), dtype=torch.int32, device=DEV)
+    x = make(1, sum(lengths), sum(lengths), 2 * hk, hk, 64, torch.float32, 34)
+    check("long packed", *x, 0.125, 700, 5, cu)
+
+
 def test_packed_queries_and_keys():
     """Packed continuations: each sequence's queries against more (or fewer) keys."""
     nq, nk = [5, 64, 0, 40, 9], [70, 64, 12, 10, 0]
