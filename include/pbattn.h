@@ -77,6 +77,11 @@ int pbattn_abi_version(void);
  *   o          [B, Tq, Hq, D] dense, dtype, written
  *   lse        [B, Tq, Hq] dense float32, written; may be NULL
  *   D          64, 128 or 256 (narrower heads zero-padded by the caller)
+ *
+ * A call without sequences or queries (B, num_seqs or Tq 0) launches nothing and
+ * writes nothing, the backward call's neither: where tokens of no sequence are
+ * left (num_seqs 0), or keys without queries (Tq 0), the caller fills o with
+ * zeros, lse with -infinity and the gradients with zeros.
  */
 int pbattn_window_fwd(const void *q, const void *k, const void *v, int dtype, const int64_t *strides,
                       const int32_t *cu_q, const int32_t *cu_k, int num_seqs, void *o, float *lse, int B, int Tq,

@@ -150,6 +150,23 @@ def test_packed_queries_and_keys():
     check("packed continuations, no window", *x, 0.125, None, 0, cq, ck)
 
 
+def test_calls_without_sequences_or_queries():
+    """What the launches leave out is filled in: zeros, and lse -inf."""
+    q, k, v, go, glse = make(1, 7, 7, 4, 2, 64, torch.bfloat16, 35)
+    none = torch.zeros(1, dtype=torch.int32, device=DEV)
+    for dtype in (torch.int32, torch.int64):
+        leaves = [x.detach().requires_grad_(True) for x in (q, k, v)]
+        o, lse = at.window_attention(*leaves, 0.125, 3, 1, none.to(dtype), return_lse=True)
+        assert torch.count_nonzero(o) == 0 and torch.isneginf(lse).all()
+        assert all(torch.count_nonzero(g) == 0 for g in torch.autograd.grad((o, lse), leaves, (go, glse)))
+    for shape in ((1, 0, 4, 64), (0, 7, 4, 64)):
+        q = torch.randn(shape, device=DEV).to(torch.bfloat16).requires_grad_(True)
+        kv = [torch.randn(shape[0], 7, 2, 64, device=DEV).to(torch.bfloat16).requires_grad_(True) for _ in range(2)]
+        o, lse = at.window_attention(q, *kv, 0.125, return_lse=True)
+        assert o.shape == q.shape and lse.shape == q.shape[:3]
+        assert all(torch.count_nonzero(g) == 0 for g in torch.autograd.grad((o, lse), (q, *kv), (o, lse)))
+
+
 def test_many_short_sequences_equal_the_batched_call():
     """300 packed sequences of 9 tokens are the batched call, bit for bit."""
     q, k, v, go, _ = make(300, 9, 9, 4, 2, 64, torch.bfloat16, 5)
