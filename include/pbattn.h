@@ -117,7 +117,7 @@ int pbattn_window_bwd(const void *q, const void *k, const void *v, int dtype, co
                       int Hq, int Hk, int D, float scale, int window, int sinks, void *workspace,
                       size_t workspace_bytes, void *stream);
 
-/* Bytes of workspace pbattn_window_bwd needs: 8 bytes per (token, query head)
+/* Bytes of workspace pbattn_window_bwd needs: 12 bytes per (token, query head)
  * and, where the sums over queries are split, their float32 parts. 0 for
  * invalid sizes. `packed`: cu_q is given. */
 size_t pbattn_window_bwd_workspace_size(int B, int Tq, int Tk, int Hq, int Hk, int D, int num_seqs, int dtype,

@@ -29,7 +29,16 @@
 
 namespace pbgdn {
 
+// Weights are exp2(s c - lse), with lse in powers of two as one float32: off by up to
+// 2^-23 |lse|. In rows whose |lse| (natural) is beyond this, where that would reach
+// 2^-13, dq_kernel finds the largest score and the sum again; the largest is then the
+// row's origin, which its scores lose before they are scaled, and lse the sum's
+// logarithm alone. Workgroups that meet such rows (`has_large`) go the masked tiles'
+// way throughout, and take the origins off there.
+constexpr float LARGE_LSE = 1024.0f;
+
 constexpr int QR = 32;            // rows of a query tile of dkdv_kernel
+constexpr int DQ_WAVES = 4, DQ_ROWS = 32 * DQ_WAVES;  // waves and rows of a workgroup of dq_kernel
 // Rows (or a token's heads if more) of one part of the sinks' walk, by how many
 // sinks there are: a part's sums, two float32 rows a sink, against the rows of Q and
 // dO that each 32 sinks read. 16 rows a sink keep what the sums write to an eighth of
@@ -45,6 +54,8 @@ struct BwdParams {
   const float *lse, *grad_lse;
   void *dq, *dk, *dv;
   float2 *stat;       // [B][Hk][Tq G]: (lse log2(e), delta); +inf for a row that sees nothing
+  float *origin;      // as stat: zero but for rows of large scores
+  int *has_large;     // [B][Hk][f.slots]: a tile of dq_kernel has such a row
   uint32_t *range;    // float16: bits of max |do|, |v|, |dlse|
   float *part;        // [2][parts][B][Hk][Tk][D] when parts > 1
   float *tail;        // [2][tail slots][Hk][sinks][D]
@@ -197,7 +208,7 @@ __global__ __launch_bounds__(256) void range_kernel(const BwdParams p) {
 template <int DT, int D, int NW>
 struct Dkdv {
   using L = Tile<DT, D>;
-  static constexpr int BN = 32 * NW, TILE = QR * L::ROW, STAT = QR * 8, BUF = 2 * TILE + STAT, LDS = 2 * BUF;
+  static constexpr int BN = 32 * NW, TILE = QR * L::ROW, STAT = QR * 16, BUF = 2 * TILE + STAT, LDS = 2 * BUF;
   static constexpr int LOADS = QR / L::PER_DMA;  // of one tensor, all waves
   // Registers hold the sums, and K and V rows where they find room beside them
   // (two waves a SIMD up to D = 128 in 16 bits): otherwise LDS does.
@@ -286,6 +297,19 @@ __global__ __launch_bounds__(NW * 64, WAVES) void dkdv_kernel(const BwdParams p)
   }
   const int tiles = uniform(t1 > t0 ? (t1 - t0 + p.tokens - 1) / p.tokens * p.splits : 0);
 
+  // whether the tiles of dq_kernel that those tokens' rows lie in have rows of large scores
+  int some_large = 0;
+  if (tiles > 0) {
+    const int *flags = p.has_large + (static_cast<long>(b) * f.Hk + hk) * f.slots +
+                       (f.cu_q ? slot_start(f.cu_q, seq, f.Tq, G, DQ_ROWS) : 0);
+    const int last = (t1 * G - 1) / DQ_ROWS;
+    int s = t0 * G / DQ_ROWS + lane;
+    if (s <= last) some_large = flags[s];
+    if (uniform(s) + 64 <= last) {
+      for (s += 64; s <= last; s += 64) some_large |= flags[s];
+    }
+  }
+
   // this wave's keys
   const int key = j0 + wave * 32 + n;
   const int kc = key < sq.nk ? key : sq.nk - 1;
@@ -318,6 +342,7 @@ __global__ __launch_bounds__(NW * 64, WAVES) void dkdv_kernel(const BwdParams p)
 #pragma unroll
     for (int s = 0; s < S; ++s) settle(vf[s]);
   }
+  some_large = __any(some_large);
   float16_t dk[MB], dv[MB];
 #pragma unroll
   for (int m = 0; m < MB; ++m) dk[m] = dv[m] = zero16();
@@ -371,7 +396,9 @@ __global__ __launch_bounds__(NW * 64, WAVES) void dkdv_kernel(const BwdParams p)
       dma(dq_, in ? qa : OUT_OF_RANGE, to + inst * 1024);
       dma(dg_, in ? ga : OUT_OF_RANGE, to + K::TILE + inst * 1024);
     }
-    if (wave == 0) dma4(dma_desc(sp, limit * (p.splits == 1 ? G * 8L : 8L)), lane * 4, to + 2 * K::TILE);
+    const long rows = limit * (p.splits == 1 ? G : 1);
+    if (wave == 0) dma4(dma_desc(sp, rows * 8), lane * 4, to + 2 * K::TILE);
+    if (wave == NW - 1) dma4(dma_desc(p.origin + (sp - p.stat), rows * 4), lane * 4, to + 2 * K::TILE + QR * 8);
     // on to the next
     if (++split == p.splits) {
       split = 0;
@@ -436,7 +463,15 @@ __global__ __launch_bounds__(NW * 64, WAVES) void dkdv_kernel(const BwdParams p)
       L::template rows_product<1>(gt, rbase, vf, &y);
     else
       y = L::rows_product_lds(gt, vl, rbase);
-    if (!whole) {
+    if (!whole || some_large) {
+      if (some_large) {
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+          const float4_t a = stat[QR / 2 + (2 * e + 4 * h) / 4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) x[e + r] -= a[r];
+        }
+      }
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         const int pos = p_lo + static_cast<int>((acc_row(e, h) * inv) >> 16);
@@ -615,6 +650,7 @@ __global__ __launch_bounds__(NW * 64, WAVES) void dq_kernel(const BwdParams p) {
   const int groups = gridDim.x / f.slots;
   int grp, slot;
   place(blockIdx.x, groups, f.slots, grp, slot);
+  int *const has_large = p.has_large + grp * static_cast<long>(f.slots) + slot;
   const int b = uniform(grp / f.Hk), hk = grp - b * f.Hk;
   int seq = b;
   if (f.cu_q) {
@@ -656,6 +692,8 @@ __global__ __launch_bounds__(NW * 64, WAVES) void dq_kernel(const BwdParams p) {
     settle(gf[s]);
   }
   float2 st;
+  float origin = 0.0f;
+  bool large;
   {
     const unsigned char *orow = static_cast<const unsigned char *>(p.o) + out * L::ROW;
     float sum = 0.0f;
@@ -673,10 +711,12 @@ __global__ __launch_bounds__(NW * 64, WAVES) void dq_kernel(const BwdParams p) {
     sum = add_xor32(sum);
     const float lse = p.lse[out], dlse = p.grad_lse ? p.grad_lse[out] : 0.0f;
     const bool empty = lse == -INFINITY;
+    large = fabsf(lse) > LARGE_LSE && fabsf(lse) < INFINITY;
     st = make_float2(empty ? INFINITY : lse * LOG2E, empty ? 0.0f : sum - dlse);
   }
   settle(st.x);
   settle(st.y);
+  const int wave_large = __any(large);
   const float scale16 = range_scale<DT, D>(p.range);
   float16_t dq[MB];
 #pragma unroll
@@ -688,23 +728,76 @@ __global__ __launch_bounds__(NW * 64, WAVES) void dq_kernel(const BwdParams p) {
     block_sync();
     if (it + 1 < tiles) stage.tile(it + 1, lds + ((it + 1) & 1) * F::TILE);
   };
-  // Scores and dP of 32 keys, those from u0 on of the range; `whole`: every row sees all of them.
-  const auto products = [&](const unsigned char *kt, const unsigned char *vt, int u0, bool whole, float16_t &x,
-                            float16_t &y) __attribute__((always_inline)) {
+  // Scores (and dP) of 32 keys, those from u0 on of the range; `whole`: every row sees all of them.
+  const auto scores = [&](const unsigned char *kt, int u0, bool whole, float16_t &x) __attribute__((always_inline)) {
     L::template rows_product<1>(kt, rbase, qf, &x);
-    L::template rows_product<1>(vt, rbase, gf, &y);
     if (!whole) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const int u = u0 + acc_row(i, h);
+        x[i] = sees(pos, u < range.sinks ? u : u + range.delta, f.window, f.sinks) ? x[i] : -INFINITY;
+      }
+    }
+  };
+  const auto products = [&](const unsigned char *kt, const unsigned char *vt, int u0, bool whole, float16_t &x,
+                            float16_t &y) __attribute__((always_inline)) {
+    L::template rows_product<1>(kt, rbase, qf, &x);
+    L::template rows_product<1>(vt, rbase, gf, &y);
+    if (!whole || wave_large) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int u = u0 + acc_row(i, h);
         const bool seen = sees(pos, u < range.sinks ? u : u + range.delta, f.window, f.sinks);
-        x[i] = seen ? x[i] : -INFINITY;
+        x[i] = seen ? x[i] - origin : -INFINITY;
         y[i] = seen ? y[i] : 0.0f;
       }
     }
   };
   const int mine = wave_tiles(range, tiles, w_last, BN);
   int it = 0;
+  const auto again = [&]() __attribute__((always_inline)) {  // the walk from its start
+    for (; it < tiles; ++it) advance(it);
+    it = 0;
+    block_sync();
+    stage.tile(0, lds);
+  };
+  // Rows of large scores: their largest, and the sum of the weights against it, once more.
+  __shared__ int any_large[NW];
+  if (lane == 0) any_large[wave] = wave_large;
+  block_sync();
+  int walk_large = 0;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) walk_large |= any_large[w];
+  walk_large = uniform(walk_large);
+  if (threadIdx.x == 0) *has_large = walk_large;
+  if (walk_large && tiles > 0) {
+    float m = -INFINITY, l = 0.0f;
+    for (; it < mine; ++it) {
+      advance(it);
+      const unsigned char *kt = lds + (it & 1) * F::TILE;
+      const bool whole = whole_tile(range, it * BN, BN, w_first, w_last, f.window);
+#pragma unroll 1
+      for (int kb = 0; kb < BN / 32; ++kb) {
+        float16_t x;
+        scores(kt + 32 * kb * L::ROW, it * BN + 32 * kb, whole, x);
+        float most = x[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) most = fmaxf(most, x[i]);
+        most = fmaxf(m, max_xor32(most));
+        const float base = most == -INFINITY ? 0.0f : most;
+        l *= __builtin_amdgcn_exp2f((m - base) * f.c);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) l += __builtin_amdgcn_exp2f((x[i] - base) * f.c);
+        m = most;
+      }
+    }
+    l += __shfl_xor(l, 32, 64);
+    if (large) {
+      origin = m;
+      st.x = __builtin_amdgcn_logf(l);
+    }
+    again();
+  }
   if constexpr (F::EXACT_TILES > 0) {
     if (tiles > 0 && tiles <= F::EXACT_TILES) {
       float sum = 0.0f;
@@ -722,16 +815,17 @@ __global__ __launch_bounds__(NW * 64, WAVES) void dq_kernel(const BwdParams p) {
           }
         }
       }
-      for (; it < tiles; ++it) advance(it);
       sum += __shfl_xor(sum, 32, 64);
       if (st.x != INFINITY) st.y += p.grad_lse ? sum - p.grad_lse[out] : sum;
       settle(st.y);
-      it = 0;
-      block_sync();
-      stage.tile(0, lds);
+      again();
     }
   }
-  if (h == 0 && row < total) p.stat[((static_cast<long>(b) * f.Hk + hk) * f.Tq + sq.q0) * G + r] = st;
+  if (h == 0 && row < total) {
+    const long at = ((static_cast<long>(b) * f.Hk + hk) * f.Tq + sq.q0) * G + r;
+    p.stat[at] = st;
+    p.origin[at] = origin;
+  }
   for (; it < mine; ++it) {
     advance(it);
     const unsigned char *kt = lds + (it & 1) * F::TILE, *vt = kt + 2 * F::TILE;
@@ -792,16 +886,17 @@ static int launch_bwd(BwdParams &p, hipStream_t stream) {
     hipLaunchKernelGGL((range_kernel<D>), dim3(shape.cus * 8), dim3(256), 0, stream, p);
   }
   {
-    constexpr int DQ_NW = 4, DQ_BN = DT == PBGDN_F32 ? (D == 64 ? 64 : 32) : D == 256 ? 32 : 64;
+    constexpr int DQ_BN = DT == PBGDN_F32 ? (D == 64 ? 64 : 32) : D == 256 ? 32 : 64;
     constexpr int W = DT != PBGDN_F32 && D <= 128 ? 2 : 1;
-    using F = Dq<DT, D, DQ_NW, DQ_BN>;
+    using F = Dq<DT, D, DQ_WAVES, DQ_BN>;
     static std::atomic<bool> flags[MAX_DEVICES];
-    const auto kernel = dq_kernel<DT, D, DQ_NW, DQ_BN, W>;
+    const auto kernel = dq_kernel<DT, D, DQ_WAVES, DQ_BN, W>;
     if (!smem_configured(reinterpret_cast<const void *>(kernel), F::LDS, flags)) return PBGDN_ERR_LAUNCH;
-    const long slots = window_slots(f, F::BM), blocks = slots * nb * f.Hk;
+    static_assert(F::BM == DQ_ROWS);
+    const long slots = window_slots(f, DQ_ROWS), blocks = slots * nb * f.Hk;
     if (blocks > 0x7fffffffL) return PBGDN_ERR_UNSUPPORTED;
     f.slots = static_cast<int>(slots);
-    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(DQ_NW * 64), F::LDS, stream, p);
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(DQ_WAVES * 64), F::LDS, stream, p);
   }
 
   constexpr int NW = dkdv_waves<DT, D>(), BN = 32 * NW;
@@ -841,7 +936,7 @@ static int launch_bwd(BwdParams &p, hipStream_t stream) {
 
 // The workspace: statistics, the float16 range, the parts.
 struct Plan {
-  size_t stat, range, part, tail, bytes;
+  size_t stat, origin, has_large, range, part, tail, bytes;
   int parts, sinks, tail_tokens, tail_slots;
 };
 static int key_tile(int dtype, int D) {
@@ -858,7 +953,9 @@ static bool plan(Plan &w, const WindowParams &f, int dtype, int B, int D) {
   w.tail_slots = static_cast<int>(slots);
   const auto round = [](size_t x) { return (x + 255) & ~static_cast<size_t>(255); };
   w.stat = 0;
-  w.range = round(static_cast<size_t>(B) * f.Tq * f.Hq * sizeof(float2));
+  w.origin = round(static_cast<size_t>(B) * f.Tq * f.Hq * sizeof(float2));
+  w.has_large = w.origin + round(static_cast<size_t>(B) * f.Tq * f.Hq * sizeof(float));
+  w.range = w.has_large + round(static_cast<size_t>(B) * f.Hk * window_slots(f, DQ_ROWS) * sizeof(int));
   w.part = w.range + 256;
   w.tail = w.part + round(w.parts > 1 ? 2 * sizeof(float) * w.parts * B * f.Tk * f.Hk * static_cast<size_t>(D) : 0);
   w.bytes = w.tail + round(2 * sizeof(float) * slots * f.Hk * w.sinks * static_cast<size_t>(D));
@@ -916,6 +1013,8 @@ extern "C" int pbattn_window_bwd(const void *q, const void *k, const void *v, in
   p.dk = dk;
   p.dv = dv;
   p.stat = reinterpret_cast<float2 *>(ws + w.stat);
+  p.origin = reinterpret_cast<float *>(ws + w.origin);
+  p.has_large = reinterpret_cast<int *>(ws + w.has_large);
   p.range = reinterpret_cast<uint32_t *>(ws + w.range);
   p.part = reinterpret_cast<float *>(ws + w.part);
   p.tail = reinterpret_cast<float *>(ws + w.tail);

@@ -362,6 +362,52 @@ def test_lowest_scores_and_visible_nan():
     assert bad[70:90].all() and not bad[:70].any() and not bad[90:].any()
 
 
+@pytest.mark.parametrize("power", [6, 11])
+@pytest.mark.parametrize("dtype,d", [(torch.float32, 64), (torch.float32, 256), (torch.bfloat16, 64), (torch.bfloat16, 128),
+                                     (torch.bfloat16, 256), (torch.float16, 128)])
+@pytest.mark.parametrize("length,hq,hk,window,sinks,packed", [
+    (60, 4, 2, None, 0, False), (300, 4, 2, None, 0, False), (300, 6, 2, 130, 40, False), (150, 40, 1, 70, 3, False),
+    (900, 2, 1, None, 0, False), (330, 4, 2, 90, 5, True)])
+def test_gradients_of_large_scores(power, dtype, d, length, hq, hk, window, sinks, packed):
+    """Every other token's scores lie 2^11 or 2^21 off zero, all of one row by the same, which changes nothing
+    but lse: its float32 then says little of a score's distance. Small integers beside that offset keep the
+    scores exact, so the bounds are those of the tensors without it (column 0, the offset's, left out)."""
+    gen = torch.Generator().manual_seed(36)
+    _, _, v, go, _ = make(1, length, length, hq, hk, d, dtype, 36)
+    q, k = (torch.zeros(1, length, h, d) for h in (hq, hk))
+    for x in (q, k):
+        x[..., 1:5] = torch.randint(-2, 3, x[..., 1:5].shape, generator=gen).float()
+    plain = [x.to(dtype).to(DEV) for x in (q, k)]
+    q[:, 1::2, :, 0], k[..., 0] = 2.0 ** power, 2.0 ** power
+    q[:, 1::4] *= torch.tensor([-1.0] + [1.0] * (d - 1))  # below zero, too
+    q, k = (x.to(dtype).to(DEV) for x in (q, k))
+    cu = torch.tensor([0, 100, 107, 320], dtype=torch.int32, device=DEV) if packed else None
+    o, lse = at.window_attention_fwd(q, k, v, 0.5, window, sinks, cu)
+    got = (o, *at.window_attention_bwd(q, k, v, o, lse, go, 0.5, window, sinks, cu))
+    args = [f64(x)[0] for x in (*plain, v)]
+    if packed:
+        ref = oa.packed(*args, 0.5, window, sinks, cu.tolist(), cu.tolist(), f64(go)[0], None, NAMES[dtype])
+    else:
+        ref = oa.attention(*args, 0.5, window, sinks, f64(go)[0], None, NAMES[dtype])
+    for n, x in zip(("o", "dq", "dk", "dv"), got):
+        first = 1 if n in ("dq", "dk") else 0
+        compare(f"large scores {n}", x[0, ..., first:], ref[n][..., first:], ref[n + "_tol"][..., first:])
+
+
+def test_gradients_of_the_lowest_scores():
+    """Equal scores at the type's lowest value: every gradient finite, dv that of a mean."""
+    q, k, v, go, _ = make(1, 50, 50, 1, 1, 64, torch.float32, 13)
+    q[..., 1:] = 0
+    k[..., 1:] = 0
+    q[0, :, 0, 0], k[0, :, 0, 0] = 1e19, -1e19
+    o, lse = at.window_attention_fwd(q, k, v, 1.0)
+    dq, dk, dv = at.window_attention_bwd(q, k, v, o, lse, go, 1.0)
+    weight = torch.tril(torch.ones(50, 50, dtype=torch.float64, device=DEV)) / torch.arange(
+        1, 51, device=DEV, dtype=torch.float64)[:, None]
+    torch.testing.assert_close(dv[0, :, 0].double(), weight.T @ go[0, :, 0].double(), rtol=1e-5, atol=1e-5)
+    assert torch.isfinite(dq).all() and torch.isfinite(dk).all()
+
+
 @pytest.mark.parametrize("d", [64, 128, 256])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("heads,length", [((4, 2), 150), ((32, 8), 1400)])
