@@ -37,6 +37,10 @@ namespace pbgdn {
 // way throughout, and take the origins off there.
 constexpr float LARGE_LSE = 1024.0f;
 
+// float16: dkdv_kernel's weights, at most 1, are held times 2^14, for beside many
+// keys they are small: 1.5 million alike came out 1.6% off in dV as multiples of 2^-24.
+constexpr int F16_WEIGHTS = 14;
+
 constexpr int QR = 32;            // rows of a query tile of dkdv_kernel
 constexpr int DQ_WAVES = 4, DQ_ROWS = 32 * DQ_WAVES;  // waves and rows of a workgroup of dq_kernel
 // Rows (or a token's heads if more) of one part of the sinks' walk, by how many
@@ -53,7 +57,7 @@ struct BwdParams {
   const void *grad_o, *o;
   const float *lse, *grad_lse;
   void *dq, *dk, *dv;
-  float2 *stat;       // [B][Hk][Tq G]: (lse log2(e), delta); +inf for a row that sees nothing
+  float2 *stat;       // [B][Hk][Tq G]: (lse log2(e), for float16 less F16_WEIGHTS; delta); +inf for a row that sees nothing
   float *origin;      // as stat: zero but for rows of large scores
   int *has_large;     // [B][Hk][f.slots]: a tile of dq_kernel has such a row
   uint32_t *range;    // float16: bits of max |do|, |v|, |dlse|
@@ -346,7 +350,8 @@ __global__ __launch_bounds__(NW * 64, WAVES) void dkdv_kernel(const BwdParams p)
   float16_t dk[MB], dv[MB];
 #pragma unroll
   for (int m = 0; m < MB; ++m) dk[m] = dv[m] = zero16();
-  const float range = range_scale<DT, D>(p.range);
+  const float unit = DT == PBGDN_F16 ? ldexpf(1.0f, -F16_WEIGHTS) : 1.0f, scale16 = range_scale<DT, D>(p.range);
+  const float range = scale16 * unit;  // of dS, beside the weights' own
 
   // Staging of the query tiles in turn: `tokens` tokens of `heads` heads, or the
   // heads of a token in `splits` tiles. A lane's offsets into a tile do not change;
@@ -500,25 +505,25 @@ __global__ __launch_bounds__(NW * 64, WAVES) void dkdv_kernel(const BwdParams p)
   for (; i < tiles; ++i) advance(i);
 
   if (key >= sq.nk || (TAIL && key >= p.sinks)) return;
-  const float fk = p.scale / range;
+  const float fk = p.scale / scale16;
   const long row = (static_cast<long>(b) * f.Tk + sq.k0 + key) * f.Hk + hk;
   if constexpr (TAIL) {
     const long at = ((static_cast<long>(slot) * f.Hk + hk) * p.sinks + key) * D;
     const long half = static_cast<long>(p.tail_slots) * f.Hk * p.sinks * D;
     store_row<PBGDN_F32, D>(p.tail + at, dk, h, fk);
-    store_row<PBGDN_F32, D>(p.tail + half + at, dv, h, 1.0f);
+    store_row<PBGDN_F32, D>(p.tail + half + at, dv, h, unit);
   } else if (p.parts > 1) {
     const long half = static_cast<long>(p.B) * f.Tk * f.Hk * D;
     store_row<PBGDN_F32, D>(p.part + part * half + row * D, dk, h, fk);
-    store_row<PBGDN_F32, D>(p.part + (p.parts + part) * half + row * D, dv, h, 1.0f);
+    store_row<PBGDN_F32, D>(p.part + (p.parts + part) * half + row * D, dv, h, unit);
   } else if (key < p.sinks && seq < f.nseq && is_long(f, sq)) {
     const long at = ((static_cast<long>(tail_start(p, seq)) * f.Hk + hk) * p.sinks + key) * D;
     const long half = static_cast<long>(p.tail_slots) * f.Hk * p.sinks * D;
     store_row<PBGDN_F32, D>(p.tail + at, dk, h, fk);
-    store_row<PBGDN_F32, D>(p.tail + half + at, dv, h, 1.0f);
+    store_row<PBGDN_F32, D>(p.tail + half + at, dv, h, unit);
   } else {
     store_row<DT, D>(static_cast<unsigned char *>(p.dk) + row * L::ROW, dk, h, fk);
-    store_row<DT, D>(static_cast<unsigned char *>(p.dv) + row * L::ROW, dv, h, 1.0f);
+    store_row<DT, D>(static_cast<unsigned char *>(p.dv) + row * L::ROW, dv, h, unit);
   }
 }
 
@@ -823,7 +828,7 @@ __global__ __launch_bounds__(NW * 64, WAVES) void dq_kernel(const BwdParams p) {
   }
   if (h == 0 && row < total) {
     const long at = ((static_cast<long>(b) * f.Hk + hk) * f.Tq + sq.q0) * G + r;
-    p.stat[at] = st;
+    p.stat[at] = make_float2(DT == PBGDN_F16 ? st.x - F16_WEIGHTS : st.x, st.y);
     p.origin[at] = origin;
   }
   for (; it < mine; ++it) {

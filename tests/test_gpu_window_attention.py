@@ -288,6 +288,23 @@ def test_float16_gradients_of_any_size(go_scale):
     check("float16 range", *x, 0.125 / (64 if go_scale < 1 else 1), 100, 2)
 
 
+def test_float16_weights_of_many_keys():
+    """1.5 million keys that weigh alike, about 7e-7, which float16 itself holds to 5%."""
+    tq, tk, d = 64, 1_500_000, 64
+    gen = torch.Generator(device=DEV).manual_seed(37)
+    k, v = (torch.randn(1, tk, 1, d, generator=gen, device=DEV).to(torch.float16) for _ in range(2))
+    q = torch.zeros(1, tq, 1, d, dtype=torch.float16, device=DEV)
+    go = (20 + torch.randn(1, tq, 1, d, generator=gen, device=DEV)).to(torch.float16)
+    o, lse = at.window_attention_fwd(q, k, v, 0.125)
+    dv = at.window_attention_bwd(q, k, v, o, lse, go, 0.125)[2][0, :, 0]
+    share = go[0, :, 0].double() / torch.arange(tk - tq + 1, tk + 1, device=DEV, dtype=torch.float64)[:, None]
+    want = share.flip(0).cumsum(0).flip(0)  # of the queries from i on, which the key at tk - tq + i is seen by
+    want = torch.cat([want[:1].expand(tk - tq, d), want])
+    # two roundings (the weight, the result), and lse's own in float32: 16 * 2^-24
+    bound = (2 * 2.0 ** -11 + 1e-5) * want.abs() + 2.0 ** -24
+    assert ((dv.double() - want).abs() <= bound).all()
+
+
 def test_what_no_query_sees_is_never_used():
     """NaN and infinite keys and values left of every window, and past the last boundary."""
     q, k, v, go, glse = make(1, 40, 300, 4, 2, 64, torch.bfloat16, 11)
