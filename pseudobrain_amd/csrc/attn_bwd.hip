@@ -206,8 +206,8 @@ __global__ __launch_bounds__(256) void range_kernel(const BwdParams p) {
 // registers and one wave has a SIMD to itself, so its waits are not covered: 4 x
 // 2,048 tokens, 32 heads of 128 on 8, window 1,024: 270 to 300 us (700 TFLOP/s,
 // the matrix unit busy 38%); 6,011 tokens in 7 sequences, 16 heads of 256 on 2,
-// window 512: 180 us (400 TFLOP/s, 20%). The sinks' walk reads all of Q and dO
-// again for a few keys: 27 us there, 31 us for 4 x 2,048 tokens.
+// window 512: 182 to 190 us (390 TFLOP/s, 20%). The sinks' walk reads all of Q and
+// dO again for a few keys: 26 us there, 28 to 31 us for 4 x 2,048 tokens.
 // ---------------------------------------------------------------------------
 template <int DT, int D, int NW>
 struct Dkdv {
@@ -627,9 +627,9 @@ __global__ __launch_bounds__(256) void join_kernel(const BwdParams p, int sink_b
 // of 128 keys at most, the rows walk once for that sum, and again with the delta
 // corrected by it, which is kept for dkdv_kernel, so this kernel comes first.
 //
-// 4 x 2,048 tokens, 32 heads of 128 on 8, window 1,024: 192 to 211 us (770
+// 4 x 2,048 tokens, 32 heads of 128 on 8, window 1,024: 187 to 211 us (770
 // TFLOP/s, the matrix unit busy 46%); 6,011 tokens in 7 sequences, 16 heads of 256
-// on 2, window 512: 120 us at one wave a SIMD (450 TFLOP/s, 21%). Reading o for
+// on 2, window 512: 122 to 127 us at one wave a SIMD (430 TFLOP/s, 21%). Reading o for
 // delta takes 4 to 15 us of it; a pass of its own over o and grad_o took 18 to 37.
 // ---------------------------------------------------------------------------
 template <int DT, int D, int NW, int BN>
