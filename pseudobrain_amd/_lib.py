@@ -21,7 +21,7 @@ ABI_VERSION = 15
 # The attention operators (include/pbattn.h), a library of their own.
 ATTN_LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libpbattn.so")
 ATTN_DEBUG_LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libpbattn_debug.so")
-ATTN_ABI_VERSION = 1
+ATTN_ABI_VERSION = 2
 
 F32, BF16, F16 = 0, 1, 2
 OK, ERR_INVALID_ARGUMENT, ERR_UNSUPPORTED, ERR_LAUNCH, ERR_SCRATCH = 0, 1, 2, 3, 4
