@@ -20,7 +20,8 @@
  * j <= p and (j > p - window or j < sinks); window <= 0 means no window. With
  * s_ij = scale q_i . k_j over the keys that i sees, p_ij = exp(s_ij - lse_i)
  * and lse_i = log sum_j exp(s_ij), o_i = sum_j p_ij v_j. A query that sees no
- * key gets o = 0 and lse = -infinity, and adds nothing to any gradient.
+ * key gets o = 0 and lse = -infinity, and adds nothing to any gradient; no other
+ * query has that lse (one past float32's range ends at its largest values).
  * Query head h reads key head h / (Hq / Hk).
  *
  * Conventions: those of pbgdn.h (its dtype and status codes; caller-owned

@@ -42,7 +42,7 @@ struct DecodeParams {
   void *o;
   float *lse;
   float *part;     // [slots][Hk][rows][D] unnormalised outputs
-  float2 *stat;    // [slots][Hk][rows] (maximum in powers of two, sum)
+  float2 *stat;    // [slots][Hk][rows] (largest score, sum)
   int B, T, Hq, Hk, group, rows, row_tiles, window, sinks, target;
   float c;
   int negate;
@@ -482,9 +482,6 @@ __global__ __launch_bounds__(DEC_WAVES * 64, (Dec<DT, D>::OCC)) void decode_kern
 
 #pragma unroll
   for (int r = 0; r < RB; ++r) l[r] = add_xor32(add_xor16(l[r]));
-  // from here on maxima in powers of two
-#pragma unroll
-  for (int r = 0; r < RB; ++r) m[r] *= p.c;
   // join the waves into wave 0: the upper half into the lower, or one by one
   constexpr int ROUNDS = JOINS == 2 ? 2 : DEC_WAVES - 1;
 #pragma unroll
@@ -510,7 +507,7 @@ __global__ __launch_bounds__(DEC_WAVES * 64, (Dec<DT, D>::OCC)) void decode_kern
       for (int r = 0; r < RB; ++r) {
         const float m2 = src[RB * DEC_ROWS * D + (r * 16 + c) * 2], l2 = src[RB * DEC_ROWS * D + (r * 16 + c) * 2 + 1];
         const float top = fmaxf(m[r], m2), at = top == -INFINITY ? 0.0f : top;
-        const float f1 = __builtin_amdgcn_exp2f(m[r] - at), f2 = __builtin_amdgcn_exp2f(m2 - at);
+        const float f1 = __builtin_amdgcn_exp2f((m[r] - at) * p.c), f2 = __builtin_amdgcn_exp2f((m2 - at) * p.c);
         m[r] = top;
         l[r] = l[r] * f1 + l2 * f2;
 #pragma unroll
@@ -534,7 +531,7 @@ __global__ __launch_bounds__(DEC_WAVES * 64, (Dec<DT, D>::OCC)) void decode_kern
       if (!last) {
         p.stat[at] = make_float2(m[r], l[r]);
       } else if (p.lse) {
-        p.lse[at] = l[r] > 0.0f ? (m[r] + __builtin_amdgcn_logf(l[r])) * LN2 : l[r] == 0.0f ? -INFINITY : l[r];
+        p.lse[at] = row_lse(m[r], l[r], p.c);
       }
     }
     // element j of the lane's i-th matrix row: column VE (4 g + i) + j of a run of 16 VE
@@ -601,7 +598,7 @@ __global__ __launch_bounds__(256) void decode_join_kernel(const DecodeParams p) 
     }
     const float2 s = lane < n ? p.stat[at0 + lane * step] : make_float2(-INFINITY, 0.0f);
     const float top = fmaxf(m, wave_max(s.x)), base = top == -INFINITY ? 0.0f : top;
-    const float f = __builtin_amdgcn_exp2f(s.x - base), keep = __builtin_amdgcn_exp2f(m - base);
+    const float f = __builtin_amdgcn_exp2f((s.x - base) * p.c), keep = __builtin_amdgcn_exp2f((m - base) * p.c);
     m = top;
     l = l * keep + wave_sum(s.y * f);
 #pragma unroll
@@ -630,7 +627,7 @@ __global__ __launch_bounds__(256) void decode_join_kernel(const DecodeParams p) 
     for (int e = 0; e < VEC; ++e) o[e] = 0.0f;
 #pragma unroll
     for (int i = 0; i < SPLIT; ++i) {
-      const float f = __builtin_amdgcn_exp2f(stat[i][0] - base);
+      const float f = __builtin_amdgcn_exp2f((stat[i][0] - base) * p.c);
       l += stat[i][1] * f;
 #pragma unroll
       for (int e = 0; e < VEC; ++e) o[e] += acc[i][lane * VEC + e] * f;
@@ -640,7 +637,7 @@ __global__ __launch_bounds__(256) void decode_join_kernel(const DecodeParams p) 
   const long at = (static_cast<long>(b) * p.T + row / p.group) * p.Hq + hk * p.group + row % p.group;
 #pragma unroll
   for (int e = 0; e < VEC; ++e) store_elem(p.o, at * D + lane * VEC + e, DT, o[e] * inv);
-  if (p.lse && lane == 0) p.lse[at] = l > 0.0f ? (m + __builtin_amdgcn_logf(l)) * LN2 : l == 0.0f ? -INFINITY : l;
+  if (p.lse && lane == 0) p.lse[at] = row_lse(m, l, p.c);
 }
 
 // ---------------------------------------------------------------------------

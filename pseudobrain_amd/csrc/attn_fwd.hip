@@ -218,8 +218,7 @@ struct WaveRows {
   __device__ __forceinline__ void store(const WindowParams &p) const {
     const float inv = l > 0.0f ? 1.0f / l : l;  // no key seen: zeros (a NaN stays)
     if (out < 0) return;
-    if (p.lse && h == 0)
-      p.lse[out] = l > 0.0f ? (m * p.c + __builtin_amdgcn_logf(l)) * LN2 : l == 0.0f ? -INFINITY : l;
+    if (p.lse && h == 0) p.lse[out] = row_lse(m, l, p.c);
     store_row<DT, D>(static_cast<unsigned char *>(p.o) + out * L::ROW, o, h, inv);
   }
 };

@@ -350,6 +350,15 @@ __device__ __forceinline__ float max_xor32(float x) {
   return fmaxf(a, b);
 }
 
+// The logarithm of a row's softmax sum, l against its largest score m. -infinity is
+// left to rows that see no key: others end at the type's largest values.
+__device__ __forceinline__ float row_lse(float m, float l, float c) {
+  if (!(l > 0.0f)) return l == 0.0f ? -INFINITY : l;
+  const float powers = m * c;
+  const float lse = fabsf(powers) < INFINITY ? (powers + __builtin_amdgcn_logf(l)) * LN2 : m * LN2 * c;
+  return fminf(fmaxf(lse, -__FLT_MAX__), __FLT_MAX__);
+}
+
 // ---------------------------------------------------------------------------
 // Which keys a query sees: position p sees key j when j <= p and
 // (j > p - window or j < sinks). Without branches, and used to select, never to

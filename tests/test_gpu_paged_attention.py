@@ -274,6 +274,27 @@ def test_prefill_then_decode_equals_one_pass():
         torch.testing.assert_close(l1, lse[:, t:t + 1], rtol=0, atol=1e-4)
 
 
+@pytest.mark.parametrize("dtype,d", [(torch.float32, 64), (torch.bfloat16, 128), (torch.bfloat16, 256)])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("scale", [1.0, 4.0])
+@pytest.mark.parametrize("draft,hq", [(1, 2), (3, 16)])
+def test_scores_at_the_ends_of_the_range(dtype, d, sign, scale, draft, hq):
+    """Equal scores of 3.3e38 or its negative, in one part and in parts that are joined: means of the values."""
+    lengths = [40, 9000, 700]
+    q, kc, vc, table, lens = make(lengths, 16, hq, 2, d, draft, dtype, 39)
+    q.zero_(), kc.zero_()
+    q[..., 0], kc[..., 0] = 1.0, sign * 3.3e38
+    o, lse = at.paged_decode_attention(q, kc, vc, table, lens, scale, return_lse=True)
+    want = min(3.3e38 * scale, torch.finfo(torch.float32).max) * sign
+    assert torch.isfinite(lse).all() and (lse.double() - want).abs().max() <= 2 ** -7 * abs(want)
+    for b, n in enumerate(lengths):
+        v = rows(vc, table, b, n)
+        for t in range(draft):
+            mean = v[:n - draft + 1 + t].mean(0).repeat(hq // 2, 0)
+            u = max(oa.UNIT[NAMES[dtype]], n * 2.0 ** -24)
+            assert (np.abs(f64(o[b, t]) - mean) <= 4 * u * np.abs(v).max()).all()
+
+
 def test_compiled_decoding_equals_eager():
     """A decode step under torch.compile: the caches and outputs of the eager calls, no break in the graph."""
     q, kc, vc, table, lengths = make([300, 17, 90], 16, 8, 2, 64, 1, torch.bfloat16, 32)

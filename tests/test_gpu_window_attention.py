@@ -379,6 +379,34 @@ def test_lowest_scores_and_visible_nan():
     assert bad[70:90].all() and not bad[:70].any() and not bad[90:].any()
 
 
+LARGEST = torch.finfo(torch.float32).max
+
+
+@pytest.mark.parametrize("dtype,d", [(torch.float32, 64), (torch.float32, 128), (torch.bfloat16, 64), (torch.bfloat16, 256)])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("scale", [1.0, 4.0])
+@pytest.mark.parametrize("length", [50, 1500])
+def test_scores_at_the_ends_of_the_range(dtype, d, sign, scale, length):
+    """Equal scores of 3.3e38 or its negative, past the range in powers of two, and (scale 4) past it altogether:
+    means of the values, lse at the score or the range's end, gradients as of equal scores."""
+    q, k, v, go, _ = make(1, length, length, 1, 1, d, dtype, 38)
+    q.zero_(), k.zero_()
+    q[..., 0], k[..., 0] = 1.0, sign * 3.3e38
+    o, lse = at.window_attention_fwd(q, k, v, scale)
+    dq, dk, dv = at.window_attention_bwd(q, k, v, o, lse, go, scale)
+    n = torch.arange(1, length + 1, device=DEV, dtype=torch.float64)[:, None]
+    mean = v[0, :, 0].double().cumsum(0) / n
+    u = max(oa.UNIT[NAMES[dtype]], length * 2.0 ** -24)
+    assert ((o[0, :, 0].double() - mean).abs() <= 4 * u * v.double().abs().max()).all()
+    want = min(3.3e38 * scale, LARGEST) * sign
+    assert (lse.double() - want).abs().max() <= 2 ** -7 * abs(want) and torch.isfinite(lse).all()
+    share = (go[0, :, 0].double() / n).flip(0).cumsum(0).flip(0)
+    size = (go[0, :, 0].double().abs() / n).flip(0).cumsum(0).flip(0)
+    assert ((dv[0, :, 0].double() - share).abs() <= 4 * u * size + 1e-6).all()
+    # (column 0 is 0 x 3.3e38 in dq, or its rounding)
+    assert torch.isfinite(dk).all() and torch.count_nonzero(dq[..., 1:]) == 0
+
+
 @pytest.mark.parametrize("power", [6, 11])
 @pytest.mark.parametrize("dtype,d", [(torch.float32, 64), (torch.float32, 256), (torch.bfloat16, 64), (torch.bfloat16, 128),
                                      (torch.bfloat16, 256), (torch.float16, 128)])
