@@ -21,134 +21,9 @@
 // less than the host's 13 to 15.
 #include <type_traits>
 
-#include "attn.hpp"
-#include "attn_tile.hpp"
-#include "device.hpp"
+#include "attn_decode.hpp"
 
 namespace pbgdn {
-
-constexpr int DEC_WAVES = 4;         // waves of a workgroup
-constexpr int DEC_KEYS = 32;         // keys of a block
-constexpr int DEC_MIN = DEC_WAVES;   // fewest blocks of a part: one a wave
-constexpr int DEC_ROWS = 16;         // rows of a matrix tile
-constexpr int JOIN_SPLIT_ROWS = 2048;  // up to here four waves join a row's parts
-
-struct DecodeParams {
-  const unsigned char *q, *k, *v;
-  long token, head;  // strides of the caches, bytes
-  int page_rows;     // a page's stride in token strides
-  int page, num_pages, max_pages;
-  const int32_t *table, *lengths;
-  void *o;
-  float *lse;
-  float *part;     // [slots][Hk][rows][D] unnormalised outputs
-  float2 *stat;    // [slots][Hk][rows] (largest score, sum)
-  int B, T, Hq, Hk, group, rows, row_tiles, window, sinks, target;
-  float c;
-  int negate;
-};
-
-// The keys sequence b's queries see, and its blocks.
-__device__ __forceinline__ int seq_length(const DecodeParams &p, int b) {
-  const int n = p.num_pages > 0 ? p.lengths[b] : 0;
-  return n > 0 ? n : 0;
-}
-__device__ __forceinline__ KeyRange seq_keys(const DecodeParams &p, int len) {
-  return key_range(len - p.T, len - 1, p.window, p.sinks);
-}
-__device__ __forceinline__ int len_blocks(const DecodeParams &p, int len) {
-  return (seq_keys(p, len).count + DEC_KEYS - 1) / DEC_KEYS;
-}
-__device__ __forceinline__ int seq_blocks(const DecodeParams &p, int b) { return len_blocks(p, seq_length(p, b)); }
-
-// The shares: every part takes `per` blocks (the last of a sequence what is
-// left), a sequence at least one part. Every wave works them out for itself: the
-// first 256 sequences' blocks, four a lane, are read once and together.
-__device__ __forceinline__ int wave_sum_int(int x) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off, 64);
-  return x;
-}
-__device__ __forceinline__ long wave_sum_long(long x) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off, 64);
-  return x;
-}
-struct Shares {
-  static constexpr int HELD = 4;
-  int held[HELD];  // blocks of sequences 64 i + lane
-  int per;
-
-  __device__ __forceinline__ Shares(const DecodeParams &p, int lane) {
-    if (p.B == 1) {  // one request: nothing to add up over the lanes
-      held[0] = seq_blocks(p, 0);
-      share(p, held[0]);
-      return;
-    }
-    long total = 0;
-    int len[HELD];  // (read by every lane, so that the four reads are in flight together)
-#pragma unroll
-    for (int i = 0; i < HELD; ++i) len[i] = p.lengths[64 * i + lane < p.B ? 64 * i + lane : p.B - 1];
-#pragma unroll
-    for (int i = 0; i < HELD; ++i) settle(len[i]);
-#pragma unroll
-    for (int i = 0; i < HELD; ++i) {
-      const bool any = (64 * i + lane < p.B) & (p.num_pages > 0) & (len[i] > 0);
-      held[i] = any ? len_blocks(p, len[i]) : 0;
-      total += held[i];
-    }
-    for (int b = 64 * HELD + lane; b < p.B; b += 64) total += seq_blocks(p, b);
-    share(p, wave_sum_long(total));
-  }
-  __device__ __forceinline__ void share(const DecodeParams &p, long total) {
-    const int even = total <= 0x7fffffff - p.target
-                         ? (static_cast<int>(total) + p.target - 1) / p.target
-                         : static_cast<int>((total + p.target - 1) / p.target);
-    const int whole = (even + DEC_MIN - 1) / DEC_MIN * DEC_MIN;
-    per = uniform(whole > DEC_MIN ? whole : DEC_MIN);
-  }
-  __device__ __forceinline__ int parts(int blocks) const { return blocks > per ? (blocks + per - 1) / per : 1; }
-};
-// Whose slot it is: a scan over the sequences, 64 at a time. seq = -1 past the last.
-struct Share {
-  int seq, part, parts, per;
-};
-__device__ __forceinline__ Share share_of_slot(const DecodeParams &p, int slot, int lane) {
-  const Shares all(p, lane);
-  Share s{-1, 0, 0, all.per};
-  if (p.B == 1) {
-    s.parts = all.parts(all.held[0]);
-    s.part = slot;
-    s.seq = slot < s.parts ? 0 : -1;
-    return s;
-  }
-  int base = 0;
-  const auto look = [&](int b0, int blocks) __attribute__((always_inline)) {
-    const int mine = b0 + lane < p.B ? all.parts(blocks) : 0;
-    int scan = mine;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const int x = __shfl_up(scan, off, 64);
-      if (lane >= off) scan += x;
-    }
-    const uint64_t past = __ballot(base + scan > slot);
-    if (past) {
-      const int l = __builtin_ctzll(past);
-      s.seq = b0 + l;
-      s.parts = __shfl(mine, l, 64);
-      s.part = slot - (base + __shfl(scan, l, 64) - s.parts);
-    }
-    base += __shfl(scan, 63, 64);
-    return past != 0;
-  };
-#pragma unroll
-  for (int i = 0; i < Shares::HELD; ++i) {
-    if (64 * i >= p.B || look(64 * i, all.held[i])) return s;
-  }
-  for (int b0 = 64 * Shares::HELD; b0 < p.B; b0 += 64)
-    if (look(b0, b0 + lane < p.B ? seq_blocks(p, b0 + lane) : 0)) break;
-  return s;
-}
 
 template <int DT, int D>
 struct Dec {
@@ -162,10 +37,10 @@ struct Dec {
   static constexpr int OT = D / 16;                 // 16-wide output tiles: VLOADS * VE
   // Rows up to 256 bytes: 32 keys at a time. Wider ones 16, and Q in LDS where a
   // wave has two row blocks of it (its registers hold the sums, 16 keys and their
-  // values): two waves a SIMD up to 512 bytes.
+  // values): two waves a SIMD up to 512 bytes, three up to 128.
   static constexpr int KG = ROW <= 256 ? 2 : 1;     // 16-key groups at a time
   static constexpr bool q_in_lds(int rb) { return ROW > 512 || (ROW == 512 && rb == 2); }
-  static constexpr int OCC = ROW <= 512 ? 2 : 1;
+  static constexpr int OCC = ROW <= 128 ? 3 : ROW <= 512 ? 2 : 1;
 };
 
 // Scores of 16 keys: x += K rows (a lane's units) times Q rows.
@@ -179,16 +54,6 @@ __device__ __forceinline__ float4_t key_mma(v4u32_t k, v4u32_t q, float4_t x) {
   } else {
     return Elem<DT>::mma16(k, q, x);
   }
-}
-
-// max / sum over the four lanes (one of each 16) that hold a row.
-__device__ __forceinline__ float max_rows(float x) {
-  float a = x, b = x;
-  swap16(a, b);
-  a = fmaxf(a, b);
-  b = a;
-  swap32(a, b);
-  return fmaxf(a, b);
 }
 
 template <int DT, int D, int RB>
@@ -480,164 +345,9 @@ __global__ __launch_bounds__(DEC_WAVES * 64, (Dec<DT, D>::OCC)) void decode_kern
   }
   if constexpr (Q_LDS) __syncthreads();  // Q's place is the joins'
 
-#pragma unroll
-  for (int r = 0; r < RB; ++r) l[r] = add_xor32(add_xor16(l[r]));
-  // join the waves into wave 0: the upper half into the lower, or one by one
-  constexpr int ROUNDS = JOINS == 2 ? 2 : DEC_WAVES - 1;
-#pragma unroll
-  for (int round = 0; round < ROUNDS; ++round) {
-    const int from = JOINS == 2 ? DEC_WAVES / 2 >> round : round + 1, count = JOINS == 2 ? from : 1;
-    if (wave >= from && wave < from + count) {
-      float *dst = merge[wave - from];
-#pragma unroll
-      for (int r = 0; r < RB; ++r) {
-#pragma unroll
-        for (int j = 0; j < OT; ++j)
-          *reinterpret_cast<float4_t *>(dst + ((r * OT + j) * 64 + lane) * 4) = o[r][j];
-        if (g == 0) {
-          dst[RB * DEC_ROWS * D + (r * 16 + c) * 2] = m[r];
-          dst[RB * DEC_ROWS * D + (r * 16 + c) * 2 + 1] = l[r];
-        }
-      }
-    }
-    __syncthreads();
-    if (wave < count) {
-      const float *src = merge[wave];
-#pragma unroll
-      for (int r = 0; r < RB; ++r) {
-        const float m2 = src[RB * DEC_ROWS * D + (r * 16 + c) * 2], l2 = src[RB * DEC_ROWS * D + (r * 16 + c) * 2 + 1];
-        const float top = fmaxf(m[r], m2), at = top == -INFINITY ? 0.0f : top;
-        const float f1 = __builtin_amdgcn_exp2f((m[r] - at) * p.c), f2 = __builtin_amdgcn_exp2f((m2 - at) * p.c);
-        m[r] = top;
-        l[r] = l[r] * f1 + l2 * f2;
-#pragma unroll
-        for (int j = 0; j < OT; ++j)
-          o[r][j] = o[r][j] * f1 + *reinterpret_cast<const float4_t *>(src + ((r * OT + j) * 64 + lane) * 4) * f2;
-      }
-    }
-    __syncthreads();
-  }
+  join_waves<RB, D, JOINS>(merge, m, l, o, wave, lane, p.c);
   if (wave != 0) return;
-
-#pragma unroll
-  for (int r = 0; r < RB; ++r) {
-    const int row = row0 + r * DEC_ROWS + c;
-    if (row >= p.rows) continue;
-    const bool last = share.parts == 1;
-    const float f = last && l[r] > 0.0f ? 1.0f / l[r] : 1.0f;
-    const long at = last ? (static_cast<long>(b) * p.T + row / p.group) * p.Hq + hk * p.group + row % p.group
-                         : (static_cast<long>(slot) * p.Hk + hk) * p.rows + row;
-    if (g == 0) {
-      if (!last) {
-        p.stat[at] = make_float2(m[r], l[r]);
-      } else if (p.lse) {
-        p.lse[at] = row_lse(m[r], l[r], p.c);
-      }
-    }
-    // element j of the lane's i-th matrix row: column VE (4 g + i) + j of a run of 16 VE
-#pragma unroll
-    for (int x = 0; x < K::VLOADS; ++x)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int e = 0; e < K::VE; e += 4) {
-          const long d = at * D + x * 16 * K::VE + (4 * g + i) * K::VE + e;
-          const float4_t y = {o[r][x * K::VE + e][i] * f, o[r][x * K::VE + e + 1][i] * f,
-                              o[r][x * K::VE + e + 2][i] * f, o[r][x * K::VE + e + 3][i] * f};
-          if (!last || !K::SHORT) {
-            *reinterpret_cast<float4_t *>((last ? static_cast<float *>(p.o) : p.part) + d) = y;
-          } else if constexpr (K::SHORT) {
-            *reinterpret_cast<v2u32_t *>(static_cast<unsigned char *>(p.o) + 2 * d) =
-                v2u32_t{E::pack(y[0], y[1]), E::pack(y[2], y[3])};
-          }
-        }
-  }
-}
-
-// Joins a sequence's parts, SPLIT waves to a (sequence, query row and head),
-// eight parts of a wave at a time: their outputs and their weights' statistics,
-// one a lane, are fetched together. Four waves a row where there are few rows,
-// one where there are many.
-template <int DT, int D, int SPLIT>
-__global__ __launch_bounds__(256) void decode_join_kernel(const DecodeParams p) {
-  constexpr int VEC = D / 64, ROWS = 4 / SPLIT, AT_ONCE = 8;  // ROWS: rows of a workgroup
-  __shared__ float acc[SPLIT > 1 ? 4 : 1][D], stat[4][2];
-  PBGDN_POISON_LDS(acc, sizeof(acc));
-  PBGDN_POISON_SYNC();
-  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), w = wave % SPLIT;
-  const int tiles = (p.rows + ROWS - 1) / ROWS;
-  int id = blockIdx.x;
-  const int row = id % tiles * ROWS + wave / SPLIT;
-  id /= tiles;
-  const int hk = id % p.Hk, b = id / p.Hk;
-  const Shares all(p, lane);
-  const int parts = uniform(all.parts(seq_blocks(p, b)));
-  if (parts == 1) return;  // written by the first kernel
-  if (SPLIT == 1 && row >= p.rows) return;
-  int first = 0;  // the sequence's first slot
-  if (b > 0) {
-#pragma unroll
-    for (int i = 0; i < Shares::HELD; ++i)
-      if (64 * i + lane < b) first += all.parts(all.held[i]);
-    for (int i = 64 * Shares::HELD + lane; i < b; i += 64) first += all.parts(seq_blocks(p, i));
-    first = uniform(wave_sum_int(first));
-  }
-  float m = -INFINITY, l = 0.0f, o[VEC];
-#pragma unroll
-  for (int e = 0; e < VEC; ++e) o[e] = 0.0f;
-  for (int i0 = w; i0 < parts; i0 += AT_ONCE * SPLIT) {  // this wave's parts: i0, i0 + SPLIT, ...
-    const int count = (parts - i0 + SPLIT - 1) / SPLIT, n = count < AT_ONCE ? count : AT_ONCE;
-    const long at0 = (static_cast<long>(first + i0) * p.Hk + hk) * p.rows + row;
-    const long step = static_cast<long>(SPLIT) * p.Hk * p.rows;
-    float x[AT_ONCE][VEC];
-#pragma unroll
-    for (int i = 0; i < AT_ONCE; ++i) {
-      const float *src = p.part + (at0 + (i < n ? i : 0) * step) * D + lane * VEC;
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) x[i][e] = src[e];
-    }
-    const float2 s = lane < n ? p.stat[at0 + lane * step] : make_float2(-INFINITY, 0.0f);
-    const float top = fmaxf(m, wave_max(s.x)), base = top == -INFINITY ? 0.0f : top;
-    const float f = __builtin_amdgcn_exp2f((s.x - base) * p.c), keep = __builtin_amdgcn_exp2f((m - base) * p.c);
-    m = top;
-    l = l * keep + wave_sum(s.y * f);
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) o[e] *= keep;
-#pragma unroll
-    for (int i = 0; i < AT_ONCE; ++i) {
-      const float fi = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), i));
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) o[e] += i < n ? x[i][e] * fi : 0.0f;
-    }
-  }
-  if constexpr (SPLIT > 1) {
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) acc[wave][lane * VEC + e] = o[e];
-    if (lane == 0) {
-      stat[wave][0] = m;
-      stat[wave][1] = l;
-    }
-    __syncthreads();
-    if (wave != 0) return;
-#pragma unroll
-    for (int i = 1; i < SPLIT; ++i) m = fmaxf(m, stat[i][0]);
-    const float base = m == -INFINITY ? 0.0f : m;
-    l = 0.0f;
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) o[e] = 0.0f;
-#pragma unroll
-    for (int i = 0; i < SPLIT; ++i) {
-      const float f = __builtin_amdgcn_exp2f((stat[i][0] - base) * p.c);
-      l += stat[i][1] * f;
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) o[e] += acc[i][lane * VEC + e] * f;
-    }
-  }
-  const float inv = l > 0.0f ? 1.0f / l : l;
-  const long at = (static_cast<long>(b) * p.T + row / p.group) * p.Hq + hk * p.group + row % p.group;
-#pragma unroll
-  for (int e = 0; e < VEC; ++e) store_elem(p.o, at * D + lane * VEC + e, DT, o[e] * inv);
-  if (p.lse && lane == 0) p.lse[at] = row_lse(m, l, p.c);
+  store_decoded<DT, D, RB, K::VE>(p, share, b, hk, row0, slot, lane, m, l, o);
 }
 
 // ---------------------------------------------------------------------------
@@ -673,23 +383,14 @@ __global__ __launch_bounds__(256) void paged_write_kernel(const WriteParams p) {
 
 template <int DT, int D>
 static int launch_decode(DecodeParams &p, hipStream_t stream) {
-  const long slots = static_cast<long>(p.target) + p.B;
   const auto run = [&](auto kernel, int rb) {
-    p.row_tiles = (p.rows + rb * DEC_ROWS - 1) / (rb * DEC_ROWS);
-    const long blocks = slots * p.Hk * p.row_tiles;
-    if (blocks > 0x7fffffffL || static_cast<long>(p.B) * p.Hk * p.rows > 0x7fffffffL) return false;
-    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(DEC_WAVES * 64), 0, stream, p);
-    return true;
+    const unsigned blocks = decode_blocks(p, rb);
+    if (blocks) hipLaunchKernelGGL(kernel, dim3(blocks), dim3(DEC_WAVES * 64), 0, stream, p);
+    return blocks != 0;
   };
   const bool ok = p.rows <= DEC_ROWS ? run(decode_kernel<DT, D, 1>, 1) : run(decode_kernel<DT, D, 2>, 2);
   if (!ok) return PBGDN_ERR_UNSUPPORTED;
-  const long rows = static_cast<long>(p.B) * p.Hk * p.rows;
-  if (rows <= JOIN_SPLIT_ROWS) {
-    hipLaunchKernelGGL((decode_join_kernel<DT, D, 4>), dim3(static_cast<unsigned>(rows)), dim3(256), 0, stream, p);
-  } else {
-    const unsigned blocks = static_cast<unsigned>(p.B * p.Hk * ((p.rows + 3) / 4));
-    hipLaunchKernelGGL((decode_join_kernel<DT, D, 1>), dim3(blocks), dim3(256), 0, stream, p);
-  }
+  launch_join<DT, D>(p, stream);
   return hipGetLastError() == hipSuccess ? PBGDN_OK : PBGDN_ERR_LAUNCH;
 }
 
@@ -714,9 +415,6 @@ static int decode_target(int Hk, int rows, int row_bytes) {
   const int tiles = (rows + 2 * DEC_ROWS - 1) / (2 * DEC_ROWS);
   const int t = (row_bytes <= 256 ? 8 : 4) * shape.cus / (Hk * tiles);
   return t > 1 ? t : 1;
-}
-static bool decode_sizes_ok(int B, int T, int Hq, int Hk, int D) {
-  return B >= 0 && T >= 1 && T <= PBATTN_MAX_DRAFT && Hq > 0 && Hk > 0 && Hq % Hk == 0 && D > 0;
 }
 
 // The cache's strides in bytes; false when they cannot be.
@@ -775,30 +473,12 @@ extern "C" int pbattn_paged_decode(const void *q, const void *k_cache, const voi
   p.lengths = lengths;
   p.o = o;
   p.lse = lse;
-  p.B = B;
-  p.T = T;
-  p.Hq = Hq;
-  p.Hk = Hk;
-  p.group = Hq / Hk;
-  p.rows = p.group * T;
-  p.window = window <= 0 || window > NO_WINDOW ? NO_WINDOW : window;
-  p.sinks = sinks < NO_WINDOW ? sinks : NO_WINDOW;
-  // (no more parts than the table's pages, or the window, can need)
-  long most = static_cast<long>(max_pages) * page_size;
-  if (most > static_cast<long>(p.window) + T + p.sinks) most = static_cast<long>(p.window) + T + p.sinks;
-  most = (most + DEC_MIN * DEC_KEYS - 1) / (DEC_MIN * DEC_KEYS) * B;
-  const int wanted = decode_target(Hk, p.rows, D * attn_bytes(dtype));
-  p.target = most < wanted ? static_cast<int>(most > 1 ? most : 1) : wanted;
-  const float c = __builtin_fabsf(scale) * LOG2E;
-  p.c = c > 1.17549435e-38f ? c : 1.17549435e-38f;
-  p.negate = scale < 0.0f;
-  const size_t rows = (static_cast<size_t>(p.target) + B) * Hk * p.rows;
-  p.part = static_cast<float *>(workspace);
-  p.stat = reinterpret_cast<float2 *>(p.part + rows * D);
+  decode_call(p, B, T, Hq, Hk, scale, window, sinks, decode_target(Hk, Hq / Hk * T, D * attn_bytes(dtype)));
+  const size_t used = decode_workspace(p, workspace, D);
   hipStream_t s = static_cast<hipStream_t>(stream);
   debug_poison(o, static_cast<size_t>(B) * T * Hq * D * attn_bytes(dtype), s);
   if (lse) debug_poison(lse, static_cast<size_t>(B) * T * Hq * sizeof(float), s);
-  debug_poison(workspace, rows * (D * sizeof(float) + sizeof(float2)), s);
+  debug_poison(workspace, used, s);
   switch (dtype) {
     case PBGDN_F32: return dispatch_decode<PBGDN_F32>(p, D, s);
     case PBGDN_BF16: return dispatch_decode<PBGDN_BF16>(p, D, s);
