@@ -10,6 +10,9 @@
  *                          sequence over a paged key-value cache, split over
  *                          the cache's length and joined
  *   pbattn_paged_write     new keys and values into the cache's pages
+ *   pbattn_fp4_decode, pbattn_fp4_write, pbattn_fp4_read
+ *                          the cache held in 4 bits: decoding over it, its writes,
+ *                          its contexts read back
  *
  * The reference computes this half of WindowedHybridLayer.mix
  * (pseudobrain/transplant.py:989-997) with PyTorch's attention in training and
@@ -53,7 +56,7 @@ extern "C" {
 #endif
 
 /* Raised with every function that is added or changed. */
-#define PBATTN_ABI_VERSION 2
+#define PBATTN_ABI_VERSION 3
 
 /* Most query tokens a sequence may have in pbattn_paged_decode. */
 #define PBATTN_MAX_DRAFT 16
@@ -172,6 +175,68 @@ size_t pbattn_paged_decode_workspace_size(int B, int T, int Hq, int Hk, int D);
 int pbattn_paged_write(const void *k, const void *v, int dtype, const int64_t *kv_strides, void *k_cache,
                        void *v_cache, const int64_t *strides, int page_size, int num_pages, const int64_t *slots,
                        int N, int Hk, int D, void *stream);
+
+/* Most sequences of a call that works packed sequences out from their lengths
+ * (pbattn_fp4_read, pbattn_pages_extend, pbattn_pages_release). */
+#define PBATTN_MAX_REQUESTS 4096
+
+/*
+ * The cache held in 4 bits. 32 consecutive values of a head share a scale s, a
+ * power of two; each is held as the nearest of +-{0, 0.5, 1, 1.5, 2, 3, 4, 6} s
+ * (ties to the even code; codes 0 to 7, 8 more for a negative value). s is
+ * 2^(e - 2), where 2^e <= x < 2^(e + 1) for the largest |x| of the 32, and twice
+ * that where x >= 1.75 2^e, held as the byte e - 2 + 127 kept within [2, 252]
+ * (smaller values round to zero or 2^-126, larger ones are cut to 6 2^125). A byte
+ * of 255 marks 32 values among which one is infinite or NaN: all of them read as
+ * NaN. Byte i of a row of codes holds value 2 i in its lower half and 2 i + 1 in the
+ * upper one.
+ *
+ *   k_cache, v_cache   codes: pages of page_size tokens, rows of D / 2 bytes; token
+ *                      i of page g at byte g strides[0] + i strides[1], key head h
+ *                      strides[2] further on. Strides are multiples of D / 2,
+ *                      strides[0] of strides[1] too
+ *   k_scale, v_scale   their scales, laid out alike: rows of D / 32 bytes, every
+ *                      stride a sixteenth of the codes'
+ *   D                  64, 128 or 256; bases aligned to 16 bytes
+ */
+
+/*
+ * pbattn_paged_decode over such a cache: the same arguments besides, and the same
+ * results for the values that the cache stands for. q in any of the three types;
+ * scores and outputs of float16 and float32 rows are as exact as over a cache of
+ * their own type (their products are taken in two and three parts).
+ */
+int pbattn_fp4_decode(const void *q, int dtype, const void *k_cache, const void *v_cache, const void *k_scale,
+                      const void *v_scale, const int64_t *strides, int page_size, int num_pages,
+                      const int32_t *page_table, int max_pages, const int32_t *lengths, void *o, float *lse, int B,
+                      int T, int Hq, int Hk, int D, float scale, int window, int sinks, void *workspace,
+                      size_t workspace_bytes, void *stream);
+
+/* Bytes of workspace pbattn_fp4_decode needs; 0 for invalid sizes. */
+size_t pbattn_fp4_decode_workspace_size(int B, int T, int Hq, int Hk, int D);
+
+/* pbattn_paged_write into such a cache: k, v of `dtype` by kv_strides are rounded as
+ * said above. */
+int pbattn_fp4_write(const void *k, const void *v, int dtype, const int64_t *kv_strides, void *k_cache, void *v_cache,
+                     void *k_scale, void *v_scale, const int64_t *strides, int page_size, int num_pages,
+                     const int64_t *slots, int N, int Hk, int D, void *stream);
+
+/*
+ * Reads B sequences back, packed in their order: the first lengths[b] keys and
+ * values of each, as pbattn_window_fwd takes them for a prompt's next queries.
+ *
+ *   page_table, lengths   as in pbattn_paged_decode (a length below 0 counts as 0)
+ *   k, v         [tokens, Hk, D] dense, dtype (exact in bfloat16 and float32; float16
+ *                ends at its own range), written: zeros for the keys of absent pages
+ *                and for tokens past the last sequence
+ *   cu_seqlens   [B + 1] int32, written: where each sequence starts and ends, cut at
+ *                `tokens`
+ *   B            at most PBATTN_MAX_REQUESTS
+ */
+int pbattn_fp4_read(const void *k_cache, const void *v_cache, const void *k_scale, const void *v_scale,
+                    const int64_t *strides, int page_size, int num_pages, const int32_t *page_table, int max_pages,
+                    const int32_t *lengths, void *k, void *v, int dtype, int32_t *cu_seqlens, int B, int tokens, int Hk,
+                    int D, void *stream);
 
 #ifdef __cplusplus
 }

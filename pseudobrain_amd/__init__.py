@@ -5,6 +5,9 @@ attention that a hybrid layer runs beside it in pseudobrain_amd.attention."""
 from .attention import (  # noqa: F401
     paged_cache_write, paged_decode_attention, window_attention, window_attention_bwd, window_attention_fwd,
 )
+from .fp4 import (  # noqa: F401
+    Fp4Cache, fp4_cache, paged_cache_read_fp4, paged_cache_write_fp4, paged_decode_attention_fp4,
+)
 from .gated_deltanet import (  # noqa: F401
     CHUNK, KERNELS, SEQUENTIAL_MAX, chunk_bwd, chunk_decumulate, chunk_fwd, chunk_fwd_slots, chunk_residuals,
     chunk_slots_, delta_rule_hip, delta_rule_sequential, gated_delta_chunk, gated_delta_chunk_backward,

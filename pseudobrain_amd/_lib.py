@@ -21,7 +21,7 @@ ABI_VERSION = 15
 # The attention operators (include/pbattn.h), a library of their own.
 ATTN_LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libpbattn.so")
 ATTN_DEBUG_LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libpbattn_debug.so")
-ATTN_ABI_VERSION = 2
+ATTN_ABI_VERSION = 3
 
 F32, BF16, F16 = 0, 1, 2
 OK, ERR_INVALID_ARGUMENT, ERR_UNSUPPORTED, ERR_LAUNCH, ERR_SCRATCH = 0, 1, 2, 3, 4
@@ -80,6 +80,11 @@ ATTN_SIGNATURES = {
                              _vp, _sz, _vp], _i),
     "pbattn_paged_decode_workspace_size": ([_i, _i, _i, _i, _i], _sz),
     "pbattn_paged_write": ([_vp, _vp, _i, _vp, _vp, _vp, _vp, _i, _i, _vp, _i, _i, _i, _vp], _i),
+    "pbattn_fp4_decode": ([_vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _i, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _f, _i,
+                           _i, _vp, _sz, _vp], _i),
+    "pbattn_fp4_decode_workspace_size": ([_i, _i, _i, _i, _i], _sz),
+    "pbattn_fp4_write": ([_vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _vp, _i, _i, _i, _vp], _i),
+    "pbattn_fp4_read": ([_vp, _vp, _vp, _vp, _vp, _i, _i, _vp, _i, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _i, _vp], _i),
 }
 
 _lock = threading.Lock()
