@@ -13,6 +13,9 @@
  *   pbattn_fp4_decode, pbattn_fp4_write, pbattn_fp4_read
  *                          the cache held in 4 bits: decoding over it, its writes,
  *                          its contexts read back
+ *   pbattn_pages_extend, pbattn_pages_release
+ *                          the pages, slots and positions of new tokens from the
+ *                          requests' lengths; pages given back
  *
  * The reference computes this half of WindowedHybridLayer.mix
  * (pseudobrain/transplant.py:989-997) with PyTorch's attention in training and
@@ -237,6 +240,48 @@ int pbattn_fp4_read(const void *k_cache, const void *v_cache, const void *k_scal
                     const int64_t *strides, int page_size, int num_pages, const int32_t *page_table, int max_pages,
                     const int32_t *lengths, void *k, void *v, int dtype, int32_t *cu_seqlens, int B, int tokens, int Hk,
                     int D, void *stream);
+
+/*
+ * The pages of a paged cache from its requests' lengths, on the device: a pool of free
+ * pages, kept as a stack, from which requests take pages as they grow and to which they
+ * give them back. Page i of a request holds its tokens i page_size .. (i + 1) page_size
+ * - 1, entry i of its row of page_table (rows table_row entries apart) says which it is.
+ *
+ *   free_pages   [capacity] int32, the pool's pages from its bottom up
+ *   num_free     [1] int32, how many of them there are (kept within [0, capacity])
+ *   B            at most PBATTN_MAX_REQUESTS; max_pages page_size at most 2^31 - 1
+ *
+ * pbattn_pages_extend: request b, of lengths[b] tokens, gets counts[b] more (none where
+ * it is not positive). Requests are gone through in order; one is granted if
+ *   its tokens, and those asked for by all requests before it, are at most `tokens`,
+ *   they and its lengths[b] (not negative) fit max_pages pages, and
+ *   it needs no new page, or the pages that requests up to it need (those of requests
+ *   that fail the first two left out) are no more than the pool's.
+ * The others get nothing. New pages come off the top of the stack, in the requests'
+ * order, and are entered in page_table; the granted tokens are packed in that order:
+ *   slots        [tokens] int64, written: page_table entry times page_size plus the
+ *                place there, as pbattn_paged_write takes it (-1 where the entry is
+ *                negative), and -1 past the last token
+ *   positions    [tokens] int32, written: the token's place in its request, -1 past the last
+ *   cu_seqlens   [B + 1] int32, written: where each request's new tokens start and end
+ *   new_lengths  [B] int32, written: lengths with what was granted
+ *   new_num_free [1] int32, written
+ * pbattn_pages_release: the pages of request b whose last token lies in [first[b],
+ * end[b]) are pushed, in the requests' order (capacity ends it); page_table stays as it
+ * is. Ranges of one request that follow each other so give every page back once: the
+ * tokens that a window has left, or, up to a multiple of page_size, all of a finished
+ * request's.
+ *
+ * Neither changes lengths, counts, num_free: the same call again gives the same results.
+ * The outputs must not overlap the inputs.
+ */
+int pbattn_pages_extend(int32_t *page_table, int64_t table_row, int max_pages, const int32_t *lengths,
+                        const int32_t *counts, int B, int page_size, const int32_t *free_pages, int capacity,
+                        const int32_t *num_free, int tokens, int64_t *slots, int32_t *positions, int32_t *cu_seqlens,
+                        int32_t *new_lengths, int32_t *new_num_free, void *stream);
+int pbattn_pages_release(const int32_t *page_table, int64_t table_row, int max_pages, const int32_t *first,
+                         const int32_t *end, int B, int page_size, int32_t *free_pages, int capacity,
+                         const int32_t *num_free, int32_t *new_num_free, void *stream);
 
 #ifdef __cplusplus
 }

@@ -1,7 +1,8 @@
 """MI355X-native Gated DeltaNet operator (prefill, its backward, decode) behind the
 reference's operator API; see pseudobrain_amd.gated_deltanet. The layer-side
 prologue and epilogue around it are in pseudobrain_amd.layer, the windowed
-attention that a hybrid layer runs beside it in pseudobrain_amd.attention."""
+attention that a hybrid layer runs beside it in pseudobrain_amd.attention, its cache
+held in 4 bits in pseudobrain_amd.fp4, the cache's pages in pseudobrain_amd.pages."""
 from .attention import (  # noqa: F401
     paged_cache_write, paged_decode_attention, window_attention, window_attention_bwd, window_attention_fwd,
 )
@@ -15,3 +16,4 @@ from .gated_deltanet import (  # noqa: F401
     recurrent_step_, register_reference_ops, select_kernel,
 )
 from .layer import decode_layer_step, layer_epilogue, layer_prologue, layer_prologue_varlen  # noqa: F401,E402
+from .pages import paged_cache_extend, paged_cache_release  # noqa: F401,E402

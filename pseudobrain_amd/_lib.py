@@ -85,6 +85,8 @@ ATTN_SIGNATURES = {
     "pbattn_fp4_decode_workspace_size": ([_i, _i, _i, _i, _i], _sz),
     "pbattn_fp4_write": ([_vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _vp, _i, _i, _i, _vp], _i),
     "pbattn_fp4_read": ([_vp, _vp, _vp, _vp, _vp, _i, _i, _vp, _i, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _i, _vp], _i),
+    "pbattn_pages_extend": ([_vp, ctypes.c_int64, _i, _vp, _vp, _i, _i, _vp, _i, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp], _i),
+    "pbattn_pages_release": ([_vp, ctypes.c_int64, _i, _vp, _vp, _i, _i, _vp, _i, _vp, _vp, _vp], _i),
 }
 
 _lock = threading.Lock()

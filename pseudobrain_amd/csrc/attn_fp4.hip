@@ -4,7 +4,7 @@
 
 #include "attn_decode.hpp"
 #include "attn_fp4.hpp"
-#include "attn_pages.hpp"
+#include "pages.hpp"
 
 namespace pbgdn {
 
