@@ -16,6 +16,9 @@
  *   pbattn_pages_extend, pbattn_pages_release
  *                          the pages, slots and positions of new tokens from the
  *                          requests' lengths; pages given back
+ *   pbattn_qk_norm_rope, pbattn_qk_norm_rope_bwd
+ *                          what queries and keys go through before they are attended:
+ *                          norms of each head and the rotation by position
  *
  * The reference computes this half of WindowedHybridLayer.mix
  * (pseudobrain/transplant.py:989-997) with PyTorch's attention in training and
@@ -282,6 +285,55 @@ int pbattn_pages_extend(int32_t *page_table, int64_t table_row, int max_pages, c
 int pbattn_pages_release(const int32_t *page_table, int64_t table_row, int max_pages, const int32_t *first,
                          const int32_t *end, int B, int page_size, int32_t *free_pages, int capacity,
                          const int32_t *num_free, int32_t *new_num_free, void *stream);
+
+/*
+ * Norms of queries and keys for each head, and the rotation by their positions, in one
+ * pass: for a row x of D values, with r = (mean x^2 + eps)^(-1/2) and the weight w,
+ *   y_i = x_i r (w_i + weight_offset),
+ *   (y_a, y_b) -> (y_a cos - y_b sin, y_b cos + y_a sin)   for the R / 2 pairs (a, b)
+ * of the first R values: i and R / 2 + i, or with `interleaved` 2 i and 2 i + 1; the
+ * others stay. float32 throughout, rounded once.
+ *
+ *   q, k         [B, T, Hq, D] and [B, T, Hk, D] dtype by `strides` (batch, token, head of
+ *                q, then of k: 6 values, elements, not negative), the innermost axis
+ *                dense. Where strides and bases are multiples of 16 bytes and D and R of
+ *                16 (float32: of 8) rows are moved in whole units; any others work too,
+ *                slower
+ *   q_weight, k_weight   [D] of weight_dtype
+ *   cos, sin     [rows, R / 2] float32: the angles of position i in row i
+ *   positions    int32, or int64 with positions64, by pos_strides (batch, token;
+ *                elements, 0 to repeat): rows of the tables. A token whose position lies
+ *                outside them (-1 for padding) gets zeros
+ *   q_out, k_out dense, dtype, written; 16-byte aligned
+ *   D            up to 256; R even, 0 (norms alone) to D
+ */
+int pbattn_qk_norm_rope(const void *q, const void *k, int dtype, const int64_t *strides, const void *q_weight,
+                        const void *k_weight, int weight_dtype, float weight_offset, const float *cos, const float *sin,
+                        int rows, const void *positions, int positions64, const int64_t *pos_strides, void *q_out,
+                        void *k_out, int B, int T, int Hq, int Hk, int D, int R, float eps, int interleaved, void *stream);
+
+/*
+ * Its gradients: with g the gradient of an output row turned back by its angles and
+ * u = g (w + weight_offset),
+ *   dx = r (u - x r^2 mean(u x)),  dw = sum over tokens and heads of g x r
+ *   grad_q, grad_k        dense, dtype, 16-byte aligned
+ *   dq, dk                dense, dtype, written (zeros for tokens without a position,
+ *                         which add nothing to dw)
+ *   dq_weight, dk_weight  [D] weight_dtype, written, 16-byte aligned
+ *   workspace             at least pbattn_qk_norm_rope_bwd_workspace_size bytes, 16-byte
+ *                         aligned; needs no initialisation
+ * Sums are taken in a fixed order. A call without tokens writes nothing, the weights'
+ * gradients neither.
+ */
+int pbattn_qk_norm_rope_bwd(const void *q, const void *k, int dtype, const int64_t *strides, const void *q_weight,
+                            const void *k_weight, int weight_dtype, float weight_offset, const float *cos,
+                            const float *sin, int rows, const void *positions, int positions64, const int64_t *pos_strides,
+                            const void *grad_q, const void *grad_k, void *dq, void *dk, void *dq_weight, void *dk_weight,
+                            int B, int T, int Hq, int Hk, int D, int R, float eps, int interleaved, void *workspace,
+                            size_t workspace_bytes, void *stream);
+
+/* Bytes of workspace pbattn_qk_norm_rope_bwd needs on the current device; 0 for an invalid width. */
+size_t pbattn_qk_norm_rope_bwd_workspace_size(int D);
 
 #ifdef __cplusplus
 }

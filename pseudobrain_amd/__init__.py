@@ -2,7 +2,8 @@
 reference's operator API; see pseudobrain_amd.gated_deltanet. The layer-side
 prologue and epilogue around it are in pseudobrain_amd.layer, the windowed
 attention that a hybrid layer runs beside it in pseudobrain_amd.attention, its cache
-held in 4 bits in pseudobrain_amd.fp4, the cache's pages in pseudobrain_amd.pages."""
+held in 4 bits in pseudobrain_amd.fp4, the cache's pages in pseudobrain_amd.pages, the
+norms and rotation of its queries and keys in pseudobrain_amd.rope."""
 from .attention import (  # noqa: F401
     paged_cache_write, paged_decode_attention, window_attention, window_attention_bwd, window_attention_fwd,
 )
@@ -17,3 +18,4 @@ from .gated_deltanet import (  # noqa: F401
 )
 from .layer import decode_layer_step, layer_epilogue, layer_prologue, layer_prologue_varlen  # noqa: F401,E402
 from .pages import paged_cache_extend, paged_cache_release  # noqa: F401,E402
+from .rope import qk_norm_rope, rope_tables  # noqa: F401,E402

@@ -87,6 +87,11 @@ ATTN_SIGNATURES = {
     "pbattn_fp4_read": ([_vp, _vp, _vp, _vp, _vp, _i, _i, _vp, _i, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _i, _vp], _i),
     "pbattn_pages_extend": ([_vp, ctypes.c_int64, _i, _vp, _vp, _i, _i, _vp, _i, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp], _i),
     "pbattn_pages_release": ([_vp, ctypes.c_int64, _i, _vp, _vp, _i, _i, _vp, _i, _vp, _vp, _vp], _i),
+    "pbattn_qk_norm_rope": ([_vp, _vp, _i, _vp, _vp, _vp, _i, _f, _vp, _vp, _i, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i,
+                             _i, _f, _i, _vp], _i),
+    "pbattn_qk_norm_rope_bwd": ([_vp, _vp, _i, _vp, _vp, _vp, _i, _f, _vp, _vp, _i, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp,
+                                 _vp, _i, _i, _i, _i, _i, _i, _f, _i, _vp, _sz, _vp], _i),
+    "pbattn_qk_norm_rope_bwd_workspace_size": ([_i], _sz),
 }
 
 _lock = threading.Lock()

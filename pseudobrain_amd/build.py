@@ -30,7 +30,8 @@ SOURCES = ("abi.hip", "recurrent.hip", "chunk.hip", "chunk_prep.hip", "chunk_sca
            "layer.hip", "decode_layer.hip", "device.hip")
 ATTN_LIB = os.path.join(PKG, "libpbattn.so")
 ATTN_DEBUG_LIB = os.path.join(PKG, "libpbattn_debug.so")
-ATTN_SOURCES = ("attn_fwd.hip", "attn_bwd.hip", "attn_decode.hip", "attn_fp4.hip", "pages.hip", "device.hip")
+ATTN_SOURCES = ("attn_fwd.hip", "attn_bwd.hip", "attn_decode.hip", "attn_fp4.hip", "pages.hip", "rope.hip",
+                "device.hip")
 ARCH = "gfx950"
 
 # Packed fp32 VALU instructions are disabled (-packed-fp32-ops): the kernels
