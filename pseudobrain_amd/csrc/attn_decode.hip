@@ -25,6 +25,8 @@
 
 namespace pbgdn {
 
+constexpr int JOIN_SPLIT_ROWS = 2048;  // up to here four waves join a row's parts
+
 template <int DT, int D>
 struct Dec {
   using E = Elem<DT>;
@@ -347,7 +349,7 @@ __global__ __launch_bounds__(DEC_WAVES * 64, (Dec<DT, D>::OCC)) void decode_kern
 
   join_waves<RB, D, JOINS>(merge, m, l, o, wave, lane, p.c);
   if (wave != 0) return;
-  store_decoded<DT, D, RB, K::VE>(p, share, b, hk, row0, slot, lane, m, l, o);
+  store_decoded<DT, D, RB, K::VE>(p, share.parts == 1, b, hk, row0, slot, lane, m, l, o);
 }
 
 // ---------------------------------------------------------------------------
@@ -390,7 +392,7 @@ static int launch_decode(DecodeParams &p, hipStream_t stream) {
   };
   const bool ok = p.rows <= DEC_ROWS ? run(decode_kernel<DT, D, 1>, 1) : run(decode_kernel<DT, D, 2>, 2);
   if (!ok) return PBGDN_ERR_UNSUPPORTED;
-  launch_join<DT, D>(p, stream);
+  launch_join<DT, D, Shares>(p, static_cast<long>(p.B) * p.Hk * p.rows <= JOIN_SPLIT_ROWS, 4, stream);
   return hipGetLastError() == hipSuccess ? PBGDN_OK : PBGDN_ERR_LAUNCH;
 }
 

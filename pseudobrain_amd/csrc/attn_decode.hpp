@@ -14,7 +14,6 @@ constexpr int DEC_WAVES = 4;         // waves of a workgroup
 constexpr int DEC_KEYS = 32;         // keys of a block
 constexpr int DEC_MIN = DEC_WAVES;   // fewest blocks of a part: one a wave
 constexpr int DEC_ROWS = 16;         // rows of a matrix tile
-constexpr int JOIN_SPLIT_ROWS = 2048;  // up to here four waves join a row's parts
 
 struct DecodeParams {
   const unsigned char *q, *k, *v;
@@ -27,6 +26,7 @@ struct DecodeParams {
   float *part;     // [slots][Hk][rows][D] unnormalised outputs
   float2 *stat;    // [slots][Hk][rows] (largest score, sum)
   int B, T, Hq, Hk, group, rows, row_tiles, window, sinks, target;
+  int join_rows;   // query rows that a workgroup joins
   float c;
   int negate;
 };
@@ -91,6 +91,20 @@ struct Shares {
     per = uniform(whole > DEC_MIN ? whole : DEC_MIN);
   }
   __device__ __forceinline__ int parts(int blocks) const { return blocks > per ? (blocks + per - 1) / per : 1; }
+
+  // Sequence b's parts, and its first slot.
+  __device__ __forceinline__ int parts_of(const DecodeParams &p, int b, int) const { return uniform(parts(seq_blocks(p, b))); }
+  __device__ __forceinline__ int first_of(const DecodeParams &p, int b, int lane) const {
+    int first = 0;
+    if (b > 0) {
+#pragma unroll
+      for (int i = 0; i < HELD; ++i)
+        if (64 * i + lane < b) first += parts(held[i]);
+      for (int i = 64 * HELD + lane; i < b; i += 64) first += parts(seq_blocks(p, i));
+      first = uniform(wave_sum_int(first));
+    }
+    return first;
+  }
 };
 // Whose slot it is: a scan over the sequences, 64 at a time. seq = -1 past the last.
 struct Share {
@@ -188,12 +202,12 @@ __device__ __forceinline__ void join_waves(float (&merge)[JOINS][RB * DEC_ROWS *
   }
 }
 
-// Wave 0's rows: to the part's place, or, where the sequence has one part, divided
-// by their sums to o and lse. Tile x VE + e of o holds columns VE (4 g + i) + e of
+// Wave 0's rows: to the part's place, or, where it is the sequence's only one (last),
+// divided by their sums to o and lse. Tile x VE + e of o holds columns VE (4 g + i) + e of
 // the x-th run of 16 VE.
 template <int DT, int D, int RB, int VE>
-__device__ __forceinline__ void store_decoded(const DecodeParams &p, const Share &share, int b, int hk, int row0, int slot,
-                                              int lane, const float (&m)[RB], const float (&l)[RB],
+__device__ __forceinline__ void store_decoded(const DecodeParams &p, bool last, int b, int hk, int row0, int slot, int lane,
+                                               const float (&m)[RB], const float (&l)[RB],
                                               const float4_t (&o)[RB][D / 16]) {
   using E = Elem<DT>;
   constexpr bool SHORT = E::BYTES == 2;
@@ -203,7 +217,6 @@ __device__ __forceinline__ void store_decoded(const DecodeParams &p, const Share
   for (int r = 0; r < RB; ++r) {
     const int row = row0 + r * DEC_ROWS + c;
     if (row >= p.rows) continue;
-    const bool last = share.parts == 1;
     const float f = last && l[r] > 0.0f ? 1.0f / l[r] : 1.0f;
     const long at = last ? (static_cast<long>(b) * p.T + row / p.group) * p.Hq + hk * p.group + row % p.group
                          : (static_cast<long>(slot) * p.Hk + hk) * p.rows + row;
@@ -237,99 +250,93 @@ __device__ __forceinline__ void store_decoded(const DecodeParams &p, const Share
 // Joins a sequence's parts, SPLIT waves to a (sequence, query row and head),
 // eight parts of a wave at a time: their outputs and their weights' statistics,
 // one a lane, are fetched together. Four waves a row where there are few rows,
-// one where there are many.
-template <int DT, int D, int SPLIT>
+// one where there are many. Division says which parts they are.
+template <int DT, int D, int SPLIT, typename Division>
 static __global__ __launch_bounds__(256) void decode_join_kernel(const DecodeParams p) {
   constexpr int VEC = D / 64, ROWS = 4 / SPLIT, AT_ONCE = 8;  // ROWS: rows of a workgroup
   __shared__ float acc[SPLIT > 1 ? 4 : 1][D], stat[4][2];
   PBGDN_POISON_LDS(acc, sizeof(acc));
   PBGDN_POISON_SYNC();
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), w = wave % SPLIT;
-  const int tiles = (p.rows + ROWS - 1) / ROWS;
+  const int tiles = (p.rows + p.join_rows - 1) / p.join_rows;
   int id = blockIdx.x;
-  const int row = id % tiles * ROWS + wave / SPLIT;
+  const int row0 = id % tiles * p.join_rows, row1 = row0 + p.join_rows < p.rows ? row0 + p.join_rows : p.rows;
   id /= tiles;
   const int hk = id % p.Hk, b = id / p.Hk;
-  const Shares all(p, lane);
-  const int parts = uniform(all.parts(seq_blocks(p, b)));
+  const Division all(p, lane);
+  const int parts = all.parts_of(p, b, lane);
   if (parts == 1) return;  // written by the first kernel
-  if (SPLIT == 1 && row >= p.rows) return;
-  int first = 0;  // the sequence's first slot
-  if (b > 0) {
-#pragma unroll
-    for (int i = 0; i < Shares::HELD; ++i)
-      if (64 * i + lane < b) first += all.parts(all.held[i]);
-    for (int i = 64 * Shares::HELD + lane; i < b; i += 64) first += all.parts(seq_blocks(p, i));
-    first = uniform(wave_sum_int(first));
-  }
-  float m = -INFINITY, l = 0.0f, o[VEC];
-#pragma unroll
-  for (int e = 0; e < VEC; ++e) o[e] = 0.0f;
-  for (int i0 = w; i0 < parts; i0 += AT_ONCE * SPLIT) {  // this wave's parts: i0, i0 + SPLIT, ...
-    const int count = (parts - i0 + SPLIT - 1) / SPLIT, n = count < AT_ONCE ? count : AT_ONCE;
-    const long at0 = (static_cast<long>(first + i0) * p.Hk + hk) * p.rows + row;
-    const long step = static_cast<long>(SPLIT) * p.Hk * p.rows;
-    float x[AT_ONCE][VEC];
-#pragma unroll
-    for (int i = 0; i < AT_ONCE; ++i) {
-      const float *src = p.part + (at0 + (i < n ? i : 0) * step) * D + lane * VEC;
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) x[i][e] = src[e];
-    }
-    const float2 s = lane < n ? p.stat[at0 + lane * step] : make_float2(-INFINITY, 0.0f);
-    const float top = fmaxf(m, wave_max(s.x)), base = top == -INFINITY ? 0.0f : top;
-    const float f = __builtin_amdgcn_exp2f((s.x - base) * p.c), keep = __builtin_amdgcn_exp2f((m - base) * p.c);
-    m = top;
-    l = l * keep + wave_sum(s.y * f);
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) o[e] *= keep;
-#pragma unroll
-    for (int i = 0; i < AT_ONCE; ++i) {
-      const float fi = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), i));
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) o[e] += i < n ? x[i][e] * fi : 0.0f;
-    }
-  }
-  if constexpr (SPLIT > 1) {
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) acc[wave][lane * VEC + e] = o[e];
-    if (lane == 0) {
-      stat[wave][0] = m;
-      stat[wave][1] = l;
-    }
-    __syncthreads();
-    if (wave != 0) return;
-#pragma unroll
-    for (int i = 1; i < SPLIT; ++i) m = fmaxf(m, stat[i][0]);
-    const float base = m == -INFINITY ? 0.0f : m;
-    l = 0.0f;
+  const int first = all.first_of(p, b, lane);
+  for (int row = row0 + wave / SPLIT; row < row1; row += ROWS) {
+    float m = -INFINITY, l = 0.0f, o[VEC];
 #pragma unroll
     for (int e = 0; e < VEC; ++e) o[e] = 0.0f;
+    for (int i0 = w; i0 < parts; i0 += AT_ONCE * SPLIT) {  // this wave's parts: i0, i0 + SPLIT, ...
+      const int count = (parts - i0 + SPLIT - 1) / SPLIT, n = count < AT_ONCE ? count : AT_ONCE;
+      const long at0 = (static_cast<long>(first + i0) * p.Hk + hk) * p.rows + row;
+      const long step = static_cast<long>(SPLIT) * p.Hk * p.rows;
+      float x[AT_ONCE][VEC];
 #pragma unroll
-    for (int i = 0; i < SPLIT; ++i) {
-      const float f = __builtin_amdgcn_exp2f((stat[i][0] - base) * p.c);
-      l += stat[i][1] * f;
+      for (int i = 0; i < AT_ONCE; ++i) {
+        const float *src = p.part + (at0 + (i < n ? i : 0) * step) * D + lane * VEC;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) o[e] += acc[i][lane * VEC + e] * f;
+        for (int e = 0; e < VEC; ++e) x[i][e] = src[e];
+      }
+      const float2 s = lane < n ? p.stat[at0 + lane * step] : make_float2(-INFINITY, 0.0f);
+      const float top = fmaxf(m, wave_max(s.x)), base = top == -INFINITY ? 0.0f : top;
+      const float f = __builtin_amdgcn_exp2f((s.x - base) * p.c), keep = __builtin_amdgcn_exp2f((m - base) * p.c);
+      m = top;
+      l = l * keep + wave_sum(s.y * f);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) o[e] *= keep;
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; ++i) {
+        const float fi = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), i));
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) o[e] += i < n ? x[i][e] * fi : 0.0f;
+      }
     }
-  }
-  const float inv = l > 0.0f ? 1.0f / l : l;
-  const long at = (static_cast<long>(b) * p.T + row / p.group) * p.Hq + hk * p.group + row % p.group;
+    if constexpr (SPLIT > 1) {
 #pragma unroll
-  for (int e = 0; e < VEC; ++e) store_elem(p.o, at * D + lane * VEC + e, DT, o[e] * inv);
-  if (p.lse && lane == 0) p.lse[at] = row_lse(m, l, p.c);
+      for (int e = 0; e < VEC; ++e) acc[wave][lane * VEC + e] = o[e];
+      if (lane == 0) {
+        stat[wave][0] = m;
+        stat[wave][1] = l;
+      }
+      __syncthreads();
+      if (wave != 0) continue;  // (one row a workgroup: join_rows is 1)
+#pragma unroll
+      for (int i = 1; i < SPLIT; ++i) m = fmaxf(m, stat[i][0]);
+      const float base = m == -INFINITY ? 0.0f : m;
+      l = 0.0f;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) o[e] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < SPLIT; ++i) {
+        const float f = __builtin_amdgcn_exp2f((stat[i][0] - base) * p.c);
+        l += stat[i][1] * f;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) o[e] += acc[i][lane * VEC + e] * f;
+      }
+    }
+    const float inv = l > 0.0f ? 1.0f / l : l;
+    const long at = (static_cast<long>(b) * p.T + row / p.group) * p.Hq + hk * p.group + row % p.group;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) store_elem(p.o, at * D + lane * VEC + e, DT, o[e] * inv);
+    if (p.lse && lane == 0) p.lse[at] = row_lse(m, l, p.c);
+  }
 }
 
-// Launches the join of parts (decode_join_kernel) for a call whose parts have been.
-template <int DT, int D>
-static void launch_join(const DecodeParams &p, hipStream_t stream) {
-  const long rows = static_cast<long>(p.B) * p.Hk * p.rows;
-  if (rows <= JOIN_SPLIT_ROWS) {
-    hipLaunchKernelGGL((decode_join_kernel<DT, D, 4>), dim3(static_cast<unsigned>(rows)), dim3(256), 0, stream, p);
-  } else {
-    const unsigned blocks = static_cast<unsigned>(p.B * p.Hk * ((p.rows + 3) / 4));
-    hipLaunchKernelGGL((decode_join_kernel<DT, D, 1>), dim3(blocks), dim3(256), 0, stream, p);
-  }
+// Launches the join of parts (decode_join_kernel) for a call whose parts have been: four
+// waves a row (`split`), or one, of which a workgroup takes `rows` one after the other.
+template <int DT, int D, typename Division>
+static void launch_join(DecodeParams &p, bool split, int rows, hipStream_t stream) {
+  p.join_rows = split ? 1 : rows;
+  const unsigned blocks = static_cast<unsigned>(p.B * p.Hk * ((p.rows + p.join_rows - 1) / p.join_rows));
+  if (split)
+    hipLaunchKernelGGL((decode_join_kernel<DT, D, 4, Division>), dim3(blocks), dim3(256), 0, stream, p);
+  else
+    hipLaunchKernelGGL((decode_join_kernel<DT, D, 1, Division>), dim3(blocks), dim3(256), 0, stream, p);
 }
 
 // The grid of a call's parts for kernels of rb row tiles a workgroup; 0 where it
@@ -345,7 +352,8 @@ inline bool decode_sizes_ok(int B, int T, int Hq, int Hk, int D) {
 }
 
 // What a decoding call's arguments make of the parameters besides the caches' addresses
-// and strides: `wanted` parts over all sequences, no more than the table's pages, or the window, can need.
+// and strides: `wanted` parts over all sequences, no more than the table's pages, or the
+// window, can need.
 inline void decode_call(DecodeParams &p, int B, int T, int Hq, int Hk, float scale, int window, int sinks, int wanted) {
   p.B = B;
   p.T = T;

@@ -1,5 +1,12 @@
 // The cache held in 4 bits (attn_fp4.hpp): decoding over it (pbattn_fp4_decode),
 // its writes (pbattn_fp4_write) and its reading back (pbattn_fp4_read).
+//
+// Decoding reads 17 bytes for 32 values instead of 64, so what a bfloat16 cache's kernel
+// does beside its loads would cost as much as they do. Codes become bfloat16 operands by
+// one conversion for two values, scale included; a value row's codes are fetched as they
+// lie and transposed by byte permutations after it. Distances of rows and scales are
+// worked out once, a lane for each key, and go through LDS to the lanes that need them.
+// A block's loads go out a whole block ahead, and page table entries one before that.
 #include <type_traits>
 
 #include "attn_decode.hpp"
@@ -9,8 +16,108 @@
 namespace pbgdn {
 
 struct Fp4DecodeParams {
-  DecodeParams d;                       // k, v, token, head: the codes'
-  const unsigned char *k_scale, *v_scale;  // their strides: a sixteenth of the codes'
+  DecodeParams d;                          // k, v, head: the codes'
+  const unsigned char *k_scale, *v_scale;  // laid out as the codes are, a sixteenth of every stride
+  uint32_t page_step, token_step;          // a page's and a token's stride of the codes in 16 bytes, of the scales in bytes
+  uint32_t page_mul;                       // j / page = (2 j page_mul) >> 32 >> page_shift for 0 <= j < 2^31
+  int page_shift;
+};
+
+// How the work is divided: the keys of all sequences, in order, are one line of quads
+// (four blocks of keys, one for each wave of a workgroup; a sequence that sees no key has
+// one too), of which workgroup w of a (row tile, key head) takes `per` from w per on,
+// whatever sequences they belong to. Its piece of sequence b is part w + b: the pairs
+// (w, b) that meet follow each other, and w + b rises from each to the next. So as many
+// workgroups as fit the GPU at once share the work evenly, and each starts once.
+__device__ __forceinline__ long uniform_long(long x) {
+  return static_cast<long>(static_cast<uint64_t>(static_cast<uint32_t>(uniform(static_cast<int>(x >> 32)))) << 32 |
+                           static_cast<uint32_t>(uniform(static_cast<int>(x))));
+}
+struct Walk {
+  static constexpr int HELD = 4;
+  int held[HELD];  // quads of sequences 64 i + lane
+  long per, total;
+
+  __device__ __forceinline__ static int quads_of(const DecodeParams &p, int len) {
+    const int n = (len_blocks(p, len) + DEC_WAVES - 1) / DEC_WAVES;
+    return n > 1 ? n : 1;
+  }
+  __device__ __forceinline__ static int quads(const DecodeParams &p, int b) { return quads_of(p, seq_length(p, b)); }
+
+  __device__ __forceinline__ Walk(const DecodeParams &p, int lane) {
+    if (p.B == 1) {  // one request: nothing to add up over the lanes
+      held[0] = quads(p, 0);
+      total = held[0];
+    } else {
+      total = 0;
+      int len[HELD];  // (read by every lane, so that the four reads are in flight together)
+#pragma unroll
+      for (int i = 0; i < HELD; ++i) len[i] = p.lengths[64 * i + lane < p.B ? 64 * i + lane : p.B - 1];
+#pragma unroll
+      for (int i = 0; i < HELD; ++i) settle(len[i]);
+#pragma unroll
+      for (int i = 0; i < HELD; ++i) {
+        held[i] = 64 * i + lane < p.B ? quads_of(p, ((p.num_pages > 0) & (len[i] > 0)) ? len[i] : 0) : 0;
+        total += held[i];
+      }
+      for (int b = 64 * HELD + lane; b < p.B; b += 64) total += quads(p, b);
+      total = wave_sum_long(total);
+    }
+    total = uniform_long(total);
+    const long target = p.target;
+    per = uniform_long(total <= 0x7fffffff - target ? (static_cast<int>(total) + p.target - 1) / p.target
+                                                    : (total + target - 1) / target);
+  }
+  // Whose quad x < total is, and where that sequence starts.
+  __device__ __forceinline__ int find(const DecodeParams &p, long x, int lane, long &start) const {
+    start = 0;
+    if (p.B == 1) return 0;
+    int found = 0;
+    const auto look = [&](int b0, int mine) __attribute__((always_inline)) {
+      int scan = mine;
+#pragma unroll
+      for (int off = 1; off < 64; off <<= 1) {
+        const int y = __shfl_up(scan, off, 64);
+        if (lane >= off) scan += y;
+      }
+      const uint64_t past = __ballot(start + scan > x);
+      if (past) {
+        const int l = __builtin_ctzll(past);
+        found = b0 + l;
+        start += __shfl(scan, l, 64) - __shfl(mine, l, 64);
+        return true;
+      }
+      start += __shfl(scan, 63, 64);
+      return false;
+    };
+#pragma unroll
+    for (int i = 0; i < HELD; ++i)
+      if (64 * i >= p.B || look(64 * i, held[i])) return found;
+    for (int b0 = 64 * HELD; b0 < p.B; b0 += 64)
+      if (look(b0, b0 + lane < p.B ? quads(p, b0 + lane) : 0)) break;
+    return found;
+  }
+  // Sequence b's first quad.
+  __device__ __forceinline__ long start_of(const DecodeParams &p, int b, int lane) const {
+    if (b == 0) return 0;
+    long x = 0;
+#pragma unroll
+    for (int i = 0; i < HELD; ++i)
+      if (64 * i + lane < b) x += held[i];
+    for (int i = 64 * HELD + lane; i < b; i += 64) x += quads(p, i);
+    return wave_sum_long(x);
+  }
+  __device__ __forceinline__ int workgroup_of(long x) const {
+    return x <= 0x7fffffff ? static_cast<int>(x) / static_cast<int>(per) : static_cast<int>(x / per);
+  }
+  // Sequence b's parts, and its first slot.
+  __device__ __forceinline__ int parts_of(const DecodeParams &p, int b, int lane) const {
+    const long first = start_of(p, b, lane);
+    return uniform(workgroup_of(first + quads(p, b) - 1) - workgroup_of(first) + 1);
+  }
+  __device__ __forceinline__ int first_of(const DecodeParams &p, int b, int lane) const {
+    return uniform(workgroup_of(start_of(p, b, lane))) + b;
+  }
 };
 
 // Q and the weights enter bfloat16 products as one, two or three parts that sum up to
@@ -38,388 +145,6 @@ __device__ __forceinline__ void split_pair(float x, float y, uint32_t *out) {
   }
 }
 
-template <int DT, int D>
-struct Fp4 {
-  static constexpr int N = Parts<DT>::N;
-  static constexpr int ROW = D / 2;           // bytes of a key's codes
-  static constexpr int SROW = D / FP4_BLOCK;  // and of its scales
-  static constexpr int KSTEPS = D / 32;       // matrix steps of a score
-  static constexpr int KW = ROW / 16;         // words a lane reads of a key: one a step
-  static constexpr int KSCALES = D == 256 ? 2 : 1;  // and of its scales
-  static constexpr int OT = D / 16;           // output tiles: values a lane reads of a value row
-  static constexpr int VW = D == 64 ? 1 : OT / 8;   // words that hold them
-  static constexpr int KG = 2, KEYS = 16 * KG;      // keys at a time
-  // Q in LDS where its parts would take more than 64 registers.
-  static constexpr bool q_in_lds(int rb) { return KSTEPS * N * rb > 16; }
-  // First of the eight columns that lane group g takes in matrix step s.
-  __device__ static constexpr int column(int g, int s) {
-    return D == 64 ? 16 * g + 8 * s : 128 * (s / 4) + 32 * g + 8 * (s % 4);
-  }
-};
-
-template <int DT, int D, int RB>
-__global__ __launch_bounds__(DEC_WAVES * 64, 2) void fp4_decode_kernel(const Fp4DecodeParams pp) {
-  using K = Fp4<DT, D>;
-  using E = Elem<PBGDN_BF16>;
-  constexpr int KS = K::KSTEPS, OT = K::OT, KG = K::KG, KEYS = K::KEYS, N = K::N;
-  constexpr bool Q_LDS = K::q_in_lds(RB);
-  constexpr int JOINS = RB * D <= 256 ? 2 : 1;
-  constexpr int Q_UNITS = Q_LDS ? RB * N * KS * 64 : 1;  // 16-byte units: [row tile][part][step][lane]
-  typedef float Merge[JOINS][RB * DEC_ROWS * (D + 2)];
-  __shared__ union {  // Q's place is the joins' afterwards
-    Merge merge;
-    v4u32_t q[Q_UNITS];
-  } lds;
-  PBGDN_POISON_LDS(&lds, sizeof(lds));
-  PBGDN_POISON_SYNC();
-  v4u32_t *const q_lds = lds.q;
-  const DecodeParams &p = pp.d;
-
-  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
-  const int c = lane & 15, g = lane >> 4;
-  const int slots = p.target + p.B, id = uniform(blockIdx.x / slots), slot = blockIdx.x - id * slots;
-  const int row0 = uniform(id / p.Hk) * (RB * DEC_ROWS), hk = uniform(id % p.Hk);
-  const Share share = share_of_slot(p, slot, lane);
-  if (share.seq < 0) return;
-  const int b = uniform(share.seq), len = uniform(seq_length(p, b));
-  const KeyRange range = seq_keys(p, len);
-  // this wave's KEYS-wide blocks of the part: begin + wave, then every DEC_WAVES-th
-  const int blocks = (range.count + KEYS - 1) / KEYS;
-  const int begin = uniform(share.part * share.per * (DEC_KEYS / KEYS));
-  const int end_ = begin + share.per * (DEC_KEYS / KEYS);
-  const int end = uniform(end_ < blocks ? end_ : blocks);
-
-  // this lane's rows of Q (column c of every row tile), in parts; in LDS, each wave brings in a share
-  v4u32_t qf[Q_LDS ? 1 : RB][Q_LDS ? 1 : N][Q_LDS ? 1 : KS];
-  int pos[RB];
-  constexpr int QB = DT == PBGDN_F32 ? 4 : 2;  // bytes of an element of Q
-#pragma unroll
-  for (int r = 0; r < RB; ++r) {
-    const int row = row0 + r * DEC_ROWS + c;
-    const int rr = row < p.rows ? row : p.rows - 1;
-    const int t = rr / p.group;
-    pos[r] = len - p.T + t;
-    const unsigned char *src = p.q + ((static_cast<long>(b) * p.T + t) * p.Hq + hk * p.group + rr - t * p.group) * (D * QB);
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      if (Q_LDS && s % DEC_WAVES != wave) continue;
-      v4u32_t part[N];
-      if constexpr (DT == PBGDN_BF16) {
-        part[0] = *reinterpret_cast<const v4u32_t *>(src + K::column(g, s) * 2);
-        if (p.negate) part[0] ^= 0x80008000u;
-      } else {
-        float x[8];
-        if constexpr (DT == PBGDN_F16) {
-          const half8_t h = *reinterpret_cast<const half8_t *>(src + K::column(g, s) * 2);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] = static_cast<float>(h[e]);
-        } else {
-          const float4_t lo = *reinterpret_cast<const float4_t *>(src + K::column(g, s) * 4),
-                         hi = *reinterpret_cast<const float4_t *>(src + K::column(g, s) * 4 + 16);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            x[e] = lo[e];
-            x[4 + e] = hi[e];
-          }
-        }
-#pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-          uint32_t w[N];
-          split_pair<N>(p.negate ? -x[e] : x[e], p.negate ? -x[e + 1] : x[e + 1], w);
-#pragma unroll
-          for (int i = 0; i < N; ++i) part[i][e / 2] = w[i];
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        if constexpr (Q_LDS)
-          q_lds[((r * N + i) * KS + s) * 64 + lane] = part[i];
-        else
-          qf[r][i][s] = part[i];
-      }
-    }
-  }
-  if constexpr (Q_LDS) __syncthreads();
-  float m[RB], l[RB];
-  float4_t o[RB][OT];
-#pragma unroll
-  for (int r = 0; r < RB; ++r) {
-    m[r] = -INFINITY;
-    l[r] = 0.0f;
-#pragma unroll
-    for (int j = 0; j < OT; ++j) o[r][j] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
-  }
-
-  const unsigned char *kbase = p.k + hk * p.head, *vbase = p.v + hk * p.head;
-  const unsigned char *ksbase = pp.k_scale + hk * (p.head / 16), *vsbase = pp.v_scale + hk * (p.head / 16);
-  const int32_t *table = p.table + static_cast<long>(b) * p.max_pages;
-  // Key `lane` (modulo KEYS) of a block: its page, and its place there (-1: there is none); then its row in the cache.
-  const auto lookup = [&](int blk, int &page, int &place) __attribute__((always_inline)) {
-    const uint32_t u = static_cast<uint32_t>(blk) * KEYS + lane % KEYS, last = range.count - 1;  // (past a range's end too)
-    const int v = static_cast<int>(u < last ? u : last), j = v < range.sinks ? v : v + range.delta;
-    const int pg = j / p.page;
-    page = table[pg < p.max_pages ? pg : p.max_pages - 1];
-    place = ((u <= last) & (pg < p.max_pages)) ? j - pg * p.page : -1;
-  };
-  const auto cache_row = [&](int page, int place) __attribute__((always_inline)) {
-    return ((place >= 0) & (page >= 0) & (page < p.num_pages)) ? page * p.page_rows + place : -1;
-  };
-  // A key's row as lane (c, g) takes it: unit g of key 16 kb + c; its scales.
-  uint32_t kf[KG][K::KW], ks[KG][K::KSCALES];
-  // Values: lane (c, .) takes columns OT c .. of the keys that its weights belong to.
-  uint32_t vf[4 * KG][K::VW], vs[4 * KG];
-  const auto load_keys = [&](int rows) __attribute__((always_inline)) {
-    const int safe = rows >= 0 ? rows : 0;
-#pragma unroll
-    for (int kb = 0; kb < KG; ++kb) {
-      const long row = __shfl(safe, 16 * kb + c, 64);
-      const unsigned char *src = kbase + row * p.token, *ss = ksbase + row * (p.token / 16);
-      if constexpr (D == 64) {
-        const v2u32_t w = __builtin_nontemporal_load(reinterpret_cast<const v2u32_t *>(src + g * 8));
-        kf[kb][0] = w[0];
-        kf[kb][1] = w[1];
-        ks[kb][0] = ss[g / 2];
-      } else {
-#pragma unroll
-        for (int h = 0; h < D / 128; ++h) {
-          const v4u32_t w = __builtin_nontemporal_load(reinterpret_cast<const v4u32_t *>(src + h * 64 + g * 16));
-#pragma unroll
-          for (int e = 0; e < 4; ++e) kf[kb][4 * h + e] = w[e];
-          ks[kb][h] = ss[4 * h + g];
-        }
-      }
-    }
-  };
-  const auto load_values = [&](int rows) __attribute__((always_inline)) {
-    const int safe = rows >= 0 ? rows : 0;
-#pragma unroll
-    for (int i = 0; i < 4 * KG; ++i) {
-      const long row = __shfl(safe, i / 4 * 16 + 4 * g + i % 4, 64);
-      const unsigned char *src = vbase + row * p.token + c * (OT / 2);
-      if constexpr (D == 64) {
-        vf[i][0] = __builtin_nontemporal_load(reinterpret_cast<const uint16_t *>(src));
-      } else if constexpr (D == 128) {
-        vf[i][0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t *>(src));
-      } else {
-        const v2u32_t w = __builtin_nontemporal_load(reinterpret_cast<const v2u32_t *>(src));
-        vf[i][0] = w[0];
-        vf[i][1] = w[1];
-      }
-      vs[i] = vsbase[row * (p.token / 16) + c * OT / FP4_BLOCK];
-    }
-  };
-  // A block's keys are fetched while the one before is weighed, its values while the
-  // scores are formed; the pages of the block after are asked for before those values.
-  int valid = -1, page = -1, place = -1;
-  if (begin + wave < end) {
-    lookup(begin + wave, page, place);
-    valid = cache_row(page, place);
-    lookup(begin + wave + DEC_WAVES, page, place);
-    load_keys(valid);
-    load_values(valid);
-  }
-  const auto step = [&](int blk, auto last) __attribute__((always_inline)) {
-    constexpr bool more = !decltype(last)::value;
-    const bool all = __ballot(valid >= 0) == ~0ull;
-    float4_t sc[RB][KG];
-#pragma unroll
-    for (int r = 0; r < RB; ++r)
-#pragma unroll
-      for (int kb = 0; kb < KG; ++kb) sc[r][kb] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      v4u32_t a[KG];
-#pragma unroll
-      for (int kb = 0; kb < KG; ++kb) a[kb] = fp4_unpack8(kf[kb][s], fp4_scale(ks[kb][D == 256 ? s / 4 : 0]));
-#pragma unroll
-      for (int i = 0; i < N; ++i)
-#pragma unroll
-        for (int r = 0; r < RB; ++r) {
-          v4u32_t q;
-          if constexpr (Q_LDS)
-            q = q_lds[((r * N + i) * KS + s) * 64 + lane];
-          else
-            q = qf[r][i][s];
-#pragma unroll
-          for (int kb = 0; kb < KG; ++kb) sc[r][kb] = E::mma16(a[kb], q, sc[r][kb]);
-        }
-    }
-    const int next = more ? cache_row(page, place) : -1;
-    if constexpr (more) load_keys(next);
-    if (!all) {  // values of absent keys: zeros, whatever the row they were read from holds
-#pragma unroll
-      for (int i = 0; i < 4 * KG; ++i) {
-        const bool in = __shfl(valid, i / 4 * 16 + 4 * g + i % 4, 64) >= 0;
-#pragma unroll
-        for (int x = 0; x < K::VW; ++x) vf[i][x] = in ? vf[i][x] : 0u;
-        vs[i] = in ? vs[i] : 127u;
-      }
-    }
-    const int u0 = blk * KEYS;
-    const int j0 = u0 < range.sinks ? u0 : u0 + range.delta, j1 = u0 + KEYS - 1 + range.delta;
-    const bool whole = all && u0 >= range.sinks && j1 <= len - p.T && j0 > len - 1 - p.window;
-#pragma unroll
-    for (int r = 0; r < RB; ++r) {
-      float4_t (&s)[KG] = sc[r];
-      if (!whole) {
-#pragma unroll
-        for (int i = 0; i < 4 * KG; ++i) {
-          const int key = i / 4 * 16 + 4 * g + i % 4, u = u0 + key;
-          const int j = u < range.sinks ? u : u + range.delta;
-          const bool seen = (__shfl(valid, key, 64) >= 0) & sees(pos[r], j, p.window, p.sinks);
-          s[i / 4][i % 4] = seen ? s[i / 4][i % 4] : -INFINITY;
-        }
-      }
-      float mx = s[0][0];
-#pragma unroll
-      for (int i = 1; i < 4 * KG; ++i) mx = fmaxf(mx, s[i / 4][i % 4]);
-      mx = max_rows(mx);
-      if (__any((mx - m[r]) * p.c > LAG)) {
-        const float top = fmaxf(m[r], mx);
-        const float alpha = __builtin_amdgcn_exp2f((m[r] - (top == -INFINITY ? 0.0f : top)) * p.c);
-        m[r] = top;
-        l[r] *= alpha;
-#pragma unroll
-        for (int j = 0; j < OT; ++j) o[r][j] *= alpha;
-      }
-      const float base = m[r] == -INFINITY ? 0.0f : m[r], at = base * p.c;
-      const bool far = __any(fabsf(at) > EXACT_SCORES);
-      float sum = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 4 * KG; ++i) {
-        const float x = s[i / 4][i % 4];
-        s[i / 4][i % 4] = __builtin_amdgcn_exp2f(far ? (x - base) * p.c : __builtin_fmaf(x, p.c, -at));
-        sum += s[i / 4][i % 4];
-      }
-      l[r] += sum;
-    }
-    // O^T += V^T P; element e of the lane's values makes output tile e
-    v4u32_t w[RB][KG / 2][N];
-#pragma unroll
-    for (int r = 0; r < RB; ++r)
-#pragma unroll
-      for (int h = 0; h < KG / 2; ++h)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float x = sc[r][2 * h + i / 2][2 * (i % 2)], y = sc[r][2 * h + i / 2][2 * (i % 2) + 1];
-          if constexpr (N == 1) {
-            w[r][h][0][i] = E::pack(x, y);
-          } else {
-            uint32_t part[N];
-            split_pair<N>(x, y, part);
-#pragma unroll
-            for (int n = 0; n < N; ++n) w[r][h][n][i] = part[n];
-          }
-        }
-    const auto pair_of_tiles = [&](auto E0) __attribute__((always_inline)) {  // tiles 2 e and 2 e + 1
-      constexpr int e = decltype(E0)::value;
-#pragma unroll
-      for (int h = 0; h < KG / 2; ++h) {
-        uint32_t x[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = fp4_pair<e % 4>(vf[8 * h + i][e / 4], fp4_scale(vs[8 * h + i]));
-        v4u32_t lo, hi;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          lo[i] = __builtin_amdgcn_perm(x[2 * i + 1], x[2 * i], 0x05040100u);
-          hi[i] = __builtin_amdgcn_perm(x[2 * i + 1], x[2 * i], 0x07060302u);
-        }
-#pragma unroll
-        for (int n = 0; n < N; ++n)
-#pragma unroll
-          for (int r = 0; r < RB; ++r) {
-            o[r][2 * e] = E::mma16(lo, w[r][h][n], o[r][2 * e]);
-            o[r][2 * e + 1] = E::mma16(hi, w[r][h][n], o[r][2 * e + 1]);
-          }
-      }
-    };
-    pair_of_tiles(std::integral_constant<int, 0>{});
-    pair_of_tiles(std::integral_constant<int, 1>{});
-    if constexpr (OT >= 8) {
-      pair_of_tiles(std::integral_constant<int, 2>{});
-      pair_of_tiles(std::integral_constant<int, 3>{});
-    }
-    if constexpr (OT >= 16) {
-      pair_of_tiles(std::integral_constant<int, 4>{});
-      pair_of_tiles(std::integral_constant<int, 5>{});
-      pair_of_tiles(std::integral_constant<int, 6>{});
-      pair_of_tiles(std::integral_constant<int, 7>{});
-    }
-    if constexpr (more) {
-      lookup(blk + 2 * DEC_WAVES, page, place);
-      load_values(next);
-      valid = next;
-    }
-  };
-  int blk = begin + wave;
-  for (; blk + DEC_WAVES < end; blk += DEC_WAVES) step(blk, std::false_type{});
-  if (blk < end) step(blk, std::true_type{});
-  // A value that some tokens see and others do not enters all rows' products, with
-  // weight zero where it is not seen: harmless unless its scale is that of NaN (or
-  // infinite). Outputs that end so are worked out again, key by key, from what their
-  // token sees alone.
-  if (p.T > 1) {
-#pragma unroll
-    for (int r = 0; r < RB; ++r) {
-      float nought = 0.0f;
-#pragma unroll
-      for (int j = 0; j < OT; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) nought = __builtin_fmaf(o[r][j][i], 0.0f, nought);  // zero, or NaN
-      if (!__any(nought != 0.0f)) continue;
-#pragma unroll
-      for (int j = 0; j < OT; ++j) o[r][j] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
-      const int row = row0 + r * DEC_ROWS + c, rr = row < p.rows ? row : p.rows - 1, t = rr / p.group;
-      const unsigned char *qrow = p.q + ((static_cast<long>(b) * p.T + t) * p.Hq + hk * p.group + rr - t * p.group) * (D * QB);
-      const float base = m[r] == -INFINITY ? 0.0f : m[r], sign = p.negate ? -1.0f : 1.0f;
-      const auto value = [&](const unsigned char *codes, const unsigned char *scales, int d) __attribute__((always_inline)) {
-        return bf16_bits_to_float(static_cast<u16>(fp4_pair<0>(codes[d / 2] >> (d % 2 * 4), fp4_scale(scales[d / FP4_BLOCK]))));
-      };
-      for (int at = begin + wave; at < end; at += DEC_WAVES) {
-        int pg, place_;
-        lookup(at, pg, place_);
-        const int rows = cache_row(pg, place_);
-        for (int key = 0; key < KEYS; ++key) {
-          const int slot_ = __shfl(rows, key, 64), u = at * KEYS + key, j = u < range.sinks ? u : u + range.delta;
-          if (slot_ < 0) continue;
-          const long cr = static_cast<long>(slot_) * p.token;
-          float dot = 0.0f;
-          for (int d = g * (D / 4); d < (g + 1) * (D / 4); ++d)
-            dot += value(kbase + cr, ksbase + cr / 16, d) * load_elem(qrow, d, DT);
-          dot = add_xor32(add_xor16(dot)) * sign;
-          if (!sees(pos[r], j, p.window, p.sinks)) continue;
-          const float w = __builtin_amdgcn_exp2f((dot - base) * p.c);
-#pragma unroll
-          for (int e = 0; e < OT; ++e)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) o[r][e][i] += w * value(vbase + cr, vsbase + cr / 16, (4 * g + i) * OT + e);
-        }
-      }
-    }
-  }
-  if constexpr (Q_LDS) __syncthreads();
-  join_waves<RB, D, JOINS>(lds.merge, m, l, o, wave, lane, p.c);
-  if (wave != 0) return;
-  store_decoded<DT, D, RB, OT>(p, share, b, hk, row0, slot, lane, m, l, o);
-}
-
-// ---------------------------------------------------------------------------
-// Writes: eight values of a key and of a value a thread, four threads a scale.
-// ---------------------------------------------------------------------------
-struct Fp4Cache {
-  unsigned char *k, *v, *k_scale, *v_scale;
-  long page_stride, token, head;  // of the codes, bytes; the scales': a sixteenth
-  long total;                     // slots
-  int page;
-};
-struct Fp4WriteParams {
-  const unsigned char *k, *v;
-  long k_token, k_head, v_token, v_head;
-  Fp4Cache cache;
-  const int64_t *slots;
-  int eighths, N, Hk;  // groups of eight values of a head
-};
-
 // Eight values from src as float32.
 template <int DT>
 __device__ __forceinline__ void load8(const unsigned char *src, float *x) {
@@ -439,6 +164,473 @@ __device__ __forceinline__ void load8(const unsigned char *src, float *x) {
     }
   }
 }
+
+// Read past the caches (ONCE) or through them.
+template <bool ONCE, typename T>
+__device__ __forceinline__ T load_keys(const T *p) {
+  if constexpr (ONCE) return __builtin_nontemporal_load(p);
+  return *p;
+}
+
+template <int DT, int D>
+struct Fp4 {
+  static constexpr int N = Parts<DT>::N;
+  static constexpr int ROW = D / 2;           // bytes of a key's codes
+  static constexpr int SROW = D / FP4_BLOCK;  // and of its scales
+  static constexpr int KSTEPS = D / 32;       // matrix steps of a score
+  static constexpr int KW = ROW / 16;         // words a lane reads of a key: one a step
+  static constexpr int KSCALES = D == 256 ? 2 : 1;  // and of its scales
+  static constexpr int OT = D / 16;           // output tiles: values a lane reads of a value row
+  static constexpr int VW = D == 64 ? 1 : OT / 8;   // words that hold them
+  static constexpr int KG = 2, KEYS = 16 * KG;      // keys at a time
+  static constexpr int SW = SROW / 4 > 0 ? SROW / 4 : 1;  // words that hold a key's scales
+  // First of the eight columns that lane group g takes in matrix step s.
+  __device__ static constexpr int column(int g, int s) {
+    return D == 64 ? 16 * g + 8 * s : 128 * (s / 4) + 32 * g + 8 * (s % 4);
+  }
+};
+
+// A wave's own LDS accesses before this come before those after it.
+__device__ __forceinline__ void wave_lds_order() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+}
+
+// Which of 16 keys is row m of their matrix product, so that the values of keys 4 i ..
+// 4 i + 3, next to each other where their rows are, are those of element i of the
+// result's lane groups.
+__device__ __forceinline__ int key_of(int m) { return 4 * (m % 4) + m / 4; }
+
+// NEAR: the caches' offsets fit 32 bits. ONCE: no other row tile reads the cache, so that
+// keys are loaded past the caches (values not: a row's are fetched in pieces).
+template <int DT, int D, int RB, bool NEAR, bool ONCE>
+__global__ __launch_bounds__(DEC_WAVES * 64, 2) void fp4_decode_kernel(const Fp4DecodeParams pp) {
+  using K = Fp4<DT, D>;
+  using E = Elem<PBGDN_BF16>;
+  constexpr int KS = K::KSTEPS, OT = K::OT, KG = K::KG, KEYS = K::KEYS, N = K::N;
+  constexpr int JOINS = RB * D <= 256 ? 2 : 1;
+  __shared__ __attribute__((aligned(16))) float merge[JOINS][RB * DEC_ROWS * (D + 2)];
+  __shared__ v4u32_t q_lds[RB * N * KS * 64];  // [row tile][part][step][lane]
+  __shared__ struct {
+    __attribute__((aligned(16))) uint32_t at[KEYS];
+    unsigned char scales[2 * KEYS * K::SROW];  // of the keys, then of the values
+  } lds_keys[DEC_WAVES];
+  PBGDN_POISON_LDS(merge, sizeof(merge));
+  PBGDN_POISON_LDS(q_lds, sizeof(q_lds));
+  PBGDN_POISON_LDS(lds_keys, sizeof(lds_keys));
+  PBGDN_POISON_SYNC();
+  const DecodeParams &p = pp.d;
+
+  const int thread = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  // Workgroups go to the XCDs in turn: the heads and row tiles of a piece follow each
+  // other on one XCD, whose L2 they share (rows of a token next to each other lie in one
+  // line; row tiles read the same ones).
+  const int heads = p.Hk * p.row_tiles, turn = blockIdx.x >> 3;
+  const int w = uniform(turn / heads * 8 + (blockIdx.x & 7)), id = turn - turn / heads * heads;
+  const int row0 = uniform(id / p.Hk) * (RB * DEC_ROWS), hk = uniform(id % p.Hk);
+  const Walk walk(p, thread);
+  const long x_end = (w + 1) * walk.per < walk.total ? (w + 1) * walk.per : walk.total;
+  long x_at = w * walk.per, start;
+  if (w >= p.target || x_at >= walk.total) return;
+  int b = uniform(walk.find(p, x_at, thread, start));
+  start = uniform_long(start);
+  for (; x_at < x_end && b < p.B; ++b) {
+    // (opaque: what follows from the lane is worked out where it is used, for each part
+    // again, instead of being kept in registers that the main loop needs)
+    const int lane = static_cast<int>(opaque(thread)), c = lane & 15, g = lane >> 4;
+    const int len = uniform(seq_length(p, b));
+    const KeyRange range = seq_keys(p, len);
+    const int quads = uniform(Walk::quads_of(p, len));
+    const int quad0 = uniform(static_cast<int>(x_at - start));
+    const int quad1 = uniform(static_cast<int>(x_end - start < quads ? x_end - start : quads));
+    const bool alone = quad0 == 0 && quad1 == quads;  // the sequence's only part
+    const int slot = w + b;
+    x_at = start + quad1;
+    start += quads;
+    // this wave's KEYS-wide blocks of the part: begin + wave, then every DEC_WAVES-th
+    static_assert(KEYS == DEC_KEYS, "quads are of such blocks");
+    const int blocks = (range.count + KEYS - 1) / KEYS, begin = quad0 * DEC_WAVES;
+    const int end = uniform(quad1 * DEC_WAVES < blocks ? quad1 * DEC_WAVES : blocks);
+
+    // this lane's rows of Q (column c of every row tile), in parts; each wave brings in a share
+    int pos[RB];
+    constexpr int QB = DT == PBGDN_F32 ? 4 : 2;  // bytes of an element of Q
+#pragma unroll
+    for (int r = 0; r < RB; ++r) {
+      const int row = row0 + r * DEC_ROWS + c;
+      const int rr = row < p.rows ? row : p.rows - 1;
+      const int t = rr / p.group;
+      pos[r] = len - p.T + t;
+      const unsigned char *src = p.q + ((static_cast<long>(b) * p.T + t) * p.Hq + hk * p.group + rr - t * p.group) * (D * QB);
+      for (int s = wave; s < KS; s += DEC_WAVES) {
+        const unsigned char *eight = src + K::column(g, s) * QB;
+        v4u32_t part[N];
+        if constexpr (DT == PBGDN_BF16) {
+          part[0] = *reinterpret_cast<const v4u32_t *>(eight);
+          if (p.negate) part[0] ^= 0x80008000u;
+        } else {
+          float x[8];
+          load8<DT>(eight, x);
+#pragma unroll
+          for (int e = 0; e < 8; e += 2) {
+            uint32_t y[N];
+            split_pair<N>(p.negate ? -x[e] : x[e], p.negate ? -x[e + 1] : x[e + 1], y);
+#pragma unroll
+            for (int i = 0; i < N; ++i) part[i][e / 2] = y[i];
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) q_lds[((r * N + i) * KS + s) * 64 + lane] = part[i];
+      }
+    }
+    __syncthreads();
+    float m[RB], l[RB];
+    float4_t o[RB][OT];
+#pragma unroll
+    for (int r = 0; r < RB; ++r) {
+      m[r] = -INFINITY;
+      l[r] = 0.0f;
+#pragma unroll
+      for (int j = 0; j < OT; ++j) o[r][j] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+
+    const unsigned char *kbase = p.k + hk * p.head, *vbase = p.v + hk * p.head;
+    const unsigned char *ksbase = pp.k_scale + hk * (p.head / 16), *vsbase = pp.v_scale + hk * (p.head / 16);
+    const int32_t *table = p.table + static_cast<long>(b) * p.max_pages;
+    // Where a block's keys lie, key lane % KEYS a lane: its page and its place there (-1:
+    // there is none), and then its row's distance from the caches' bases (of a row that
+    // exists, in any case).
+    struct Place {
+      int page, place;
+    };
+    const auto lookup = [&](int blk) __attribute__((always_inline)) {
+      const uint32_t u = static_cast<uint32_t>(blk) * KEYS + lane % KEYS, last = range.count - 1;  // (past a range's end too)
+      const int v = static_cast<int>(u < last ? u : last), j = v < range.sinks ? v : v + range.delta;
+      const int pg = static_cast<int>(__umulhi(2u * j, pp.page_mul) >> pp.page_shift);
+      return Place{table[pg < p.max_pages ? pg : p.max_pages - 1], ((u <= last) & (pg < p.max_pages)) ? j - pg * p.page : -1};
+    };
+    const auto exists = [&](const Place &x) __attribute__((always_inline)) {
+      return (x.place >= 0) & (x.page >= 0) & (x.page < p.num_pages);
+    };
+    const auto distance = [&](const Place &x) __attribute__((always_inline)) {
+      return exists(x) ? (x.page * pp.page_step + x.place * pp.token_step) << (NEAR ? 4 : 0) : 0u;
+    };
+    // A block as a lane takes it: unit g of key 16 kb + c of every group of keys, columns
+    // OT c .. of the values that its weights belong to, and the scales of one key (lanes
+    // below KEYS) or value. The scales and the distances go to their users through LDS,
+    // where a wave has a place of its own.
+    struct Block {
+      uint32_t k[KG][K::KW], v[4 * KG][K::VW], scales[K::SW];
+      bool held;  // key lane % KEYS exists
+    };
+    uint32_t *const at = lds_keys[wave].at;
+    unsigned char *const scales = lds_keys[wave].scales;
+    const auto publish = [&](const Place &x) __attribute__((always_inline)) {
+      const uint32_t d = distance(x);
+      wave_lds_order();
+      if (lane < KEYS) at[lane] = d;
+      wave_lds_order();
+      return d;
+    };
+    const unsigned char *const my_scales = lane < KEYS ? ksbase : vsbase;
+    const auto codes = [&](const unsigned char *base, uint32_t d, uint32_t lane_at) __attribute__((always_inline)) {
+      return NEAR ? base + (d + lane_at) : base + lane_at + (static_cast<uint64_t>(d) << 4);
+    };
+    const auto load = [&](Block &x, const Place &pl) __attribute__((always_inline)) {
+      x.held = exists(pl);
+      const unsigned char *ss = my_scales + (publish(pl) >> (NEAR ? 4 : 0));
+      if constexpr (D == 64) {
+        x.scales[0] = *reinterpret_cast<const uint16_t *>(ss);
+      } else if constexpr (D == 128) {
+        x.scales[0] = *reinterpret_cast<const uint32_t *>(ss);
+      } else {
+        const v2u32_t w = *reinterpret_cast<const v2u32_t *>(ss);
+        x.scales[0] = w[0];
+        x.scales[1] = w[1];
+      }
+#pragma unroll
+      for (int kb = 0; kb < KG; ++kb) {
+        const unsigned char *src = codes(kbase, at[16 * kb + key_of(c)], g * (D == 64 ? 8 : 16));
+        if constexpr (D == 64) {
+          const v2u32_t w = load_keys<ONCE>(reinterpret_cast<const v2u32_t *>(src));
+          x.k[kb][0] = w[0];
+          x.k[kb][1] = w[1];
+        } else {
+#pragma unroll
+          for (int h = 0; h < D / 128; ++h) {
+            const v4u32_t w = load_keys<ONCE>(reinterpret_cast<const v4u32_t *>(src + h * 64));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x.k[kb][4 * h + e] = w[e];
+          }
+        }
+      }
+#pragma unroll
+      for (int kb = 0; kb < KG; ++kb) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const unsigned char *src = codes(vbase, at[16 * kb + 4 * i + g], c * (OT / 2));
+          if constexpr (D == 64) {
+            x.v[4 * kb + i][0] = *reinterpret_cast<const uint16_t *>(src);
+          } else if constexpr (D == 128) {
+            x.v[4 * kb + i][0] = *reinterpret_cast<const uint32_t *>(src);
+          } else {
+            const v2u32_t w = *reinterpret_cast<const v2u32_t *>(src);
+            x.v[4 * kb + i][0] = w[0];
+            x.v[4 * kb + i][1] = w[1];
+          }
+        }
+      }
+    };
+    // One block of keys, cur; the next one's loads go out before it is worked on, and
+    // before them the page table's entries of the one after: loads come back in order.
+    Place pl{-1, -1};  // of the next block
+    const auto step = [&](int blk, Block &cur, Block &next, auto last) __attribute__((always_inline)) {
+      constexpr bool more = !decltype(last)::value;
+      if constexpr (more) {
+        const Place after = lookup(blk + 2 * DEC_WAVES);
+        load(next, pl);
+        pl = after;
+      }
+      // absent keys get a scale of one: finite values, whatever the row they were read from
+      // holds, which their weights of zero cancel
+#pragma unroll
+      for (int i = 0; i < K::SW; ++i) cur.scales[i] = cur.held ? cur.scales[i] : 0x7f7f7f7fu;
+      wave_lds_order();
+      if constexpr (D == 64) {
+        reinterpret_cast<uint16_t *>(scales)[lane] = static_cast<uint16_t>(cur.scales[0]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < K::SW; ++i) reinterpret_cast<uint32_t *>(scales)[K::SW * lane + i] = cur.scales[i];
+      }
+      wave_lds_order();
+      const uint64_t held = __ballot(cur.held);
+      float4_t sc[RB][KG];
+#pragma unroll
+      for (int r = 0; r < RB; ++r)
+#pragma unroll
+        for (int kb = 0; kb < KG; ++kb) sc[r][kb] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+      float ks[KG][K::KSCALES];
+#pragma unroll
+      for (int kb = 0; kb < KG; ++kb)
+#pragma unroll
+        for (int h = 0; h < K::KSCALES; ++h)
+          ks[kb][h] = fp4_scale(scales[(16 * kb + key_of(c)) * K::SROW + (D == 64 ? g / 2 : 4 * h + g)]);
+      float vs[4 * KG];
+#pragma unroll
+      for (int i = 0; i < 4 * KG; ++i)
+        vs[i] = fp4_scale(scales[(KEYS + i / 4 * 16 + 4 * (i % 4) + g) * K::SROW + c * OT / FP4_BLOCK]);
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        v4u32_t a[KG];
+#pragma unroll
+        for (int kb = 0; kb < KG; ++kb) a[kb] = fp4_unpack8(cur.k[kb][s], ks[kb][D == 256 ? s / 4 : 0]);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+          for (int r = 0; r < RB; ++r) {
+            const v4u32_t q = q_lds[((r * N + i) * KS + s) * 64 + lane];
+#pragma unroll
+            for (int kb = 0; kb < KG; ++kb) sc[r][kb] = E::mma16(a[kb], q, sc[r][kb]);
+          }
+      }
+      const int u0 = blk * KEYS;
+      const int j0 = u0 < range.sinks ? u0 : u0 + range.delta, j1 = u0 + KEYS - 1 + range.delta;
+      const bool whole = held == ~0ull && u0 >= range.sinks && j1 <= len - p.T && j0 > len - 1 - p.window;
+#pragma unroll
+      for (int r = 0; r < RB; ++r) {
+        float4_t (&s)[KG] = sc[r];
+        if (!whole) {
+#pragma unroll
+          for (int i = 0; i < 4 * KG; ++i) {
+            const int key = i / 4 * 16 + 4 * (i % 4) + g, u = u0 + key;
+            const int j = u < range.sinks ? u : u + range.delta;
+            const bool seen = ((held >> key) & 1) & sees(pos[r], j, p.window, p.sinks);
+            s[i / 4][i % 4] = seen ? s[i / 4][i % 4] : -INFINITY;
+          }
+        }
+        float mx = s[0][0];
+#pragma unroll
+        for (int i = 1; i < 4 * KG; ++i) mx = fmaxf(mx, s[i / 4][i % 4]);
+        mx = max_rows(mx);
+        if (__any((mx - m[r]) * p.c > LAG)) {
+          const float top = fmaxf(m[r], mx);
+          const float alpha = __builtin_amdgcn_exp2f((m[r] - (top == -INFINITY ? 0.0f : top)) * p.c);
+          m[r] = top;
+          l[r] *= alpha;
+#pragma unroll
+          for (int j = 0; j < OT; ++j) o[r][j] *= alpha;
+        }
+        const float base = m[r] == -INFINITY ? 0.0f : m[r], at = base * p.c;
+        float sum = 0.0f;
+        if (__any(fabsf(at) > EXACT_SCORES)) {
+#pragma unroll
+          for (int i = 0; i < 4 * KG; ++i) s[i / 4][i % 4] = (s[i / 4][i % 4] - base) * p.c;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4 * KG; ++i) s[i / 4][i % 4] = __builtin_fmaf(s[i / 4][i % 4], p.c, -at);
+        }
+#pragma unroll
+        for (int i = 0; i < 4 * KG; ++i) {
+          s[i / 4][i % 4] = __builtin_amdgcn_exp2f(s[i / 4][i % 4]);
+          sum += s[i / 4][i % 4];
+        }
+        l[r] += sum;
+      }
+      // O^T += V^T P; element e of the lane's values makes output tile e
+      v4u32_t w[RB][KG / 2][N];
+#pragma unroll
+      for (int r = 0; r < RB; ++r)
+#pragma unroll
+        for (int h = 0; h < KG / 2; ++h)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float x = sc[r][2 * h + i / 2][2 * (i % 2)], y = sc[r][2 * h + i / 2][2 * (i % 2) + 1];
+            if constexpr (N == 1) {
+              w[r][h][0][i] = E::pack(x, y);
+            } else {
+              uint32_t part[N];
+              split_pair<N>(x, y, part);
+#pragma unroll
+              for (int n = 0; n < N; ++n) w[r][h][n][i] = part[n];
+            }
+          }
+      const auto pair_of_tiles = [&](auto E0) __attribute__((always_inline)) {  // tiles 2 e and 2 e + 1
+        constexpr int e = decltype(E0)::value;
+#pragma unroll
+        for (int h = 0; h < KG / 2; ++h) {
+          uint32_t x[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] = fp4_pair<e % 4>(cur.v[8 * h + i][e / 4], vs[8 * h + i]);
+          v4u32_t lo, hi;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            lo[i] = __builtin_amdgcn_perm(x[2 * i + 1], x[2 * i], 0x05040100u);
+            hi[i] = __builtin_amdgcn_perm(x[2 * i + 1], x[2 * i], 0x07060302u);
+          }
+#pragma unroll
+          for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int r = 0; r < RB; ++r) {
+              o[r][2 * e] = E::mma16(lo, w[r][h][n], o[r][2 * e]);
+              o[r][2 * e + 1] = E::mma16(hi, w[r][h][n], o[r][2 * e + 1]);
+            }
+        }
+      };
+      pair_of_tiles(std::integral_constant<int, 0>{});
+      pair_of_tiles(std::integral_constant<int, 1>{});
+      if constexpr (OT >= 8) {
+        pair_of_tiles(std::integral_constant<int, 2>{});
+        pair_of_tiles(std::integral_constant<int, 3>{});
+      }
+      if constexpr (OT >= 16) {
+        pair_of_tiles(std::integral_constant<int, 4>{});
+        pair_of_tiles(std::integral_constant<int, 5>{});
+        pair_of_tiles(std::integral_constant<int, 6>{});
+        pair_of_tiles(std::integral_constant<int, 7>{});
+      }
+    };
+    if (begin + wave < end) {
+      Block x, y;
+      const Place first = lookup(begin + wave);
+      pl = lookup(begin + wave + DEC_WAVES);
+      load(x, first);
+      int blk = begin + wave;
+      for (; blk + 2 * DEC_WAVES < end; blk += 2 * DEC_WAVES) {
+        step(blk, x, y, std::false_type{});
+        step(blk + DEC_WAVES, y, x, std::false_type{});
+      }
+      if (blk + DEC_WAVES < end) {
+        step(blk, x, y, std::false_type{});
+        step(blk + DEC_WAVES, y, x, std::true_type{});
+      } else {
+        step(blk, x, y, std::true_type{});
+      }
+    }
+    // A value that some tokens see and others do not enters all rows' products, with
+    // weight zero where it is not seen: harmless unless its scale is that of NaN (or
+    // infinite). Outputs that end so are worked out again, key by key, from what their
+    // token sees alone.
+    if (p.T > 1) {
+#pragma unroll
+      for (int r = 0; r < RB; ++r) {
+        float nought = 0.0f;
+#pragma unroll
+        for (int j = 0; j < OT; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) nought = __builtin_fmaf(o[r][j][i], 0.0f, nought);  // zero, or NaN
+        if (!__any(nought != 0.0f)) continue;
+#pragma unroll
+        for (int j = 0; j < OT; ++j) o[r][j] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        const int row = row0 + r * DEC_ROWS + c, rr = row < p.rows ? row : p.rows - 1, t = rr / p.group;
+        const unsigned char *qrow = p.q + ((static_cast<long>(b) * p.T + t) * p.Hq + hk * p.group + rr - t * p.group) * (D * QB);
+        const float base = m[r] == -INFINITY ? 0.0f : m[r], sign = p.negate ? -1.0f : 1.0f;
+        for (int at = begin + wave; at < end; at += DEC_WAVES) {
+          const Place mine = lookup(at);
+          const uint64_t held = __ballot(exists(mine));
+          const int steps = static_cast<int>(distance(mine));
+          for (int key = 0; key < KEYS; ++key) {
+            const uint64_t sr = static_cast<uint32_t>(__shfl(steps, key, 64)) >> (NEAR ? 4 : 0), cr = sr << 4;
+            const int u = at * KEYS + key, j = u < range.sinks ? u : u + range.delta;
+            if (!((held >> key) & 1)) continue;
+            float dot = 0.0f;
+#pragma unroll 1
+            for (int d = g * (D / 4); d < (g + 1) * (D / 4); d += 8) {
+              const v4u32_t k = fp4_unpack8(*reinterpret_cast<const uint32_t *>(kbase + cr + d / 2),
+                                            fp4_scale(ksbase[sr + d / FP4_BLOCK]));
+              float x[8];
+              load8<DT>(qrow + d * QB, x);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) dot += E::low(k[e]) * x[2 * e] + E::high(k[e]) * x[2 * e + 1];
+            }
+            dot = add_xor32(add_xor16(dot)) * sign;
+            if (!sees(pos[r], j, p.window, p.sinks)) continue;
+            const float w = __builtin_amdgcn_exp2f((dot - base) * p.c);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int d = (4 * g + i) * OT;
+              const float vs = fp4_scale(vsbase[sr + d / FP4_BLOCK]);
+#pragma unroll
+              for (int e = 0; e < OT; e += 8) {
+                const unsigned char *src = vbase + cr + (d + e) / 2;
+                uint32_t word;
+                if constexpr (D == 64)
+                  word = *reinterpret_cast<const uint16_t *>(src);
+                else
+                  word = *reinterpret_cast<const uint32_t *>(src);
+                const v4u32_t v = fp4_unpack8(word, vs);
+#pragma unroll
+                for (int x = 0; x < 8 && e + x < OT; ++x)
+                  o[r][e + x][i] += w * (x % 2 ? E::high(v[x / 2]) : E::low(v[x / 2]));
+              }
+              __builtin_amdgcn_sched_barrier(0);  // (not all the values at once, in so many registers)
+            }
+          }
+        }
+      }
+    }
+    const int lane_ = static_cast<int>(opaque(thread));
+    join_waves<RB, D, JOINS>(merge, m, l, o, wave, lane_, p.c);
+    if (wave == 0) store_decoded<DT, D, RB, OT>(p, alone, b, hk, row0, slot, lane_, m, l, o);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Writes: eight values of a key and of a value a thread, four threads a scale.
+// ---------------------------------------------------------------------------
+struct Fp4Cache {
+  unsigned char *k, *v, *k_scale, *v_scale;
+  long page_stride, token, head;  // of the codes, bytes; the scales': a sixteenth
+  long total;                     // slots
+  int page;
+};
+struct Fp4WriteParams {
+  const unsigned char *k, *v;
+  long k_token, k_head, v_token, v_head;
+  Fp4Cache cache;
+  const int64_t *slots;
+  int eighths, N, Hk;  // groups of eight values of a head
+};
 
 // Codes of the eight values of each of four neighbouring lanes, and their scale.
 __device__ __forceinline__ uint32_t quantise(const float *x, uint32_t &scale) {
@@ -568,35 +760,59 @@ __global__ __launch_bounds__(SCAN_THREADS) void fp4_read_kernel(const Fp4ReadPar
   }
 }
 
-template <int DT, int D>
+// Row tiles of 16 that a workgroup takes at once: two where that keeps its registers
+// within those of two waves a SIMD.
+static int fp4_row_tiles(int D, int rows) { return rows > DEC_ROWS && D < 256 ? 2 : 1; }
+
+// Workgroups of a (row tile, key head): together as many as the GPU holds at once.
+static int fp4_target(int Hk, int rows, int D) {
+  DeviceShape shape;
+  if (!device_shape(shape)) shape.cus = 256;
+  const int rb = fp4_row_tiles(D, rows), tiles = (rows + rb * DEC_ROWS - 1) / (rb * DEC_ROWS);
+  const int held = rb == 1 && D < 256 ? 3 : 2;  // of a CU
+  const long t = static_cast<long>(held) * shape.cus / (static_cast<long>(Hk) * tiles);
+  return t > 1 ? static_cast<int>(t) : 1;
+}
+
+template <int DT, int D, bool NEAR>
 static int launch_fp4(Fp4DecodeParams &p, hipStream_t stream) {
-  const auto run = [&](auto kernel, int rb) {
-    const unsigned blocks = decode_blocks(p.d, rb);
-    if (blocks) hipLaunchKernelGGL(kernel, dim3(blocks), dim3(DEC_WAVES * 64), 0, stream, p);
-    return blocks != 0;
+  const int rb = fp4_row_tiles(D, p.d.rows);
+  p.d.row_tiles = (p.d.rows + rb * DEC_ROWS - 1) / (rb * DEC_ROWS);
+  const long blocks = (p.d.target + 7L) / 8 * 8 * p.d.Hk * p.d.row_tiles;
+  if (blocks > 0x7fffffffL || static_cast<long>(p.d.B) * p.d.Hk * p.d.rows > 0x7fffffffL) return PBGDN_ERR_UNSUPPORTED;
+  const auto run = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(DEC_WAVES * 64), 0, stream, p);
   };
-  const bool ok = p.d.rows <= DEC_ROWS ? run(fp4_decode_kernel<DT, D, 1>, 1) : run(fp4_decode_kernel<DT, D, 2>, 2);
-  if (!ok) return PBGDN_ERR_UNSUPPORTED;
-  launch_join<DT, D>(p.d, stream);
+  if constexpr (D == 256) {
+    if (p.d.row_tiles == 1 && NEAR)
+      run(fp4_decode_kernel<DT, D, 1, NEAR, NEAR>);
+    else
+      run(fp4_decode_kernel<DT, D, 1, NEAR, false>);
+  } else {
+    if (rb == 1)
+      run(fp4_decode_kernel<DT, D, 1, NEAR, NEAR>);
+    else if (p.d.row_tiles == 1 && NEAR)
+      run(fp4_decode_kernel<DT, D, 2, NEAR, NEAR>);
+    else
+      run(fp4_decode_kernel<DT, D, 2, NEAR, false>);
+  }
+  // Four waves a row where a sequence may have more parts than one fetches at once; else
+  // eight rows a workgroup, which all take the same sums over the lengths.
+  launch_join<DT, D, Walk>(p.d, p.d.target > 8L * p.d.B, 8, stream);
   return hipGetLastError() == hipSuccess ? PBGDN_OK : PBGDN_ERR_LAUNCH;
 }
 
-template <int DT>
+template <int DT, bool NEAR>
 static int dispatch_fp4(Fp4DecodeParams &p, int D, hipStream_t stream) {
   switch (D) {
-    case 64: return launch_fp4<DT, 64>(p, stream);
-    case 128: return launch_fp4<DT, 128>(p, stream);
-    default: return launch_fp4<DT, 256>(p, stream);
+    case 64: return launch_fp4<DT, 64, NEAR>(p, stream);
+    case 128: return launch_fp4<DT, 128, NEAR>(p, stream);
+    default: return launch_fp4<DT, 256, NEAR>(p, stream);
   }
 }
-
-// Parts wanted over all sequences.
-static int fp4_target(int Hk, int rows) {
-  DeviceShape shape;
-  if (!device_shape(shape)) shape.cus = 256;
-  const int tiles = (rows + 2 * DEC_ROWS - 1) / (2 * DEC_ROWS);
-  const int t = 8 * shape.cus / (Hk * tiles);
-  return t > 1 ? t : 1;
+template <int DT>
+static int dispatch_fp4(Fp4DecodeParams &p, int D, bool near, hipStream_t stream) {
+  return near ? dispatch_fp4<DT, true>(p, D, stream) : dispatch_fp4<DT, false>(p, D, stream);
 }
 
 static bool fp4_width(int D) { return D == 64 || D == 128 || D == 256; }
@@ -628,9 +844,9 @@ static int fp4_cache(Fp4Cache &c, const void *k, const void *v, const void *ks, 
 
 extern "C" size_t pbattn_fp4_decode_workspace_size(int B, int T, int Hq, int Hk, int D) {
   using namespace pbgdn;
-  if (!decode_sizes_ok(B, T, Hq, Hk, D)) return 0;
+  if (!decode_sizes_ok(B, T, Hq, Hk, D) || !fp4_width(D)) return 0;
   const int rows = Hq / Hk * T;
-  const size_t slots = static_cast<size_t>(fp4_target(Hk, rows)) + B;
+  const size_t slots = static_cast<size_t>(fp4_target(Hk, rows, D)) + B;
   return slots * Hk * rows * (D * sizeof(float) + sizeof(float2));
 }
 
@@ -653,8 +869,10 @@ extern "C" int pbattn_fp4_decode(const void *q, int dtype, const void *k_cache, 
   Fp4Cache cache;
   const int status = fp4_cache(cache, k_cache, v_cache, k_scale, v_scale, strides, page_size, num_pages, D);
   if (status != PBGDN_OK) return status;
-  const long page_rows = cache.token > 0 ? cache.page_stride / cache.token : 0;
-  if (page_rows * (num_pages > 0 ? num_pages - 1 : 0) + page_size > 0x7fffffffL) return PBGDN_ERR_UNSUPPORTED;
+  const long pages = num_pages > 0 ? num_pages - 1 : 0;
+  const long reach = (cache.page_stride / 16) * pages + (cache.token / 16) * (page_size - 1L);
+  if (reach > 0xffffffffL) return PBGDN_ERR_UNSUPPORTED;
+  const bool near = reach < (1L << 28) - D / 32;  // (a row's own bytes within 4 GiB, too)
   if (workspace_bytes < pbattn_fp4_decode_workspace_size(B, T, Hq, Hk, D)) return PBGDN_ERR_INVALID_ARGUMENT;
   Fp4DecodeParams pp{};
   DecodeParams &p = pp.d;
@@ -663,9 +881,13 @@ extern "C" int pbattn_fp4_decode(const void *q, int dtype, const void *k_cache, 
   p.v = cache.v;
   pp.k_scale = cache.k_scale;
   pp.v_scale = cache.v_scale;
-  p.token = cache.token;
   p.head = cache.head;
-  p.page_rows = static_cast<int>(page_rows);
+  pp.page_step = static_cast<uint32_t>(pages > 0 ? cache.page_stride / 16 : 0);
+  pp.token_step = static_cast<uint32_t>(page_size > 1 ? cache.token / 16 : 0);
+  // with 2^(s - 1) < page <= 2^s, floor(2^(31 + s) / page) + 1 is 2^(31 + s) / page and at
+  // most one more, which adds less than 1 / page to any quotient below 2^31 / page
+  while ((1L << pp.page_shift) < page_size) ++pp.page_shift;
+  pp.page_mul = static_cast<uint32_t>((1ULL << (31 + pp.page_shift)) / page_size + 1);
   p.page = page_size;
   p.num_pages = max_pages > 0 ? num_pages : 0;  // (no table: no keys)
   p.max_pages = max_pages;
@@ -673,16 +895,16 @@ extern "C" int pbattn_fp4_decode(const void *q, int dtype, const void *k_cache, 
   p.lengths = lengths;
   p.o = o;
   p.lse = lse;
-  decode_call(p, B, T, Hq, Hk, scale, window, sinks, fp4_target(Hk, Hq / Hk * T));
+  decode_call(p, B, T, Hq, Hk, scale, window, sinks, fp4_target(Hk, Hq / Hk * T, D));
   const size_t used = decode_workspace(p, workspace, D);
   hipStream_t s = static_cast<hipStream_t>(stream);
   debug_poison(o, static_cast<size_t>(B) * T * Hq * D * attn_bytes(dtype), s);
   if (lse) debug_poison(lse, static_cast<size_t>(B) * T * Hq * sizeof(float), s);
   debug_poison(workspace, used, s);
   switch (dtype) {
-    case PBGDN_F32: return dispatch_fp4<PBGDN_F32>(pp, D, s);
-    case PBGDN_BF16: return dispatch_fp4<PBGDN_BF16>(pp, D, s);
-    default: return dispatch_fp4<PBGDN_F16>(pp, D, s);
+    case PBGDN_F32: return dispatch_fp4<PBGDN_F32>(pp, D, near, s);
+    case PBGDN_BF16: return dispatch_fp4<PBGDN_BF16>(pp, D, near, s);
+    default: return dispatch_fp4<PBGDN_F16>(pp, D, near, s);
   }
 }
 

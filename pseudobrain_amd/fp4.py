@@ -60,12 +60,11 @@ def fp4_cache(pages: int, page: int, heads: int, width: int, device="cuda", head
 
 
 @_plan
-def _fp4_plan(k, k_stride, v, v_stride, ks, ks_stride, vs, vs_stride, dtypes):
-    """Checked sizes (pages, page, Hk, D) of a cache of these shapes and strides, and the stride array."""
-    if len(k) != 4 or v != k or len(ks) != 4 or vs != ks or ks[:3] != k[:3] or ks[3] * 16 != k[3]:
-        raise ValueError("expected a cache of codes k, v [pages, page, Hk, D / 2] and scales [pages, page, Hk, D / 32]")
-    if dtypes != (torch.uint8,) * 4:
-        raise ValueError("codes and scales are uint8")
+def _fp4_plan(k, k_stride, ks, ks_stride):
+    """Checked sizes (pages, page, Hk, D) of a cache of codes and scales of these shapes and
+    strides, and the stride array."""
+    if len(k) != 4 or len(ks) != 4 or ks[:3] != k[:3] or ks[3] * 16 != k[3]:
+        raise ValueError(_FP4_SHAPES)
     pages, page, heads, row = k
     if page < 1 or heads < 1:
         raise ValueError("a cache has at least one token a page and one head")
@@ -81,17 +80,28 @@ def _fp4_plan(k, k_stride, v, v_stride, ks, ks_stride, vs, vs_stride, dtypes):
         return p or t * page, t, h
 
     at = steps(k, k_stride)
-    if at is None or at[0] % at[1] or any(steps(s, st) != at for s, st in ((v, v_stride), (ks, ks_stride), (vs, vs_stride))):
-        raise ValueError("codes and scales must be laid out alike: dense rows, equal strides in rows that are multiples of "
-                         "one (the scales' a sixteenth of the codes'), pages a whole number of tokens apart")
+    if at is None or at[0] % at[1] or steps(ks, ks_stride) != at:
+        raise ValueError(_FP4_LAYOUT)
     return (pages, page, heads, 2 * row), (ctypes.c_int64 * 3)(*(row * x for x in at))
+
+
+_FP4_SHAPES = "expected a cache of codes k, v [pages, page, Hk, D / 2] and scales [pages, page, Hk, D / 32]"
+_FP4_LAYOUT = ("codes and scales must be laid out alike: dense rows, equal strides in rows that are multiples of one (the "
+               "scales' a sixteenth of the codes'), pages a whole number of tokens apart")
 
 
 def _fp4(cache):
     """_fp4_plan of a cache, and its tensors' addresses."""
     k, v, ks, vs = cache
-    plan = _fp4_plan(k.shape, k.stride(), v.shape, v.stride(), ks.shape, ks.stride(), vs.shape, vs.stride(),
-                     (k.dtype, v.dtype, ks.dtype, vs.dtype))
+    if not k.dtype == v.dtype == ks.dtype == vs.dtype == torch.uint8:
+        raise ValueError("codes and scales are uint8")
+    shape, stride, s_shape, s_stride = k.shape, k.stride(), ks.shape, ks.stride()
+    if v.shape != shape or vs.shape != s_shape:
+        raise ValueError(_FP4_SHAPES)
+    plan = _fp4_plan(shape, stride, s_shape, s_stride)
+    if (v.stride() != stride or vs.stride() != s_stride) and (
+            list(_fp4_plan(shape, v.stride(), s_shape, vs.stride())[1]) != list(plan[1])):
+        raise ValueError(_FP4_LAYOUT)
     at = k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr()
     if (at[0] | at[1] | at[2] | at[3]) % 16:
         raise ValueError("codes and scales must be aligned to 16 bytes")
@@ -230,7 +240,7 @@ def _read(cache, page_table, lengths, tokens, dtype):
     code = _read_plan(shape, page_table.shape, lengths.shape, int(tokens), dtype)
     page_table, lengths = _boundaries(page_table), _boundaries(lengths)
     k, v = (torch.empty(tokens, *shape[2:], dtype=dtype, device=dev) for _ in range(2))
-    cu = torch.empty(lengths.shape[0] + 1, dtype=torch.int32, device=dev)
+    cu = lengths.new_empty(lengths.shape[0] + 1)
     _launch("pbattn_fp4_read", _lib.attn_lib().pbattn_fp4_read, dev, *at, steps, shape[1], shape[0], page_table.data_ptr(),
             page_table.shape[1], lengths.data_ptr(), k.data_ptr(), v.data_ptr(), code, cu.data_ptr(), lengths.shape[0],
             tokens, shape[2], shape[3])

@@ -57,8 +57,7 @@ def _extend(page_table, lengths, counts, free_pages, num_free, page, tokens):
     if not 0 <= tokens < 2**31:
         raise ValueError("tokens must be a number of tokens below 2^31")
     slots = torch.empty(tokens, dtype=torch.int64, device=dev)
-    positions, cu, new_lengths, new_free = (torch.empty(n, dtype=torch.int32, device=dev)
-                                            for n in (tokens, batch + 1, batch, 1))
+    positions, cu, new_lengths, new_free = [lengths.new_empty(n) for n in (tokens, batch + 1, batch, 1)]
     _launch("pbattn_pages_extend", _lib.attn_lib().pbattn_pages_extend, dev, page_table.data_ptr(), row, max_pages,
             lengths.data_ptr(), counts.data_ptr(), batch, page, free_pages.data_ptr(), capacity, num_free.data_ptr(), tokens,
             slots.data_ptr(), positions.data_ptr(), cu.data_ptr(), new_lengths.data_ptr(), new_free.data_ptr())
@@ -109,7 +108,7 @@ def paged_cache_extend(page_table, lengths, counts, free_pages, num_free, page: 
 
 def _release(page_table, first, end, free_pages, num_free, page):
     dev, (row, max_pages, batch, capacity), first, end, num_free = _pool(page_table, first, end, free_pages, num_free, page)
-    new_free = torch.empty(1, dtype=torch.int32, device=dev)
+    new_free = first.new_empty(1)
     _launch("pbattn_pages_release", _lib.attn_lib().pbattn_pages_release, dev, page_table.data_ptr(), row, max_pages,
             first.data_ptr(), end.data_ptr(), batch, page, free_pages.data_ptr(), capacity, num_free.data_ptr(),
             new_free.data_ptr())

@@ -32,10 +32,8 @@ def rope_tables(positions: int, rotary: int, base: float = 10000.0, device="cuda
     return angle.cos().float(), angle.sin().float()
 
 
-@_plan
-def _rope_plan(q, k, dtypes, qw, kw, cos, sin, tables, positions, pos_dtype):
-    """Checked sizes (B, T, Hq, Hk, D, R) of a call with tensors of these shapes, and the
-    dtype codes of the rows and of the weights."""
+def _rope_sizes(q, k, dtype, k_dtype, qw, kw, w_dtype, kw_dtype, cos, sin, cos_dtype, sin_dtype, positions, pos_dtype):
+    """Checked sizes (B, T, Hq, Hk, D, R) of a call with tensors of these shapes and types."""
     if len(q) != 4 or len(k) != 4 or q[:2] != k[:2] or q[3] != k[3]:
         raise ValueError("expected q [B,T,Hq,D] and k [B,T,Hk,D]")
     batch, length, hq, d = q
@@ -46,9 +44,10 @@ def _rope_plan(q, k, dtypes, qw, kw, cos, sin, tables, positions, pos_dtype):
         raise ValueError(f"no kernel for head widths above {MAX_WIDTH} (got {d})")
     if qw != (d,) or kw != (d,):
         raise ValueError("expected a weight [D] for q and for k")
-    if dtypes[1] != dtypes[0] or dtypes[3] != dtypes[2]:
+    if k_dtype != dtype or kw_dtype != w_dtype:
         raise ValueError("q and k must have one dtype, and their weights one")
-    if len(cos) != 2 or sin != cos or tables != (torch.float32, torch.float32):
+    _dtype_code(dtype), _dtype_code(w_dtype)
+    if len(cos) != 2 or sin != cos or cos_dtype != torch.float32 or sin_dtype != torch.float32:
         raise ValueError("expected float32 tables cos and sin [positions, R / 2] of one shape")
     if 2 * cos[1] > d:
         raise ValueError("the tables rotate more values than a head has")
@@ -57,71 +56,74 @@ def _rope_plan(q, k, dtypes, qw, kw, cos, sin, tables, positions, pos_dtype):
     if len(positions) not in (1, 2) or positions[-1] not in (1, length) or (
             len(positions) == 2 and positions[0] not in (1, batch)):
         raise ValueError("expected positions [T] or [B,T] (or what broadcasts to it)")
-    return (batch, length, hq, hk, d, 2 * cos[1]), _dtype_code(dtypes[0]), _dtype_code(dtypes[2])
-
-
-def _check(q, k, q_weight, k_weight, cos, sin, positions):
-    return _rope_plan(q.shape, k.shape, (q.dtype, k.dtype, q_weight.dtype, k_weight.dtype), q_weight.shape, k_weight.shape,
-                      cos.shape, sin.shape, (cos.dtype, sin.dtype), positions.shape, positions.dtype)
+    return batch, length, hq, hk, d, 2 * cos[1]
 
 
 @_plan
-def _row_steps(q, q_stride, k, k_stride):
-    """The stride array of rows of these shapes, None if an innermost axis is not dense."""
-    if any(x[3] > 1 and stride[3] != 1 for x, stride in ((q, q_stride), (k, k_stride))):
-        return None
-    return _steps((q, q_stride), (k, k_stride))
+def _rope_plan(q_stride, k_stride, pos_stride, *call):
+    """_rope_sizes of a call, the dtype codes of its rows and weights, the stride arrays of
+    the rows (None if an innermost axis is not dense) and of the positions, and whether those
+    have 64 bits."""
+    sizes = _rope_sizes(*call)
+    q, k, positions = call[0], call[1], call[12]
+    dense = all(x[3] == 1 or stride[3] == 1 for x, stride in ((q, q_stride), (k, k_stride)))
+    lead = 2 - len(positions)
+    pos_steps = _steps(((1,) * lead + tuple(positions) + (1,), (0,) * lead + tuple(pos_stride) + (1,)))
+    return (sizes, _dtype_code(call[2]), _dtype_code(call[6]), _steps((q, q_stride), (k, k_stride)) if dense else None,
+            pos_steps, int(call[13] == torch.int64))
 
 
-@_plan
-def _position_steps(shape, stride):
-    return _steps(((1,) * (2 - len(shape)) + tuple(shape) + (1,), (0,) * (2 - len(shape)) + tuple(stride) + (1,)))
+def _call(q, k, q_weight, k_weight, cos, sin, positions):
+    return (q.shape, k.shape, q.dtype, k.dtype, q_weight.shape, k_weight.shape, q_weight.dtype, k_weight.dtype, cos.shape,
+            sin.shape, cos.dtype, sin.dtype, positions.shape, positions.dtype)
 
 
-def _operands(q, k, q_weight, k_weight, cos, sin, positions):
-    """The tensors as the kernels read them, and the arguments that say where: (tensors to
-    keep, arguments up to the outputs without the offset)."""
-    q, k = _aligned(q, 16), _aligned(k, 16)
-    steps = _row_steps(q.shape, q.stride(), k.shape, k.stride())
-    if steps is None:
-        q, k = q.contiguous(), k.contiguous()
-        steps = _row_steps(q.shape, q.stride(), k.shape, k.stride())
-    q_weight, k_weight, cos, sin = (_aligned(x.contiguous(), 16) for x in (q_weight, k_weight, cos, sin))
-    return (q, k, q_weight, k_weight, cos, sin, positions), steps, _position_steps(positions.shape, positions.stride())
+def _operands(q, k, q_weight, k_weight, cos, sin, positions, weight_offset):
+    """The device, the checked sizes, the tensors as the kernels read them (to be kept until
+    the launch) and the arguments that name them."""
+    args = (q, k, q_weight, k_weight, cos, sin, positions)
+    plan = _rope_plan(q.stride(), k.stride(), positions.stride(), *_call(*args))
+    dev = _one_device(*args)
+    if (plan[3] is None or (q.data_ptr() | k.data_ptr() | q_weight.data_ptr() | k_weight.data_ptr() | cos.data_ptr()
+                            | sin.data_ptr()) % 16
+            or not (q_weight.is_contiguous() and k_weight.is_contiguous() and cos.is_contiguous() and sin.is_contiguous())):
+        # (the strides are taken last: a copy for the alignment may have others than its view)
+        q, k = (_aligned(x if x.stride(3) == 1 or x.shape[3] == 1 else x.contiguous(), 16) for x in (q, k))
+        args = (q, k, *(_aligned(x.contiguous(), 16) for x in args[2:6]), positions)
+        plan = _rope_plan(q.stride(), k.stride(), positions.stride(), *_call(*args))
+    sizes, code, wcode, steps, pos_steps, pos64 = plan
+    return dev, sizes, args, (q.data_ptr(), k.data_ptr(), code, steps, args[2].data_ptr(), args[3].data_ptr(), wcode,
+                              weight_offset, args[4].data_ptr(), args[5].data_ptr(), cos.shape[0], positions.data_ptr(),
+                              pos64, pos_steps)
 
 
 def _forward(q, k, q_weight, k_weight, cos, sin, positions, eps, weight_offset, interleaved):
-    sizes, code, wcode = _check(q, k, q_weight, k_weight, cos, sin, positions)
-    dev = _one_device(q, k, q_weight, k_weight, cos, sin, positions)
-    (q, k, q_weight, k_weight, cos, sin, positions), steps, pos_steps = _operands(
-        q, k, q_weight, k_weight, cos, sin, positions)
-    q_out, k_out = (torch.empty(x.shape, dtype=x.dtype, device=dev) for x in (q, k))
-    _launch("pbattn_qk_norm_rope", _lib.attn_lib().pbattn_qk_norm_rope, dev, q.data_ptr(), k.data_ptr(), code, steps,
-            q_weight.data_ptr(), k_weight.data_ptr(), wcode, weight_offset, cos.data_ptr(), sin.data_ptr(), cos.shape[0],
-            positions.data_ptr(), int(positions.dtype == torch.int64), pos_steps, q_out.data_ptr(), k_out.data_ptr(), *sizes,
+    dev, sizes, kept, args = _operands(q, k, q_weight, k_weight, cos, sin, positions, weight_offset)
+    q_out, k_out = q.new_empty(q.shape), k.new_empty(k.shape)
+    _launch("pbattn_qk_norm_rope", _lib.attn_lib().pbattn_qk_norm_rope, dev, *args, q_out.data_ptr(), k_out.data_ptr(), *sizes,
             eps, int(interleaved))
     return q_out, k_out
 
 
+@_plan
+def _workspace_size(width: int, device_index: int) -> int:
+    with torch.cuda.device(device_index):  # (the size depends on the device's compute units)
+        return _lib.attn_lib().pbattn_qk_norm_rope_bwd_workspace_size(width)
+
+
 def _backward(q, k, q_weight, k_weight, cos, sin, positions, grad_q, grad_k, eps, weight_offset, interleaved):
-    sizes, code, wcode = _check(q, k, q_weight, k_weight, cos, sin, positions)
-    dev = _one_device(q, k, q_weight, k_weight, cos, sin, positions, grad_q, grad_k)
+    dev, sizes, kept, args = _operands(q, k, q_weight, k_weight, cos, sin, positions, weight_offset)
+    _one_device(q, grad_q, grad_k)
     if grad_q.shape != q.shape or grad_k.shape != k.shape:
         raise ValueError("grad_q and grad_k must have q's and k's shapes")
-    (q, k, q_weight, k_weight, cos, sin, positions), steps, pos_steps = _operands(
-        q, k, q_weight, k_weight, cos, sin, positions)
     grad_q, grad_k = (_aligned(x.to(q.dtype).contiguous(), 16) for x in (grad_q, grad_k))
-    dq, dk, dqw, dkw = (torch.empty(x.shape, dtype=x.dtype, device=dev) for x in (q, k, q_weight, k_weight))
+    dq, dk, dqw, dkw = (x.new_empty(x.shape) for x in (q, k, q_weight, k_weight))
     if sizes[0] == 0 or sizes[1] == 0:
         return dq, dk, dqw.zero_(), dkw.zero_()
-    lib = _lib.attn_lib()
-    with torch.cuda.device(dev):  # (the size depends on the device's compute units)
-        nbytes = lib.pbattn_qk_norm_rope_bwd_workspace_size(sizes[4])
+    nbytes = _workspace_size(sizes[4], dev.index)
     workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    _launch("pbattn_qk_norm_rope_bwd", lib.pbattn_qk_norm_rope_bwd, dev, q.data_ptr(), k.data_ptr(), code, steps,
-            q_weight.data_ptr(), k_weight.data_ptr(), wcode, weight_offset, cos.data_ptr(), sin.data_ptr(), cos.shape[0],
-            positions.data_ptr(), int(positions.dtype == torch.int64), pos_steps, grad_q.data_ptr(), grad_k.data_ptr(),
-            dq.data_ptr(), dk.data_ptr(), dqw.data_ptr(), dkw.data_ptr(), *sizes, eps, int(interleaved),
+    _launch("pbattn_qk_norm_rope_bwd", _lib.attn_lib().pbattn_qk_norm_rope_bwd, dev, *args, grad_q.data_ptr(),
+            grad_k.data_ptr(), dq.data_ptr(), dk.data_ptr(), dqw.data_ptr(), dkw.data_ptr(), *sizes, eps, int(interleaved),
             workspace.data_ptr(), nbytes)
     return dq, dk, dqw, dkw
 
@@ -205,13 +207,13 @@ def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps: float = 1e-
     in reverse mode (a forward-mode tangent raises; the tables get no gradient)."""
     args = (q, k, q_weight, k_weight, cos, sin, positions)
     _no_tangents("qk_norm_rope", *args[:6])
-    _check(*args)
-    if eps < 0 or eps != eps or eps == float("inf"):
+    if not 0 <= eps < float("inf"):
         raise ValueError(f"eps must be a number not below 0, got {eps}")
-    if torch.is_grad_enabled() and (cos.requires_grad or sin.requires_grad):
+    if (cos.requires_grad or sin.requires_grad) and torch.is_grad_enabled():
         raise RuntimeError("qk_norm_rope has no gradient for its tables: detach cos and sin")
-    _one_device(*args)
-    args += (float(eps), float(weight_offset), bool(interleaved))
-    if not _untraced(*args[:7]):
-        return qk_norm_rope_op(*args)
-    return (_QkNormRope.apply if grad_needed(*args[:4]) else _forward)(*args)
+    rest = float(eps), float(weight_offset), bool(interleaved)
+    if not _untraced(*args):
+        _rope_sizes(*_call(*args))
+        _one_device(*args)
+        return qk_norm_rope_op(*args, *rest)
+    return (_QkNormRope.apply if grad_needed(*args[:4]) else _forward)(*args, *rest)
