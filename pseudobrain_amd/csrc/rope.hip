@@ -34,10 +34,11 @@ struct RopeParams {
   const float *cos, *sin;
   const void *pos;
   long pos_batch, pos_token;       // elements
-  float *part;                     // [workgroups][2][D] sums for the weights' gradients
-  long tokens, items;              // tokens of all batch rows; pieces of work of a wave
+  float *part;                     // [workgroups][D] sums for the weights' gradients
+  long tokens;                     // of all batch rows
   int T, H[2], D, R, rows;         // rows: of the angles' tables
-  int split;                       // waves a token's heads are divided over
+  int split[2];                    // waves a token's heads of q, or k, are divided over
+  int blocks_q;                    // workgroups of q; the others are k's
   int wdt, pos64, interleaved;
   float eps, offset;
 };
@@ -128,29 +129,45 @@ __device__ __forceinline__ void turn(float *v, const float *c, const float *s, b
   }
 }
 
+// The workgroup's sums over its waves to its place.
+__device__ __forceinline__ void store_sums(const RopeParams &p, const float (&sums)[ROPE_WAVES][ROPE_MAX_D]) {
+  __syncthreads();
+  for (int i = threadIdx.x; i < p.D; i += ROPE_WAVES * 64) {
+    float y = 0.0f;
+#pragma unroll
+    for (int wave = 0; wave < ROPE_WAVES; ++wave) y += sums[wave][i];
+    p.part[static_cast<long>(blockIdx.x) * p.D + i] = y;
+  }
+}
+
+// Workgroups are q's or k's, so that one set of weights, and in the backward of their
+// sums, is in registers: six waves a SIMD in the forward, four in the backward.
 template <int DT, int G, bool PAIRS, bool BWD>
-__global__ __launch_bounds__(ROPE_WAVES * 64) void rope_kernel(const RopeParams p) {
+__global__ __launch_bounds__(ROPE_WAVES * 64, 4) void rope_kernel(const RopeParams p) {
   using U = Unit<DT>;
   constexpr int E = U::E, ROWS = 64 / G;  // rows of a wave at a time
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), j = lane % G, group = lane / G;
   const int lanes = p.D / (2 * E), half = p.R / (2 * E);  // lanes of a row; those that rotate
   const bool mine = j < lanes, turns = j < half;
   const int u0 = PAIRS ? 2 * j : turns ? j : 2 * j, u1 = PAIRS || !turns ? u0 + 1 : j + half;
-  const int groups_q = (p.H[0] + ROWS - 1) / ROWS, groups = groups_q + (p.H[1] + ROWS - 1) / ROWS;
-  float w[2][2 * E];
+  const bool key = static_cast<int>(blockIdx.x) >= p.blocks_q;
+  const int block = key ? blockIdx.x - p.blocks_q : blockIdx.x, blocks = key ? gridDim.x - p.blocks_q : p.blocks_q;
+  const int heads = key ? p.H[1] : p.H[0], groups = (heads + ROWS - 1) / ROWS, split = key ? p.split[1] : p.split[0];
+  const unsigned char *const x_base = key ? p.x[1] : p.x[0], *const g_base = key ? p.g[1] : p.g[0];
+  unsigned char *const out_base = key ? p.out[1] : p.out[0];
+  const long batch_step = key ? p.batch[1] : p.batch[0], token_step = key ? p.token[1] : p.token[0],
+             head_step = key ? p.head[1] : p.head[0];
+  float w[2 * E];
+  load_weights<E>(key ? p.w[1] : p.w[0], p.wdt, mine ? u0 : 0, p.offset, w);
+  load_weights<E>(key ? p.w[1] : p.w[0], p.wdt, mine ? u1 : 0, p.offset, w + E);
+  float dw[BWD ? 2 * E : 1];
 #pragma unroll
-  for (int x = 0; x < 2; ++x) {
-    load_weights<E>(p.w[x], p.wdt, mine ? u0 : 0, p.offset, w[x]);
-    load_weights<E>(p.w[x], p.wdt, mine ? u1 : 0, p.offset, w[x] + E);
-  }
-  float dw[2][BWD ? 2 * E : 1];
-#pragma unroll
-  for (int i = 0; i < (BWD ? 2 * E : 1); ++i) dw[0][i] = dw[1][i] = 0.0f;
+  for (int i = 0; i < (BWD ? 2 * E : 1); ++i) dw[i] = 0.0f;
 
-  for (long item = blockIdx.x * static_cast<long>(ROPE_WAVES) + wave; item < p.items;
-       item += static_cast<long>(gridDim.x) * ROPE_WAVES) {
-    const long tok = item / p.split;
-    const int first = static_cast<int>(item - tok * p.split);
+  for (long item = block * static_cast<long>(ROPE_WAVES) + wave; item < p.tokens * split;
+       item += static_cast<long>(blocks) * ROPE_WAVES) {
+    const long tok = item / split;
+    const int first = static_cast<int>(item - tok * split);
     const int b = static_cast<int>(tok / p.T), t = static_cast<int>(tok - static_cast<long>(b) * p.T);
     const long row = angle_row(p, b, t);
     const bool known = row >= 0;
@@ -168,36 +185,30 @@ __global__ __launch_bounds__(ROPE_WAVES * 64) void rope_kernel(const RopeParams 
         s[e + i] = y[i];
       }
     }
-    for (int i = first; i < groups; i += p.split) {
-      const bool key = i >= groups_q;  // (the same for the whole wave)
-      const int h = (key ? i - groups_q : i) * ROWS + group, heads = key ? p.H[1] : p.H[0];
+    for (int i = first; i < groups; i += split) {
+      const int h = i * ROWS + group;
       const bool here = mine & (h < heads);
       const long at = (tok * heads + h) * p.D * (16 / E);  // of a dense row, bytes
       v4u32_t a = {0, 0, 0, 0}, d = {0, 0, 0, 0}, ga = {0, 0, 0, 0}, gd = {0, 0, 0, 0};
       if (here & known) {
-        const unsigned char *src = (key ? p.x[1] : p.x[0]) + b * (key ? p.batch[1] : p.batch[0]) +
-                                   t * (key ? p.token[1] : p.token[0]) + h * (key ? p.head[1] : p.head[0]);
+        const unsigned char *src = x_base + b * batch_step + t * token_step + h * head_step;
         a = *reinterpret_cast<const v4u32_t *>(src + u0 * 16);
         d = *reinterpret_cast<const v4u32_t *>(src + u1 * 16);
         if constexpr (BWD) {
-          const unsigned char *g = (key ? p.g[1] : p.g[0]) + at;
-          ga = *reinterpret_cast<const v4u32_t *>(g + u0 * 16);
-          gd = *reinterpret_cast<const v4u32_t *>(g + u1 * 16);
+          ga = *reinterpret_cast<const v4u32_t *>(g_base + at + u0 * 16);
+          gd = *reinterpret_cast<const v4u32_t *>(g_base + at + u1 * 16);
         }
       }
-      float v[2 * E], ww[2 * E];
+      float v[2 * E];
       U::unpack(a, v);
       U::unpack(d, v + E);
       float ss = 0.0f;
 #pragma unroll
-      for (int e = 0; e < 2 * E; ++e) {
-        ss = __builtin_fmaf(v[e], v[e], ss);
-        ww[e] = key ? w[1][e] : w[0][e];
-      }
+      for (int e = 0; e < 2 * E; ++e) ss = __builtin_fmaf(v[e], v[e], ss);
       if constexpr (!BWD) {
         const float r = 1.0f / sqrtf(row_sum<G>(ss) / p.D + p.eps);
 #pragma unroll
-        for (int e = 0; e < 2 * E; ++e) v[e] = v[e] * r * ww[e];
+        for (int e = 0; e < 2 * E; ++e) v[e] = v[e] * r * w[e];
         turn<E, PAIRS, false>(v, c, s, turns);
       } else {
         float g[2 * E];
@@ -206,23 +217,17 @@ __global__ __launch_bounds__(ROPE_WAVES * 64) void rope_kernel(const RopeParams 
         turn<E, PAIRS, true>(g, c, s, turns);
         float ux = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 2 * E; ++e) ux = __builtin_fmaf(g[e] * ww[e], v[e], ux);
+        for (int e = 0; e < 2 * E; ++e) ux = __builtin_fmaf(g[e] * w[e], v[e], ux);
         const float r = 1.0f / sqrtf(row_sum<G>(ss) / p.D + p.eps), f = r * r * (row_sum<G>(ux) / p.D);
         if (here & known) {
 #pragma unroll
-          for (int e = 0; e < 2 * E; ++e) {
-            const float hx = g[e] * (v[e] * r);
-            if (key)
-              dw[1][e] += hx;
-            else
-              dw[0][e] += hx;
-          }
+          for (int e = 0; e < 2 * E; ++e) dw[e] += g[e] * (v[e] * r);
         }
 #pragma unroll
-        for (int e = 0; e < 2 * E; ++e) v[e] = r * (g[e] * ww[e] - v[e] * f);
+        for (int e = 0; e < 2 * E; ++e) v[e] = r * (g[e] * w[e] - v[e] * f);
       }
       if (here) {
-        unsigned char *dst = (key ? p.out[1] : p.out[0]) + at;
+        unsigned char *dst = out_base + at;
         const v4u32_t zero = {0, 0, 0, 0};  // a row without a position
         *reinterpret_cast<v4u32_t *>(dst + u0 * 16) = known ? U::pack(v) : zero;
         *reinterpret_cast<v4u32_t *>(dst + u1 * 16) = known ? U::pack(v + E) : zero;
@@ -230,26 +235,17 @@ __global__ __launch_bounds__(ROPE_WAVES * 64) void rope_kernel(const RopeParams 
     }
   }
   if constexpr (BWD) {
-    __shared__ float sums[ROPE_WAVES][2][ROPE_MAX_D];
+    __shared__ float sums[ROPE_WAVES][ROPE_MAX_D];
     PBGDN_POISON_LDS(sums, sizeof(sums));
     PBGDN_POISON_SYNC();
 #pragma unroll
-    for (int x = 0; x < 2; ++x)
+    for (int e = 0; e < 2 * E; ++e) {
+      float y = dw[e];
 #pragma unroll
-      for (int e = 0; e < 2 * E; ++e) {
-        float y = dw[x][e];
-#pragma unroll
-        for (int off = G; off < 64; off *= 2) y += __shfl_xor(y, off, 64);
-        if (mine & (group == 0)) sums[wave][x][(e < E ? u0 : u1) * E + e % E] = y;
-      }
-    __syncthreads();
-    for (int i = threadIdx.x; i < 2 * p.D; i += ROPE_WAVES * 64) {
-      const int x = i / p.D, col = i - x * p.D;
-      float y = 0.0f;
-#pragma unroll
-      for (int wv = 0; wv < ROPE_WAVES; ++wv) y += sums[wv][x][col];
-      p.part[static_cast<long>(blockIdx.x) * 2 * p.D + i] = y;
+      for (int off = G; off < 64; off *= 2) y += __shfl_xor(y, off, 64);
+      if (mine & (group == 0)) sums[wave][(e < E ? u0 : u1) * E + e % E] = y;
     }
+    store_sums(p, sums);
   }
 }
 
@@ -259,16 +255,18 @@ template <int DT, bool BWD>
 __global__ __launch_bounds__(ROPE_WAVES * 64) void rope_any_kernel(const RopeParams p) {
   constexpr int N = ROPE_MAX_D / 64;
   constexpr int BYTES = DT == PBGDN_F32 ? 4 : 2;
-  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), heads = p.H[0] + p.H[1];
-  float dw[2][N];
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const int key = static_cast<int>(blockIdx.x) >= p.blocks_q, heads = p.H[key];
+  const int block = key ? blockIdx.x - p.blocks_q : blockIdx.x, blocks = key ? gridDim.x - p.blocks_q : p.blocks_q;
+  float dw[N];
 #pragma unroll
-  for (int e = 0; e < N; ++e) dw[0][e] = dw[1][e] = 0.0f;
-  for (long item = blockIdx.x * static_cast<long>(ROPE_WAVES) + wave; item < p.tokens * heads;
-       item += static_cast<long>(gridDim.x) * ROPE_WAVES) {
+  for (int e = 0; e < N; ++e) dw[e] = 0.0f;
+  for (long item = block * static_cast<long>(ROPE_WAVES) + wave; item < p.tokens * heads;
+       item += static_cast<long>(blocks) * ROPE_WAVES) {
     const long tok = item / heads;
-    const int hh = static_cast<int>(item - tok * heads), key = hh >= p.H[0], h = key ? hh - p.H[0] : hh;
+    const int h = static_cast<int>(item - tok * heads);
     const int b = static_cast<int>(tok / p.T), t = static_cast<int>(tok - static_cast<long>(b) * p.T);
-    const long row = angle_row(p, b, t), at = (tok * p.H[key] + h) * p.D;
+    const long row = angle_row(p, b, t), at = item * p.D;
     if (row < 0) {
       for (int i = lane; i < p.D; i += 64) store_elem(p.out[key], at + i, DT, 0.0f);
       continue;
@@ -303,11 +301,7 @@ __global__ __launch_bounds__(ROPE_WAVES * 64) void rope_any_kernel(const RopePar
       const int i = lane + 64 * e;
       if (i >= p.D) continue;
       if constexpr (BWD) {
-        const float hx = y[e] * (v[e] * r);
-        if (key)
-          dw[1][e] += hx;
-        else
-          dw[0][e] += hx;
+        dw[e] += y[e] * (v[e] * r);
         store_elem(p.out[key], at + i, DT, r * (y[e] * weight(i) - v[e] * f));
       } else {
         store_elem(p.out[key], at + i, DT, y[e] * r);
@@ -315,45 +309,42 @@ __global__ __launch_bounds__(ROPE_WAVES * 64) void rope_any_kernel(const RopePar
     }
   }
   if constexpr (BWD) {
-    __shared__ float sums[ROPE_WAVES][2][ROPE_MAX_D];
+    __shared__ float sums[ROPE_WAVES][ROPE_MAX_D];
     PBGDN_POISON_LDS(sums, sizeof(sums));
     PBGDN_POISON_SYNC();
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-      sums[wave][0][lane + 64 * e] = dw[0][e];
-      sums[wave][1][lane + 64 * e] = dw[1][e];
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < 2 * p.D; i += ROPE_WAVES * 64) {
-      const int x = i / p.D, col = i - x * p.D;
-      float y = 0.0f;
-#pragma unroll
-      for (int wv = 0; wv < ROPE_WAVES; ++wv) y += sums[wv][x][col];
-      p.part[static_cast<long>(blockIdx.x) * 2 * p.D + i] = y;
-    }
+    for (int e = 0; e < N; ++e) sums[wave][lane + 64 * e] = dw[e];
+    store_sums(p, sums);
   }
 }
 
-// The weights' gradients from the workgroups' sums, in a fixed order: 64 columns of both
-// a workgroup, each of 16 waves a sixteenth of the sums.
-constexpr int ROPE_JOIN_WAVES = 16;
-__global__ __launch_bounds__(ROPE_JOIN_WAVES * 64) void rope_join_kernel(const float *part, int n, int D, void *dq, void *dk,
-                                                                        int wdt) {
-  __shared__ float sums[ROPE_JOIN_WAVES][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = blockIdx.x * 64 + lane;
+// The weights' gradients from the workgroups' sums, in a fixed order: 16 columns a
+// workgroup, every 64th sum a thread.
+constexpr int JOIN_COLS = 16, JOIN_ROWS = 64;
+__global__ __launch_bounds__(JOIN_COLS * JOIN_ROWS) void rope_join_kernel(const float *part, int blocks_q, int blocks, int D,
+                                                                          void *dq, void *dk, int wdt) {
+  __shared__ float sums[JOIN_ROWS][JOIN_COLS];
+  PBGDN_POISON_LDS(sums, sizeof(sums));
+  PBGDN_POISON_SYNC();
+  const int tiles = (D + JOIN_COLS - 1) / JOIN_COLS;
+  const bool key = static_cast<int>(blockIdx.x) >= tiles;
+  const int c = threadIdx.x % JOIN_COLS, r = threadIdx.x / JOIN_COLS;
+  const int col = (key ? blockIdx.x - tiles : blockIdx.x) * JOIN_COLS + c, end = key ? blocks : blocks_q;
   float x = 0.0f;
-  if (col < 2 * D)
-    for (int i = wave; i < n; i += ROPE_JOIN_WAVES) x += part[static_cast<long>(i) * 2 * D + col];
-  sums[wave][lane] = x;
-  __syncthreads();
-  if (wave != 0 || col >= 2 * D) return;
-  x = 0.0f;
+  if (col < D) {
+#pragma unroll 8
+    for (int i = (key ? blocks_q : 0) + r; i < end; i += JOIN_ROWS) x += part[static_cast<long>(i) * D + col];
+  }
+  sums[r][c] = x;
 #pragma unroll
-  for (int w = 0; w < ROPE_JOIN_WAVES; ++w) x += sums[w][lane];
-  store_elem(col < D ? dq : dk, col < D ? col : col - D, wdt, x);
+  for (int n = JOIN_ROWS / 2; n > 0; n /= 2) {
+    __syncthreads();
+    if (r < n) sums[r][c] += sums[r + n][c];
+  }
+  if (r == 0 && col < D) store_elem(key ? dk : dq, col, wdt, sums[0][c]);
 }
 
-// Workgroups of the backward: four a CU, the most whose sums are kept.
+// Most workgroups of the backward: as many as the GPU holds at once, four a CU.
 static long rope_bwd_blocks() {
   DeviceShape shape;
   if (!device_shape(shape)) shape.cus = 256;
@@ -421,36 +412,50 @@ static bool rope_units(const RopeParams &p, int dtype, std::initializer_list<con
   return true;
 }
 
+// Workgroups for items of q and of k: one for every four, or, where that is more than
+// `most`, as many of them as their share of the work; at least one each.
+static unsigned rope_blocks(RopeParams &p, long items_q, long items_k, long most) {
+  long nq = (items_q + ROPE_WAVES - 1) / ROPE_WAVES, nk = (items_k + ROPE_WAVES - 1) / ROPE_WAVES;
+  if (nq + nk > most) {
+    nq = most * p.H[0] / (p.H[0] + p.H[1]);
+    nq = nq < 1 ? 1 : nq < most ? nq : most - 1;
+    nk = most - nq;
+  }
+  p.blocks_q = static_cast<int>(nq);
+  return static_cast<unsigned>(nq + nk);
+}
+
 template <bool BWD>
-static int launch_rope(RopeParams &p, int dtype, bool units, long most, int &blocks, hipStream_t stream) {
-  const auto go = [&](auto kernel, long items) {
-    const long want = (items + ROPE_WAVES - 1) / ROPE_WAVES, n = want < most ? want : most;
-    blocks = static_cast<int>(n);
-    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(n)), dim3(ROPE_WAVES * 64), 0, stream, p);
+static int launch_rope(RopeParams &p, int dtype, bool units, long most, unsigned &blocks, hipStream_t stream) {
+  const auto go = [&](auto kernel, long items_q, long items_k) {
+    blocks = rope_blocks(p, items_q, items_k, most);
+    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(ROPE_WAVES * 64), 0, stream, p);
   };
   if (!units) {
-    const long items = p.tokens * (p.H[0] + p.H[1]);
+    const long nq = p.tokens * p.H[0], nk = p.tokens * p.H[1];
     switch (dtype) {
-      case PBGDN_F32: go(rope_any_kernel<PBGDN_F32, BWD>, items); break;
-      case PBGDN_BF16: go(rope_any_kernel<PBGDN_BF16, BWD>, items); break;
-      default: go(rope_any_kernel<PBGDN_F16, BWD>, items); break;
+      case PBGDN_F32: go(rope_any_kernel<PBGDN_F32, BWD>, nq, nk); break;
+      case PBGDN_BF16: go(rope_any_kernel<PBGDN_BF16, BWD>, nq, nk); break;
+      default: go(rope_any_kernel<PBGDN_F16, BWD>, nq, nk); break;
     }
     return hipGetLastError() == hipSuccess ? PBGDN_OK : PBGDN_ERR_LAUNCH;
   }
   const int lanes = p.D / (dtype == PBGDN_F32 ? 8 : 16);
   const auto by_pairs = [&](auto DT, auto G) {
     constexpr int dt = decltype(DT)::value, g = decltype(G)::value, rows = 64 / g;
-    const int groups = (p.H[0] + rows - 1) / rows + (p.H[1] + rows - 1) / rows;
-    // a token's heads on as many waves as it takes to have 16 a CU
+    // a token's heads on as many pieces as it takes to have 16 a CU, in the backward, whose
+    // workgroups take piece after piece, 64: its last round is then a small part
     DeviceShape shape;
     if (!device_shape(shape)) shape.cus = 256;
-    const long want = (16L * shape.cus + p.tokens - 1) / p.tokens;
-    p.split = static_cast<int>(want < groups ? want : groups);
-    p.items = p.tokens * p.split;
+    const long want = ((BWD ? 64L : 16L) * shape.cus + p.tokens - 1) / p.tokens;
+    for (int a = 0; a < 2; ++a) {
+      const int groups = (p.H[a] + rows - 1) / rows;
+      p.split[a] = static_cast<int>(want < groups ? want : groups);
+    }
     if (p.interleaved)
-      go(rope_kernel<dt, g, true, BWD>, p.items);
+      go(rope_kernel<dt, g, true, BWD>, p.tokens * p.split[0], p.tokens * p.split[1]);
     else
-      go(rope_kernel<dt, g, false, BWD>, p.items);
+      go(rope_kernel<dt, g, false, BWD>, p.tokens * p.split[0], p.tokens * p.split[1]);
   };
   const auto by_lanes = [&](auto DT) {
     if (lanes <= 4)
@@ -488,12 +493,12 @@ extern "C" int pbattn_qk_norm_rope(const void *q, const void *k, int dtype, cons
   hipStream_t s = static_cast<hipStream_t>(stream);
   debug_poison(q_out, static_cast<size_t>(p.tokens) * Hq * D * attn_bytes(dtype), s);
   debug_poison(k_out, static_cast<size_t>(p.tokens) * Hk * D * attn_bytes(dtype), s);
-  int blocks;
+  unsigned blocks;
   return launch_rope<false>(p, dtype, rope_units(p, dtype, {q, k, q_weight, k_weight, cos, sin}), 0x7fffffffL / 64, blocks, s);
 }
 
 extern "C" size_t pbattn_qk_norm_rope_bwd_workspace_size(int D) {
-  return D > 0 && D <= pbgdn::ROPE_MAX_D ? static_cast<size_t>(pbgdn::rope_bwd_blocks()) * 2 * D * sizeof(float) : 0;
+  return D > 0 && D <= pbgdn::ROPE_MAX_D ? static_cast<size_t>(pbgdn::rope_bwd_blocks()) * D * sizeof(float) : 0;
 }
 
 extern "C" int pbattn_qk_norm_rope_bwd(const void *q, const void *k, int dtype, const int64_t *strides, const void *q_weight,
@@ -521,11 +526,11 @@ extern "C" int pbattn_qk_norm_rope_bwd(const void *q, const void *k, int dtype, 
   debug_poison(dq, static_cast<size_t>(p.tokens) * Hq * D * attn_bytes(dtype), s);
   debug_poison(dk, static_cast<size_t>(p.tokens) * Hk * D * attn_bytes(dtype), s);
   debug_poison(workspace, pbattn_qk_norm_rope_bwd_workspace_size(D), s);
-  int blocks = 0;
+  unsigned blocks = 0;
   const int launched = launch_rope<true>(p, dtype, rope_units(p, dtype, {q, k, q_weight, k_weight, cos, sin}),
                                          rope_bwd_blocks(), blocks, s);
   if (launched != PBGDN_OK) return launched;
-  hipLaunchKernelGGL(rope_join_kernel, dim3((2 * D + 63) / 64), dim3(ROPE_JOIN_WAVES * 64), 0, s, p.part, blocks, D, dq_weight,
-                     dk_weight, weight_dtype);
+  hipLaunchKernelGGL(rope_join_kernel, dim3(2 * ((D + JOIN_COLS - 1) / JOIN_COLS)), dim3(JOIN_COLS * JOIN_ROWS), 0, s, p.part,
+                     p.blocks_q, static_cast<int>(blocks), D, dq_weight, dk_weight, weight_dtype);
   return hipGetLastError() == hipSuccess ? PBGDN_OK : PBGDN_ERR_LAUNCH;
 }
