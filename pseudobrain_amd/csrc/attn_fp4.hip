@@ -202,10 +202,14 @@ __device__ __forceinline__ void wave_lds_order() {
 // result's lane groups.
 __device__ __forceinline__ int key_of(int m) { return 4 * (m % 4) + m / 4; }
 
+// Workgroups of a CU at once (waves of a SIMD), by the registers that the sums of RB row
+// tiles and two blocks of keys and values take.
+constexpr int fp4_held(int D, int RB) { return RB == 2 || D == 256 ? 2 : D == 128 ? 3 : 4; }
+
 // NEAR: the caches' offsets fit 32 bits. ONCE: no other row tile reads the cache, so that
 // keys are loaded past the caches (values not: a row's are fetched in pieces).
 template <int DT, int D, int RB, bool NEAR, bool ONCE>
-__global__ __launch_bounds__(DEC_WAVES * 64, 2) void fp4_decode_kernel(const Fp4DecodeParams pp) {
+__global__ __launch_bounds__(DEC_WAVES * 64, (fp4_held(D, RB))) void fp4_decode_kernel(const Fp4DecodeParams pp) {
   using K = Fp4<DT, D>;
   using E = Elem<PBGDN_BF16>;
   constexpr int KS = K::KSTEPS, OT = K::OT, KG = K::KG, KEYS = K::KEYS, N = K::N;
@@ -712,7 +716,7 @@ __device__ __forceinline__ void store8(unsigned char *dst, uint32_t w, float sca
 
 template <int DT>
 __global__ __launch_bounds__(SCAN_THREADS) void fp4_read_kernel(const Fp4ReadParams p) {
-  constexpr int BYTES = DT == PBGDN_F32 ? 4 : 2;
+  constexpr int BYTES = DT == PBGDN_F32 ? 4 : 2, AT_ONCE = 4;
   __shared__ int start[MAX_REQUESTS];
   __shared__ long waves[SCAN_WAVES], rows[READ_TOKENS];
   PBGDN_POISON_LDS(start, sizeof(start));
@@ -742,21 +746,32 @@ __global__ __launch_bounds__(SCAN_THREADS) void fp4_read_kernel(const Fp4ReadPar
     rows[threadIdx.x] = row;
   }
   __syncthreads();
-  const int per = p.Hk * p.eighths;
-  for (int i = threadIdx.x; i < n * per; i += SCAN_THREADS) {
-    const int tok = i / per, x = i - tok * per, hd = x / p.eighths, u = x - hd * p.eighths;
-    const long row = rows[tok];
-    uint32_t k = 0, v = 0, ks = 127, vs = 127;
-    if (row >= 0) {
-      const long from = row + hd * p.cache.head, scales = from / 16 + u / 4;
-      k = __builtin_nontemporal_load(reinterpret_cast<const uint32_t *>(p.cache.k + from + u * 4));
-      v = __builtin_nontemporal_load(reinterpret_cast<const uint32_t *>(p.cache.v + from + u * 4));
-      ks = p.cache.k_scale[scales];
-      vs = p.cache.v_scale[scales];
+  const int per = p.Hk * p.eighths, end = n * per;
+  for (int i0 = threadIdx.x; i0 < end; i0 += AT_ONCE * SCAN_THREADS) {
+    uint32_t k[AT_ONCE], v[AT_ONCE], ks[AT_ONCE], vs[AT_ONCE];
+#pragma unroll
+    for (int j = 0; j < AT_ONCE; ++j) {
+      const int i = i0 + j * SCAN_THREADS, tok = i < end ? i / per : 0, x = i - tok * per;
+      const int hd = x / p.eighths, u = x - hd * p.eighths;
+      const long row = i < end ? rows[tok] : -1;
+      k[j] = v[j] = 0;
+      ks[j] = vs[j] = 127;
+      if (row >= 0) {
+        const long from = row + hd * p.cache.head, scales = from / 16 + u / 4;
+        k[j] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t *>(p.cache.k + from + u * 4));
+        v[j] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t *>(p.cache.v + from + u * 4));
+        ks[j] = p.cache.k_scale[scales];
+        vs[j] = p.cache.v_scale[scales];
+      }
     }
-    const long to = (static_cast<long>(first + tok) * per + x) * (8 * BYTES);
-    store8<DT>(static_cast<unsigned char *>(p.k) + to, k, fp4_scale(ks));
-    store8<DT>(static_cast<unsigned char *>(p.v) + to, v, fp4_scale(vs));
+#pragma unroll
+    for (int j = 0; j < AT_ONCE; ++j) {
+      const int i = i0 + j * SCAN_THREADS;
+      if (i >= end) break;
+      const long to = (static_cast<long>(first) * per + i) * (8 * BYTES);
+      store8<DT>(static_cast<unsigned char *>(p.k) + to, k[j], fp4_scale(ks[j]));
+      store8<DT>(static_cast<unsigned char *>(p.v) + to, v[j], fp4_scale(vs[j]));
+    }
   }
 }
 
@@ -769,8 +784,7 @@ static int fp4_target(int Hk, int rows, int D) {
   DeviceShape shape;
   if (!device_shape(shape)) shape.cus = 256;
   const int rb = fp4_row_tiles(D, rows), tiles = (rows + rb * DEC_ROWS - 1) / (rb * DEC_ROWS);
-  const int held = rb == 1 && D < 256 ? 3 : 2;  // of a CU
-  const long t = static_cast<long>(held) * shape.cus / (static_cast<long>(Hk) * tiles);
+  const long t = static_cast<long>(fp4_held(D, rb)) * shape.cus / (static_cast<long>(Hk) * tiles);
   return t > 1 ? static_cast<int>(t) : 1;
 }
 
@@ -973,10 +987,10 @@ extern "C" int pbattn_fp4_read(const void *k_cache, const void *v_cache, const v
   p.Hk = Hk;
   p.eighths = D / 8;
   p.num_pages = num_pages;
-  // Tokens of a workgroup: as many as leave the GPU four workgroups a CU, READ_TOKENS at most.
+  // Tokens of a workgroup: as many as leave the GPU eight workgroups a CU, READ_TOKENS at most.
   DeviceShape shape;
   if (!device_shape(shape)) shape.cus = 256;
-  const int even = (tokens + 4 * shape.cus - 1) / (4 * shape.cus);
+  const int even = (tokens + 8 * shape.cus - 1) / (8 * shape.cus);
   p.per_block = even < 1 ? 1 : even > READ_TOKENS ? READ_TOKENS : even;
   if (static_cast<long>(p.per_block) * Hk * p.eighths > 0x7fffffffL) return PBGDN_ERR_UNSUPPORTED;
   const int blocks = (tokens + p.per_block - 1) / p.per_block;
