@@ -793,7 +793,7 @@ static int launch_fp4(Fp4DecodeParams &p, hipStream_t stream) {
   const int rb = fp4_row_tiles(D, p.d.rows);
   p.d.row_tiles = (p.d.rows + rb * DEC_ROWS - 1) / (rb * DEC_ROWS);
   const long blocks = (p.d.target + 7L) / 8 * 8 * p.d.Hk * p.d.row_tiles;
-  if (blocks > 0x7fffffffL || static_cast<long>(p.d.B) * p.d.Hk * p.d.rows > 0x7fffffffL) return PBGDN_ERR_UNSUPPORTED;
+  if (blocks > 0xffffffL || static_cast<long>(p.d.B) * p.d.Hk * p.d.rows > 0x7fffffffL) return PBGDN_ERR_UNSUPPORTED;
   const auto run = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(DEC_WAVES * 64), 0, stream, p);
   };

@@ -24,6 +24,7 @@ namespace pbgdn {
 
 constexpr int ROPE_WAVES = 4;
 constexpr int ROPE_MAX_D = 256;
+constexpr long ROPE_MOST = 1 << 20;  // workgroups of a launch; waves take piece after piece where there are more
 
 struct RopeParams {
   const unsigned char *x[2];       // q, k
@@ -494,7 +495,7 @@ extern "C" int pbattn_qk_norm_rope(const void *q, const void *k, int dtype, cons
   debug_poison(q_out, static_cast<size_t>(p.tokens) * Hq * D * attn_bytes(dtype), s);
   debug_poison(k_out, static_cast<size_t>(p.tokens) * Hk * D * attn_bytes(dtype), s);
   unsigned blocks;
-  return launch_rope<false>(p, dtype, rope_units(p, dtype, {q, k, q_weight, k_weight, cos, sin}), 0x7fffffffL / 64, blocks, s);
+  return launch_rope<false>(p, dtype, rope_units(p, dtype, {q, k, q_weight, k_weight, cos, sin}), ROPE_MOST, blocks, s);
 }
 
 extern "C" size_t pbattn_qk_norm_rope_bwd_workspace_size(int D) {

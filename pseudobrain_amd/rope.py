@@ -111,13 +111,19 @@ def _workspace_size(width: int, device_index: int) -> int:
         return _lib.attn_lib().pbattn_qk_norm_rope_bwd_workspace_size(width)
 
 
+def _gradient(x, grad):
+    """The gradient of a result as the kernel reads it: dense, in x's dtype."""
+    if grad.shape != x.shape:
+        raise ValueError("grad_q and grad_k must have q's and k's shapes")
+    return _aligned((grad if grad.dtype == x.dtype else grad.to(x.dtype)).contiguous(), 16)
+
+
 def _backward(q, k, q_weight, k_weight, cos, sin, positions, grad_q, grad_k, eps, weight_offset, interleaved):
     dev, sizes, kept, args = _operands(q, k, q_weight, k_weight, cos, sin, positions, weight_offset)
     _one_device(q, grad_q, grad_k)
-    if grad_q.shape != q.shape or grad_k.shape != k.shape:
-        raise ValueError("grad_q and grad_k must have q's and k's shapes")
-    grad_q, grad_k = (_aligned(x.to(q.dtype).contiguous(), 16) for x in (grad_q, grad_k))
-    dq, dk, dqw, dkw = (x.new_empty(x.shape) for x in (q, k, q_weight, k_weight))
+    grad_q, grad_k = _gradient(q, grad_q), _gradient(k, grad_k)
+    dq, dk = q.new_empty(q.shape), k.new_empty(k.shape)
+    dqw, dkw = q_weight.new_empty(sizes[4]), k_weight.new_empty(sizes[4])
     if sizes[0] == 0 or sizes[1] == 0:
         return dq, dk, dqw.zero_(), dkw.zero_()
     nbytes = _workspace_size(sizes[4], dev.index)

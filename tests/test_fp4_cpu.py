@@ -57,6 +57,22 @@ def test_ties_scales_and_ends():
     assert data[0, 0] == 0x06 and data[8, 0] == 0x0f  # value 0 in the lower half; a negative value's code
 
 
+def test_pages_by_multiplication():
+    """The decoding kernel's j / page: the upper half of 2 j m, shifted, is the quotient for
+    every 0 <= j < 2^31 (shown by j at and around multiples of the page, and at the ends)."""
+    rng = np.random.default_rng(3)
+    pages = [1, 2, 3, 7, 16, 100, 528, 4097, 2 ** 20 - 1, 2 ** 30 + 1, 2 ** 31 - 1, *rng.integers(1, 2 ** 31, 200).tolist()]
+    for page in pages:
+        shift = (page - 1).bit_length()
+        m = (1 << (31 + shift)) // page + 1
+        assert m < 2 ** 32
+        top = (2 ** 31 - 1) // page * page
+        some = [x * page for x in rng.integers(0, top // page + 1, 50).tolist()]
+        for j in {0, 1, 2 ** 31 - 1, *(x + d for x in (top, *some) for d in (-1, 0, 1))}:
+            if 0 <= j < 2 ** 31:
+                assert ((2 * j * m) >> 32) >> shift == j // page
+
+
 # ----------------------------------------------------------------------------
 # The C ABI.
 # ----------------------------------------------------------------------------

@@ -112,6 +112,10 @@ def test_large_batches():
     lengths = [(i * 37) % 200 for i in range(300)]
     x = make(lengths, 16, 4, 2, 64, 1, torch.bfloat16, 22)
     check("batch of 300", *x, 0.125)
+    lengths = [(i * 37) % 23 for i in range(1500)]
+    lengths[700], lengths[1499] = 3000, 1000
+    x = make(lengths, 16, 4, 2, 64, 1, torch.bfloat16, 23)
+    check("batch of 1500", *x, 0.125)
 
 
 def test_large_and_small_rows_of_float32_and_float16():
