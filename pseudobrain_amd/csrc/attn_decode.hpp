@@ -157,16 +157,18 @@ __device__ __forceinline__ float max_rows(float x) {
   return fmaxf(a, b);
 }
 // The waves' running sums o (scores' maxima m, weights' sums l) into wave 0's: the
-// upper half into the lower, or one by one where JOINS is 1. Element 4 g + i of o's
+// upper half into the lower, or one by one where JOINS is 1. With HEADS = 2 the waves of
+// each parity are a head's of their own and end in waves 0 and 1. Element 4 g + i of o's
 // columns j lies in element i of o[.][j]; every lane of a column holds m and l.
-template <int RB, int D, int JOINS>
+template <int RB, int D, int JOINS, int HEADS = 1>
 __device__ __forceinline__ void join_waves(float (&merge)[JOINS][RB * DEC_ROWS * (D + 2)], float (&m)[RB], float (&l)[RB],
                                            float4_t (&o)[RB][D / 16], int wave, int lane, float pc) {
   constexpr int OT = D / 16;
   const int c = lane & 15, g = lane >> 4;
 #pragma unroll
   for (int r = 0; r < RB; ++r) l[r] = add_xor32(add_xor16(l[r]));
-  constexpr int ROUNDS = JOINS == 2 ? 2 : DEC_WAVES - 1;
+  static_assert(HEADS == 1 || (HEADS == 2 && JOINS == 2), "pairs of waves are joined");
+  constexpr int ROUNDS = JOINS == 2 ? 3 - HEADS : DEC_WAVES - 1;
 #pragma unroll
   for (int round = 0; round < ROUNDS; ++round) {
     const int from = JOINS == 2 ? DEC_WAVES / 2 >> round : round + 1, count = JOINS == 2 ? from : 1;

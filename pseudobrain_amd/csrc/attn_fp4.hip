@@ -206,22 +206,24 @@ __device__ __forceinline__ int key_of(int m) { return 4 * (m % 4) + m / 4; }
 // tiles and two blocks of keys and values take.
 constexpr int fp4_held(int D, int RB) { return RB == 2 || D == 256 ? 2 : D == 128 ? 3 : 4; }
 
-// NEAR: the caches' offsets fit 32 bits. ONCE: no other row tile reads the cache, so that
-// keys are loaded past the caches (values not: a row's are fetched in pieces).
-template <int DT, int D, int RB, bool NEAR, bool ONCE>
+// NEAR: the caches' offsets fit 32 bits. ONCE: no other workgroup reads the same lines, so
+// that keys are loaded past the caches (values not: a row's are fetched in pieces). HEADS:
+// key heads of a workgroup, whose waves they share by parity: two where the rows of
+// neighbouring heads lie side by side, and are so fetched together.
+template <int DT, int D, int RB, bool NEAR, bool ONCE, int HEADS>
 __global__ __launch_bounds__(DEC_WAVES * 64, (fp4_held(D, RB))) void fp4_decode_kernel(const Fp4DecodeParams pp) {
   using K = Fp4<DT, D>;
   using E = Elem<PBGDN_BF16>;
   constexpr int KS = K::KSTEPS, OT = K::OT, KG = K::KG, KEYS = K::KEYS, N = K::N;
-  constexpr int JOINS = RB * D <= 256 ? 2 : 1;
+  constexpr int JOINS = RB * D <= 256 ? 2 : 1, HW = DEC_WAVES / HEADS;  // HW: waves of a head
   __shared__ __attribute__((aligned(16))) float merge[JOINS][RB * DEC_ROWS * (D + 2)];
-  __shared__ v4u32_t q_lds[RB * N * KS * 64];  // [row tile][part][step][lane]
+  __shared__ v4u32_t q_of[HEADS][RB * N * KS * 64];  // [row tile][part][step][lane]
   __shared__ struct {
     __attribute__((aligned(16))) uint32_t at[KEYS];
     unsigned char scales[2 * KEYS * K::SROW];  // of the keys, then of the values
   } lds_keys[DEC_WAVES];
   PBGDN_POISON_LDS(merge, sizeof(merge));
-  PBGDN_POISON_LDS(q_lds, sizeof(q_lds));
+  PBGDN_POISON_LDS(q_of, sizeof(q_of));
   PBGDN_POISON_LDS(lds_keys, sizeof(lds_keys));
   PBGDN_POISON_SYNC();
   const DecodeParams &p = pp.d;
@@ -230,9 +232,11 @@ __global__ __launch_bounds__(DEC_WAVES * 64, (fp4_held(D, RB))) void fp4_decode_
   // Workgroups go to the XCDs in turn: the heads and row tiles of a piece follow each
   // other on one XCD, whose L2 they share (rows of a token next to each other lie in one
   // line; row tiles read the same ones).
-  const int heads = p.Hk * p.row_tiles, turn = blockIdx.x >> 3;
-  const int w = uniform(turn / heads * 8 + (blockIdx.x & 7)), id = turn - turn / heads * heads;
-  const int row0 = uniform(id / p.Hk) * (RB * DEC_ROWS), hk = uniform(id % p.Hk);
+  const int groups = p.Hk / HEADS, pieces = groups * p.row_tiles, turn = blockIdx.x >> 3;
+  const int w = uniform(turn / pieces * 8 + (blockIdx.x & 7)), id = turn - turn / pieces * pieces;
+  const int row0 = uniform(id / groups) * (RB * DEC_ROWS), hk = uniform(id % groups * HEADS + wave % HEADS);
+  const int hw = wave / HEADS;  // this wave among its head's
+  v4u32_t *const q_lds = q_of[wave % HEADS];
   const Walk walk(p, thread);
   const long x_end = (w + 1) * walk.per < walk.total ? (w + 1) * walk.per : walk.total;
   long x_at = w * walk.per, start;
@@ -252,7 +256,7 @@ __global__ __launch_bounds__(DEC_WAVES * 64, (fp4_held(D, RB))) void fp4_decode_
     const int slot = w + b;
     x_at = start + quad1;
     start += quads;
-    // this wave's KEYS-wide blocks of the part: begin + wave, then every DEC_WAVES-th
+    // this wave's KEYS-wide blocks of the part: begin + hw, then every HW-th
     static_assert(KEYS == DEC_KEYS, "quads are of such blocks");
     const int blocks = (range.count + KEYS - 1) / KEYS, begin = quad0 * DEC_WAVES;
     const int end = uniform(quad1 * DEC_WAVES < blocks ? quad1 * DEC_WAVES : blocks);
@@ -267,7 +271,7 @@ __global__ __launch_bounds__(DEC_WAVES * 64, (fp4_held(D, RB))) void fp4_decode_
       const int t = rr / p.group;
       pos[r] = len - p.T + t;
       const unsigned char *src = p.q + ((static_cast<long>(b) * p.T + t) * p.Hq + hk * p.group + rr - t * p.group) * (D * QB);
-      for (int s = wave; s < KS; s += DEC_WAVES) {
+      for (int s = hw; s < KS; s += HW) {
         const unsigned char *eight = src + K::column(g, s) * QB;
         v4u32_t part[N];
         if constexpr (DT == PBGDN_BF16) {
@@ -392,7 +396,7 @@ __global__ __launch_bounds__(DEC_WAVES * 64, (fp4_held(D, RB))) void fp4_decode_
     const auto step = [&](int blk, Block &cur, Block &next, auto last) __attribute__((always_inline)) {
       constexpr bool more = !decltype(last)::value;
       if constexpr (more) {
-        const Place after = lookup(blk + 2 * DEC_WAVES);
+        const Place after = lookup(blk + 2 * HW);
         load(next, pl);
         pl = after;
       }
@@ -534,19 +538,19 @@ __global__ __launch_bounds__(DEC_WAVES * 64, (fp4_held(D, RB))) void fp4_decode_
         pair_of_tiles(std::integral_constant<int, 7>{});
       }
     };
-    if (begin + wave < end) {
+    if (begin + hw < end) {
       Block x, y;
-      const Place first = lookup(begin + wave);
-      pl = lookup(begin + wave + DEC_WAVES);
+      const Place first = lookup(begin + hw);
+      pl = lookup(begin + hw + HW);
       load(x, first);
-      int blk = begin + wave;
-      for (; blk + 2 * DEC_WAVES < end; blk += 2 * DEC_WAVES) {
+      int blk = begin + hw;
+      for (; blk + 2 * HW < end; blk += 2 * HW) {
         step(blk, x, y, std::false_type{});
-        step(blk + DEC_WAVES, y, x, std::false_type{});
+        step(blk + HW, y, x, std::false_type{});
       }
-      if (blk + DEC_WAVES < end) {
+      if (blk + HW < end) {
         step(blk, x, y, std::false_type{});
-        step(blk + DEC_WAVES, y, x, std::true_type{});
+        step(blk + HW, y, x, std::true_type{});
       } else {
         step(blk, x, y, std::true_type{});
       }
@@ -569,7 +573,7 @@ __global__ __launch_bounds__(DEC_WAVES * 64, (fp4_held(D, RB))) void fp4_decode_
         const int row = row0 + r * DEC_ROWS + c, rr = row < p.rows ? row : p.rows - 1, t = rr / p.group;
         const unsigned char *qrow = p.q + ((static_cast<long>(b) * p.T + t) * p.Hq + hk * p.group + rr - t * p.group) * (D * QB);
         const float base = m[r] == -INFINITY ? 0.0f : m[r], sign = p.negate ? -1.0f : 1.0f;
-        for (int at = begin + wave; at < end; at += DEC_WAVES) {
+        for (int at = begin + hw; at < end; at += HW) {
           const Place mine = lookup(at);
           const uint64_t held = __ballot(exists(mine));
           const int steps = static_cast<int>(distance(mine));
@@ -614,8 +618,8 @@ __global__ __launch_bounds__(DEC_WAVES * 64, (fp4_held(D, RB))) void fp4_decode_
       }
     }
     const int lane_ = static_cast<int>(opaque(thread));
-    join_waves<RB, D, JOINS>(merge, m, l, o, wave, lane_, p.c);
-    if (wave == 0) store_decoded<DT, D, RB, OT>(p, alone, b, hk, row0, slot, lane_, m, l, o);
+    join_waves<RB, D, JOINS, HEADS>(merge, m, l, o, wave, lane_, p.c);
+    if (wave < HEADS) store_decoded<DT, D, RB, OT>(p, alone, b, hk, row0, slot, lane_, m, l, o);
   }
 }
 
@@ -779,36 +783,47 @@ __global__ __launch_bounds__(SCAN_THREADS) void fp4_read_kernel(const Fp4ReadPar
 // within those of two waves a SIMD.
 static int fp4_row_tiles(int D, int rows) { return rows > DEC_ROWS && D < 256 ? 2 : 1; }
 
-// Workgroups of a (row tile, key head): together as many as the GPU holds at once.
-static int fp4_target(int Hk, int rows, int D) {
+// Key heads of a workgroup: two where the rows of neighbouring heads lie side by side and
+// are shorter than a line. Rows in token order, times with one head and with two: 64
+// contexts up to 8,192 tokens, 8 heads of 64, 66 and 49 us; 16 up to 4,000, 16 heads of
+// 128, 38.5 and 33; 64 up to 16,384, 8 heads of 128, 155 and 152 (142 with four, which took
+// 4% longer in the others; heads before tokens 106: memory gives more in longer runs).
+static int fp4_heads(int Hk, int rows, int D, bool beside) {
+  return beside && D < 256 && rows <= DEC_ROWS && Hk % 2 == 0 ? 2 : 1;
+}
+
+// Workgroups of a row tile and `heads` key heads: together as many as the GPU holds at once.
+static int fp4_target(int Hk, int rows, int D, int heads) {
   DeviceShape shape;
   if (!device_shape(shape)) shape.cus = 256;
   const int rb = fp4_row_tiles(D, rows), tiles = (rows + rb * DEC_ROWS - 1) / (rb * DEC_ROWS);
-  const long t = static_cast<long>(fp4_held(D, rb)) * shape.cus / (static_cast<long>(Hk) * tiles);
+  const long t = static_cast<long>(fp4_held(D, rb)) * shape.cus / (static_cast<long>(Hk / heads) * tiles);
   return t > 1 ? static_cast<int>(t) : 1;
 }
 
 template <int DT, int D, bool NEAR>
-static int launch_fp4(Fp4DecodeParams &p, hipStream_t stream) {
+static int launch_fp4(Fp4DecodeParams &p, int heads, hipStream_t stream) {
   const int rb = fp4_row_tiles(D, p.d.rows);
   p.d.row_tiles = (p.d.rows + rb * DEC_ROWS - 1) / (rb * DEC_ROWS);
-  const long blocks = (p.d.target + 7L) / 8 * 8 * p.d.Hk * p.d.row_tiles;
+  const long blocks = (p.d.target + 7L) / 8 * 8 * (p.d.Hk / heads) * p.d.row_tiles;
   if (blocks > 0xffffffL || static_cast<long>(p.d.B) * p.d.Hk * p.d.rows > 0x7fffffffL) return PBGDN_ERR_UNSUPPORTED;
   const auto run = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(DEC_WAVES * 64), 0, stream, p);
   };
   if constexpr (D == 256) {
     if (p.d.row_tiles == 1 && NEAR)
-      run(fp4_decode_kernel<DT, D, 1, NEAR, NEAR>);
+      run(fp4_decode_kernel<DT, D, 1, NEAR, NEAR, 1>);
     else
-      run(fp4_decode_kernel<DT, D, 1, NEAR, false>);
+      run(fp4_decode_kernel<DT, D, 1, NEAR, false, 1>);
   } else {
-    if (rb == 1)
-      run(fp4_decode_kernel<DT, D, 1, NEAR, NEAR>);
+    if (NEAR && heads == 2)
+      run(fp4_decode_kernel<DT, D, 1, NEAR, false, NEAR ? 2 : 1>);
+    else if (rb == 1)
+      run(fp4_decode_kernel<DT, D, 1, NEAR, NEAR, 1>);
     else if (p.d.row_tiles == 1 && NEAR)
-      run(fp4_decode_kernel<DT, D, 2, NEAR, NEAR>);
+      run(fp4_decode_kernel<DT, D, 2, NEAR, NEAR, 1>);
     else
-      run(fp4_decode_kernel<DT, D, 2, NEAR, false>);
+      run(fp4_decode_kernel<DT, D, 2, NEAR, false, 1>);
   }
   // Four waves a row where a sequence may have more parts than one fetches at once; else
   // eight rows a workgroup, which all take the same sums over the lengths.
@@ -817,16 +832,16 @@ static int launch_fp4(Fp4DecodeParams &p, hipStream_t stream) {
 }
 
 template <int DT, bool NEAR>
-static int dispatch_fp4(Fp4DecodeParams &p, int D, hipStream_t stream) {
+static int dispatch_fp4(Fp4DecodeParams &p, int D, int heads, hipStream_t stream) {
   switch (D) {
-    case 64: return launch_fp4<DT, 64, NEAR>(p, stream);
-    case 128: return launch_fp4<DT, 128, NEAR>(p, stream);
-    default: return launch_fp4<DT, 256, NEAR>(p, stream);
+    case 64: return launch_fp4<DT, 64, NEAR>(p, heads, stream);
+    case 128: return launch_fp4<DT, 128, NEAR>(p, heads, stream);
+    default: return launch_fp4<DT, 256, NEAR>(p, heads, stream);
   }
 }
 template <int DT>
-static int dispatch_fp4(Fp4DecodeParams &p, int D, bool near, hipStream_t stream) {
-  return near ? dispatch_fp4<DT, true>(p, D, stream) : dispatch_fp4<DT, false>(p, D, stream);
+static int dispatch_fp4(Fp4DecodeParams &p, int D, bool near, int heads, hipStream_t stream) {
+  return near ? dispatch_fp4<DT, true>(p, D, heads, stream) : dispatch_fp4<DT, false>(p, D, heads, stream);
 }
 
 static bool fp4_width(int D) { return D == 64 || D == 128 || D == 256; }
@@ -860,7 +875,7 @@ extern "C" size_t pbattn_fp4_decode_workspace_size(int B, int T, int Hq, int Hk,
   using namespace pbgdn;
   if (!decode_sizes_ok(B, T, Hq, Hk, D) || !fp4_width(D)) return 0;
   const int rows = Hq / Hk * T;
-  const size_t slots = static_cast<size_t>(fp4_target(Hk, rows, D)) + B;
+  const size_t slots = static_cast<size_t>(fp4_target(Hk, rows, D, fp4_heads(Hk, rows, D, true))) + B;
   return slots * Hk * rows * (D * sizeof(float) + sizeof(float2));
 }
 
@@ -887,6 +902,7 @@ extern "C" int pbattn_fp4_decode(const void *q, int dtype, const void *k_cache, 
   const long reach = (cache.page_stride / 16) * pages + (cache.token / 16) * (page_size - 1L);
   if (reach > 0xffffffffL) return PBGDN_ERR_UNSUPPORTED;
   const bool near = reach < (1L << 28) - D / 32;  // (a row's own bytes within 4 GiB, too)
+  const int heads = fp4_heads(Hk, Hq / Hk * T, D, near && cache.head == D / 2);
   if (workspace_bytes < pbattn_fp4_decode_workspace_size(B, T, Hq, Hk, D)) return PBGDN_ERR_INVALID_ARGUMENT;
   Fp4DecodeParams pp{};
   DecodeParams &p = pp.d;
@@ -909,16 +925,16 @@ extern "C" int pbattn_fp4_decode(const void *q, int dtype, const void *k_cache, 
   p.lengths = lengths;
   p.o = o;
   p.lse = lse;
-  decode_call(p, B, T, Hq, Hk, scale, window, sinks, fp4_target(Hk, Hq / Hk * T, D));
+  decode_call(p, B, T, Hq, Hk, scale, window, sinks, fp4_target(Hk, Hq / Hk * T, D, heads));
   const size_t used = decode_workspace(p, workspace, D);
   hipStream_t s = static_cast<hipStream_t>(stream);
   debug_poison(o, static_cast<size_t>(B) * T * Hq * D * attn_bytes(dtype), s);
   if (lse) debug_poison(lse, static_cast<size_t>(B) * T * Hq * sizeof(float), s);
   debug_poison(workspace, used, s);
   switch (dtype) {
-    case PBGDN_F32: return dispatch_fp4<PBGDN_F32>(pp, D, near, s);
-    case PBGDN_BF16: return dispatch_fp4<PBGDN_BF16>(pp, D, near, s);
-    default: return dispatch_fp4<PBGDN_F16>(pp, D, near, s);
+    case PBGDN_F32: return dispatch_fp4<PBGDN_F32>(pp, D, near, heads, s);
+    case PBGDN_BF16: return dispatch_fp4<PBGDN_BF16>(pp, D, near, heads, s);
+    default: return dispatch_fp4<PBGDN_F16>(pp, D, near, heads, s);
   }
 }
 
