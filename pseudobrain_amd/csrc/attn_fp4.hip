@@ -108,7 +108,7 @@ struct Walk {
     return wave_sum_long(x);
   }
   __device__ __forceinline__ int workgroup_of(long x) const {
-    return x <= 0x7fffffff ? static_cast<int>(x) / static_cast<int>(per) : static_cast<int>(x / per);
+    return x <= 0x7fffffff && per <= 0x7fffffff ? static_cast<int>(x) / static_cast<int>(per) : static_cast<int>(x / per);
   }
   // Sequence b's parts, and its first slot.
   __device__ __forceinline__ int parts_of(const DecodeParams &p, int b, int lane) const {
@@ -945,7 +945,7 @@ extern "C" int pbattn_fp4_write(const void *k, const void *v, int dtype, const i
   if (N < 0 || Hk <= 0 || D <= 0 || !attn_dtype(dtype) || !kv_strides || !strides || page_size <= 0 || num_pages < 0) {
     return PBGDN_ERR_INVALID_ARGUMENT;
   }
-  if (!fp4_width(D)) return PBGDN_ERR_UNSUPPORTED;
+  if (!fp4_width(D) || static_cast<long>(Hk) * D > 0x7fffffffL) return PBGDN_ERR_UNSUPPORTED;
   if (N == 0 || num_pages == 0) return PBGDN_OK;
   if (!k || !v || !slots || !aligned16(k) || !aligned16(v)) return PBGDN_ERR_INVALID_ARGUMENT;
   const int bytes = attn_bytes(dtype);
@@ -984,7 +984,7 @@ extern "C" int pbattn_fp4_read(const void *k_cache, const void *v_cache, const v
       max_pages < 0) {
     return PBGDN_ERR_INVALID_ARGUMENT;
   }
-  if (!fp4_width(D) || B > MAX_REQUESTS) return PBGDN_ERR_UNSUPPORTED;
+  if (!fp4_width(D) || B > MAX_REQUESTS || static_cast<long>(Hk) * D > 0x7fffffffL) return PBGDN_ERR_UNSUPPORTED;
   if (!cu_seqlens || (B > 0 && !lengths) || (B > 0 && max_pages > 0 && !page_table) ||
       (tokens > 0 && (!k || !v || !aligned16(k) || !aligned16(v)))) {
     return PBGDN_ERR_INVALID_ARGUMENT;
@@ -1006,10 +1006,11 @@ extern "C" int pbattn_fp4_read(const void *k_cache, const void *v_cache, const v
   // Tokens of a workgroup: as many as leave the GPU eight workgroups a CU, READ_TOKENS at most.
   DeviceShape shape;
   if (!device_shape(shape)) shape.cus = 256;
-  const int even = (tokens + 8 * shape.cus - 1) / (8 * shape.cus);
-  p.per_block = even < 1 ? 1 : even > READ_TOKENS ? READ_TOKENS : even;
-  if (static_cast<long>(p.per_block) * Hk * p.eighths > 0x7fffffffL) return PBGDN_ERR_UNSUPPORTED;
-  const int blocks = (tokens + p.per_block - 1) / p.per_block;
+  const long even = (tokens + 8L * shape.cus - 1) / (8L * shape.cus);
+  p.per_block = static_cast<int>(even < 1 ? 1 : even > READ_TOKENS ? READ_TOKENS : even);
+  while (p.per_block > 1 && static_cast<long>(p.per_block) * Hk * p.eighths > 0x3fffffffL) p.per_block /= 2;  // (32-bit counts)
+  const long blocks = (tokens + static_cast<long>(p.per_block) - 1) / p.per_block;
+  if (blocks > 0xffffffL) return PBGDN_ERR_UNSUPPORTED;  // (a launch has less than 2^32 threads)
   const dim3 grid(static_cast<unsigned>(blocks > 0 ? blocks : 1));
   hipStream_t s = static_cast<hipStream_t>(stream);
   const size_t bytes = static_cast<size_t>(tokens) * Hk * D * attn_bytes(dtype);

@@ -373,7 +373,7 @@ static int rope_params(RopeParams &p, const void *q, const void *k, int dtype, c
   for (int a = 0; a < 6; ++a)
     if (strides[a] < 0) return PBGDN_ERR_INVALID_ARGUMENT;
   if (pos_strides[0] < 0 || pos_strides[1] < 0) return PBGDN_ERR_INVALID_ARGUMENT;
-  if (heads > 0x7fffffffL) return PBGDN_ERR_UNSUPPORTED;
+  if (heads > 0x7fffff00L) return PBGDN_ERR_UNSUPPORTED;
   const void *x[2] = {q, k}, *w[2] = {qw, kw};
   for (int a = 0; a < 2; ++a) {
     p.x[a] = static_cast<const unsigned char *>(x[a]);

@@ -123,7 +123,7 @@ def _decode_plan(q, dtype, cache, table, lengths, window, sinks, device_index: i
         raise ValueError("q must have the cache's head width and a multiple of its heads")
     if not 1 <= length <= MAX_DRAFT:
         raise ValueError(f"paged decoding takes 1 to {MAX_DRAFT} query tokens a sequence, got {length}")
-    if len(table) != 2 or table[0] != batch or lengths != (batch,):
+    if len(table) != 2 or table[0] != batch or lengths != (batch,) or table[1] >= 2**31:
         raise ValueError("expected page_table [B, max_pages] and lengths [B]")
     code, sizes = _dtype_code(dtype), (batch, length, hq, hk, d)
     with torch.cuda.device(device_index):  # (the workspace depends on the device's compute units)
@@ -189,6 +189,8 @@ def _write(k, v, cache, slots):
     code = _dtype_code(k.dtype)
     if slots.dtype not in (torch.int32, torch.int64):
         raise ValueError("slots must be int32 or int64")
+    if slots.numel() >= 2**31:
+        raise ValueError("paged_cache_write_fp4 takes less than 2^31 tokens")
     k, v, kv_steps = _write_operands(k, v, shape, k.dtype, slots.shape)
     if slots.dtype != torch.int64 or slots.ndim != 1 or not slots.is_contiguous():
         slots = slots.reshape(-1).to(torch.int64).contiguous()
@@ -225,7 +227,7 @@ def paged_cache_write_fp4(k, v, cache, slots) -> None:
 @_plan
 def _read_plan(cache, table, lengths, tokens: int, dtype):
     """The checked code of `dtype` for a read of these shapes."""
-    if len(table) != 2 or lengths != table[:1]:
+    if len(table) != 2 or lengths != table[:1] or table[1] >= 2**31:
         raise ValueError("expected page_table [B, max_pages] and lengths [B]")
     if table[0] > MAX_REQUESTS:
         raise ValueError(f"paged_cache_read_fp4 takes at most {MAX_REQUESTS} sequences, got {table[0]}")

@@ -28,7 +28,7 @@ def _pool_plan(table, stride, dtypes, a, b, free, free_stride, num_free, page: i
     """Checked sizes (row stride, max_pages, B, capacity) of a call with tensors of these shapes."""
     if len(table) != 2 or a != table[:1] or b != a:
         raise ValueError("expected page_table [B, max_pages] and a number for each of its B requests")
-    if len(free) != 1 or num_free != (1,):
+    if len(free) != 1 or num_free != (1,) or free[0] >= 2**31:
         raise ValueError("expected free_pages [capacity] and num_free [1]")
     if dtypes != (torch.int32, torch.int32):
         raise ValueError("page_table and free_pages are written in place: both must be int32")

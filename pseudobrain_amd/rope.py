@@ -66,6 +66,8 @@ def _rope_plan(q_stride, k_stride, pos_stride, *call):
     have 64 bits."""
     sizes = _rope_sizes(*call)
     q, k, positions = call[0], call[1], call[12]
+    if max(*q, *k, call[8][0]) >= 2**31:
+        raise ValueError("q, k and the tables must have less than 2^31 rows an axis")
     dense = all(x[3] == 1 or stride[3] == 1 for x, stride in ((q, q_stride), (k, k_stride)))
     lead = 2 - len(positions)
     pos_steps = _steps(((1,) * lead + tuple(positions) + (1,), (0,) * lead + tuple(pos_stride) + (1,)))

@@ -137,6 +137,7 @@ def write(**over):
     (dict(vn=FAKE + 4), _lib.ERR_INVALID_ARGUMENT),
     (dict(slots=None), _lib.ERR_INVALID_ARGUMENT),
     (dict(kv=strides(256, 128, 250, 128)), _lib.ERR_INVALID_ARGUMENT),
+    (dict(Hk=1 << 24), _lib.ERR_UNSUPPORTED),  # a token of 2^31 values
 ])
 def test_write_rejects(over, code):
     assert write(**over) == code
@@ -159,6 +160,8 @@ def read(**over):
     (dict(cu=None), _lib.ERR_INVALID_ARGUMENT),
     (dict(lengths=None), _lib.ERR_INVALID_ARGUMENT),
     (dict(table=None), _lib.ERR_INVALID_ARGUMENT),
+    (dict(Hk=1 << 24), _lib.ERR_UNSUPPORTED),
+    (dict(tokens=2**31 - 1), _lib.ERR_UNSUPPORTED),  # more threads than a launch has
 ])
 def test_read_rejects(over, code):
     assert read(**over) == code
@@ -190,7 +193,7 @@ def test_calls_refuse():
 
 
 def test_call_shapes_are_checked(monkeypatch):
-    monkeypatch.setattr(fc, "_one_device", lambda *t: t[0].device)
+    monkeypatch.setattr(fc, "_one_device", lambda *t: torch.device("cuda", 0))
     monkeypatch.setattr(fc, "_launch", lambda *args: pytest.fail("launched"))
     cache, table, lengths = empty(), torch.zeros(2, 3, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
     for q, message in ((torch.zeros(2, 1, 4, 128), "head width"), (torch.zeros(2, 1, 3, 64), "multiple"),
@@ -204,6 +207,13 @@ def test_call_shapes_are_checked(monkeypatch):
         fc.paged_cache_read_fp4(cache, table, lengths, -1)
     with pytest.raises(ValueError, match="lengths"):
         fc.paged_cache_read_fp4(cache, table, lengths[:1], 4)
+    long = table[:, :1].expand(2, 2**32)  # (more pages than a 32-bit count says)
+    with pytest.raises(ValueError, match="expected page_table"):
+        fc.paged_cache_read_fp4(cache, long, lengths, 4)
+    with pytest.raises(ValueError, match="expected page_table"):
+        fc.paged_decode_attention_fp4(torch.zeros(2, 1, 4, 64), cache, long, lengths, 1.0)
+    with pytest.raises(ValueError, match="less than"):
+        fc.paged_cache_write_fp4(*[torch.zeros(1, 2, 64).expand(2**32, 2, 64)] * 2, cache, lengths[:1].expand(2**32))
     many = fc.MAX_REQUESTS + 1
     with pytest.raises(ValueError, match="at most"):
         fc.paged_cache_read_fp4(cache, table[:1].expand(many, 3), lengths[:1].expand(many), 4)

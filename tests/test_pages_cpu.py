@@ -119,3 +119,6 @@ def test_calls_refuse(monkeypatch):
             pg.paged_cache_extend(*args, 3)
     with pytest.raises(ValueError, match="tokens"):
         pg.paged_cache_extend(*good.values(), -1)
+    i32 = torch.int32
+    with pytest.raises(ValueError, match="free_pages"):  # (a pool that a 32-bit count calls empty)
+        pg._pool_plan((2, 4), (4, 1), (i32, i32), (2,), (2,), (2**32,), (1,), (1,), 16)

@@ -164,6 +164,10 @@ def test_calls_refuse():
             (dict(positions=torch.zeros(3, 3).long()), "broadcasts"), (dict(eps=-1.0), "eps"), (dict(eps=float("nan")), "eps")):
         with pytest.raises(ValueError, match=message):
             rope.qk_norm_rope(**{**tensors(), **over})
+    for over in (dict(q=torch.zeros(1, 1, 4, 32).expand(1, 2**32, 4, 32), k=torch.zeros(1, 1, 2, 32).expand(1, 2**32, 2, 32)),
+                 dict(cos=torch.zeros(1, 8).expand(2**32, 8), sin=torch.zeros(1, 8).expand(2**32, 8))):
+        with pytest.raises(ValueError, match="less than"):  # (sizes that 32-bit counts call zero)
+            rope.qk_norm_rope(**{**tensors(), "positions": torch.zeros(1).long(), **over})
     with pytest.raises(ValueError, match="above 256"):
         rope.qk_norm_rope(**tensors(d=264))
     with pytest.raises(ValueError, match="float64"):
