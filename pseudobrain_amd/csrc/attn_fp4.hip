@@ -428,8 +428,20 @@ __global__ __launch_bounds__(DEC_WAVES * 64, (fp4_held(D, RB))) void fp4_decode_
 #pragma unroll
       for (int i = 0; i < 4 * KG; ++i)
         vs[i] = fp4_scale(scales[(KEYS + i / 4 * 16 + 4 * (i % 4) + g) * K::SROW + c * OT / FP4_BLOCK]);
+      // Q's parts are read a matrix step ahead where there are registers for them (64 contexts up
+      // to 8,192 tokens, 32 heads of 128, eight drafted tokens: 93.2 and 90.5 us; 256-wide float32
+      // 67.8 and 64.4).
+      constexpr int AHEAD = N == 1 || D == 256 ? 2 : 1;
+      v4u32_t qs[AHEAD][N * RB];
+      const auto read_q = [&](int s) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < N * RB; ++i) qs[s % AHEAD][i] = q_lds[((i % RB * N + i / RB) * KS + s) * 64 + lane];
+      };
+#pragma unroll
+      for (int s = 0; s < AHEAD - 1; ++s) read_q(s);
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
+        if (s + AHEAD - 1 < KS) read_q(s + AHEAD - 1);
         v4u32_t a[KG];
 #pragma unroll
         for (int kb = 0; kb < KG; ++kb) a[kb] = fp4_unpack8(cur.k[kb][s], ks[kb][D == 256 ? s / 4 : 0]);
@@ -437,7 +449,7 @@ __global__ __launch_bounds__(DEC_WAVES * 64, (fp4_held(D, RB))) void fp4_decode_
         for (int i = 0; i < N; ++i)
 #pragma unroll
           for (int r = 0; r < RB; ++r) {
-            const v4u32_t q = q_lds[((r * N + i) * KS + s) * 64 + lane];
+            const v4u32_t q = qs[s % AHEAD][i * RB + r];
 #pragma unroll
             for (int kb = 0; kb < KG; ++kb) sc[r][kb] = E::mma16(a[kb], q, sc[r][kb]);
           }
