@@ -13,6 +13,10 @@
 // or nothing is rotated). A row takes D / 16 lanes (float32: D / 8), the sums over it
 // DPP moves. A wave takes a token's heads one group of rows after the other and keeps
 // the token's angles and the weights in registers.
+//
+// 19,001 tokens of 32 heads of 128 on 8, bf16: forward 76 us, 5.2 TB/s; 8,192 tokens:
+// forward 29 us, backward 50 (5.1 TB/s), its sums joined in 4; what a large copy reaches
+// is 5.1. 64 tokens: 4.2 us, the launch.
 #include <initializer_list>
 #include <type_traits>
 

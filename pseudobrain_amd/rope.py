@@ -80,12 +80,12 @@ def _call(q, k, q_weight, k_weight, cos, sin, positions):
             sin.shape, cos.dtype, sin.dtype, positions.shape, positions.dtype)
 
 
-def _operands(q, k, q_weight, k_weight, cos, sin, positions, weight_offset):
+def _operands(q, k, q_weight, k_weight, cos, sin, positions, weight_offset, *grads):
     """The device, the checked sizes, the tensors as the kernels read them (to be kept until
     the launch) and the arguments that name them."""
     args = (q, k, q_weight, k_weight, cos, sin, positions)
     plan = _rope_plan(q.stride(), k.stride(), positions.stride(), *_call(*args))
-    dev = _one_device(*args)
+    dev = _one_device(*args, *grads)
     if (plan[3] is None or (q.data_ptr() | k.data_ptr() | q_weight.data_ptr() | k_weight.data_ptr() | cos.data_ptr()
                             | sin.data_ptr()) % 16
             or not (q_weight.is_contiguous() and k_weight.is_contiguous() and cos.is_contiguous() and sin.is_contiguous())):
@@ -117,12 +117,13 @@ def _gradient(x, grad):
     """The gradient of a result as the kernel reads it: dense, in x's dtype."""
     if grad.shape != x.shape:
         raise ValueError("grad_q and grad_k must have q's and k's shapes")
-    return _aligned((grad if grad.dtype == x.dtype else grad.to(x.dtype)).contiguous(), 16)
+    if grad.dtype == x.dtype and grad.is_contiguous() and not grad.data_ptr() % 16:
+        return grad
+    return _aligned(grad.to(x.dtype).contiguous(), 16)
 
 
 def _backward(q, k, q_weight, k_weight, cos, sin, positions, grad_q, grad_k, eps, weight_offset, interleaved):
-    dev, sizes, kept, args = _operands(q, k, q_weight, k_weight, cos, sin, positions, weight_offset)
-    _one_device(q, grad_q, grad_k)
+    dev, sizes, kept, args = _operands(q, k, q_weight, k_weight, cos, sin, positions, weight_offset, grad_q, grad_k)
     grad_q, grad_k = _gradient(q, grad_q), _gradient(k, grad_k)
     dq, dk = q.new_empty(q.shape), k.new_empty(k.shape)
     dqw, dkw = q_weight.new_empty(sizes[4]), k_weight.new_empty(sizes[4])
@@ -174,10 +175,10 @@ def _gradients(backward):
     def formula(ctx, grad_q, grad_k):
         if grad_q is None and grad_k is None:
             return (None,) * 10
-        q, k = ctx.saved_tensors[:2]
-        grad_q = torch.zeros_like(q) if grad_q is None else grad_q
-        grad_k = torch.zeros_like(k) if grad_k is None else grad_k
-        return *backward(*ctx.saved_tensors, grad_q, grad_k, *ctx.rest), *(None,) * 6
+        saved = ctx.saved_tensors
+        grad_q = torch.zeros_like(saved[0]) if grad_q is None else grad_q
+        grad_k = torch.zeros_like(saved[1]) if grad_k is None else grad_k
+        return *backward(*saved, grad_q, grad_k, *ctx.rest), None, None, None, None, None, None
     return formula
 
 

@@ -167,10 +167,11 @@ def test_absent_pages_and_stale_rows():
 @pytest.mark.parametrize("d,dtype", [(64, torch.float32), (64, torch.float16), (128, torch.bfloat16), (256, torch.bfloat16),
                                      (256, torch.float32)])
 @pytest.mark.parametrize("group", [1, 3, 8])
-def test_a_bad_value_reaches_only_the_tokens_that_see_it(d, dtype, group):
+@pytest.mark.parametrize("heads_first", [False, True])
+def test_a_bad_value_reaches_only_the_tokens_that_see_it(d, dtype, group, heads_first):
     """Scales of NaN among the drafts and at the window's edge, in values and keys."""
     draft, window, lengths = 4, 50, [200, 131]
-    q, cache, table, lens = make(lengths, 16, 2 * group, 2, d, draft, dtype, 31)
+    q, cache, table, lens = make(lengths, 16, 2 * group, 2, d, draft, dtype, 31, heads_first)
     clean = fc.paged_decode_attention_fp4(q, cache, table, lens, d ** -0.5, window, 3)
     bad = {0: (200 - 1, 200 - 4 - window + 1, 200 - 2), 1: (131 - 2, 131 - 4 - window + 2, 131 - 1)}
     for b, (x, y, key) in bad.items():
