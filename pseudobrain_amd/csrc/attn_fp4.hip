@@ -128,13 +128,14 @@ struct Walk {
 };
 
 // Q and the weights enter bfloat16 products as one, two or three parts that sum up to
-// them: bfloat16 rows as they are, float16 rows in two, float32 rows in three, all of
-// them exactly; the weights of bfloat16 rows are rounded once to 2^-9, those of the
-// others cut to 16 and 24 bits. So the cache's values, exact in bfloat16, meet every
-// type of row in the same kernel.
+// them. Q: bfloat16 rows as they are, float16 rows in two, float32 rows in three, all of
+// them exactly. The weights: two parts, cut to 16 bits, whose error (2^-15) is small beside
+// a 16-bit result's own rounding, and for float32 rows three, which are all of their 24 bits.
+// So the cache's values, exact in bfloat16, meet every type of row in the same kernel.
 template <int DT>
 struct Parts {
   static constexpr int N = DT == PBGDN_BF16 ? 1 : DT == PBGDN_F16 ? 2 : 3;
+  static constexpr int WEIGHT = DT == PBGDN_F32 ? 3 : 2;
 };
 // The upper halves of two words.
 __device__ __forceinline__ uint32_t upper_halves(uint32_t lo, uint32_t hi) {
@@ -181,7 +182,7 @@ __device__ __forceinline__ T load_keys(const T *p) {
 
 template <int DT, int D>
 struct Fp4 {
-  static constexpr int N = Parts<DT>::N;
+  static constexpr int N = Parts<DT>::N, W = Parts<DT>::WEIGHT;
   static constexpr int ROW = D / 2;           // bytes of a key's codes
   static constexpr int SROW = D / FP4_BLOCK;  // and of its scales
   static constexpr int KSTEPS = D / 32;       // matrix steps of a score
@@ -221,7 +222,7 @@ template <int DT, int D, int RB, bool NEAR, bool ONCE, int HEADS>
 __global__ __launch_bounds__(DEC_WAVES * 64, (fp4_held(D, RB))) void fp4_decode_kernel(const Fp4DecodeParams pp) {
   using K = Fp4<DT, D>;
   using E = Elem<PBGDN_BF16>;
-  constexpr int KS = K::KSTEPS, OT = K::OT, KG = K::KG, KEYS = K::KEYS, N = K::N;
+  constexpr int KS = K::KSTEPS, OT = K::OT, KG = K::KG, KEYS = K::KEYS, N = K::N, W = K::W;
   constexpr int JOINS = RB * D <= 256 ? 2 : 1, HW = DEC_WAVES / HEADS;  // HW: waves of a head
   __shared__ __attribute__((aligned(16))) float merge[JOINS][RB * DEC_ROWS * (D + 2)];
   __shared__ v4u32_t q_of[HEADS][RB * N * KS * 64];  // [row tile][part][step][lane]
@@ -505,7 +506,7 @@ __global__ __launch_bounds__(DEC_WAVES * 64, (fp4_held(D, RB))) void fp4_decode_
         l[r] += sum;
       }
       // O^T += V^T P; element e of the lane's values makes output tile e
-      v4u32_t w[RB][KG / 2][N];
+      v4u32_t w[RB][KG / 2][W];
 #pragma unroll
       for (int r = 0; r < RB; ++r)
 #pragma unroll
@@ -513,14 +514,10 @@ __global__ __launch_bounds__(DEC_WAVES * 64, (fp4_held(D, RB))) void fp4_decode_
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float x = sc[r][2 * h + i / 2][2 * (i % 2)], y = sc[r][2 * h + i / 2][2 * (i % 2) + 1];
-            if constexpr (N == 1) {
-              w[r][h][0][i] = E::pack(x, y);
-            } else {
-              uint32_t part[N];
-              split_pair<N>(x, y, part);
+            uint32_t part[W];
+            split_pair<W>(x, y, part);
 #pragma unroll
-              for (int n = 0; n < N; ++n) w[r][h][n][i] = part[n];
-            }
+            for (int n = 0; n < W; ++n) w[r][h][n][i] = part[n];
           }
       const auto pair_of_tiles = [&](auto E0) __attribute__((always_inline)) {  // tiles 2 e and 2 e + 1
         constexpr int e = decltype(E0)::value;
@@ -536,7 +533,7 @@ __global__ __launch_bounds__(DEC_WAVES * 64, (fp4_held(D, RB))) void fp4_decode_
             hi[i] = __builtin_amdgcn_perm(x[2 * i + 1], x[2 * i], 0x07060302u);
           }
 #pragma unroll
-          for (int n = 0; n < N; ++n)
+          for (int n = 0; n < W; ++n)
 #pragma unroll
             for (int r = 0; r < RB; ++r) {
               o[r][2 * e] = E::mma16(lo, w[r][h][n], o[r][2 * e]);

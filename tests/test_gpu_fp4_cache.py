@@ -101,6 +101,25 @@ def test_head_groups_and_drafts(hq, hk, draft):
     check("groups, window", *x, 0.125, 20, 2)
 
 
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("draft,hq", [(1, 4), (3, 16)])
+def test_a_result_is_rounded_once(d, dtype, draft, hq):
+    """Weights do not lose the bits that a result of q's type can show: they enter the products in
+    two parts, cut to 16 bits (off by less than 2^-15 of themselves), for float32 rows in three, all
+    of their bits. So the bound is a float32 kernel's (oracle/attention.py), 2^-15 of the sum of
+    magnitudes, and one rounding of the result."""
+    q, cache, table, lengths = make([300, 5, 1000], 16, hq, 2, d, draft, dtype, d + 3)
+    o = fc.paged_decode_attention_fp4(q, cache, table, lengths, d ** -0.5, 200, 3)
+    u, cut = (0.0, 0.0) if dtype == torch.float32 else (oa.UNIT[NAMES[dtype]], 2.0 ** -15)
+    for b, n in enumerate(lengths.tolist()):
+        k, v = rows(cache, table, b, n)
+        ref = oa.attention(f64(q[b]), k, v, d ** -0.5, 200, 3)
+        size = oa.attention(f64(q[b]), k, np.abs(v), d ** -0.5, 200, 3)["o"]
+        tol = ref["o_tol"] + u * np.abs(ref["o"]) + 1.01 * cut * size + oa.TINY[NAMES[dtype]]
+        compare(f"rounded once, {n}", o[b], ref["o"], tol)
+
+
 def test_long_contexts_are_split_and_joined():
     x = make([20000, 3, 9000], 64, 8, 1, 128, 1, torch.bfloat16, 20)
     check("split", *x, 128 ** -0.5)
