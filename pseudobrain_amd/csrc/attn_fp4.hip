@@ -129,8 +129,9 @@ struct Walk {
 
 // Q and the weights enter bfloat16 products as one, two or three parts that sum up to
 // them. Q: bfloat16 rows as they are, float16 rows in two, float32 rows in three, all of
-// them exactly. The weights: two parts, cut to 16 bits, whose error (2^-15) is small beside
-// a 16-bit result's own rounding, and for float32 rows three, which are all of their 24 bits.
+// them exactly. The weights: two parts, which round them to 16 bits (2^-16: small beside a
+// 16-bit result's own rounding, and to either side), and for float32 rows three, which are
+// all of their 24 bits.
 // So the cache's values, exact in bfloat16, meet every type of row in the same kernel.
 template <int DT>
 struct Parts {
@@ -141,16 +142,18 @@ struct Parts {
 __device__ __forceinline__ uint32_t upper_halves(uint32_t lo, uint32_t hi) {
   return __builtin_amdgcn_perm(hi, lo, 0x07060302u);
 }
-// Two values as N pairs of bfloat16, cut, not rounded (no part passes the type's range).
+// Two values as N pairs of bfloat16: all but the last cut, not rounded (no part passes the
+// type's range), the last, what is left, rounded to nearest.
 template <int N>
 __device__ __forceinline__ void split_pair(float x, float y, uint32_t *out) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
+  for (int i = 0; i < N - 1; ++i) {
     const uint32_t a = __float_as_uint(x), b = __float_as_uint(y);
     out[i] = upper_halves(a, b);
     x -= __uint_as_float(a & 0xffff0000u);
     y -= __uint_as_float(b & 0xffff0000u);
   }
+  out[N - 1] = Elem<PBGDN_BF16>::pack(x, y);
 }
 
 // Eight values from src as float32.

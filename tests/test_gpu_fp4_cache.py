@@ -106,7 +106,7 @@ def test_head_groups_and_drafts(hq, hk, draft):
 @pytest.mark.parametrize("draft,hq", [(1, 4), (3, 16)])
 def test_a_result_is_rounded_once(d, dtype, draft, hq):
     """Weights do not lose the bits that a result of q's type can show: they enter the products in
-    two parts, cut to 16 bits (off by less than 2^-15 of themselves), for float32 rows in three, all
+    two parts of 16 bits (off by less than 2^-15 of themselves), for float32 rows in three, all
     of their bits. So the bound is a float32 kernel's (oracle/attention.py), 2^-15 of the sum of
     magnitudes, and one rounding of the result."""
     q, cache, table, lengths = make([300, 5, 1000], 16, hq, 2, d, draft, dtype, d + 3)
@@ -118,6 +118,30 @@ def test_a_result_is_rounded_once(d, dtype, draft, hq):
         size = oa.attention(f64(q[b]), k, np.abs(v), d ** -0.5, 200, 3)["o"]
         tol = ref["o_tol"] + u * np.abs(ref["o"]) + 1.01 * cut * size + oa.TINY[NAMES[dtype]]
         compare(f"rounded once, {n}", o[b], ref["o"], tol)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_weights_are_rounded_to_nearest(d, dtype):
+    """Six keys of weight 1 and value 1, eleven of weight 6 / 11 and value -1: their sum is what
+    the weights lose. 6 / 11 has 0.909 steps of 2^-16 behind its 16 bits: cut off they would leave
+    11 / 12 0.909 2^-16 = 1.27e-5 of the output; rounded to nearest, a weight is off by at most
+    2^-17, the output by 11 / 12 of that, and by 2^-19 for float32 arithmetic on 17 terms (17
+    2^-24 at most) and the exponential (2^-21 and less)."""
+    q, cache, table, lengths = make([17], 32, 1, 1, d, 1, dtype, d)
+    q.zero_()
+    for x in cache[:2]:
+        x.zero_()
+    for x in cache[2:]:
+        x.fill_(127)
+    q[..., 0] = -1.0
+    page = table[0, 0].item()
+    cache.k[page, 6:17, 0, 0] = 0x02  # 1 in the row's first value: a score of -scale
+    cache.v[page, :6], cache.v[page, 6:17] = 0x22, 0xaa  # 1 and -1
+    o = fc.paged_decode_attention_fp4(q, cache, table, lengths, float(np.log(11 / 6)))
+    bound = (0.0 if dtype == torch.float32 else 11 / 12 * 2.0 ** -17) + 2.0 ** -19
+    print(f"[weights] {np.abs(f64(o)).max():.3e} of {bound:.3e}", flush=True)
+    assert np.abs(f64(o)).max() <= bound
 
 
 def test_long_contexts_are_split_and_joined():
