@@ -270,8 +270,8 @@ int pbattn_fp4_read(const void *k_cache, const void *v_cache, const void *k_scal
  *   new_lengths  [B] int32, written: lengths with what was granted
  *   new_num_free [1] int32, written
  * pbattn_pages_release: the pages of request b whose last token lies in [first[b],
- * end[b]) are pushed, in the requests' order (capacity ends it); page_table stays as it
- * is. Ranges of one request that follow each other so give every page back once: the
+ * end[b]) are pushed, in the requests' order (capacity ends it); entries below 0, which
+ * are no pages, are left out, and page_table stays as it is. Ranges of one request that follow each other so give every page back once: the
  * tokens that a window has left, or, up to a multiple of page_size, all of a finished
  * request's.
  *

@@ -29,8 +29,8 @@ def extend(table, lengths, counts, pool, page, tokens):
 
 
 def release(table, first, end, pool, page, capacity):
-    """Pushes onto `pool` in place, up to `capacity`."""
+    """Pushes onto `pool` in place, up to `capacity`; an entry below 0 is no page."""
     for row, lo, hi in zip(table, first, end):
         for i, entry in enumerate(row):
-            if lo <= i * page + page - 1 < hi and len(pool) < capacity:
+            if lo <= i * page + page - 1 < hi and entry >= 0 and len(pool) < capacity:
                 pool.append(entry)

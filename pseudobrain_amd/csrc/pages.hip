@@ -5,8 +5,8 @@
 // token or page: every workgroup forms the sums for itself (a scan over at most 4,096
 // requests in LDS), finds its pieces' requests by bisection and writes them, so that a
 // call is one launch and needs nothing kept between workgroups. Bound by latency: the
-// launch, the requests' numbers, three scans, the table's entry (64 requests: release 2.8
-// us, extend 4.7; 233 with 4,000 tokens 2.8 and 6.2).
+// launch, the requests' numbers, three scans, the table's entry (64 requests: release 4.0
+// us, extend 4.8; 233 with 4,000 tokens 4.2 and 5.7).
 #include "attn.hpp"
 #include "pages.hpp"
 #include "device.hpp"
@@ -123,12 +123,23 @@ __global__ __launch_bounds__(SCAN_THREADS) void extend_kernel(const PoolParams p
   }
 }
 
-__global__ __launch_bounds__(SCAN_THREADS) void release_kernel(const PoolParams p) {
-  __shared__ int start[MAX_REQUESTS];
-  __shared__ long waves[SCAN_WAVES];
+// The entries of all ranges, in the requests' order, are one list, of which each workgroup
+// takes a run: it counts the pages before its own and pushes those in it. An entry below 0 is
+// no page (the caches' other operators skip it too) and must not come back as one. (64 requests,
+// one page each 3.9 us; a request's 16,384 pages 8.8; 256 requests of 1,024 pages 111: a run's
+// start costs the reading of all before it, which a serving step, of few pages, does not notice.)
+constexpr int RELEASE_THREADS = 512, RELEASE_WAVES = RELEASE_THREADS / 64;
+constexpr int RELEASE_BLOCKS = 64;  // most workgroups
+
+__global__ __launch_bounds__(RELEASE_THREADS) void release_kernel(const PoolParams p) {
+  constexpr int AT_ONCE = 16;  // entries of a thread in flight
+  __shared__ long start[MAX_REQUESTS], table_of[MAX_REQUESTS];  // first entry in the list; entry k is table[table_of + k]
+  __shared__ long waves[RELEASE_WAVES], counts[RELEASE_WAVES];
   PBGDN_POISON_LDS(start, sizeof(start));
+  PBGDN_POISON_LDS(table_of, sizeof(table_of));
   PBGDN_POISON_SYNC();
-  const int each = (p.B + SCAN_THREADS - 1) / SCAN_THREADS, b0 = threadIdx.x * each;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int each = (p.B + RELEASE_THREADS - 1) / RELEASE_THREADS, b0 = threadIdx.x * each;
   const int b1 = b0 + each < p.B ? b0 + each : p.B, pool = pool_height(p);
   // pages whose last token lies in [first, end): from first / page up to end / page
   const auto low = [&](int b) { return p.a[b] > 0 ? p.a[b] / p.page : 0; };
@@ -139,19 +150,75 @@ __global__ __launch_bounds__(SCAN_THREADS) void release_kernel(const PoolParams 
   long sum = 0, total;
   for (int b = b0; b < b1; ++b) sum += pages(b);
   long at = block_scan(sum, waves, total);
-  const long room = p.capacity - pool;
-  if (total > room) total = room;  // (more than the pool can have given)
   for (int b = b0; b < b1; ++b) {
-    start[b] = static_cast<int>(at < total ? at : total);
+    start[b] = at;
+    table_of[b] = b * p.table_row + low(b) - at;
     at += pages(b);
   }
-  if (blockIdx.x == 0 && threadIdx.x == 0) *p.num_free_out = pool + static_cast<int>(total);
   __syncthreads();
-  for (long k = blockIdx.x * static_cast<long>(SCAN_THREADS) + threadIdx.x; k < total;
-       k += static_cast<long>(gridDim.x) * SCAN_THREADS) {
-    const int b = sequence_of(start, p.B, static_cast<int>(k));
-    p.free_pages[pool + k] = p.table[b * p.table_row + low(b) + (k - start[b])];
+  const long even = (total + gridDim.x - 1) / gridDim.x, run = (even + RELEASE_THREADS - 1) / RELEASE_THREADS * RELEASE_THREADS;
+  const long k0 = blockIdx.x * run, k1 = k0 + run < total ? k0 + run : total;
+  if (blockIdx.x > 0 && k0 >= total) return;
+  // Entries k + 64 i of the list below `end` (-1 past it). Where a request's have ended it is the
+  // next one's, or one that bisection finds.
+  int top = 1;
+  while (top < p.B) top *= 2;
+  const auto entries = [&](auto &x, long k, long end) __attribute__((always_inline)) {
+    constexpr int N = sizeof(x) / sizeof(x[0]);
+    int b = -1;
+    long from = 0, next = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i, k += 64) {
+      if (k >= next && k < end) {
+        const auto ends = [&] { return b + 1 < p.B ? start[b + 1] : end; };
+        ++b;
+        next = ends();
+        if (i == 0 || k >= next) {
+          b = 0;
+          for (int step = top / 2; step > 0; step /= 2)  // the last b with start[b] <= k
+            if (b + step < p.B && start[b + step] <= k) b += step;
+          next = ends();
+        }
+        from = table_of[b];
+      }
+      x[i] = k < end ? p.table[from + k] : -1;
+    }
+  };
+  // pages of the threads before this one, in `all` those of all of them
+  const auto ranks = [&](long mine, long &all) __attribute__((always_inline)) {
+    __syncthreads();
+    if (lane == 0) counts[wave] = mine;
+    __syncthreads();
+    long before = 0;
+    all = 0;
+#pragma unroll
+    for (int w = 0; w < RELEASE_WAVES; ++w) {
+      if (w < wave) before += counts[w];
+      all += counts[w];
+    }
+    return before;
+  };
+  long before = 0;
+  if (k0 > 0) {
+    long mine = 0;
+    for (long first = 0; first < k0; first += AT_ONCE * RELEASE_THREADS) {
+      int x[AT_ONCE];
+      entries(x, first + wave * (64 * AT_ONCE) + lane, k0);
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; ++i) mine += __popcll(__ballot(x[i] >= 0));
+    }
+    ranks(mine, before);
   }
+  for (long first = k0; first < k1; first += RELEASE_THREADS) {
+    int x[1];
+    long held;
+    entries(x, first + threadIdx.x, k1);
+    const uint64_t there = __ballot(x[0] >= 0);
+    const long to = pool + before + ranks(__popcll(there), held) + __popcll(there & ((1ull << lane) - 1));
+    if (x[0] >= 0 && to < p.capacity) p.free_pages[to] = x[0];  // (past it: more than the pool can have given)
+    before += held;
+  }
+  if (k1 == total && threadIdx.x == 0) *p.num_free_out = static_cast<int>(pool + before < p.capacity ? pool + before : p.capacity);
 }
 
 static int pool_params(PoolParams &p, int32_t *table, int64_t table_row, int max_pages, const int32_t *a, const int32_t *b,
@@ -209,9 +276,9 @@ extern "C" int pbattn_pages_release(const int32_t *page_table, int64_t table_row
   const int status = pool_params(p, const_cast<int32_t *>(page_table), table_row, max_pages, first, end, B, page_size,
                                  free_pages, capacity, num_free, new_num_free);
   if (status != PBGDN_OK) return status;
-  // as many threads as there are pages to give at most, 64 workgroups of them
-  const long blocks = (static_cast<long>(B) * max_pages + SCAN_THREADS - 1) / SCAN_THREADS;
-  hipLaunchKernelGGL(release_kernel, dim3(static_cast<unsigned>(blocks < 1 ? 1 : blocks < 64 ? blocks : 64)),
-                     dim3(SCAN_THREADS), 0, static_cast<hipStream_t>(stream), p);
+  // as many threads as there are pages to give at most, up to RELEASE_BLOCKS workgroups of them
+  const long blocks = (static_cast<long>(B) * max_pages + RELEASE_THREADS - 1) / RELEASE_THREADS;
+  hipLaunchKernelGGL(release_kernel, dim3(static_cast<unsigned>(blocks < 1 ? 1 : blocks < RELEASE_BLOCKS ? blocks : RELEASE_BLOCKS)),
+                     dim3(RELEASE_THREADS), 0, static_cast<hipStream_t>(stream), p);
   return hipGetLastError() == hipSuccess ? PBGDN_OK : PBGDN_ERR_LAUNCH;
 }

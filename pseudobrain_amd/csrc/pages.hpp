@@ -13,7 +13,8 @@ constexpr int SCAN_WAVES = SCAN_THREADS / 64;
 
 // Sum of x over the threads before this one, in `total` over all of them. (64 bits:
 // neither wrong counts nor many large ones may wrap around.)
-__device__ __forceinline__ long block_scan(long x, long (&waves)[SCAN_WAVES], long &total) {
+template <int WAVES>
+__device__ __forceinline__ long block_scan(long x, long (&waves)[WAVES], long &total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   long scan = x;
 #pragma unroll
@@ -27,7 +28,7 @@ __device__ __forceinline__ long block_scan(long x, long (&waves)[SCAN_WAVES], lo
   long before = 0;
   total = 0;
 #pragma unroll
-  for (int w = 0; w < SCAN_WAVES; ++w) {
+  for (int w = 0; w < WAVES; ++w) {
     if (w < wave) before += waves[w];
     total += waves[w];
   }
@@ -36,7 +37,8 @@ __device__ __forceinline__ long block_scan(long x, long (&waves)[SCAN_WAVES], lo
 
 // The last b in [0, n) with start[b] <= t, 0 where there is none: the sequence of
 // token t when start[0] = 0 and a next sequence starts past it.
-__device__ __forceinline__ int sequence_of(const int *start, int n, int t) {
+template <typename T>
+__device__ __forceinline__ int sequence_of(const T *start, int n, T t) {
   int lo = 0, hi = n - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;

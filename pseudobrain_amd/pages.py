@@ -130,8 +130,9 @@ def _(page_table, first, end, free_pages, num_free, page):
 
 def paged_cache_release(page_table, first, end, free_pages, num_free, page: int):
     """Give pages back: those of request b whose last token lies in [first[b], end[b]) (int
-    [B] both) are pushed on the pool, free_pages in place, in the requests' order. Returns
-    the new num_free, int32 [1]; page_table stays as it is.
+    [B] both) are pushed on the pool, free_pages in place, in the requests' order; entries
+    below 0 are no pages and are left out. Returns the new num_free, int32 [1]; page_table
+    stays as it is.
 
     Ranges that follow each other give every page back once: a window's, as it moves on
     (first no less than the sinks' pages times `page`), and in the end the rest, end rounded

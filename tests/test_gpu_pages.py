@@ -93,6 +93,39 @@ def test_release(page):
         assert free.tolist() == pool + [-7] * (capacity - len(pool))
 
 
+@pytest.mark.parametrize("batch,width", [(1, 3), (7, 40), (1, 70000), (5, 9000), (300, 500), (4096, 6)])
+@pytest.mark.parametrize("absent", [0.0, 0.3, 1.0])
+def test_absent_entries_do_not_come_back_as_pages(batch, width, absent):
+    """Ranges with entries below 0 among them, in one workgroup's run and over many, pools with room for
+    all and for some."""
+    page, rng = 4, random.Random(batch + width)
+    gen = torch.Generator().manual_seed(batch)
+    rows = torch.randint(10 ** 6, (batch, width), generator=gen)
+    rows[torch.rand(batch, width, generator=gen) < absent] = -1
+    rows = rows.tolist()
+    first = [rng.choice([0, 0, 0, 5, page * width]) for _ in range(batch)]
+    end = [rng.choice([page * width, page * width, 10 ** 9, page * (width // 2) + 1, 0]) for _ in first]
+    first[0], end[0] = 0, page * width
+    for start, spare in ((3, batch * width), (3, batch * width // 3), (0, 0)):
+        pool = list(range(start))
+        free = ints(pool + [-7] * spare)
+        left = pg.paged_cache_release(ints(rows), ints(first), ints(end), free, ints([start]), page)
+        op.release(rows, first, end, pool, page, start + spare)
+        assert left.tolist() == [len(pool)]
+        assert free.tolist() == pool + [-7] * (start + spare - len(pool))
+
+
+def test_a_pool_over_absent_entries_grants_pages():
+    """A request that held its window's pages alone gives them back; what the pool then grants is pages."""
+    table, free = ints([[-1, -1, 5, -1, 6]]), ints([9, -7, -7, -7])
+    num_free = pg.paged_cache_release(table, ints([0]), ints([20]), free, ints([1]), 4)
+    assert num_free.tolist() == [3] and free.tolist() == [9, 5, 6, -7]
+    slots, *_, left = pg.paged_cache_extend(table, ints([0]), ints([20]), free, num_free, 4, 20)
+    assert left.tolist() == [3] and slots.tolist() == [-1] * 20  # five pages are not there
+    slots, *_, left = pg.paged_cache_extend(table, ints([0]), ints([12]), free, num_free, 4, 12)
+    assert left.tolist() == [0] and slots.tolist() == [*range(24, 28), *range(20, 24), *range(36, 40)]
+
+
 def test_empty_calls_and_strided_tables():
     none = ints([])
     slots, positions, cu, after, left = pg.paged_cache_extend(none.view(0, 3), none, none, ints([4, 5]), ints([2]), 16, 6)

@@ -43,6 +43,12 @@ def test_no_page_is_held_twice_or_lost():
     assert refused > 50
 
 
+def test_absent_entries_are_not_released():
+    pool = [7]
+    op.release([[3, -1, 4], [-1, -1, -1]], [0, 0], [12, 12], pool, 4, 9)
+    assert pool == [7, 3, 4]
+
+
 def extend(**over):
     args = dict(table=FAKE, row=4, max_pages=4, lengths=FAKE, counts=FAKE, B=2, page=16, free=FAKE, capacity=9,
                 num_free=FAKE, tokens=3, slots=FAKE, positions=FAKE, cu=FAKE, after=FAKE, left=FAKE, stream=None)
