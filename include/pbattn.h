@@ -274,6 +274,10 @@ int pbattn_fp4_read(const void *k_cache, const void *v_cache, const void *k_scal
  * are no pages, are left out, and page_table stays as it is. Ranges of one request that follow each other so give every page back once: the
  * tokens that a window has left, or, up to a multiple of page_size, all of a finished
  * request's.
+ * Which pages a request holds follows from its length: whoever lowers one (drafted tokens
+ * that were not accepted) releases [new length, old length), both rounded up to a multiple
+ * of page_size, before the next pbattn_pages_extend, which takes pages past the new length
+ * as not yet held and would enter others in their place.
  *
  * Neither changes lengths, counts, num_free: the same call again gives the same results.
  * The outputs must not overlap the inputs.

@@ -10,6 +10,14 @@ i page + page - 1 and is entry i of its row of page_table.
   paged_cache_extend   pages, slots and positions for the requests' new tokens
   paged_cache_release  pages whose tokens are no longer needed back to the pool
 
+Which pages a request holds follows from its length. A length that is lowered, as by drafted
+tokens that were not accepted, leaves pages behind that the next extension would replace by
+others and the pool would never see again: they are released first, from the new length to the
+old one, both rounded up to whole pages,
+
+    up = lambda n: (n + page - 1) // page * page
+    num_free = paged_cache_release(page_table, up(accepted), up(lengths), free_pages, num_free, page)
+
 Lengths, counts and num_free are read, never changed: both return the new ones, and the
 same call again gives the same results. On the GPU only; a missing library or a CPU
 tensor raises.
@@ -97,7 +105,8 @@ def paged_cache_extend(page_table, lengths, counts, free_pages, num_free, page: 
       num_free     int32 [1]: pages left
 
     A request's place that is not granted shows as an unchanged length; ask again once pages
-    have been released."""
+    have been released. Pages past lengths[b] count as not held: where a length was lowered they
+    have to be released before (see the module)."""
     args = (page_table, lengths, counts, free_pages, num_free)
     if not _untraced(*args):
         return paged_cache_extend_op(*args, int(page), int(tokens))
@@ -135,8 +144,9 @@ def paged_cache_release(page_table, first, end, free_pages, num_free, page: int)
     stays as it is.
 
     Ranges that follow each other give every page back once: a window's, as it moves on
-    (first no less than the sinks' pages times `page`), and in the end the rest, end rounded
-    up to a whole page. A page must not be given back twice."""
+    (first no less than the sinks' pages times `page`), from behind, as a length is lowered
+    (both ends rounded up to whole pages), and in the end the rest, end rounded up to a whole
+    page. A page must not be given back twice."""
     args = (page_table, first, end, free_pages, num_free)
     if not _untraced(*args):
         return paged_cache_release_op(*args, int(page))

@@ -144,6 +144,47 @@ def test_requests_come_and_go():
     assert engine.num_free.item() == pages and sorted(engine.free.tolist()) == list(range(pages))
 
 
+def test_drafts_partly_accepted():
+    """Four drafted tokens a step, of which the device accepts some: rejected tokens' pages go back
+    before the next step, their rows are written again, and no page is lost."""
+    rows, pages, draft, steps = 3, 30, 4, 25
+    engine = Engine(rows, pages, 4)
+    engine.prefill([30, 1, 16])
+    counts = torch.full((rows,), draft, dtype=torch.int32, device=DEV)
+
+    def up(n):
+        return (n + PAGE - 1) // PAGE * PAGE
+
+    for i in range(steps):
+        slots, positions, cu = engine.place(counts, rows * draft)
+        assert cu.tolist() == [0, 4, 8, 12]
+        q, k, v = engine.tokens(rows * draft)
+        qr, kr = engine.normed(q, k, positions)
+        paged_cache_write_fp4(kr[0], v[0], engine.cache, slots)
+        o = paged_decode_attention_fp4(qr.view(rows, draft, HQ, D), engine.cache, engine.table, engine.lengths, SCALE,
+                                       WINDOW, SINKS)
+        engine.note(kr, v, cu.tolist())
+        for b in range(rows):
+            ref = engine.expect(b, f64(qr[0, draft * b:draft * (b + 1)]))
+            compare(f"step {i}, drafts of {b}", o[b], ref["o"], ref["o_tol"])
+        rejected = torch.randint(0, draft + 1, (rows,), generator=engine.gen, device=DEV)
+        accepted = (engine.lengths - rejected).to(torch.int32)
+        engine.num_free = paged_cache_release(engine.table, up(accepted), up(engine.lengths), engine.free, engine.num_free,
+                                              PAGE)
+        for b, n in enumerate(rejected.tolist()):
+            for seen in engine.seen[b]:
+                del seen[len(seen) - n:]
+        engine.lengths = accepted
+        held = [engine.table[b, j].item() for b in range(rows)
+                for j in [*range(min(KEPT, up(accepted[b].item())) // PAGE),
+                          *range(engine.low[b].item() // PAGE, up(accepted[b].item()) // PAGE)]]
+        free = engine.free[:engine.num_free.item()].tolist()
+        assert sorted(held + free) == list(range(pages))
+    for b in range(rows):
+        engine.finish(b)
+    assert engine.num_free.item() == pages and sorted(engine.free.tolist()) == list(range(pages))
+
+
 def test_a_pool_that_is_too_small():
     """What does not fit waits, and neither the others nor the pool notice."""
     engine = Engine(3, 6, 2)

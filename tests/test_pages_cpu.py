@@ -43,6 +43,27 @@ def test_no_page_is_held_twice_or_lost():
     assert refused > 50
 
 
+@pytest.mark.parametrize("released", [True, False])
+def test_drafts_that_are_not_accepted(released):
+    """Lengths that go back: with the pages between released first none is lost, without they are."""
+    rng = random.Random(1)
+    page, batch, width, capacity, draft = 4, 3, 40, 40, 6
+    pool, table = list(range(capacity)), [[-1] * width for _ in range(batch)]
+    lengths = [0] * batch
+    for _ in range(30):
+        before = lengths
+        *_, lengths = op.extend(table, lengths, [draft] * batch, pool, page, draft * batch)
+        accepted = [min(n, m + rng.randint(0, draft)) for n, m in zip(lengths, before)]
+        if released:
+            up = [[-(-n // page) * page for n in x] for x in (accepted, lengths)]
+            op.release(table, *up, pool, page, capacity)
+        lengths = accepted
+        held = [row[i] for row, n in zip(table, lengths) for i in range(-(-n // page))]
+        assert len(set(held + pool)) == len(held) + len(pool)
+        assert not released or len(held) + len(pool) == capacity
+    assert min(lengths) > 5 * page and (released or len(held) + len(pool) < capacity)
+
+
 def test_absent_entries_are_not_released():
     pool = [7]
     op.release([[3, -1, 4], [-1, -1, -1]], [0, 0], [12, 12], pool, 4, 9)
