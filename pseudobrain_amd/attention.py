@@ -194,8 +194,11 @@ def _window_operands(q, k, v, gradients: bool = False):
 
 
 def _boundaries(cu):
+    """Whole numbers as the kernels read them: dense int32, those outside its range at its ends."""
     if cu is None or (cu.dtype == torch.int32 and cu.is_contiguous()):
         return cu
+    if cu.dtype == torch.int64:
+        cu = cu.clamp(-2**31, 2**31 - 1)
     return cu.to(torch.int32).contiguous()
 
 

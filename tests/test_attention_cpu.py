@@ -490,3 +490,14 @@ def test_oracle_gradients_against_differences(tq, tk, window, sinks):
             x[at_] = keep
             # the difference's own error: 1e-10 (third derivatives) and 1e-16 / 1e-5
             np.testing.assert_allclose((ends[0] - ends[1]) / 2e-5, r[n][at_], atol=1e-8)
+
+
+def test_numbers_past_32_bits_do_not_wrap_around():
+    """Lengths, tables and boundaries of 64 bits: what 32 do not hold stays as large, or as small, as they go."""
+    x = torch.tensor([[5, 2**32 + 3, -2**32 + 5], [2**62, -2**63, -1]])
+    want = torch.tensor([[5, 2**31 - 1, -2**31], [2**31 - 1, -2**31, -1]], dtype=torch.int32)
+    for y in (x, x.t().contiguous().t()):
+        got = at._boundaries(y)
+        assert got.dtype == torch.int32 and got.is_contiguous() and torch.equal(got, want)
+    assert torch.equal(at._boundaries(x[:, ::2]), want[:, ::2]) and at._boundaries(want) is want
+    assert torch.equal(at._boundaries(torch.tensor([3, 4], dtype=torch.int16)), torch.tensor([3, 4], dtype=torch.int32))

@@ -395,6 +395,20 @@ def test_read_of_many_sequences(batch):
             np.testing.assert_array_equal(f64(x)[seen], ref[:tokens][seen])
 
 
+def test_numbers_past_32_bits():
+    """64-bit lengths and table entries that 32 bits do not hold: no such keys, no such pages."""
+    q, cache, table, lengths = make([90, 40, 60], 16, 4, 2, 64, 1, torch.bfloat16, 41)
+    far, lens = table.long(), lengths.long()
+    far[0, 2] += 2**32
+    lens[1] -= 2**32
+    hole, none = table.clone(), lengths.clone()
+    hole[0, 2], none[1] = -1, 0
+    assert torch.equal(fc.paged_decode_attention_fp4(q, cache, far, lens, 0.125),
+                       fc.paged_decode_attention_fp4(q, cache, hole, none, 0.125))
+    for x, y in zip(fc.paged_cache_read_fp4(cache, far, lens, 150), fc.paged_cache_read_fp4(cache, hole, none, 150)):
+        assert torch.equal(x, y)
+
+
 def test_empty_reads():
     cache = filled(4, 8, 2, 64, 2)
     none = torch.zeros(0, dtype=torch.int32, device=DEV)

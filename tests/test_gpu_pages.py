@@ -126,6 +126,20 @@ def test_a_pool_over_absent_entries_grants_pages():
     assert left.tolist() == [0] and slots.tolist() == [*range(24, 28), *range(20, 24), *range(36, 40)]
 
 
+def test_numbers_past_32_bits():
+    """64-bit lengths, counts and ranges that 32 bits do not hold."""
+    far = torch.iinfo(torch.int64).max
+    free = ints([0, 0, 0, 0])
+    left = pg.paged_cache_release(ints([[4, 5], [6, 7]]), ints([0, far], torch.int64), ints([far, far], torch.int64), free,
+                                  ints([1], torch.int64), 16)
+    assert left.tolist() == [3] and free.tolist() == [0, 4, 5, 0]
+    slots, _, cu, after, left = pg.paged_cache_extend(
+        ints([[-1, -1]] * 4), ints([0, 2**32, 5 - 2**32, 0], torch.int64), ints([3, 1, 1, 2**32 + 1], torch.int64),
+        ints([8, 9]), ints([2**32 + 1], torch.int64), 16, 9)
+    assert cu.tolist() == [0, 3, 3, 3, 3] and slots.tolist() == [144, 145, 146] + [-1] * 6
+    assert after.tolist() == [3, 2**31 - 1, -2**31, 0] and left.tolist() == [1]
+
+
 def test_empty_calls_and_strided_tables():
     none = ints([])
     slots, positions, cu, after, left = pg.paged_cache_extend(none.view(0, 3), none, none, ints([4, 5]), ints([2]), 16, 6)
