@@ -39,10 +39,10 @@ struct Dec {
   static constexpr int OT = D / 16;                 // 16-wide output tiles: VLOADS * VE
   // Rows up to 256 bytes: 32 keys at a time. Wider ones 16, and Q in LDS where a
   // wave has two row blocks of it (its registers hold the sums, 16 keys and their
-  // values): two waves a SIMD up to 512 bytes, three up to 128.
+  // values): two waves a SIMD up to 512 bytes.
   static constexpr int KG = ROW <= 256 ? 2 : 1;     // 16-key groups at a time
   static constexpr bool q_in_lds(int rb) { return ROW > 512 || (ROW == 512 && rb == 2); }
-  static constexpr int OCC = ROW <= 128 ? 3 : ROW <= 512 ? 2 : 1;
+  static constexpr int OCC = ROW <= 512 ? 2 : 1;
 };
 
 // Scores of 16 keys: x += K rows (a lane's units) times Q rows.
@@ -347,9 +347,12 @@ __global__ __launch_bounds__(DEC_WAVES * 64, (Dec<DT, D>::OCC)) void decode_kern
   }
   if constexpr (Q_LDS) __syncthreads();  // Q's place is the joins'
 
-  join_waves<RB, D, JOINS>(merge, m, l, o, wave, lane, p.c);
+  // (opaque: what follows from the lane is worked out here, not kept through the main loop: 166
+  // registers for 169 in the 64-wide kernels of two row tiles, and so three waves a SIMD)
+  const int lane_ = static_cast<int>(opaque(lane));
+  join_waves<RB, D, JOINS>(merge, m, l, o, wave, lane_, p.c);
   if (wave != 0) return;
-  store_decoded<DT, D, RB, K::VE>(p, share.parts == 1, b, hk, row0, slot, lane, m, l, o);
+  store_decoded<DT, D, RB, K::VE>(p, share.parts == 1, b, hk, row0, slot, lane_, m, l, o);
 }
 
 // ---------------------------------------------------------------------------

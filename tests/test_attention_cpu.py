@@ -446,6 +446,24 @@ def test_no_mfma_result_is_read_early(monkeypatch):
     assert not problems, "\n".join(problems[:20])
 
 
+def test_narrow_decoding_keeps_its_registers(tmp_path):
+    """The 64-wide 16-bit decoding kernels: no register spilled, and few enough of them for three waves
+    a SIMD (168 of 512; two waves take 10 to 15% more time)."""
+    out = tmp_path / "decode.s"
+    subprocess.run([build.hipcc(), *build.HIPCC_FLAGS, f"-I{build.INCLUDE}", "--cuda-device-only", "-S",
+                    os.path.join(build.CSRC, "attn_decode.hip"), "-o", str(out)], check=True, capture_output=True)
+    meta = out.read_text().split("amdhsa.kernels:")[1]
+    found = 0
+    for entry in re.split(r"\n  - \.", meta)[1:]:
+        name = re.search(r"\.name:\s+(\S+)", entry).group(1)
+        if not re.search(r"decode_kernelILi[12]ELi64E", name):
+            continue
+        number = {k: int(re.search(rf"{k}:\s+(\d+)", entry).group(1)) for k in ("vgpr_count", "vgpr_spill_count")}
+        assert number["vgpr_spill_count"] == 0 and number["vgpr_count"] <= 168, (name, number)
+        found += 1
+    assert found == 4
+
+
 # ----------------------------------------------------------------------------
 # The oracle.
 # ----------------------------------------------------------------------------
