@@ -395,7 +395,7 @@ static int launch_decode(DecodeParams &p, hipStream_t stream) {
   };
   const bool ok = p.rows <= DEC_ROWS ? run(decode_kernel<DT, D, 1>, 1) : run(decode_kernel<DT, D, 2>, 2);
   if (!ok) return PBGDN_ERR_UNSUPPORTED;
-  launch_join<DT, D, Shares>(p, static_cast<long>(p.B) * p.Hk * p.rows <= JOIN_SPLIT_ROWS, 4, stream);
+  launch_join<DT, D, 4, Shares>(p, static_cast<long>(p.B) * p.Hk * p.rows <= JOIN_SPLIT_ROWS, stream);
   return hipGetLastError() == hipSuccess ? PBGDN_OK : PBGDN_ERR_LAUNCH;
 }
 

@@ -26,7 +26,6 @@ struct DecodeParams {
   float *part;     // [slots][Hk][rows][D] unnormalised outputs
   float2 *stat;    // [slots][Hk][rows] (largest score, sum)
   int B, T, Hq, Hk, group, rows, row_tiles, window, sinks, target;
-  int join_rows;   // query rows that a workgroup joins
   float c;
   int negate;
 };
@@ -252,24 +251,28 @@ __device__ __forceinline__ void store_decoded(const DecodeParams &p, bool last, 
 // Joins a sequence's parts, SPLIT waves to a (sequence, query row and head),
 // eight parts of a wave at a time: their outputs and their weights' statistics,
 // one a lane, are fetched together. Four waves a row where there are few rows,
-// one where there are many. Division says which parts they are.
-template <int DT, int D, int SPLIT, typename Division>
+// one where there are many. A workgroup takes PER rows, as many of them at a time as it has
+// waves for. Division says which parts they are.
+template <int DT, int D, int SPLIT, int PER, typename Division>
 static __global__ __launch_bounds__(256) void decode_join_kernel(const DecodeParams p) {
-  constexpr int VEC = D / 64, ROWS = 4 / SPLIT, AT_ONCE = 8;  // ROWS: rows of a workgroup
+  constexpr int VEC = D / 64, ROWS = 4 / SPLIT, AT_ONCE = 8;  // ROWS: rows of a workgroup at a time
+  static_assert(SPLIT == 1 || PER == ROWS, "a row's waves meet once");
   __shared__ float acc[SPLIT > 1 ? 4 : 1][D], stat[4][2];
   PBGDN_POISON_LDS(acc, sizeof(acc));
   PBGDN_POISON_SYNC();
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), w = wave % SPLIT;
-  const int tiles = (p.rows + p.join_rows - 1) / p.join_rows;
+  const int tiles = (p.rows + PER - 1) / PER;
   int id = blockIdx.x;
-  const int row0 = id % tiles * p.join_rows, row1 = row0 + p.join_rows < p.rows ? row0 + p.join_rows : p.rows;
+  const int row0 = id % tiles * PER, row1 = row0 + PER < p.rows ? row0 + PER : p.rows;
+  int row = row0 + wave / SPLIT;
   id /= tiles;
   const int hk = id % p.Hk, b = id / p.Hk;
   const Division all(p, lane);
   const int parts = all.parts_of(p, b, lane);
   if (parts == 1) return;  // written by the first kernel
+  if (SPLIT == 1 && row >= row1) return;
   const int first = all.first_of(p, b, lane);
-  for (int row = row0 + wave / SPLIT; row < row1; row += ROWS) {
+  do {
     float m = -INFINITY, l = 0.0f, o[VEC];
 #pragma unroll
     for (int e = 0; e < VEC; ++e) o[e] = 0.0f;
@@ -306,7 +309,7 @@ static __global__ __launch_bounds__(256) void decode_join_kernel(const DecodePar
         stat[wave][1] = l;
       }
       __syncthreads();
-      if (wave != 0) continue;  // (one row a workgroup: join_rows is 1)
+      if (wave != 0) return;
 #pragma unroll
       for (int i = 1; i < SPLIT; ++i) m = fmaxf(m, stat[i][0]);
       const float base = m == -INFINITY ? 0.0f : m;
@@ -326,19 +329,20 @@ static __global__ __launch_bounds__(256) void decode_join_kernel(const DecodePar
 #pragma unroll
     for (int e = 0; e < VEC; ++e) store_elem(p.o, at * D + lane * VEC + e, DT, o[e] * inv);
     if (p.lse && lane == 0) p.lse[at] = row_lse(m, l, p.c);
-  }
+    row += ROWS;
+  } while (PER > ROWS && row < row1);
 }
 
 // Launches the join of parts (decode_join_kernel) for a call whose parts have been: four
-// waves a row (`split`), or one, of which a workgroup takes `rows` one after the other.
-template <int DT, int D, typename Division>
-static void launch_join(DecodeParams &p, bool split, int rows, hipStream_t stream) {
-  p.join_rows = split ? 1 : rows;
-  const unsigned blocks = static_cast<unsigned>(p.B * p.Hk * ((p.rows + p.join_rows - 1) / p.join_rows));
+// waves a row (`split`), or one, of which a workgroup takes ROWS, four at a time.
+template <int DT, int D, int ROWS, typename Division>
+static void launch_join(const DecodeParams &p, bool split, hipStream_t stream) {
+  const int per = split ? 1 : ROWS;
+  const unsigned blocks = static_cast<unsigned>(p.B * p.Hk * ((p.rows + per - 1) / per));
   if (split)
-    hipLaunchKernelGGL((decode_join_kernel<DT, D, 4, Division>), dim3(blocks), dim3(256), 0, stream, p);
+    hipLaunchKernelGGL((decode_join_kernel<DT, D, 4, 1, Division>), dim3(blocks), dim3(256), 0, stream, p);
   else
-    hipLaunchKernelGGL((decode_join_kernel<DT, D, 1, Division>), dim3(blocks), dim3(256), 0, stream, p);
+    hipLaunchKernelGGL((decode_join_kernel<DT, D, 1, ROWS, Division>), dim3(blocks), dim3(256), 0, stream, p);
 }
 
 // The grid of a call's parts for kernels of rb row tiles a workgroup; 0 where it

@@ -849,7 +849,7 @@ static int launch_fp4(Fp4DecodeParams &p, int heads, hipStream_t stream) {
   }
   // Four waves a row where a sequence may have more parts than one fetches at once; else
   // eight rows a workgroup, which all take the same sums over the lengths.
-  launch_join<DT, D, Walk>(p.d, p.d.target > 8L * p.d.B, 8, stream);
+  launch_join<DT, D, 8, Walk>(p.d, p.d.target > 8L * p.d.B, stream);
   return hipGetLastError() == hipSuccess ? PBGDN_OK : PBGDN_ERR_LAUNCH;
 }
 
