@@ -388,6 +388,8 @@ __global__ __launch_bounds__(256) void paged_write_kernel(const WriteParams p) {
 
 template <int DT, int D>
 static int launch_decode(DecodeParams &p, hipStream_t stream) {
+  const bool split = static_cast<long>(p.B) * p.Hk * p.rows <= JOIN_SPLIT_ROWS;
+  if (join_blocks(p, split, 4) > MAX_BLOCKS) return PBGDN_ERR_UNSUPPORTED;
   const auto run = [&](auto kernel, int rb) {
     const unsigned blocks = decode_blocks(p, rb);
     if (blocks) hipLaunchKernelGGL(kernel, dim3(blocks), dim3(DEC_WAVES * 64), 0, stream, p);
@@ -395,7 +397,7 @@ static int launch_decode(DecodeParams &p, hipStream_t stream) {
   };
   const bool ok = p.rows <= DEC_ROWS ? run(decode_kernel<DT, D, 1>, 1) : run(decode_kernel<DT, D, 2>, 2);
   if (!ok) return PBGDN_ERR_UNSUPPORTED;
-  launch_join<DT, D, 4, Shares>(p, static_cast<long>(p.B) * p.Hk * p.rows <= JOIN_SPLIT_ROWS, stream);
+  launch_join<DT, D, 4, Shares>(p, split, stream);
   return hipGetLastError() == hipSuccess ? PBGDN_OK : PBGDN_ERR_LAUNCH;
 }
 

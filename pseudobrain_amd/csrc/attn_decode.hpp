@@ -333,16 +333,21 @@ static __global__ __launch_bounds__(256) void decode_join_kernel(const DecodePar
   } while (PER > ROWS && row < row1);
 }
 
+constexpr long MAX_BLOCKS = 0xffffff;  // of 256 threads: a launch has less than 2^32
+
 // Launches the join of parts (decode_join_kernel) for a call whose parts have been: four
 // waves a row (`split`), or one, of which a workgroup takes ROWS, four at a time.
+inline long join_blocks(const DecodeParams &p, bool split, int rows) {
+  const int per = split ? 1 : rows;
+  return static_cast<long>(p.B) * p.Hk * ((p.rows + per - 1) / per);
+}
 template <int DT, int D, int ROWS, typename Division>
 static void launch_join(const DecodeParams &p, bool split, hipStream_t stream) {
-  const int per = split ? 1 : ROWS;
-  const unsigned blocks = static_cast<unsigned>(p.B * p.Hk * ((p.rows + per - 1) / per));
+  const dim3 grid(static_cast<unsigned>(join_blocks(p, split, ROWS)));
   if (split)
-    hipLaunchKernelGGL((decode_join_kernel<DT, D, 4, 1, Division>), dim3(blocks), dim3(256), 0, stream, p);
+    hipLaunchKernelGGL((decode_join_kernel<DT, D, 4, 1, Division>), grid, dim3(256), 0, stream, p);
   else
-    hipLaunchKernelGGL((decode_join_kernel<DT, D, 1, ROWS, Division>), dim3(blocks), dim3(256), 0, stream, p);
+    hipLaunchKernelGGL((decode_join_kernel<DT, D, 1, ROWS, Division>), grid, dim3(256), 0, stream, p);
 }
 
 // The grid of a call's parts for kernels of rb row tiles a workgroup; 0 where it
@@ -350,7 +355,7 @@ static void launch_join(const DecodeParams &p, bool split, hipStream_t stream) {
 inline unsigned decode_blocks(DecodeParams &p, int rb) {
   p.row_tiles = (p.rows + rb * DEC_ROWS - 1) / (rb * DEC_ROWS);
   const long blocks = (static_cast<long>(p.target) + p.B) * p.Hk * p.row_tiles;
-  return blocks > 0x7fffffffL || static_cast<long>(p.B) * p.Hk * p.rows > 0x7fffffffL ? 0u : static_cast<unsigned>(blocks);
+  return blocks > MAX_BLOCKS || static_cast<long>(p.B) * p.Hk * p.rows > 0x7fffffffL ? 0u : static_cast<unsigned>(blocks);
 }
 
 inline bool decode_sizes_ok(int B, int T, int Hq, int Hk, int D) {

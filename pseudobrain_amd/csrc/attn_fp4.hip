@@ -828,7 +828,13 @@ static int launch_fp4(Fp4DecodeParams &p, int heads, hipStream_t stream) {
   const int rb = fp4_row_tiles(D, p.d.rows);
   p.d.row_tiles = (p.d.rows + rb * DEC_ROWS - 1) / (rb * DEC_ROWS);
   const long blocks = (p.d.target + 7L) / 8 * 8 * (p.d.Hk / heads) * p.d.row_tiles;
-  if (blocks > 0xffffffL || static_cast<long>(p.d.B) * p.d.Hk * p.d.rows > 0x7fffffffL) return PBGDN_ERR_UNSUPPORTED;
+  // Joined by four waves a row where a sequence may have more parts than one fetches at once;
+  // else eight rows a workgroup, which all take the same sums over the lengths.
+  const bool split = p.d.target > 8L * p.d.B;
+  if (blocks > MAX_BLOCKS || join_blocks(p.d, split, 8) > MAX_BLOCKS ||
+      static_cast<long>(p.d.B) * p.d.Hk * p.d.rows > 0x7fffffffL) {
+    return PBGDN_ERR_UNSUPPORTED;
+  }
   const auto run = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(DEC_WAVES * 64), 0, stream, p);
   };
@@ -847,9 +853,7 @@ static int launch_fp4(Fp4DecodeParams &p, int heads, hipStream_t stream) {
     else
       run(fp4_decode_kernel<DT, D, 2, NEAR, false, 1>);
   }
-  // Four waves a row where a sequence may have more parts than one fetches at once; else
-  // eight rows a workgroup, which all take the same sums over the lengths.
-  launch_join<DT, D, 8, Walk>(p.d, p.d.target > 8L * p.d.B, stream);
+  launch_join<DT, D, 8, Walk>(p.d, split, stream);
   return hipGetLastError() == hipSuccess ? PBGDN_OK : PBGDN_ERR_LAUNCH;
 }
 
@@ -1032,7 +1036,7 @@ extern "C" int pbattn_fp4_read(const void *k_cache, const void *v_cache, const v
   p.per_block = static_cast<int>(even < 1 ? 1 : even > READ_TOKENS ? READ_TOKENS : even);
   while (p.per_block > 1 && static_cast<long>(p.per_block) * Hk * p.eighths > 0x3fffffffL) p.per_block /= 2;  // (32-bit counts)
   const long blocks = (tokens + static_cast<long>(p.per_block) - 1) / p.per_block;
-  if (blocks > 0xffffffL) return PBGDN_ERR_UNSUPPORTED;  // (a launch has less than 2^32 threads)
+  if (blocks > MAX_BLOCKS) return PBGDN_ERR_UNSUPPORTED;
   const dim3 grid(static_cast<unsigned>(blocks > 0 ? blocks : 1));
   hipStream_t s = static_cast<hipStream_t>(stream);
   const size_t bytes = static_cast<size_t>(tokens) * Hk * D * attn_bytes(dtype);

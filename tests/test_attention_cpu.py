@@ -162,6 +162,12 @@ def decode(**over):
     return _lib.attn_lib().pbattn_paged_decode(*args.values())
 
 
+def test_decoding_of_more_threads_than_a_launch_has_is_refused():
+    """2^24 workgroups of 256 threads, in the parts' join or their own launch: told before either."""
+    assert decode(B=1 << 22, Hq=16, Hk=4) == _lib.ERR_UNSUPPORTED
+    assert decode(B=1 << 23, Hq=2, Hk=2) == _lib.ERR_UNSUPPORTED
+
+
 @pytest.mark.parametrize("over,code", [
     (dict(dtype=-1), _lib.ERR_INVALID_ARGUMENT),
     (dict(T=0), _lib.ERR_INVALID_ARGUMENT),

@@ -124,6 +124,11 @@ def test_decode_rejects(over, code):
     assert decode(B=0) == _lib.OK
 
 
+def test_a_join_of_more_threads_than_a_launch_has_is_refused():
+    """2^24 workgroups of 256 threads: told before the parts are worked out."""
+    assert decode(B=1 << 22, Hq=32, Hk=4) == _lib.ERR_UNSUPPORTED
+
+
 def write(**over):
     args = dict(kn=FAKE, vn=FAKE, dtype=1, kv=strides(256, 128, 256, 128), k=FAKE, v=FAKE, ks=FAKE, vs=FAKE, strides=ROWS,
                 page=16, pages=8, slots=FAKE, N=3, Hk=2, D=128, stream=None)
