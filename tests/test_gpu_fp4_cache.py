@@ -144,6 +144,16 @@ def test_weights_are_rounded_to_nearest(d, dtype):
     assert np.abs(f64(o)).max() <= bound
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("hq,hk,draft", [(6, 3, 1), (3, 3, 5), (24, 3, 3), (7, 1, 1), (20, 1, 1)])
+def test_an_odd_number_of_heads(d, dtype, hq, hk, draft):
+    """Heads whose rows share lines with the next one's, and one head alone."""
+    for heads_first, page in ((False, 16), (True, 2)):
+        x = make([300, 5, 1000], page, hq, hk, d, draft, dtype, d + hk, heads_first)
+        check("odd heads", *x, d ** -0.5, 400, 3)
+
+
 def test_long_contexts_are_split_and_joined():
     x = make([20000, 3, 9000], 64, 8, 1, 128, 1, torch.bfloat16, 20)
     check("split", *x, 128 ** -0.5)
