@@ -270,6 +270,45 @@ def test_offsets_past_32_bits():
         compare("past 32 bits", o[0], ref["o"], ref["o_tol"])
 
 
+def test_every_kernel_past_32_bits():
+    """Decoding over codes beyond 4 GiB: each width, type and number of row tiles, pages at both ends of
+    the cache, drafts, the last of which sees keys and values whose scale is that of NaN."""
+    if torch.cuda.mem_get_info()[0] < 14 << 30:
+        pytest.skip("needs 14 GiB of free device memory")
+    pages, page, n, draft = 16900, 16, 75, 4  # 4.4 GB of codes each
+    whole = fc.fp4_cache(pages, page, 128, 256, DEV, False)
+    lengths = torch.tensor([n, 0], dtype=torch.int32, device=DEV)
+    first = torch.tensor([pages - 1, 0, pages - 3, 1, pages - 2], dtype=torch.int32, device=DEV)
+    table = torch.stack((first, first))
+    slots = (first.long()[:, None] * page + torch.arange(page, device=DEV)).flatten()[:n]
+    hk = 2
+    for d in (64, 128, 256):
+        cache = [x.view(pages, page, 128 * 256 // d, -1)[:, :, :hk] for x in whole]  # its first heads
+        for dtype in (torch.float32, torch.bfloat16, torch.float16):
+            gen = torch.Generator().manual_seed(d)
+            k, v = (torch.randn(n, hk, d, generator=gen).to(torch.bfloat16).to(DEV) for _ in range(2))
+            held_k, held_v = (of.values(*of.quantise(f64(x))) for x in (k, v))
+            for group, t in ((3, 1), (2, draft), (8, draft)):
+                for bad in (False, True) if t > 1 else (False,):
+                    q = torch.randn(2, t, hk * group, d, generator=gen).to(dtype).to(DEV)
+                    fc.paged_cache_write_fp4(k, v, cache, slots)  # (and over the last one's scales of NaN)
+                    if bad:
+                        cache[2][first[(n - 1) // page].long(), (n - 1) % page] = 255
+                        cache[3][first[(n - 2) // page].long(), (n - 2) % page, :, -1] = 255
+                    print(f"[past 32 bits] {d} {dtype} rows {group * t} bad {bad}", flush=True)
+                    o = fc.paged_decode_attention_fp4(q, cache, table, lengths, d ** -0.5, 60, 3)
+                    assert torch.count_nonzero(o[1]) == 0
+                    for i in range(t):
+                        m = n - t + 1 + i
+                        if bad and i == t - 1:
+                            assert torch.isnan(o[0, i]).all()
+                            continue
+                        ref = oa.attention(f64(q[0, i:i + 1]), held_k[:m], held_v[:m], d ** -0.5, 60, 3, dtype=NAMES[dtype])
+                        got, hidden = o[0, i:i + 1], d - 32 if bad and i == t - 2 else d
+                        assert not torch.isfinite(got[..., hidden:]).any()
+                        compare(f"token {i}", got[..., :hidden], ref["o"][..., :hidden], ref["o_tol"][..., :hidden])
+
+
 @pytest.mark.parametrize("dtype,d", [(torch.float32, 64), (torch.bfloat16, 128), (torch.bfloat16, 256), (torch.float16, 128)])
 @pytest.mark.parametrize("sign", [1.0, -1.0])
 @pytest.mark.parametrize("draft,hq", [(1, 2), (3, 16)])
