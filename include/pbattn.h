@@ -296,7 +296,8 @@ int pbattn_pages_release(const int32_t *page_table, int64_t table_row, int max_p
  *   y_i = x_i r (w_i + weight_offset),
  *   (y_a, y_b) -> (y_a cos - y_b sin, y_b cos + y_a sin)   for the R / 2 pairs (a, b)
  * of the first R values: i and R / 2 + i, or with `interleaved` 2 i and 2 i + 1; the
- * others stay. float32 throughout, rounded once.
+ * others stay. float32 throughout, rounded once; rows whose squares float32 does not hold
+ * are scaled by a power of two for them.
  *
  *   q, k         [B, T, Hq, D] and [B, T, Hk, D] dtype by `strides` (batch, token, head of
  *                q, then of k: 6 values, elements, not negative), the innermost axis

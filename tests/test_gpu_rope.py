@@ -126,6 +126,29 @@ def test_large_and_small_rows(dtype, size, d):
     check("sizes", x, eps=1e-6)
 
 
+@pytest.mark.parametrize("dtype,size", [(torch.float32, 2.0**127), (torch.bfloat16, 2.0**127), (torch.float32, 1e25),
+                                        (torch.float32, 1e-25), (torch.bfloat16, 1e-30)])
+@pytest.mark.parametrize("d", [64, 50, 256])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rows_whose_squares_float32_does_not_hold(dtype, size, d, interleaved):
+    """Rows near the ends of the range among ordinary ones, with an eps of no weight beside them."""
+    x = make(1, 6, 8, 3, d, 20 if d == 50 else 32, dtype, 15)
+    for n in ("q", "k"):
+        x[n] /= x[n].abs().max()
+        x[n][0, 1:3] = (x[n][0, 1:3].float() * size).to(dtype)
+        x[n][0, 4, 1] = (x[n][0, 4, 1].float() * size).to(dtype)
+    check("ends of the range", x, eps=0.0 if size < 1 else 1e-6, interleaved=interleaved)
+
+
+def test_ordinary_values_of_eps_count_beside_small_rows():
+    """Tiny rows under an ordinary eps, and an eps of their own size (as the float32 that the kernels
+    take: 1e-44 lies between two that are 2^-149 apart)."""
+    x = make(1, 6, 4, 2, 64, 32, torch.float32, 16)
+    x["q"], x["k"] = x["q"] * 1e-25, x["k"] * 1e-22
+    for eps in (1e-6, 1e-35, 1e-44):
+        check("eps", x, eps=float(np.float32(eps)))
+
+
 @pytest.mark.parametrize("d", [64, 50])
 def test_a_bad_value_stays_in_its_row(d):
     """An infinity or NaN reaches its own row alone, an infinity no value that is not rotated with it."""
