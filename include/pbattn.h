@@ -208,9 +208,10 @@ int pbattn_paged_write(const void *k, const void *v, int dtype, const int64_t *k
 
 /*
  * pbattn_paged_decode over such a cache: the same arguments besides, and the same
- * results for the values that the cache stands for. q in any of the three types;
- * scores and outputs of float16 and float32 rows are as exact as over a cache of
- * their own type (their products are taken in two and three parts).
+ * results for the values that the cache stands for. q in any of the three types.
+ * Queries enter the products exactly (float16 and float32 rows in two and three
+ * parts), the weights of 16-bit rows in two parts, rounded to 16 bits (off by 2^-16
+ * at most), those of float32 rows in three, with all of their 24.
  */
 int pbattn_fp4_decode(const void *q, int dtype, const void *k_cache, const void *v_cache, const void *k_scale,
                       const void *v_scale, const int64_t *strides, int page_size, int num_pages,

@@ -8,12 +8,13 @@
 // worked out once, a lane for each key, and go through LDS to the lanes that need them.
 // A block's loads go out a whole block ahead, and page table entries one before that.
 //
-// 64 contexts up to 16,384 tokens, 32 heads of 128 on 8, bf16: 95 us, 5.9 TB/s, what
-// reading alone reaches (a bfloat16 cache takes 365). 233 contexts behind a window of
-// 4,096, 16 heads of 256 on 2, four drafted tokens: 120 us for 79 us of bytes, bound by
-// issue: both tiles of 16 rows unpack the cache for themselves (one drafted token: 80).
+// 64 contexts up to 16,384 tokens, 32 heads of 128 on 8, bf16: 99 us, 5.7 TB/s; reading
+// alone reaches 5.9 (a bfloat16 cache takes 365). 233 contexts behind a window of
+// 4,096, 16 heads of 256 on 2, four drafted tokens: 130 us for 79 us of bytes, bound by
+// issue: both tiles of 16 rows unpack the cache for themselves (one drafted token: 77).
 // Two tiles a workgroup leave one wave a SIMD or spill: 126 to 128 us for the 136 of the
-// whole call, but float16 rows 79 for 58 and float32 rows 110 for 64 (64 contexts).
+// whole call (weights in one part), but float16 rows 79 for 58 and float32 rows 110 for 64
+// (64 contexts).
 #include <type_traits>
 
 #include "attn_decode.hpp"
@@ -131,7 +132,9 @@ struct Walk {
 // them. Q: bfloat16 rows as they are, float16 rows in two, float32 rows in three, all of
 // them exactly. The weights: two parts, which round them to 16 bits (2^-16: small beside a
 // 16-bit result's own rounding, and to either side), and for float32 rows three, which are
-// all of their 24 bits.
+// all of their 24 bits. (One part for bfloat16 rows takes 107 us for 113 with 64 contexts up
+// to 16,384 tokens, and leaves an error of 2^-9 in every weight: 0.0021 to 0.0023 against 64
+// bits, for the 0.0017 of the result's own rounding.)
 // So the cache's values, exact in bfloat16, meet every type of row in the same kernel.
 template <int DT>
 struct Parts {
@@ -214,7 +217,9 @@ __device__ __forceinline__ void wave_lds_order() {
 __device__ __forceinline__ int key_of(int m) { return 4 * (m % 4) + m / 4; }
 
 // Workgroups of a CU at once (waves of a SIMD), by the registers that the sums of RB row
-// tiles and two blocks of keys and values take.
+// tiles and two blocks of keys and values take. Four at D = 64 spill 2 to 5 registers (64
+// contexts up to 8,192 tokens, 24 heads on 8: heads before tokens 49 us, 52 with three and
+// no spill; float16, two drafted tokens 52.5 and 54; tokens first 50 and 48).
 constexpr int fp4_held(int D, int RB) { return RB == 2 || D == 256 ? 2 : D == 128 ? 3 : 4; }
 
 // NEAR: the caches' offsets fit 32 bits. ONCE: no other workgroup reads the same lines, so

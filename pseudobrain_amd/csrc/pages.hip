@@ -5,8 +5,8 @@
 // token or page: every workgroup forms the sums for itself (a scan over at most 4,096
 // requests in LDS), finds its pieces' requests by bisection and writes them, so that a
 // call is one launch and needs nothing kept between workgroups. Bound by latency: the
-// launch, the requests' numbers, three scans, the table's entry (64 requests: release 4.0
-// us, extend 4.8; 233 with 4,000 tokens 4.2 and 5.7).
+// launch, the requests' numbers, three scans, the table's entry (64 requests: release 3.6
+// us, extend 4.7; 233 with 4,000 tokens 4.1 and 6.1).
 #include "attn.hpp"
 #include "pages.hpp"
 #include "device.hpp"

@@ -166,7 +166,9 @@ def paged_decode_attention_fp4(q, cache, page_table, lengths, scale: float, wind
     """paged_decode_attention over a 4-bit cache (k, v, k_scale, v_scale): q [B,T,Hq,D] in
     float32, bfloat16 or float16, the T newest tokens of each sequence, against the values
     that the cache stands for; page_table, lengths, window, sinks, return_lse and out as
-    there. Nothing but q's own type limits the result: a float32 q gets float32 products."""
+    there. Results are as exact as q's own type: softmax weights enter the products with 16 bits
+    for a 16-bit q and with all of float32's 24 for a float32 one, sums are float32, and the
+    result is rounded once."""
     _inference_only("paged_decode_attention_fp4", q)
     if _untraced(q, *cache, page_table, lengths):
         o, lse = _decode(q, cache, page_table, lengths, scale, window, sinks, out, return_lse)
