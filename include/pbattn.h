@@ -62,7 +62,7 @@ extern "C" {
 #endif
 
 /* Raised with every function that is added or changed. */
-#define PBATTN_ABI_VERSION 3
+#define PBATTN_ABI_VERSION 4
 
 /* Most query tokens a sequence may have in pbattn_paged_decode. */
 #define PBATTN_MAX_DRAFT 16
