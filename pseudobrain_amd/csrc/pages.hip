@@ -126,7 +126,7 @@ __global__ __launch_bounds__(SCAN_THREADS) void extend_kernel(const PoolParams p
 // The entries of all ranges, in the requests' order, are one list, of which each workgroup
 // takes a run: it counts the pages before its own and pushes those in it. An entry below 0 is
 // no page (the caches' other operators skip it too) and must not come back as one. (64 requests,
-// one page each 3.9 us; a request's 16,384 pages 8.8; 256 requests of 1,024 pages 111: a run's
+// one page each 3.9 us; a request's 16,384 pages 6.6; 256 requests of 1,024 pages 74: a run's
 // start costs the reading of all before it, which a serving step, of few pages, does not notice.)
 constexpr int RELEASE_THREADS = 512, RELEASE_WAVES = RELEASE_THREADS / 64;
 constexpr int RELEASE_BLOCKS = 64;  // most workgroups
@@ -159,30 +159,34 @@ __global__ __launch_bounds__(RELEASE_THREADS) void release_kernel(const PoolPara
   const long even = (total + gridDim.x - 1) / gridDim.x, run = (even + RELEASE_THREADS - 1) / RELEASE_THREADS * RELEASE_THREADS;
   const long k0 = blockIdx.x * run, k1 = k0 + run < total ? k0 + run : total;
   if (blockIdx.x > 0 && k0 >= total) return;
-  // Entries k + 64 i of the list below `end` (-1 past it). Where a request's have ended it is the
-  // next one's, or one that bisection finds.
+  // Entries k + 64 i of the list below `end` (-1 past it, where the last is read, so that all
+  // loads are in flight together). Where a request's have ended it is the next one's, or one that
+  // bisection finds.
   int top = 1;
   while (top < p.B) top *= 2;
+  int b = -1;  // whose the last entry was, where that request's entries lie and the next one's begin
+  long from = 0, next = 0;
   const auto entries = [&](auto &x, long k, long end) __attribute__((always_inline)) {
     constexpr int N = sizeof(x) / sizeof(x[0]);
-    int b = -1;
-    long from = 0, next = 0;
 #pragma unroll
-    for (int i = 0; i < N; ++i, k += 64) {
-      if (k >= next && k < end) {
-        const auto ends = [&] { return b + 1 < p.B ? start[b + 1] : end; };
+    for (int i = 0; i < N; ++i) {
+      const long at = k + 64 * i < end ? k + 64 * i : end - 1;
+      if (at >= next) {
+        const auto ends = [&] { return b + 1 < p.B ? start[b + 1] : total; };
         ++b;
         next = ends();
-        if (i == 0 || k >= next) {
+        if (at >= next) {
           b = 0;
-          for (int step = top / 2; step > 0; step /= 2)  // the last b with start[b] <= k
-            if (b + step < p.B && start[b + step] <= k) b += step;
+          for (int step = top / 2; step > 0; step /= 2)  // the last b with start[b] <= at
+            if (b + step < p.B && start[b + step] <= at) b += step;
           next = ends();
         }
         from = table_of[b];
       }
-      x[i] = k < end ? p.table[from + k] : -1;
+      x[i] = p.table[from + at];
     }
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = k + 64 * i < end ? x[i] : -1;
   };
   // pages of the threads before this one, in `all` those of all of them
   const auto ranks = [&](long mine, long &all) __attribute__((always_inline)) {
